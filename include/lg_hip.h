@@ -268,6 +268,69 @@ int    lg_hip_attention_noalloc(const float *d_q, const uint16_t *d_kc, const ui
                                 int n_head_kv, int hd, int seq, int window, int pos, float *d_out, void *stream);
 int    lg_hip_attention_noalloc_init(void);
 size_t lg_hip_attention_noalloc_limit(void);
+/* ---- operators of a batched decode step: what a program that serves many sequences calls between its matrix products -----
+ * No counterpart in the reference, which serves one conversation from one cache.  The pointers called d_ are device memory on the
+ * current device; nothing is allocated, the launches go to `stream` (a hipStream_t of that device, NULL = the default stream) and the
+ * call returns without waiting; a stream under capture takes it.  Working memory (d_work, aligned to 256 bytes, at least as
+ * many bytes as the _workspace function says for the same sizes) holds nothing from call to call: calls on one stream may share it, calls
+ * that can overlap may not, captured or eager.  Calls may come from several threads. */
+
+/* A KV cache in pages.  Position t of a sequence is row t % page_size of page table[t / page_size]; a slot is page * page_size + row.
+ * Keys and values of one layer, binary16: value i of key head h of a row is k[page * page_stride + row * row_stride + h * head_dim + i].
+ * page_size a power of two of 16..256; head_dim 64, 128, 256 or 512; strides count values, are multiples of 8 and hold their rows;
+ * k and v aligned to 16 bytes.  n_pages * page_size is below 2^31. */
+struct lg_hip_pages {
+    uint16_t *k, *v;
+    int32_t n_pages, page_size, n_head_kv, head_dim;
+    int64_t row_stride, page_stride;
+};
+/* Pages and slots of a step from the lengths of n_seq (0..4096) sequences before and after it.  d_table [n_seq][max_blocks] holds the
+ * pages of every sequence; d_free [n_pages] is a stack of the free ones, *d_n_free its height.  Sequences that shrink (rejected drafts,
+ * an end) put pages back (their table entries become -1), those that grow take pages off the top.  The pages that are put back go first,
+ * so that a plan with d_len_old and d_len_new exchanged undoes a plan exactly.
+ * d_start [n_seq + 1]: the sums of new tokens before each sequence; d_slots [n_slots]: new token j of sequence i, at position
+ * len_old[i] + j, has its slot at d_start[i] + j, and what is left of n_slots is -1.  *d_status: 0, or the LG_HIP_PLAN_ bits of what was
+ * wrong; then table, stack and height are as they were, d_start is 0 and every slot -1.
+ * The table's entries in use are distinct pages: a table that names a page twice is not looked for. */
+enum { LG_HIP_PLAN_BAD_LENGTH = 1,     /* a length below 0 or above max_blocks * page_size */
+       LG_HIP_PLAN_NO_PAGES = 2,       /* not enough free pages */
+       LG_HIP_PLAN_NO_SLOTS = 4,       /* more new tokens than n_slots */
+       LG_HIP_PLAN_BAD_STACK = 8,      /* a height outside 0..n_pages, also with the pages that come back */
+       LG_HIP_PLAN_BAD_PAGE = 16 };    /* a page that moves or is written into is outside 0..n_pages-1 */
+size_t lg_hip_paged_plan_workspace(int n_seq);
+int    lg_hip_paged_plan(int n_seq, int page_size, int n_pages, int max_blocks, const int32_t *d_len_old, const int32_t *d_len_new,
+                         int32_t *d_table, int32_t *d_free, int32_t *d_n_free, int32_t *d_start, int32_t *d_slots, int n_slots,
+                         int32_t *d_status, void *d_work, size_t work_bytes, void *stream);
+/* Rows of n_tok new tokens, n_head_kv * head_dim floats each (already normed and rotated, as for lg_hip_attention), `stride` floats apart
+ * (a multiple of 4; d_k and d_v aligned to 16 bytes: parts of the rows of one product may be given), rounded to the nearest binary16
+ * and stored at their slots.  Tokens whose slot is outside 0..n_pages*page_size-1 are left out.  Of two tokens of one slot either may stay. */
+int    lg_hip_paged_write(const struct lg_hip_pages *pages, const float *d_k, const float *d_v, int64_t stride, const int32_t *d_slots,
+                          int n_tok, void *stream);
+/* Attention of one new token per sequence: out = softmax(scale * q.k) v over the positions max(0, len - window) .. len - 1 (window = 0: from 0)
+ * of its pages, the new token's own among them; n_head / n_head_kv <= 8 query heads share a key head.  q and out: n_head * head_dim floats a
+ * row, q_stride (a multiple of 4; d_q aligned to 16 bytes) and out_stride floats apart.  d_len [n_seq] is read on the device; lengths above
+ * max_len or max_blocks * page_size count as that, a sequence of length 0 or less gets zeros, positions whose page is outside 0..n_pages-1
+ * are left out.  max_len bounds the lengths that a captured call will see, and the working memory.  The rows of a verify block are
+ * sequences with the same table row and lengths one apart.  What masked positions hold does not matter; infinities and NaN in positions
+ * that are seen give outputs that are not finite in the heads that read them. */
+size_t lg_hip_paged_attention_workspace(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, int window);
+int    lg_hip_paged_attention(const struct lg_hip_pages *pages, const float *d_q, int64_t q_stride, int n_seq, int n_head, const int32_t *d_table,
+                              int max_blocks, const int32_t *d_len, int max_len, int window, float scale, float *d_out, int64_t out_stride,
+                              void *d_work, size_t work_bytes, void *stream);
+/* How a token is drawn from a row of logits.  temperature not above 0: the first largest one.  Otherwise the filters are taken in this order,
+ * on softmax(logits / temperature): top_k (0 and less: off) keeps the k likeliest, of equal logits the lower index; top_p (1 and more: off)
+ * of those the fewest whose share of them reaches it, at least one; min_p (0 and less: off; above 1 as 1) of those the ones with at least
+ * min_p times the likeliest token's probability.  NaN parameters are off, NaN logits are -inf. */
+struct lg_hip_sampling { float temperature; int32_t top_k; float top_p, min_p; };
+/* One token per row of n_vocab (1..524288) logits, `stride` floats apart, with the row's own parameters and random number u of [0, 1):
+ * with w_i = exp((l_i - max) / temperature) rounded to a multiple of 2^-44 and S the sum of the kept ones, the first token in index order
+ * whose running sum is above u * S.  All sums are of whole numbers: the token does not depend on how a row is split.  d_prob (or NULL):
+ * its share of the kept ones; d_kept (or NULL): how many tokens were kept (those of weight 0 do not count).  A row without a logit above
+ * -inf gives -1, 0, 0. */
+size_t lg_hip_sample_workspace(int rows, int n_vocab);
+int    lg_hip_sample(const float *d_logits, int64_t stride, int rows, int n_vocab, const struct lg_hip_sampling *d_params, const float *d_u,
+                     int32_t *d_tok, float *d_prob, int32_t *d_kept, void *d_work, size_t work_bytes, void *stream);
+
 /* ffn_down of a verify block of 4..8 rows on the matrix cores (lg_k_down_m), in isolation: act = rows x FF floats (quantized
  * to q8 on the device, as the gate/up kernel's epilogue does), down = FF-wide q4_0 rows of the E outputs; out = rows x E,
  * the four K-quarter slabs added by the four workgroups of a row group themselves (join = 1: a hand-over inside their XCD)

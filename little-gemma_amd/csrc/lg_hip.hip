@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "../../include/lg_hip.h"
+#include "lg_host.h"
 #include "lg_kernels.h"
 #include "lg_wide.h"
 #include "lg_fused.h"
@@ -39,6 +40,13 @@ static_assert(LG_HIP_MAX_ROWS == LG_HIP_MAX_ROWS_DEV, "row limits must agree");
 // ---- errors -----------------------------------------------------------------------------------
 static thread_local char g_err[512] = "";
 static int fail(int code, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof g_err, fmt, ap);
+    va_end(ap);
+    return code;
+}
+int lg_fail(int code, const char *fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof g_err, fmt, ap);

@@ -1,0 +1,390 @@
+// lg_pages.h — a KV cache in pages that many sequences share: its bookkeeping, the rows of new tokens, and attention of one new token per sequence.
+//
+// Position t of sequence i is row t % P of page table[i][t / P] (P = page_size, a power of two of 16..256).  Free pages lie on a stack.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <hip/hip_fp16.h>
+#include <stdint.h>
+
+#define LG_PLAN_SEQS 4096           // sequences of a plan: their running sums lie in LDS
+#define LG_PLAN_WG   1024
+
+// ---- plan ------------------------------------------------------------------------------------------------------------
+enum { LG_PLAN_BAD_LEN = 1, LG_PLAN_NO_PAGES = 2, LG_PLAN_NO_SLOTS = 4, LG_PLAN_BAD_STACK = 8, LG_PLAN_BAD_PAGE = 16 };   // LG_HIP_PLAN_* of lg_hip.h
+
+struct PlanArgs {
+    const int32_t *len_old, *len_new;   // [n_seq]
+    int32_t *table;                     // [n_seq][max_blocks]
+    int32_t *stack, *n_free;            // [n_pages], its height
+    int32_t *start;                     // [n_seq + 1]
+    int32_t *slots;                     // [n_slots]
+    int32_t *status;
+    int n_seq, shift, n_pages, max_blocks, n_slots;
+};
+
+// Inclusive sum over the workgroup of one value per thread; `part`: [waves] of LDS.  *total = the sum of all.
+template <typename T>
+__device__ __forceinline__ T lg_block_scan(T v, T *part, T *total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    for (int o = 1; o < 64; o <<= 1) { const T u = __shfl_up(v, o); if (lane >= o) v += u; }
+    __syncthreads();                                        // (part may still be read from a call before)
+    if (lane == 63) part[wave] = v;
+    __syncthreads();
+    T before = 0, all = 0;
+    for (int w = 0; w < waves; ++w) { const T p = part[w]; if (w < wave) before += p; all += p; }
+    *total = all;
+    return v + before;
+}
+// The sequence that entry e belongs to: sums[i] <= e < sums[i + 1]
+__device__ __forceinline__ int lg_owner(const int32_t *sums, int n, int e) {
+    int lo = 0, hi = n;
+    while (lo < hi) { const int mid = (lo + hi) >> 1; if (sums[mid + 1] <= e) lo = mid + 1; else hi = mid; }
+    return lo;
+}
+
+// Lengths before and after a step -> pages and slots.  With nb(l) = ceil(l / P), sequence i returns max(0, nb(old) - nb(new)) pages and takes
+// max(0, nb(new) - nb(old)); all returned pages go on the stack first, the first one topmost, then the needed ones are taken from its top in
+// order, so that the plan with the lengths exchanged undoes this one exactly.  All or nothing: whatever *status reports leaves table and stack alone.
+// One workgroup: the whole step is a few thousand words (64 sequences, one new token each: 2 KB), its time is launch and a chain of
+// memory round trips, which a grid would lengthen by a launch per phase.
+__global__ __launch_bounds__(LG_PLAN_WG) void lg_k_plan(PlanArgs a) {
+    __shared__ int32_t tok[LG_PLAN_SEQS + 1], need[LG_PLAN_SEQS + 1], freed[LG_PLAN_SEQS + 1];
+    __shared__ long long part[LG_PLAN_WG / 64];
+    __shared__ int bad;
+    const int t = threadIdx.x, P = 1 << a.shift, n = a.n_seq;
+    const long long most = (long long)a.max_blocks << a.shift;
+    constexpr int CH = LG_PLAN_SEQS / LG_PLAN_WG;
+    if (t == 0) bad = 0;
+    __syncthreads();
+    auto blocks = [&](int len) { return (int)(((long long)len + P - 1) >> a.shift); };
+    // running sums: sequences t * CH .. t * CH + CH - 1 are this thread's
+    long long v[3][CH], sum[3] = { 0, 0, 0 };
+    #pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i = t * CH + c;
+        int lo = i < n ? a.len_old[i] : 0, ln = i < n ? a.len_new[i] : 0;
+        if (lo < 0 || ln < 0 || lo > most || ln > most) { atomicOr(&bad, LG_PLAN_BAD_LEN); lo = ln = 0; }
+        const int d = blocks(ln) - blocks(lo);
+        v[0][c] = ln > lo ? ln - lo : 0; v[1][c] = d > 0 ? d : 0; v[2][c] = d < 0 ? -d : 0;
+        #pragma unroll
+        for (int k = 0; k < 3; ++k) sum[k] += v[k][c];
+    }
+    long long all[3];
+    int32_t *const dst[3] = { tok, need, freed };
+    #pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        long long run = lg_block_scan(sum[k], part, &all[k]) - sum[k];
+        #pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int i = t * CH + c;
+            if (i <= n) dst[k][i] = (int32_t)run;             // (used only where the total fits, below)
+            run += v[k][c];
+        }
+        if (t == 0 && n == LG_PLAN_SEQS) dst[k][n] = (int32_t)all[k];
+    }
+    const int nf = *a.n_free;
+    if (t == 0) {
+        if (nf < 0 || nf > a.n_pages || all[2] + nf > a.n_pages) atomicOr(&bad, LG_PLAN_BAD_STACK);
+        else if (all[1] > nf + all[2]) atomicOr(&bad, LG_PLAN_NO_PAGES);
+        if (all[0] > a.n_slots) atomicOr(&bad, LG_PLAN_NO_SLOTS);
+    }
+    __syncthreads();
+    int st = bad;
+    const int nt = (int)all[0], nn = (int)all[1], ng = (int)all[2], top = nf + ng;
+    if (!st) {
+        // every page id that the step would move or write into, before anything moves
+        int ids = 0;
+        for (int e = t; e < ng; e += LG_PLAN_WG) {
+            const int i = lg_owner(freed, n, e);
+            const int id = a.table[(size_t)i * a.max_blocks + blocks(a.len_new[i]) + e - freed[i]];
+            ids |= id < 0 || id >= a.n_pages;
+        }
+        for (int e = ng + t; e < nn; e += LG_PLAN_WG) { const int id = a.stack[top - 1 - e]; ids |= id < 0 || id >= a.n_pages; }
+        for (int i = t; i < n; i += LG_PLAN_WG) {
+            const int lo = a.len_old[i];
+            if (a.len_new[i] > lo && (lo & (P - 1))) { const int id = a.table[(size_t)i * a.max_blocks + (lo >> a.shift)]; ids |= id < 0 || id >= a.n_pages; }
+        }
+        if (ids) atomicOr(&bad, LG_PLAN_BAD_PAGE);
+        __syncthreads();
+        st = bad;
+    }
+    if (!st) {
+        for (int e = t; e < ng; e += LG_PLAN_WG) {
+            const int i = lg_owner(freed, n, e);
+            int32_t *const p = a.table + (size_t)i * a.max_blocks + blocks(a.len_new[i]) + e - freed[i];
+            a.stack[top - 1 - e] = *p;
+            *p = -1;
+        }
+        __syncthreads();
+        for (int e = t; e < nn; e += LG_PLAN_WG) {
+            const int i = lg_owner(need, n, e);
+            a.table[(size_t)i * a.max_blocks + blocks(a.len_old[i]) + e - need[i]] = a.stack[top - 1 - e];
+        }
+        __syncthreads();
+    }
+    for (int s = t; s < a.n_slots; s += LG_PLAN_WG) {
+        int slot = -1;
+        if (!st && s < nt) {
+            const int i = lg_owner(tok, n, s), pos = a.len_old[i] + s - tok[i];
+            slot = a.table[(size_t)i * a.max_blocks + (pos >> a.shift)] * P + (pos & (P - 1));
+        }
+        a.slots[s] = slot;
+    }
+    for (int i = t; i <= n; i += LG_PLAN_WG) a.start[i] = st ? 0 : tok[i];
+    if (t == 0) { *a.status = st; if (!st) *a.n_free = top - nn; }
+}
+
+// ---- write -----------------------------------------------------------------------------------------------------------
+struct PageGeo {
+    uint16_t *k, *v;
+    long long row_stride, page_stride;  // values
+    int n_pages, shift;                 // page_size = 1 << shift
+};
+// New K and V rows, f32 -> binary16 (nearest even), into their slots.  Bound by memory: 6 bytes a value.  A thread takes 8 values: two 16-byte
+// loads and one 16-byte store.
+__global__ __launch_bounds__(256) void lg_k_page_write(PageGeo g, const float *k, const float *v, long long stride, const int32_t *slots, int n_tok, int units) {
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int tok = (int)(id / (2 * units)), u = (int)(id % (2 * units));
+    if (tok >= n_tok) return;
+    const int slot = slots[tok], page = slot >> g.shift;
+    if (slot < 0 || page >= g.n_pages) return;
+    const bool second = u >= units;
+    const int c = (second ? u - units : u) * 8;
+    const float4 *src = (const float4 *)((second ? v : k) + (long long)tok * stride + c);
+    const float4 x = src[0], y = src[1];
+    union { _Float16 h[8]; uint4 q; } o;
+    o.h[0] = (_Float16)x.x; o.h[1] = (_Float16)x.y; o.h[2] = (_Float16)x.z; o.h[3] = (_Float16)x.w;
+    o.h[4] = (_Float16)y.x; o.h[5] = (_Float16)y.y; o.h[6] = (_Float16)y.z; o.h[7] = (_Float16)y.w;
+    *(uint4 *)((second ? g.v : g.k) + page * g.page_stride + (slot & ((1 << g.shift) - 1)) * g.row_stride + c) = o.q;
+}
+
+// ---- attend ----------------------------------------------------------------------------------------------------------
+// One new token per sequence: o[h] = sum_t softmax_t(scale q[h].k[t, h / G]) v[t, h / G] over the keys t of [max(0, len - window), len).
+//
+// A wavefront takes tiles of 32 keys (aligned to position 0, so a page holds whole half tiles of 16) of one key head, whose G <= 8 query heads share
+// what it reads.  All products run on v_mfma_f32_16x16x32_f16.  Queries and probabilities are f32 and keep their precision: each is split into a
+// binary16 value and the binary16 of what that leaves (22 bits together), which are rows 0..7 and 8..15 of the 16 that an instruction multiplies
+// anyway, so that the second half costs nothing; the two results are added in f32.  Both are scaled by a power of two first (queries so that the largest
+// of a head lies in [2^14, 2^15), probabilities by 2^14), away from binary16's subnormals.
+//   scores, transposed: S^T = K Q^T.  A lane's 16 bytes of a key row are the operand as they lie in memory.  Lane l gets query row l % 16 and the keys
+//   4 (l / 16) .. + 3 of either half tile.
+//   values: O = P V needs 8 keys of one dimension per lane.  The order of keys inside a product is free, so it is the one in which the lane has
+//   its scores already, and no probability crosses lanes; a lane loads 16 bytes (8 dimensions) of each of its 8 key rows and turns the 8 x 8
+//   values in registers (v_perm_b32).
+// K and V never pass through LDS.  Maximum and sum run in f32; the sum is of the unsplit probabilities.
+#define LG_PA_WAVES 4
+#define LG_PA_TILE  32
+typedef _Float16 lg_h8 __attribute__((ext_vector_type(8)));
+typedef float lg_f4 __attribute__((ext_vector_type(4)));
+
+struct PageAttn {
+    PageGeo g;
+    const float *q; long long q_stride;
+    const int32_t *table, *len;
+    float *out; long long out_stride;
+    float *pm, *pl, *pacc;              // [n_seq][H][splits], [..][hd]: partials of more than one split
+    float scale;
+    int H, nkv, max_blocks, max_len, window, chunk, splits;
+};
+// The keys a sequence sees: [lo, len)
+__device__ __forceinline__ void lg_pa_range(const PageAttn &a, int seq, int &lo, int &len) {
+    const long long room = (long long)a.max_blocks << a.g.shift;
+    len = a.len[seq];
+    if (len > a.max_len) len = a.max_len;
+    if (len > room) len = (int)room;
+    if (len < 0) len = 0;
+    lo = a.window > 0 && len > a.window ? len - a.window : 0;
+}
+__device__ __forceinline__ int lg_pa_splits(const PageAttn &a, int lo, int len) {       // of a sequence: those with keys
+    const int first = lo & ~(LG_PA_TILE - 1);
+    return len > lo ? (len - first + a.chunk - 1) / a.chunk : 0;
+}
+
+template <int HD>
+__global__ __launch_bounds__(LG_PA_WAVES * 64) void lg_k_page_attn(PageAttn a) {
+    constexpr int KS = HD / 32;                     // score steps
+    constexpr int DL = HD >= 128 ? 8 : HD / 16;     // dimensions of a value load
+    constexpr int CH = HD / (16 * DL);              // value loads of a key row
+    constexpr int NT = HD / 16;                     // output tiles
+    __shared__ float s_m[LG_PA_WAVES][8], s_l[LG_PA_WAVES][8];
+    __shared__ float s_o[LG_PA_WAVES][8][HD];
+    const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
+    const int seq = unit / a.nkv, kvh = unit % a.nkv, G = a.H / a.nkv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    int lo, len;
+    lg_pa_range(a, seq, lo, len);
+    const int n_split = lg_pa_splits(a, lo, len);
+    if (split >= n_split && !(a.splits == 1)) return;
+    const int first = (lo & ~(LG_PA_TILE - 1)) + split * a.chunk, end = len < first + a.chunk ? len : first + a.chunk;
+
+    // queries: operand B of the scores, column c = query head c % 8, high part for c < 8
+    lg_h8 qf[KS];
+    float qs = 0;                                   // factor of the raw scores, in powers of two (base 2 exponent of the softmax)
+    {
+        const int h = c & 7;
+        const float *q = a.q + seq * a.q_stride + (long long)(kvh * G + (h < G ? h : 0)) * HD;
+        float top = 0;
+        #pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const float4 x = *(const float4 *)(q + s * 32 + g * 8), y = *(const float4 *)(q + s * 32 + g * 8 + 4);
+            top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
+        }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;       // top * 2^-e in [2^14, 2^15)
+        if (e < -100) e = -100;                                     // (zero and tiny rows; 2^-e stays a float)
+        const float up = __uint_as_float((unsigned)(127 - e) << 23);
+        #pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const float4 x = *(const float4 *)(q + s * 32 + g * 8), y = *(const float4 *)(q + s * 32 + g * 8 + 4);
+            const float v[8] = { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w };
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float z = v[j] * up;
+                const _Float16 hi = (_Float16)z;
+                qf[s][j] = c < 8 ? hi : (_Float16)(z - (float)hi);
+            }
+        }
+        qs = a.scale * 1.44269504088896341f * __uint_as_float((unsigned)(127 + e) << 23);
+    }
+    lg_f4 acc[NT];
+    #pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i] = (lg_f4){ 0, 0, 0, 0 };
+    float m = -INFINITY, l = 0;                     // of query row c; l of this lane's keys alone
+
+    const int32_t *table = a.table + (long long)seq * a.max_blocks;
+    const int mask = (1 << a.g.shift) - 1;
+    for (int t0 = first + wave * LG_PA_TILE; t0 < end; t0 += LG_PA_WAVES * LG_PA_TILE) {
+        bool ok[2]; long long row[2];               // of the half tiles
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int t = t0 + 16 * h, b = t >> a.g.shift;
+            const int page = b < a.max_blocks ? table[b] : -1;
+            ok[h] = page >= 0 && page < a.g.n_pages;
+            row[h] = (ok[h] ? page : 0) * a.g.page_stride + (t & mask) * a.g.row_stride + kvh * HD;
+        }
+        lg_f4 s[2] = { { 0, 0, 0, 0 }, { 0, 0, 0, 0 } };
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint16_t *kp = a.g.k + row[h] + c * a.g.row_stride + g * 8;
+            #pragma unroll
+            for (int i = 0; i < KS; ++i) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const lg_h8 *)(kp + i * 32), qf[i], s[h], 0, 0, 0);
+        }
+        // base-2 exponents; rows c and c + 8 hold the two parts of a query's score
+        float x[2][4], top = -INFINITY;
+        #pragma unroll
+        for (int h = 0; h < 2; ++h)
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float both = s[h][r] + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(s[h][r]), 0x128, 0xF, 0xF, true));   // row_ror:8
+                const int t = t0 + 16 * h + 4 * g + r;
+                x[h][r] = ok[h] && t >= lo && t < end ? both * qs : -INFINITY;
+                top = fmaxf(top, x[h][r]);
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any(top > m)) {
+            const float mn = fmaxf(m, top);
+            const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);   // (both -inf: nothing seen yet)
+            l *= f; m = mn;
+            float fr[4];
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) fr[r] = __shfl(f, (4 * g + r) & 7);
+            #pragma unroll
+            for (int i = 0; i < NT; ++i)
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][r] *= fr[r];
+        }
+        lg_h8 pf;
+        #pragma unroll
+        for (int h = 0; h < 2; ++h)
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float p = x[h][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[h][r] - m + 14.0f);
+                l += p;
+                const _Float16 hi = (_Float16)p;
+                pf[4 * h + r] = c < 8 ? hi : (_Float16)(p - (float)hi);
+            }
+        // values; a masked key's may be anything (0 * inf is not 0): zeros in its place
+        const bool whole = t0 >= lo && t0 + LG_PA_TILE <= end && ok[0] && ok[1];
+        #pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+            uint32_t w[8][DL / 2];
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int kk = 4 * g + (j & 3), h = j >> 2;
+                const uint16_t *vp = a.g.v + row[h] + kk * a.g.row_stride + ch * 128 + c * DL;
+                if constexpr (DL == 8) { const uint4 u = *(const uint4 *)vp; w[j][0] = u.x; w[j][1] = u.y; w[j][2] = u.z; w[j][3] = u.w; }
+                else { const uint2 u = *(const uint2 *)vp; w[j][0] = u.x; w[j][1] = u.y; }
+                if (!whole) {
+                    const int t = t0 + 16 * h + kk;
+                    if (!(ok[h] && t >= lo && t < end)) {
+                        #pragma unroll
+                        for (int i = 0; i < DL / 2; ++i) w[j][i] = 0;
+                    }
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < DL; ++i) {
+                union { uint32_t u[4]; lg_h8 h; } b;
+                #pragma unroll
+                for (int k2 = 0; k2 < 4; ++k2) b.u[k2] = __builtin_amdgcn_perm(w[2 * k2 + 1][i >> 1], w[2 * k2][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
+                acc[ch * DL + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, b.h, acc[ch * DL + i], 0, 0, 0);
+            }
+        }
+    }
+    // the wavefronts' parts: sums over the quarters of a tile, then the four together
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (lane < 8) { s_m[wave][lane] = m; s_l[wave][lane] = l; }
+    #pragma unroll
+    for (int i = 0; i < NT; ++i)
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float both = acc[i][r] + __shfl_xor(acc[i][r], 32);
+            if (lane < 32) s_o[wave][4 * g + r][(i / DL) * 128 + c * DL + i % DL] = both;
+        }
+    __syncthreads();
+    for (int id = threadIdx.x; id < G * HD; id += LG_PA_WAVES * 64) {
+        const int h = id / HD, d = id % HD;
+        float M = -INFINITY, L = 0, o = 0;
+        #pragma unroll
+        for (int w = 0; w < LG_PA_WAVES; ++w) M = fmaxf(M, s_m[w][h]);
+        #pragma unroll
+        for (int w = 0; w < LG_PA_WAVES; ++w) {
+            if (s_l[w][h] == 0.0f) continue;                        // no key; a score of NaN leaves its mark in the sum
+            const float f = __builtin_amdgcn_exp2f(s_m[w][h] - M);
+            L += f * s_l[w][h];
+            o += f * s_o[w][h][d];
+        }
+        const int head = kvh * G + h;
+        if (a.splits == 1) a.out[seq * a.out_stride + (long long)head * HD + d] = L == 0.0f ? 0.0f : o / L;
+        else {
+            const long long at = ((long long)seq * a.H + head) * a.splits + split;
+            a.pacc[at * HD + d] = o;
+            if (d == 0) { a.pm[at] = M; a.pl[at] = L; }
+        }
+    }
+}
+
+// The splits of a sequence, joined: a workgroup per (sequence, head), a thread per dimension.
+template <int HD>
+__global__ __launch_bounds__(HD) void lg_k_page_merge(PageAttn a) {
+    const int unit = blockIdx.x, seq = unit / a.H, head = unit % a.H, d = threadIdx.x;
+    int lo, len;
+    lg_pa_range(a, seq, lo, len);
+    const int n = lg_pa_splits(a, lo, len);
+    const long long at = (long long)unit * a.splits;
+    float M = -INFINITY, L = 0, o = 0;
+    for (int s = 0; s < n; ++s) M = fmaxf(M, a.pm[at + s]);
+    for (int s = 0; s < n; ++s) {
+        const float ls = a.pl[at + s];
+        if (ls == 0.0f) continue;                               // no key: its pages are left out
+        const float f = __builtin_amdgcn_exp2f(a.pm[at + s] - M);
+        L += f * ls;
+        o += f * a.pacc[(at + s) * HD + d];
+    }
+    a.out[seq * a.out_stride + (long long)head * HD + d] = L == 0.0f ? 0.0f : o / L;
+}

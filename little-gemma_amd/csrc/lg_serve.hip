@@ -1,0 +1,163 @@
+// lg_serve.hip — the operators of a batched decode step behind include/lg_hip.h: pages of a shared KV cache, attention over them, sampling.
+//
+// Every entry takes device pointers of the caller, allocates nothing, launches on the caller's stream and returns without waiting: a stream under
+// capture can take it.  What the host can see is checked here; what lies in device memory (lengths, page ids, slots) is checked by the kernels.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/lg_hip.h"
+#include "lg_host.h"
+#include "lg_pages.h"
+#include "lg_sample.h"
+
+static_assert(LG_PLAN_BAD_LEN == LG_HIP_PLAN_BAD_LENGTH && LG_PLAN_NO_PAGES == LG_HIP_PLAN_NO_PAGES && LG_PLAN_NO_SLOTS == LG_HIP_PLAN_NO_SLOTS &&
+              LG_PLAN_BAD_STACK == LG_HIP_PLAN_BAD_STACK && LG_PLAN_BAD_PAGE == LG_HIP_PLAN_BAD_PAGE, "status bits of a plan");
+static_assert(sizeof(SampleRow) == sizeof(struct lg_hip_sampling), "parameters of a row");
+
+static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+static int shift_of(int page_size) {                 // page_size = 1 << shift; -1: not served
+    if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) return -1;
+    return __builtin_ctz((unsigned)page_size);
+}
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// ---- plan -------------------------------------------------------------------------------------------------------
+extern "C" size_t lg_hip_paged_plan_workspace(int n_seq) { (void)n_seq; return 0; }
+
+extern "C" int lg_hip_paged_plan(int n_seq, int page_size, int n_pages, int max_blocks, const int32_t *d_len_old, const int32_t *d_len_new,
+                                 int32_t *d_table, int32_t *d_free, int32_t *d_n_free, int32_t *d_start, int32_t *d_slots, int n_slots,
+                                 int32_t *d_status, void *d_work, size_t work_bytes, void *stream) {
+    (void)d_work; (void)work_bytes;
+    const int shift = shift_of(page_size);
+    if (n_seq < 0 || n_seq > LG_PLAN_SEQS) return lg_fail(-2, "paged_plan: %d sequences (0..%d)", n_seq, LG_PLAN_SEQS);
+    if (shift < 0) return lg_fail(-2, "paged_plan: pages of %d positions (a power of two of 16..256)", page_size);
+    if (n_pages < 1 || (int64_t)n_pages * page_size > INT32_MAX || max_blocks < 1 || (int64_t)max_blocks * page_size > INT32_MAX)
+        return lg_fail(-2, "paged_plan: %d pages and %d blocks of %d positions (slots and positions are 31 bits)", n_pages, max_blocks, page_size);
+    if (n_slots < 0) return lg_fail(-2, "paged_plan: %d slots", n_slots);
+    if (!d_free || !d_n_free || !d_start || !d_status || (n_seq && (!d_len_old || !d_len_new || !d_table)) || (n_slots && !d_slots))
+        return lg_fail(-1, "paged_plan: null argument");
+    const PlanArgs a{ d_len_old, d_len_new, d_table, d_free, d_n_free, d_start, d_slots, d_status, n_seq, shift, n_pages, max_blocks, n_slots };
+    hipLaunchKernelGGL(lg_k_plan, dim3(1), dim3(LG_PLAN_WG), 0, (hipStream_t)stream, a);
+    LG_TRY(hipGetLastError());
+    return 0;
+}
+
+// ---- pages ------------------------------------------------------------------------------------------------------
+static int check_pages(const char *who, const struct lg_hip_pages *p, PageGeo *g) {
+    if (!p || !p->k || !p->v) return lg_fail(-1, "%s: null argument", who);
+    const int shift = shift_of(p->page_size);
+    if (shift < 0) return lg_fail(-2, "%s: pages of %d positions (a power of two of 16..256)", who, p->page_size);
+    if (p->n_pages < 1 || (int64_t)p->n_pages * p->page_size > INT32_MAX) return lg_fail(-2, "%s: %d pages of %d positions (slots are 31 bits)", who, p->n_pages, p->page_size);
+    const int hd = p->head_dim;
+    if (p->n_head_kv < 1 || p->n_head_kv > 1024 || (hd != 64 && hd != 128 && hd != 256 && hd != 512))
+        return lg_fail(-2, "%s: %d key heads of %d (heads of 64, 128, 256 or 512)", who, p->n_head_kv, hd);
+    const int64_t most = INT64_C(1) << 40;           // products of strides and page ids stay in 64 bits
+    if (p->row_stride < (int64_t)p->n_head_kv * hd || p->row_stride % 8 || p->row_stride > most || p->page_stride < p->row_stride * p->page_size ||
+        p->page_stride % 8 || p->page_stride > most / p->n_pages * 1024)
+        return lg_fail(-2, "%s: strides of %lld values a row and %lld a page (multiples of 8 that hold %d rows of %d)", who, (long long)p->row_stride,
+                       (long long)p->page_stride, p->page_size, p->n_head_kv * hd);
+    if (!aligned16(p->k) || !aligned16(p->v)) return lg_fail(-2, "%s: pages that are not aligned to 16 bytes", who);
+    *g = PageGeo{ p->k, p->v, p->row_stride, p->page_stride, p->n_pages, shift };
+    return 0;
+}
+
+// ---- write ------------------------------------------------------------------------------------------------------
+extern "C" int lg_hip_paged_write(const struct lg_hip_pages *p, const float *d_k, const float *d_v, int64_t stride, const int32_t *d_slots, int n_tok,
+                                  void *stream) {
+    PageGeo g;
+    const int rc = check_pages("paged_write", p, &g);
+    if (rc) return rc;
+    if (n_tok < 0) return lg_fail(-2, "paged_write: %d tokens", n_tok);
+    if (n_tok == 0) return 0;
+    if (!d_k || !d_v || !d_slots) return lg_fail(-1, "paged_write: null argument");
+    const int width = p->n_head_kv * p->head_dim;
+    if (stride < width || stride % 4 || !aligned16(d_k) || !aligned16(d_v))
+        return lg_fail(-2, "paged_write: rows of %d values, %lld apart (aligned to 16 bytes)", width, (long long)stride);
+    const int64_t groups = ((int64_t)n_tok * (width / 4) + 255) / 256;
+    if (groups > INT32_MAX) return lg_fail(-2, "paged_write: %d tokens of %d values in one call", n_tok, width);
+    hipLaunchKernelGGL(lg_k_page_write, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, g, d_k, d_v, (long long)stride, d_slots, n_tok, width / 8);
+    LG_TRY(hipGetLastError());
+    return 0;
+}
+
+// ---- attend -----------------------------------------------------------------------------------------------------
+// Keys of a split: as many as give the chip about four workgroups per CU were every sequence at its longest, 128 (a tile for each wavefront) to 1024.
+struct AttnSplit { int chunk, splits; };
+static AttnSplit split_of(int n_seq, int n_head_kv, int max_len, int window) {
+    const int64_t span = (window > 0 && window < max_len ? window : max_len) + LG_PA_TILE - 1;
+    int64_t chunk = span * n_seq * n_head_kv / 1024;
+    chunk = (chunk + 127) / 128 * 128;
+    chunk = chunk < 128 ? 128 : chunk > 1024 ? 1024 : chunk;
+    return { (int)chunk, (int)((span + chunk - 1) / chunk) };
+}
+static bool attn_shape(int n_seq, int n_head, int n_head_kv, int hd, int max_len) {
+    return n_seq >= 0 && n_head_kv >= 1 && n_head_kv <= 1024 && n_head >= 1 && n_head % n_head_kv == 0 && n_head / n_head_kv <= 8 &&
+           (hd == 64 || hd == 128 || hd == 256 || hd == 512) && max_len >= 0 && max_len <= (1 << 30);
+}
+extern "C" size_t lg_hip_paged_attention_workspace(int n_seq, int n_head, int n_head_kv, int hd, int max_len, int window) {
+    if (!attn_shape(n_seq, n_head, n_head_kv, hd, max_len)) return 0;
+    const AttnSplit s = split_of(n_seq, n_head_kv, max_len, window);
+    if (s.splits == 1) return 0;
+    const size_t slots = (size_t)n_seq * n_head * s.splits;
+    return 2 * up256(slots * 4) + slots * hd * 4;
+}
+
+template <int HD>
+static void launch_attn(const PageAttn &a, int n_seq, hipStream_t st) {
+    hipLaunchKernelGGL(lg_k_page_attn<HD>, dim3((unsigned)((int64_t)n_seq * a.nkv * a.splits)), dim3(LG_PA_WAVES * 64), 0, st, a);
+    if (a.splits > 1) hipLaunchKernelGGL(lg_k_page_merge<HD>, dim3((unsigned)((int64_t)n_seq * a.H)), dim3(HD), 0, st, a);
+}
+
+extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float *d_q, int64_t q_stride, int n_seq, int n_head, const int32_t *d_table,
+                                      int max_blocks, const int32_t *d_len, int max_len, int window, float scale, float *d_out, int64_t out_stride,
+                                      void *d_work, size_t work_bytes, void *stream) {
+    PageGeo g;
+    const int rc = check_pages("paged_attention", p, &g);
+    if (rc) return rc;
+    const int hd = p->head_dim;
+    if (!attn_shape(n_seq, n_head, p->n_head_kv, hd, max_len))
+        return lg_fail(-2, "paged_attention: %d sequences, %d query heads on %d key heads (at most 8 each), lengths up to %d", n_seq, n_head, p->n_head_kv, max_len);
+    if (max_blocks < 1 || (int64_t)max_blocks * p->page_size > INT32_MAX) return lg_fail(-2, "paged_attention: %d blocks of %d positions", max_blocks, p->page_size);
+    if (window < 0) return lg_fail(-2, "paged_attention: a window of %d", window);
+    if (n_seq == 0) return 0;
+    if (!d_q || !d_table || !d_len || !d_out) return lg_fail(-1, "paged_attention: null argument");
+    const int64_t qd = (int64_t)n_head * hd;
+    if (q_stride < qd || q_stride % 4 || !aligned16(d_q)) return lg_fail(-2, "paged_attention: query rows of %lld values, %lld apart (aligned to 16 bytes)", (long long)qd, (long long)q_stride);
+    if (out_stride < qd || ((uintptr_t)d_out & 3)) return lg_fail(-2, "paged_attention: output rows of %lld values, %lld apart", (long long)qd, (long long)out_stride);
+    const AttnSplit s = split_of(n_seq, p->n_head_kv, max_len, window);
+    if ((int64_t)n_seq * n_head * s.splits > INT32_MAX / 2) return lg_fail(-2, "paged_attention: %d sequences of %d splits in one call", n_seq, s.splits);
+    const size_t need = lg_hip_paged_attention_workspace(n_seq, n_head, p->n_head_kv, hd, max_len, window);
+    if (need && (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)))
+        return lg_fail(-2, "paged_attention: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
+    const size_t part = up256((size_t)n_seq * n_head * s.splits * 4);
+    float *const w = (float *)d_work;
+    const PageAttn a{ g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, w, need ? (float *)((char *)d_work + part) : nullptr,
+                      need ? (float *)((char *)d_work + 2 * part) : nullptr, scale, n_head, p->n_head_kv, max_blocks, max_len, window, s.chunk, s.splits };
+    hipStream_t st = (hipStream_t)stream;
+    switch (hd) {
+        case 64:  launch_attn<64>(a, n_seq, st); break;
+        case 128: launch_attn<128>(a, n_seq, st); break;
+        case 256: launch_attn<256>(a, n_seq, st); break;
+        default:  launch_attn<512>(a, n_seq, st); break;
+    }
+    LG_TRY(hipGetLastError());
+    return 0;
+}
+
+// ---- sample -----------------------------------------------------------------------------------------------------
+extern "C" size_t lg_hip_sample_workspace(int rows, int n_vocab) { (void)rows; (void)n_vocab; return 0; }
+
+extern "C" int lg_hip_sample(const float *d_logits, int64_t stride, int rows, int n_vocab, const struct lg_hip_sampling *d_params, const float *d_u,
+                             int32_t *d_tok, float *d_prob, int32_t *d_kept, void *d_work, size_t work_bytes, void *stream) {
+    (void)d_work; (void)work_bytes;
+    if (rows < 0 || rows > 65535) return lg_fail(-2, "sample: %d rows (0..65535)", rows);
+    if (n_vocab < 1 || n_vocab > LG_SAMPLE_VOCAB) return lg_fail(-2, "sample: a vocabulary of %d (1..%d)", n_vocab, LG_SAMPLE_VOCAB);
+    if (stride < n_vocab) return lg_fail(-2, "sample: rows of %d logits, %lld apart", n_vocab, (long long)stride);
+    if (rows == 0) return 0;
+    if (!d_logits || !d_params || !d_u || !d_tok) return lg_fail(-1, "sample: null argument");
+    if (((uintptr_t)d_logits | (uintptr_t)d_params) & 3) return lg_fail(-2, "sample: arguments that are not aligned to 4 bytes");
+    const SampleArgs a{ d_logits, (long long)stride, (const SampleRow *)d_params, d_u, d_tok, d_prob, d_kept, n_vocab };
+    hipLaunchKernelGGL(lg_k_sample_row, dim3(rows), dim3(LG_SAMPLE_WG), 0, (hipStream_t)stream, a);
+    LG_TRY(hipGetLastError());
+    return 0;
+}

@@ -32,6 +32,17 @@ class HipError(RuntimeError):
     pass
 
 
+class Pages(C.Structure):
+    """struct lg_hip_pages: one layer's pages of a cache that many sequences share (device pointers)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_head_kv", C.c_int32),
+                ("head_dim", C.c_int32), ("row_stride", C.c_int64), ("page_stride", C.c_int64)]
+
+
+class Sampling(C.Structure):
+    """struct lg_hip_sampling: how a token is drawn from a row of logits."""
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
 def build():
     """Compile the HIP library for gfx950 and the C backend on top of it."""
     subprocess.run(["make", "-C", CSRC, "-B", "liblg_hip.so"], check=True, stdout=subprocess.DEVNULL,
@@ -83,6 +94,17 @@ def load_hip():
     L.lg_hip_profile_step.argtypes = [C.c_void_p, C.c_void_p, i32p, C.c_int, C.c_int, C.c_int,
                                       C.POINTER(C.c_char_p), f32p, i32p,
                                       np.ctypeslib.ndpointer(np.float64, flags="C_CONTIGUOUS"), C.c_int]
+    P, I, Q, Z = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
+    L.lg_hip_paged_plan_workspace.argtypes = [I]
+    L.lg_hip_paged_plan_workspace.restype = Z
+    L.lg_hip_paged_plan.argtypes = [I] * 4 + [P] * 7 + [I, P, P, Z, P]
+    L.lg_hip_paged_write.argtypes = [P, P, P, Q, P, I, P]
+    L.lg_hip_paged_attention_workspace.argtypes = [I] * 6
+    L.lg_hip_paged_attention_workspace.restype = Z
+    L.lg_hip_paged_attention.argtypes = [P, P, Q, I, I, P, I, P, I, I, C.c_float, P, Q, P, Z, P]
+    L.lg_hip_sample_workspace.argtypes = [I, I]
+    L.lg_hip_sample_workspace.restype = Z
+    L.lg_hip_sample.argtypes = [P, Q, I, I] + [P] * 6 + [Z, P]
     _hip = L
     return L
 
