@@ -145,19 +145,36 @@ extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float 
 }
 
 // ---- sample -----------------------------------------------------------------------------------------------------
-extern "C" size_t lg_hip_sample_workspace(int rows, int n_vocab) { (void)rows; (void)n_vocab; return 0; }
+extern "C" size_t lg_hip_sample_workspace(int rows, int n_vocab) {
+    if (rows < 0 || n_vocab <= LG_SAMPLE_CAND || n_vocab > LG_SAMPLE_VOCAB) return 0;
+    return (size_t)rows * lg_sample_geo(n_vocab).row;
+}
+
+template <bool VEC>
+static void launch_sample(const SampleArgs &a, int rows, char *work, hipStream_t st) {
+    if (!work) { hipLaunchKernelGGL((lg_k_sample_finish<VEC, true>), dim3(rows), dim3(LG_SAMPLE_WG), 0, st, a, work); return; }
+    const SampleGeo g = lg_sample_geo(a.n_vocab);
+    hipLaunchKernelGGL(lg_k_sample_max<VEC>, dim3((unsigned)rows * g.maxes), dim3(LG_SAMPLE_MAX_WG), 0, st, a, work);
+    hipLaunchKernelGGL(lg_k_sample_bins<VEC>, dim3((unsigned)rows * g.slices), dim3(LG_SAMPLE_WG), 0, st, a, work);
+    hipLaunchKernelGGL(lg_k_sample_sums<VEC>, dim3((unsigned)rows * g.slices), dim3(LG_SAMPLE_WG), 0, st, a, work);
+    hipLaunchKernelGGL((lg_k_sample_finish<VEC, false>), dim3(rows), dim3(LG_SAMPLE_WG), 0, st, a, work);
+}
 
 extern "C" int lg_hip_sample(const float *d_logits, int64_t stride, int rows, int n_vocab, const struct lg_hip_sampling *d_params, const float *d_u,
                              int32_t *d_tok, float *d_prob, int32_t *d_kept, void *d_work, size_t work_bytes, void *stream) {
-    (void)d_work; (void)work_bytes;
     if (rows < 0 || rows > 65535) return lg_fail(-2, "sample: %d rows (0..65535)", rows);
     if (n_vocab < 1 || n_vocab > LG_SAMPLE_VOCAB) return lg_fail(-2, "sample: a vocabulary of %d (1..%d)", n_vocab, LG_SAMPLE_VOCAB);
     if (stride < n_vocab) return lg_fail(-2, "sample: rows of %d logits, %lld apart", n_vocab, (long long)stride);
     if (rows == 0) return 0;
     if (!d_logits || !d_params || !d_u || !d_tok) return lg_fail(-1, "sample: null argument");
     if (((uintptr_t)d_logits | (uintptr_t)d_params) & 3) return lg_fail(-2, "sample: arguments that are not aligned to 4 bytes");
+    const size_t need = lg_hip_sample_workspace(rows, n_vocab);
+    if (need && (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)))
+        return lg_fail(-2, "sample: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
     const SampleArgs a{ d_logits, (long long)stride, (const SampleRow *)d_params, d_u, d_tok, d_prob, d_kept, n_vocab };
-    hipLaunchKernelGGL(lg_k_sample_row, dim3(rows), dim3(LG_SAMPLE_WG), 0, (hipStream_t)stream, a);
+    // loads of 16 bytes where every row is aligned to that
+    if (aligned16(d_logits) && stride % 4 == 0) launch_sample<true>(a, rows, need ? (char *)d_work : nullptr, (hipStream_t)stream);
+    else launch_sample<false>(a, rows, need ? (char *)d_work : nullptr, (hipStream_t)stream);
     LG_TRY(hipGetLastError());
     return 0;
 }

@@ -99,6 +99,33 @@ def test_ties_masks_and_odd_distributions(dev, kind):
     check(dev, l.astype(np.float32), SETTINGS, rng.random(n))
 
 
+@pytest.mark.parametrize("kind", ["crowded", "equal", "outliers", "tiny temperature", "clustered", "two borders", "coarse"])
+def test_long_rows_whose_border_is_hard_to_bracket(dev, kind):
+    """More tokens in one bin than candidates are kept, a temperature whose inverse is no f32, all the likely tokens in a few groups, and
+    top-k and top-p borders far from each other and in one place."""
+    rng = np.random.default_rng(len(kind) + 50)
+    V = 60000
+    l = rows_like_logits(rng, 6, V)
+    params = [(1.0, 0, 0.9, 0.0), (1.0, 20000, 0.9, 0.0), (1.0, 20000, 1.0, 0.0), (1.0, 100, 0.95, 0.0), (1.0, 600, 0.999, 0.01), (1.0, 0, 1.0, 0.0)]
+    if kind == "crowded":                       # 50000 logits within a bin's width
+        l[:, :50000] = np.float32(3.0) + rng.normal(0, 1e-4, (6, 50000)).astype(np.float32)
+    elif kind == "equal":
+        l[:] = np.float32(-4.0)
+    elif kind == "outliers":
+        l *= np.float32(0.01)
+        l[:, 7] = -25.0; l[:, 59999] = 5.0
+    elif kind == "tiny temperature":
+        l = np.where(rng.random(l.shape) < 0.2, np.float32(1e-30), np.float32(0)).astype(np.float32)
+        params = [(1e-30, *x[1:]) for x in params[:3]] + [(1e-42, *x[1:]) for x in params[3:]]
+    elif kind == "clustered":
+        l[:, 1024:3000] += 12.0
+    elif kind == "two borders":
+        params = [(1.0, k, p, 0.0) for k, p in ((600, 0.05), (5000, 0.5), (59999, 0.3), (60000, 0.99), (513, 0.9999), (30000, 0.9999999))]
+    else:
+        l = (l.view(np.uint32) & 0xFFFF0000).view(np.float32)
+    check(dev, l, params, rng.random(6))
+
+
 def test_random_numbers_at_the_ends_and_beyond(dev):
     rng = np.random.default_rng(21)
     us = np.array([0.0, np.nextafter(np.float32(1), np.float32(0)), 1.0, 7.0, -0.5, np.nan, 2.0 ** -30, np.inf, -np.inf], np.float32)
