@@ -23,10 +23,11 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "lg_block.h"
+
 #define LG_SAMPLE_WG     1024
 #define LG_SAMPLE_VOCAB  (1 << 19)
 #define LG_SAMPLE_ONE    17592186044416.0        // 2^44
-typedef unsigned long long lg_u64;
 
 struct SampleRow { float temperature; int32_t top_k; float top_p, min_p; };     // struct lg_hip_sampling
 struct SampleArgs {
@@ -34,7 +35,7 @@ struct SampleArgs {
     const SampleRow *params;
     const float *u;
     int32_t *tok; float *prob; int32_t *kept;   // the last two may be null
-    int n_vocab;
+    int n_vocab, slices;                // workgroups of lg_k_sample_sums to a row
 };
 
 // A number that is larger for a larger logit; NaN and -inf give 0x007FFFFF, -0 what +0 gives
@@ -45,59 +46,39 @@ __device__ __forceinline__ uint32_t lg_key(float l) {
 }
 __device__ __forceinline__ float lg_unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
-// What a row's weights need: M and 1 / T (0 for a T of infinity)
-struct Weigh { double top, inv; };
-// 2^44 e^((l - top) inv), rounded.  e^x by n = rint(x / ln 2), r = x - n ln 2 and its power series up to r^12 (|r| <= 0.35: the next term is 2e-16);
-// adding 2^52 leaves the whole number in the low bits.  Below -31.5 it is 0.
+// 2^(j / 32)
+__device__ const double lg_exp2_32nds[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649,
+    1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
+// What a row's weights need: M, 32 / (T ln 2) (0 for a T of infinity), the table in LDS
+struct Weigh { double top, inv; const double *tab; };
+// 2^44 e^((l - top) / T), rounded.  With y = 32 (l - top) / (T ln 2) = n + r, n whole, it is 2^(44 + n / 32) times the power series of 2^(r / 32) (|r| <= 1/2: what
+// comes after r^5 is 2e-15).  Adding 1.5 2^52 leaves n in the low bits, adding 2^52 the result.  Beyond LG_SAMPLE_REACH it is 0.  (The series of e^r to r^12
+// without the table is 25 operations in place of 14: lg_k_sample_sums of 5 rows of 262144 21.0 -> @SUMS@ us with it.)
+#define LG_SAMPLE_REACH   31.5
 __device__ __forceinline__ lg_u64 lg_weigh(const Weigh &w, float l) {
-    const double x = l == (float)w.top ? 0.0 : ((double)l - w.top) * w.inv;
-    if (!(x >= -31.5) || l == -INFINITY) return 0;
-    const double n = __builtin_rint(x * 1.4426950408889634074);
-    double r = __builtin_fma(n, -6.93147180369123816490e-01, x);
-    r = __builtin_fma(n, -1.90821492927058770002e-10, r);
-    double p = 1.0 / 479001600.0;
-    p = __builtin_fma(p, r, 1.0 / 39916800.0);
-    p = __builtin_fma(p, r, 1.0 / 3628800.0);
-    p = __builtin_fma(p, r, 1.0 / 362880.0);
-    p = __builtin_fma(p, r, 1.0 / 40320.0);
-    p = __builtin_fma(p, r, 1.0 / 5040.0);
-    p = __builtin_fma(p, r, 1.0 / 720.0);
-    p = __builtin_fma(p, r, 1.0 / 120.0);
-    p = __builtin_fma(p, r, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
+    const double y = l == (float)w.top ? 0.0 : ((double)l - w.top) * w.inv;
+    if (!(y >= -LG_SAMPLE_REACH * 46.166241308446828384) || l == -INFINITY) return 0;
+    const double t = y + 6755399441055744.0, r = y - (t - 6755399441055744.0);
+    const int n = (int)(uint32_t)(lg_u64)__double_as_longlong(t);
+    double p = 3.9737099845494161e-11;
+    p = __builtin_fma(p, r, 9.172562701824643e-09);
+    p = __builtin_fma(p, r, 1.6938509724371821e-06);
+    p = __builtin_fma(p, r, 0.0002345961982022468);
+    p = __builtin_fma(p, r, 0.02166084939249829);
     p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    const double y = __builtin_fma(p, __longlong_as_double((lg_u64)(1023 + 44 + (int)n) << 52), 4503599627370496.0);
-    return (lg_u64)__double_as_longlong(y) & 0x000FFFFFFFFFFFFFull;
+    const double scale = __longlong_as_double(__double_as_longlong(w.tab[n & 31]) + ((long long)(44 + (n >> 5)) << 52));
+    return (lg_u64)__double_as_longlong(__builtin_fma(p, scale, 4503599627370496.0)) & 0x000FFFFFFFFFFFFFull;
 }
-__device__ __forceinline__ Weigh lg_weigher(float top, float T) { return { (double)top, T > 0 ? 1.0 / (double)T : 0.0 }; }
-
-template <typename T>
-__device__ __forceinline__ T lg_block_sum(T v, T *part) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    T all = 0;
-    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) all += part[w];
-    return all;
-}
-template <typename T>
-__device__ __forceinline__ T lg_block_run(T v, T *part, T *total) {          // inclusive
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int o = 1; o < 64; o <<= 1) { const T u = __shfl_up(v, o); if (lane >= o) v += u; }
-    __syncthreads();
-    if (lane == 63) part[wave] = v;
-    __syncthreads();
-    T before = 0, all = 0;
-    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) { const T p = part[w]; if (w < wave) before += p; all += p; }
-    *total = all;
-    return v + before;
-}
+__device__ __forceinline__ Weigh lg_weigher(float top, float T, const double *tab) { return { (double)top, T > 0 ? 46.166241308446828384 / (double)T : 0.0, tab }; }
+// (the caller's next barrier is the table's)
+__device__ __forceinline__ void lg_weigh_table(double *tab) { if (threadIdx.x < 32) tab[threadIdx.x] = lg_exp2_32nds[threadIdx.x]; }
 
 // One workgroup, one row: the border by digits of the key (4 passes of 8 bits each for top-k and top-p), then the draw.
-struct SampleLds { lg_u64 bin[256]; lg_u64 part[LG_SAMPLE_WG / 64]; uint32_t key; int idx; lg_u64 rest; };
+struct SampleLds { lg_u64 bin[256]; lg_u64 part[LG_SAMPLE_WG / 64]; uint32_t key; int idx; lg_u64 rest; };    // (tab: the caller's)
 
 // The key at which a running sum from the largest key down reaches `want` (1..sum of all), among the tokens in question with keys >= low (of key `low`
 // itself the first `ties` count); *before = the sum of the tokens with larger keys.  BY_COUNT: every token counts 1, else its weight.
@@ -132,7 +113,7 @@ __device__ uint32_t lg_border(const SampleArgs &a, const float *row, const Weigh
     return prefix;
 }
 
-__device__ void lg_sample_row(const SampleArgs &a, int r, SampleLds &s) {
+__device__ void lg_sample_row(const SampleArgs &a, int r, const double *tab, SampleLds &s) {
     const float *row = a.logits + r * a.stride;
     const SampleRow p = a.params[r];
     const int n = a.n_vocab, t = threadIdx.x;
@@ -157,19 +138,19 @@ __device__ void lg_sample_row(const SampleArgs &a, int r, SampleLds &s) {
         }
         return;
     }
-    const Weigh wg = lg_weigher(lg_unkey(best), p.temperature);
+    const Weigh wg = lg_weigher(lg_unkey(best), p.temperature, tab);
     uint32_t cut = 0; int ties = 0;                 // kept: keys > cut, and the first `ties` of those with it
     lg_u64 W = 0; unsigned count = 0;
     for (int i = t; i < n; i += LG_SAMPLE_WG) { const lg_u64 w = lg_weigh(wg, row[i]); W += w; count += w != 0; }
-    W = lg_block_sum(W, s.part);
-    count = (unsigned)lg_block_sum((lg_u64)count, s.part);
+    W = lg_block_sum<LG_SAMPLE_WG>(W, s.part);
+    count = (unsigned)lg_block_sum<LG_SAMPLE_WG>((lg_u64)count, s.part);
     if (p.top_k > 0 && (unsigned)p.top_k < count) {
         lg_u64 before;
         cut = lg_border<true>(a, row, wg, 0, 0, (lg_u64)p.top_k, &before, s);
         ties = (int)(p.top_k - before);
         lg_u64 sum = 0;
         for (int i = t; i < n; i += LG_SAMPLE_WG) if (lg_key(row[i]) > cut) sum += lg_weigh(wg, row[i]);
-        W = lg_block_sum(sum, s.part) + (lg_u64)ties * lg_weigh(wg, lg_unkey(cut));
+        W = lg_block_sum<LG_SAMPLE_WG>(sum, s.part) + (lg_u64)ties * lg_weigh(wg, lg_unkey(cut));
     }
     if (p.top_p < 1) {
         const double want_d = __builtin_ceil((double)p.top_p * (double)W);
@@ -187,8 +168,8 @@ __device__ void lg_sample_row(const SampleArgs &a, int r, SampleLds &s) {
     if (wcut < least) ties = 0;
     lg_u64 S = 0; count = 0;
     for (int i = t; i < n; i += LG_SAMPLE_WG) if (lg_key(row[i]) > cut) { const lg_u64 w = lg_weigh(wg, row[i]); if (w >= least) { S += w; ++count; } }
-    S = lg_block_sum(S, s.part) + (lg_u64)ties * wcut;
-    count = (unsigned)lg_block_sum((lg_u64)count, s.part) + ties;
+    S = lg_block_sum<LG_SAMPLE_WG>(S, s.part) + (lg_u64)ties * wcut;
+    count = (unsigned)lg_block_sum<LG_SAMPLE_WG>((lg_u64)count, s.part) + ties;
     const float u = a.u[r];
     lg_u64 target = u > 0 ? (lg_u64)__builtin_floor((u < 1 ? (double)u : 1.0) * (double)S) : 0;
     if (S && target > S - 1) target = S - 1;
@@ -201,8 +182,8 @@ __device__ void lg_sample_row(const SampleArgs &a, int r, SampleLds &s) {
         lg_u64 w = k >= cut && i < n ? lg_weigh(wg, row[i]) : 0;
         if (w < least) w = 0;
         lg_u64 all, all_ties = 0;
-        if (cut) { const int mine = k == cut, rank = tied + (int)lg_block_run((lg_u64)mine, s.part, &all_ties) - mine; if (mine && rank >= ties) w = 0; }
-        const lg_u64 upto = run + lg_block_run(w, s.part, &all);
+        if (cut) { const int mine = k == cut, rank = tied + (int)lg_block_run<LG_SAMPLE_WG>((lg_u64)mine, s.part, &all_ties) - mine; if (mine && rank >= ties) w = 0; }
+        const lg_u64 upto = run + lg_block_run<LG_SAMPLE_WG>(w, s.part, &all);
         if (w && upto > target && upto - w <= target) { s.idx = i; s.rest = w; }
         run += all; tied += (int)all_ties;
     }
@@ -219,17 +200,15 @@ __device__ void lg_sample_row(const SampleArgs &a, int r, SampleLds &s) {
 #define LG_SAMPLE_GROUP   256                    // tokens of a group: a wavefront's load of 4 each
 #define LG_SAMPLE_GROUPS  (LG_SAMPLE_VOCAB / LG_SAMPLE_GROUP)
 #define LG_SAMPLE_MAX_WG  256                    // lg_k_sample_max: 16 groups to a workgroup
-#define LG_SAMPLE_SLICE   64                     // groups of a workgroup of the two passes after it
 #define LG_SAMPLE_BINS    2048
 #define LG_SAMPLE_CAND    4096                   // candidates that a row may have
 #define LG_SAMPLE_SMALL_K 512                    // top-k up to which the groups' maxima bound the candidates well: with 1024 groups the tokens not below the
                                                  // k-th largest maximum are 1.15 k at k = 256 and 1.39 k at 512 where large logits lie anywhere in the row
 #define LG_SAMPLE_SLACK   2048                   // the estimated sum of a row's bins is trusted to 1 / 2048: four times what the comment at lg_k_sample_bins allows
-#define LG_SAMPLE_REACH   31.5                   // (max - l) / T beyond which a weight is 0
 
 struct SampleWork {                     // per row, in working memory
     uint32_t *gmax;                     // [groups] keys
-    float *smin;                        // [workgroups of lg_k_sample_max] smallest logit above -inf
+    uint32_t *smin;                     // [workgroups of lg_k_sample_max] ~key of the smallest logit above -inf, 0: none
     lg_u64 *mass; uint32_t *count;      // [LG_SAMPLE_BINS]
     lg_u64 *gsum;                       // [groups]
     lg_u64 *part;                       // [slices][3]: sum above the candidates, sum that top-p goes by (without the candidates), tokens kept above them
@@ -241,7 +220,7 @@ __host__ __device__ inline SampleGeo lg_sample_geo(int n_vocab) {
     SampleGeo g;
     g.groups = (n_vocab + LG_SAMPLE_GROUP - 1) / LG_SAMPLE_GROUP;
     g.maxes = (g.groups + 15) / 16;
-    g.slices = (g.groups + LG_SAMPLE_SLICE - 1) / LG_SAMPLE_SLICE;
+    g.slices = (g.groups + 15) / 16;                 // of the passes after it at most: 16 groups or 64 each, as lg_hip_sample chooses
     size_t at = 0;
     g.gmax = at;  at += lg_up64((size_t)g.groups * 4);
     g.smin = at;  at += lg_up64((size_t)g.maxes * 4);
@@ -256,7 +235,7 @@ __host__ __device__ inline SampleGeo lg_sample_geo(int n_vocab) {
 }
 __device__ __forceinline__ SampleWork lg_sample_work(char *base, const SampleGeo &g, int r) {
     char *const p = base + (size_t)r * g.row;
-    return { (uint32_t *)(p + g.gmax), (float *)(p + g.smin), (lg_u64 *)(p + g.mass), (uint32_t *)(p + g.count), (lg_u64 *)(p + g.gsum), (lg_u64 *)(p + g.part),
+    return { (uint32_t *)(p + g.gmax), (uint32_t *)(p + g.smin), (lg_u64 *)(p + g.mass), (uint32_t *)(p + g.count), (lg_u64 *)(p + g.gsum), (lg_u64 *)(p + g.part),
              (uint32_t *)(p + g.ncand), (lg_u64 *)(p + g.cand) };
 }
 // The first largest; a small top-k; no top-k and no top-p; a border to be found; a temperature so small that the estimates' f32 does not hold 1 / T
@@ -283,51 +262,59 @@ __device__ __forceinline__ void lg_load4(const float *row, int n, int grp, float
         for (int j = 0; j < 4; ++j) l[j] = i + j < n ? row[i + j] : -INFINITY;
 }
 
+
 template <bool VEC>
 __global__ __launch_bounds__(LG_SAMPLE_MAX_WG) void lg_k_sample_max(SampleArgs a, char *base) {
     const SampleGeo g = lg_sample_geo(a.n_vocab);
-    const int r = blockIdx.x / g.maxes, part = blockIdx.x % g.maxes, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = blockIdx.y, part = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const SampleWork w = lg_sample_work(base, g, r);
     const float *row = a.logits + r * a.stride;
-    __shared__ float s_min[LG_SAMPLE_MAX_WG / 64];
-    float l[4][4], least = INFINITY;
+    __shared__ uint32_t s_min[LG_SAMPLE_MAX_WG / 64];
+    float l[4][4];
     #pragma unroll
     for (int j = 0; j < 4; ++j) lg_load4<VEC>(row, a.n_vocab, part * 16 + wave * 4 + j, l[j]);
-    // the bins of the row are cleared on the way
-    for (int i = part * LG_SAMPLE_MAX_WG + threadIdx.x; i < LG_SAMPLE_BINS; i += g.maxes * LG_SAMPLE_MAX_WG) { w.mass[i] = 0; w.count[i] = 0; }
+    // the bins of a row that needs them are cleared on the way
+    const SampleRow p = a.params[r];
+    if (lg_row_kind(p, a.n_vocab) == LG_ROW_BORDER)
+        for (int i = part * LG_SAMPLE_MAX_WG + threadIdx.x; i < LG_SAMPLE_BINS; i += g.maxes * LG_SAMPLE_MAX_WG) { w.mass[i] = 0; w.count[i] = 0; }
     if (part == 0 && threadIdx.x == 0) *w.ncand = 0;
+    uint32_t least = 0;                                      // as ~key: the largest is the smallest logit
     #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        float m = -INFINITY;
+        uint32_t m = 0x007FFFFFu;
         #pragma unroll
-        for (int i = 0; i < 4; ++i) { m = fmaxf(m, l[j][i]); if (l[j][i] > -INFINITY) least = fminf(least, l[j][i]); }    // (fmaxf passes over NaN)
-        for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t k = lg_key(l[j][i]);
+            if (k > m) m = k;
+            if (k > 0x007FFFFFu && ~k > least) least = ~k;
+        }
+        m = lg_wave_max(m);
         const int grp = part * 16 + wave * 4 + j;
-        if (lane == 0 && grp < g.groups) w.gmax[grp] = lg_key(m);
+        if (lane == 0 && grp < g.groups) w.gmax[grp] = m;
     }
-    for (int o = 1; o < 64; o <<= 1) least = fminf(least, __shfl_xor(least, o));
-    if (lane == 0) s_min[wave] = least;
-    __syncthreads();
-    if (threadIdx.x == 0) w.smin[part] = fminf(fminf(s_min[0], s_min[1]), fminf(s_min[2], s_min[3]));
+    least = lg_block_max<LG_SAMPLE_MAX_WG>(least, s_min);
+    if (threadIdx.x == 0) w.smin[part] = least;
 }
 
 // The row's largest logit and the width of its bins, in every workgroup anew (1024 keys and 64 minima: less than a launch of their own)
-struct SampleSpan { Weigh wg; float top, scale; bool none; };      // scale: bins per unit of logit
-__device__ __forceinline__ SampleSpan lg_sample_span(const SampleRow &p, const SampleWork &w, const SampleGeo &g, uint32_t *s_key, float *s_min) {
-    uint32_t key = 0; float least = INFINITY;
-    for (int i = threadIdx.x; i < g.groups; i += LG_SAMPLE_WG) { const uint32_t k = w.gmax[i]; if (k > key) key = k; }
-    for (int i = threadIdx.x; i < g.maxes; i += LG_SAMPLE_WG) least = fminf(least, w.smin[i]);
-    for (int o = 1; o < 64; o <<= 1) { const uint32_t k = __shfl_xor((int)key, o); if (k > key) key = k; least = fminf(least, __shfl_xor(least, o)); }
+struct SampleSpan { Weigh wg; float top, scale, c; uint32_t key; };      // key: of the largest logit, 0x007FFFFF: none; scale: bins per unit of logit; c: base-2 exponents per unit
+template <int NT>
+__device__ __forceinline__ SampleSpan lg_sample_span(const SampleRow &p, const SampleWork &w, const SampleGeo &g, const double *tab, uint32_t *part) {
+    uint32_t key = 0, least = 0;
+    for (int i = threadIdx.x; i < g.groups; i += NT) { const uint32_t k = w.gmax[i]; if (k > key) key = k; }
+    for (int i = threadIdx.x; i < g.maxes; i += NT) { const uint32_t k = w.smin[i]; if (k > least) least = k; }
+    key = lg_wave_max(key); least = lg_wave_max(least);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) { s_key[threadIdx.x >> 6] = key; s_min[threadIdx.x >> 6] = least; }
+    if ((threadIdx.x & 63) == 0) { part[threadIdx.x >> 6] = key; part[NT / 64 + (threadIdx.x >> 6)] = least; }
     __syncthreads();
-    key = 0; least = INFINITY;
-    for (int i = 0; i < LG_SAMPLE_WG / 64; ++i) { if (s_key[i] > key) key = s_key[i]; least = fminf(least, s_min[i]); }
+    #pragma unroll
+    for (int i = 0; i < NT / 64; ++i) { if (part[i] > key) key = part[i]; if (part[NT / 64 + i] > least) least = part[NT / 64 + i]; }
     SampleSpan s;
-    s.none = key == 0x007FFFFFu;
+    s.key = key;
     s.top = lg_unkey(key);
-    s.wg = lg_weigher(s.top, p.temperature);
-    const float reach = (float)LG_SAMPLE_REACH * p.temperature, width = fminf(s.top - least, reach);
+    s.wg = lg_weigher(s.top, p.temperature, tab);
+    s.c = -(float)(1.4426950408889634 / (double)p.temperature);
+    const float reach = (float)LG_SAMPLE_REACH * p.temperature, width = fminf(s.top - lg_unkey(~least), reach);
     s.scale = width > 0 && width < INFINITY ? (float)LG_SAMPLE_BINS / width : 0;      // (0: all in the first bin)
     return s;
 }
@@ -337,31 +324,31 @@ __device__ __forceinline__ int lg_sample_bin(const SampleSpan &s, float l) {
     return b >= 0 ? b < (float)(LG_SAMPLE_BINS - 1) ? (int)b : LG_SAMPLE_BINS - 1 : 0;
 }
 
-template <bool VEC>
-__global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_bins(SampleArgs a, char *base) {
+// NT threads read 16 (256) or 64 (1024) groups
+template <bool VEC, int NT>
+__global__ __launch_bounds__(NT) void lg_k_sample_bins(SampleArgs a, char *base) {
     __shared__ lg_u64 mass[LG_SAMPLE_BINS];
-    __shared__ uint32_t count[LG_SAMPLE_BINS], s_key[16];
-    __shared__ float s_min[16];
+    __shared__ uint32_t count[LG_SAMPLE_BINS], part[NT / 32];
+    __shared__ double tab[32];
     const SampleGeo g = lg_sample_geo(a.n_vocab);
-    const int r = blockIdx.x / g.slices, slice = blockIdx.x % g.slices, wave = threadIdx.x >> 6;
+    const int r = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
     const SampleRow p = a.params[r];
     if (lg_row_kind(p, a.n_vocab) != LG_ROW_BORDER) return;
     const SampleWork w = lg_sample_work(base, g, r);
     const float *row = a.logits + r * a.stride;
     float l[4][4];
     #pragma unroll
-    for (int j = 0; j < 4; ++j) lg_load4<VEC>(row, a.n_vocab, slice * LG_SAMPLE_SLICE + j * 16 + wave, l[j]);
-    for (int i = threadIdx.x; i < LG_SAMPLE_BINS; i += LG_SAMPLE_WG) { mass[i] = 0; count[i] = 0; }
-    const SampleSpan s = lg_sample_span(p, w, g, s_key, s_min);                       // (its barriers are the clearing's too)
-    if (s.none) return;
+    for (int j = 0; j < 4; ++j) lg_load4<VEC>(row, a.n_vocab, slice * (NT / 16) + j * (NT / 64) + wave, l[j]);
+    lg_weigh_table(tab);
+    for (int i = threadIdx.x; i < LG_SAMPLE_BINS; i += NT) { mass[i] = 0; count[i] = 0; }
+    const SampleSpan s = lg_sample_span<NT>(p, w, g, tab, part);                      // (its barriers are the clearing's too)
+    if (s.key == 0x007FFFFFu) return;
     const bool by_count = p.top_k > 0 && p.top_k < a.n_vocab, by_mass = p.top_p < 1;
-    const float c = -(float)(1.0 / (double)p.temperature * 1.4426950408889634);
     #pragma unroll
     for (int j = 0; j < 4; ++j)
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float x = l[j][i], d = x == s.top ? 0.0f : s.top - x;
-            const float e = d * c;                                                    // in base 2; a weight of 0 starts near -45
+            const float x = l[j][i], e = x == s.top ? 0.0f : (s.top - x) * s.c;       // base 2; a weight of 0 starts near -45
             if (!(e > -46.0f)) continue;                                              // (NaN too)
             if (e < -44.0f && !lg_weigh(s.wg, x)) continue;
             const int b = lg_sample_bin(s, x);
@@ -370,7 +357,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_bins(SampleArgs a, c
             if (by_count) atomicAdd(&count[b], 1u);
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < LG_SAMPLE_BINS; i += LG_SAMPLE_WG) {
+    for (int i = threadIdx.x; i < LG_SAMPLE_BINS; i += NT) {
         if (by_mass && mass[i]) atomicAdd(&w.mass[i], mass[i]);
         if (by_count && count[i]) atomicAdd(&w.count[i], count[i]);
     }
@@ -378,17 +365,23 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_bins(SampleArgs a, c
 
 // The bins that can hold the border, from the row's estimates: the same in every workgroup of a row
 struct SampleRange { int first, last, cut; uint32_t above; };        // top-p's border is in bins first..last, top-k's in bin cut (LG_SAMPLE_BINS: none), behind `above` tokens
-struct SampleRangeLds { lg_u64 part[LG_SAMPLE_WG / 64]; SampleRange r; lg_u64 lo, hi; };
-__device__ SampleRange lg_sample_range(const SampleArgs &a, const SampleRow &p, const SampleWork &w, SampleRangeLds &s) {
-    constexpr int PT = LG_SAMPLE_BINS / LG_SAMPLE_WG;
+template <int NT>
+struct SampleRangeLds { lg_u64 part[NT / 64]; SampleRange r; lg_u64 lo, hi; };
+template <int NT>
+__device__ __forceinline__ SampleRange lg_sample_range(const SampleArgs &a, const SampleRow &p, const SampleWork &w, SampleRangeLds<NT> &s) {
+    constexpr int PT = LG_SAMPLE_BINS / NT;
     const int b0 = threadIdx.x * PT;
     const bool by_count = p.top_k > 0 && p.top_k < a.n_vocab, by_mass = p.top_p < 1;
     if (threadIdx.x == 0) s.r = { 0, LG_SAMPLE_BINS - 1, LG_SAMPLE_BINS, 0 };
+    lg_u64 m[PT];
+    if (by_mass)
+        #pragma unroll
+        for (int i = 0; i < PT; ++i) m[i] = w.mass[b0 + i];
     if (by_count) {
         lg_u64 c[PT], sum = 0, all;
         #pragma unroll
         for (int i = 0; i < PT; ++i) { c[i] = w.count[b0 + i]; sum += c[i]; }
-        lg_u64 run = lg_block_run(sum, s.part, &all) - sum;
+        lg_u64 run = lg_block_run<NT>(sum, s.part, &all) - sum;
         #pragma unroll
         for (int i = 0; i < PT; ++i) {
             if (run < (lg_u64)p.top_k && run + c[i] >= (lg_u64)p.top_k) { s.r.cut = b0 + i; s.r.above = (uint32_t)run; }
@@ -397,17 +390,16 @@ __device__ SampleRange lg_sample_range(const SampleArgs &a, const SampleRow &p, 
         __syncthreads();
     }
     if (by_mass) {
-        __syncthreads();
+        lg_u64 sum = 0, all;
+        #pragma unroll
+        for (int i = 0; i < PT; ++i) sum += m[i];
+        const lg_u64 start = lg_block_run<NT>(sum, s.part, &all) - sum;
+        lg_u64 run = start;
         const int cut = s.r.cut;
-        lg_u64 m[PT], sum = 0, all;
-        #pragma unroll
-        for (int i = 0; i < PT; ++i) { m[i] = w.mass[b0 + i]; sum += m[i]; }
-        lg_u64 run = lg_block_run(sum, s.part, &all) - sum;
-        const lg_u64 start = run;
-        if (threadIdx.x == 0) { s.lo = all; s.hi = all; }
-        __syncthreads();
-        #pragma unroll
-        for (int i = 0; i < PT; ++i) { if (b0 + i == cut) { s.lo = run; s.hi = run + m[i]; } run += m[i]; }
+        if (cut == LG_SAMPLE_BINS) { if (threadIdx.x == 0) { s.lo = all; s.hi = all; } }
+        else
+            #pragma unroll
+            for (int i = 0; i < PT; ++i) { if (b0 + i == cut) { s.lo = run; s.hi = run + m[i]; } run += m[i]; }
         __syncthreads();
         const double slack = (double)s.hi / LG_SAMPLE_SLACK;
         const double lo = (double)p.top_p * (double)s.lo - slack, hi = (double)p.top_p * (double)s.hi + slack;
@@ -419,22 +411,22 @@ __device__ SampleRange lg_sample_range(const SampleArgs &a, const SampleRow &p, 
             if (before < hi && to >= hi) s.r.last = b0 + i;
             run += m[i];
         }
-        __syncthreads();
     } else if (threadIdx.x == 0) s.r.first = s.r.last = s.r.cut;
     __syncthreads();
     SampleRange q = s.r;
     if (q.last > q.cut) q.last = q.cut;
-    __syncthreads();
     return q;
 }
 
-template <bool VEC>
-__global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_sums(SampleArgs a, char *base) {
-    __shared__ uint32_t s_key[16];
-    __shared__ float s_min[16];
-    __shared__ SampleRangeLds s_range;
+template <bool VEC, int NT>
+__global__ __launch_bounds__(NT) void lg_k_sample_sums(SampleArgs a, char *base) {
+    __shared__ uint32_t part[NT / 32], s_n;
+    __shared__ SampleRangeLds<NT> s_range;
+    __shared__ double tab[32];
+    __shared__ lg_u64 s_sum[3], s_cand[NT * 2];                            // candidates on their way out
+    constexpr uint32_t ROOM = NT * 2;
     const SampleGeo g = lg_sample_geo(a.n_vocab);
-    const int r = blockIdx.x / g.slices, slice = blockIdx.x % g.slices, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int r = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const SampleRow p = a.params[r];
     const int kind = lg_row_kind(p, a.n_vocab);
     if (kind != LG_ROW_BORDER && kind != LG_ROW_FREE) return;
@@ -442,85 +434,117 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_sums(SampleArgs a, c
     const float *row = a.logits + r * a.stride;
     float l[4][4];
     #pragma unroll
-    for (int j = 0; j < 4; ++j) lg_load4<VEC>(row, a.n_vocab, slice * LG_SAMPLE_SLICE + j * 16 + wave, l[j]);
-    const SampleSpan s = lg_sample_span(p, w, g, s_key, s_min);
-    if (s.none) return;
+    for (int j = 0; j < 4; ++j) lg_load4<VEC>(row, a.n_vocab, slice * (NT / 16) + j * (NT / 64) + wave, l[j]);
+    lg_weigh_table(tab);
+    if (threadIdx.x < 3) s_sum[threadIdx.x] = 0;
+    if (threadIdx.x == 3) s_n = 0;
     const bool border = kind == LG_ROW_BORDER, by_mass = border && p.top_p < 1;
     SampleRange q{ LG_SAMPLE_BINS, -1, LG_SAMPLE_BINS, 0 };
-    if (border) q = lg_sample_range(a, p, w, s_range);
+    if (border) q = lg_sample_range<NT>(a, p, w, s_range);
+    const SampleSpan s = lg_sample_span<NT>(p, w, g, tab, part);
+    if (s.key == 0x007FFFFFu) return;
     const lg_u64 least = lg_least(p);
-    const float c = -(float)(1.0 / (double)p.temperature * 1.4426950408889634);
     const float floor_ = !border && least > 1 ? __builtin_amdgcn_logf((float)least * 5.684341886080802e-14f) - 0.01f : -46.0f;       // (2^-44; in base 2)
-    lg_u64 above = 0, total = 0, kept = 0;
+    lg_u64 above = 0, total = 0;
+    uint32_t kept = 0;
     #pragma unroll
     for (int j = 0; j < 4; ++j) {
+        const int grp = slice * (NT / 16) + j * (NT / 64) + wave;
         lg_u64 sum = 0;
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float x = l[j][i], d = x == s.top ? 0.0f : s.top - x;
-            lg_u64 wt = 0;
-            bool cand = false;
-            if (d * c > floor_) {
-                const int b = border ? lg_sample_bin(s, x) : 0;
-                cand = border && ((b >= q.first && b <= q.last) || b == q.cut);
-                if (b < q.first || cand || (by_mass && b < q.cut)) wt = lg_weigh(s.wg, x);
-                if (by_mass && b < q.cut) total += wt;
-                if (b < q.first) { above += wt; if (wt >= least) { sum += wt; ++kept; } }
-                cand = cand && wt;
-            }
-            if (border) {
-                const unsigned long long all = __ballot(cand);
-                if (all) {
-                    uint32_t at = 0;
-                    if (lane == 0) at = atomicAdd(w.ncand, (uint32_t)__popcll(all));
-                    at = __shfl((int)at, 0) + (uint32_t)__popcll(all & ((1ull << lane) - 1));
-                    if (cand && at < LG_SAMPLE_CAND)
-                        w.cand[at] = (lg_u64)~lg_key(x) << 32 | (uint32_t)((slice * LG_SAMPLE_SLICE + j * 16 + wave) * LG_SAMPLE_GROUP + lane * 4 + i);
-                }
+            const float x = l[j][i], e = x == s.top ? 0.0f : (s.top - x) * s.c;
+            if (!(e > floor_)) continue;
+            const int b = border ? lg_sample_bin(s, x) : 0;
+            const bool cand = border && ((b >= q.first && b <= q.last) || b == q.cut);
+            if (!(b < q.first || cand || (by_mass && b < q.cut))) continue;
+            const lg_u64 wt = lg_weigh(s.wg, x);
+            if (by_mass && b < q.cut) total += wt;
+            if (b < q.first) { above += wt; if (wt >= least) { sum += wt; ++kept; } }
+            if (cand && wt) {
+                const uint32_t at = atomicAdd(&s_n, 1u);
+                const lg_u64 c = (lg_u64)~lg_key(x) << 32 | (uint32_t)(grp * LG_SAMPLE_GROUP + lane * 4 + i);
+                if (at < ROOM) s_cand[at] = c;
             }
         }
-        for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
-        const int grp = slice * LG_SAMPLE_SLICE + j * 16 + wave;
+        sum = lg_wave_total(sum);
         if (lane == 0 && grp < g.groups) w.gsum[grp] = sum;
     }
-    above = lg_block_sum(above, s_range.part);
-    total = lg_block_sum(total, s_range.part);
-    kept = lg_block_sum(kept, s_range.part);
-    if (threadIdx.x == 0) { w.part[slice * 3] = above; w.part[slice * 3 + 1] = total; w.part[slice * 3 + 2] = kept; }
-}
-
-// LDS of n words sorted, smallest first; padded to a power of two with the largest
-__device__ void lg_sample_sort(lg_u64 *v, int n) {
-    int m = 64;
-    while (m < n) m <<= 1;
-    for (int i = n + threadIdx.x; i < m; i += LG_SAMPLE_WG) v[i] = ~0ull;
+    above = lg_wave_total(above); total = lg_wave_total(total); kept = lg_wave_total(kept);
+    if (lane == 0) { atomicAdd(&s_sum[0], above); atomicAdd(&s_sum[1], total); atomicAdd(&s_sum[2], (lg_u64)kept); }
     __syncthreads();
-    for (int k = 2; k <= m; k <<= 1)
-        for (int j = k >> 1; j; j >>= 1) {
-            for (int t = threadIdx.x; t < m / 2; t += LG_SAMPLE_WG) {
-                const int i = (t & ~(j - 1)) * 2 + (t & (j - 1));
-                const lg_u64 x = v[i], y = v[i + j];
-                if ((x > y) == !(i & k)) { v[i] = y; v[i + j] = x; }
-            }
-            __syncthreads();
-        }
+    if (threadIdx.x < 3) w.part[slice * 3 + threadIdx.x] = s_sum[threadIdx.x];
+    if (border && s_n) {
+        // (what did not fit counts all the same: more than the row may have)
+        if (threadIdx.x == 0) part[0] = atomicAdd(w.ncand, s_n > ROOM ? LG_SAMPLE_CAND + 1 : s_n);
+        __syncthreads();
+        const uint32_t at = part[0], n = s_n < ROOM ? s_n : ROOM;
+        for (uint32_t i = threadIdx.x; i < n; i += NT) if (at + i < LG_SAMPLE_CAND) w.cand[at + i] = s_cand[i];
+    }
 }
 
+// One workgroup, one row.  Candidates are ~key << 32 | index: smaller is earlier in the order.  This thread's are in registers, with their measures.
+#define LG_SAMPLE_LIST    1024                   // candidates of one part of 1024 that the border's exact place is sought among
+constexpr int LG_SAMPLE_PT = LG_SAMPLE_CAND / LG_SAMPLE_WG;
 struct SampleFinishLds {
-    lg_u64 cand[LG_SAMPLE_CAND], sum[LG_SAMPLE_GROUPS], part[LG_SAMPLE_WG / 64], weight, rest;
-    uint32_t s_key[16]; float s_min[16];
-    uint32_t n, bin[1024];
-    int at, idx, before;
-    SampleRangeLds range;
+    lg_u64 sum[LG_SAMPLE_GROUPS], bin[1024], list[LG_SAMPLE_LIST], size[LG_SAMPLE_LIST], cand[LG_SAMPLE_CAND], part[LG_SAMPLE_WG / 64], last, before, rest;
+    double tab[32];
+    uint32_t key[LG_SAMPLE_WG / 32], groups[LG_SAMPLE_GROUPS];
+    uint32_t n, n_groups;
+    int at, idx;
+    SampleRangeLds<LG_SAMPLE_WG> range;
     SampleLds alone;
 };
+// The candidate at which the running sum of measures, in order, reaches `want` (1 .. the sum of all): among 1024 equal parts of the keys first, then
+// in that part.  ~0: the part holds more than LG_SAMPLE_LIST.  Measures of 0 are no candidates.
+__device__ __forceinline__ lg_u64 lg_among(const lg_u64 (&c)[LG_SAMPLE_PT], const lg_u64 (&m)[LG_SAMPLE_PT], lg_u64 want, SampleFinishLds &s) {
+    const int t = threadIdx.x;
+    uint32_t hi = 0, lo = 0;
+    #pragma unroll
+    for (int i = 0; i < LG_SAMPLE_PT; ++i) if (m[i]) { const uint32_t nk = (uint32_t)(c[i] >> 32); if (~nk > hi) hi = ~nk; if (nk > lo) lo = nk; }
+    hi = lg_wave_max(hi); lo = lg_wave_max(lo);
+    __syncthreads();
+    if ((t & 63) == 0) { s.key[t >> 6] = hi; s.key[LG_SAMPLE_WG / 64 + (t >> 6)] = lo; }
+    s.bin[t] = 0;
+    if (t == 0) { s.n = 0; s.last = ~0ull; }
+    __syncthreads();
+    #pragma unroll
+    for (int i = 0; i < LG_SAMPLE_WG / 64; ++i) { if (s.key[i] > hi) hi = s.key[i]; if (s.key[LG_SAMPLE_WG / 64 + i] > lo) lo = s.key[LG_SAMPLE_WG / 64 + i]; }
+    const uint32_t from = ~hi, span = lo - from;                             // in ~key, largest logit first
+    const int shift = span >= 1024 ? 32 - __builtin_clz(span) - 10 : 0;
+    #pragma unroll
+    for (int i = 0; i < LG_SAMPLE_PT; ++i) if (m[i]) atomicAdd(&s.bin[((uint32_t)(c[i] >> 32) - from) >> shift], m[i]);
+    __syncthreads();
+    lg_u64 all;
+    const lg_u64 mine = s.bin[t], run = lg_block_run<LG_SAMPLE_WG>(mine, s.part, &all);
+    if (run >= want && run - mine < want) { s.at = t; s.before = run - mine; }
+    __syncthreads();
+    const uint32_t part = (uint32_t)s.at;
+    const lg_u64 before = s.before;
+    #pragma unroll
+    for (int i = 0; i < LG_SAMPLE_PT; ++i)
+        if (m[i] && ((uint32_t)(c[i] >> 32) - from) >> shift == part) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < LG_SAMPLE_LIST) { s.list[at] = c[i]; s.size[at] = m[i]; } }
+    __syncthreads();
+    const uint32_t n = s.n;
+    if (n > LG_SAMPLE_LIST) return ~0ull;
+    if ((uint32_t)t < n) {
+        const lg_u64 me = s.list[t], own = s.size[t];
+        lg_u64 upto = before;
+        for (uint32_t i = 0; i < n; ++i) if (s.list[i] <= me) upto += s.size[i];
+        if (upto >= want && upto - own < want) s.last = me;
+    }
+    __syncthreads();
+    return s.last;
+}
+
 // Whole rows of up to LG_SAMPLE_CAND tokens (WHOLE: no launch came before), or what the launches before left of longer ones
 template <bool VEC, bool WHOLE>
 __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a, char *base) {
+    constexpr int PT = LG_SAMPLE_PT;
     __shared__ SampleFinishLds s;
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, n_vocab = a.n_vocab;
     const SampleRow p = a.params[r];
-    const float *row = a.logits + r * a.stride;
+    const float *row = a.logits + r * a.stride, u = a.u[r];
     const SampleGeo g = lg_sample_geo(n_vocab);
     const SampleWork w = WHOLE ? SampleWork{} : lg_sample_work(base, g, r);
     const int kind = lg_row_kind(p, n_vocab);
@@ -530,202 +554,198 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         if (a.prob) a.prob[r] = (float)prob;
         if (a.kept) a.kept[r] = kept;
     };
-    if (!WHOLE && kind == LG_ROW_ALONE) { lg_sample_row(a, r, s.alone); return; }
-    int n = 0;                                               // candidates, sorted: larger logit first, then lower index
-    lg_u64 above = 0, total = 0;                             // sum of the tokens above them; what top-p goes by, as far as it is not theirs
-    int limit = -1, open = 0;                                // candidates from `limit` on are beyond top-k; those before `open` continue the tokens above
-    int kept = 0;
-    Weigh wg;
+    lg_weigh_table(s.tab);
+    if (t == 0) { s.n = 0; s.n_groups = 0; s.at = n_vocab; s.idx = 0; }
+    lg_u64 c[PT], m[PT];                                     // this thread's candidates and their weights
+    lg_u64 above = 0, total = 0, all;                        // sum of the tokens before the candidates; what top-p goes by
+    SampleSpan span;
+    SampleRange q{ LG_SAMPLE_BINS, -1, LG_SAMPLE_BINS, 0 };
+    uint32_t kept = 0;
+    int n = 0;
     if (WHOLE) {
-        for (int i = t; i < n_vocab; i += LG_SAMPLE_WG) s.cand[i] = (lg_u64)~lg_key(row[i]) << 32 | (uint32_t)i;
-        n = n_vocab;
-        lg_sample_sort(s.cand, n);
-        const uint32_t best = ~(uint32_t)(s.cand[0] >> 32);
-        if (best == 0x007FFFFFu) { if (t == 0) answer(-1, 0, 0); return; }
-        if (kind == LG_ROW_FIRST) { if (t == 0) answer((int)(uint32_t)s.cand[0], 1, 1); return; }
-        wg = lg_weigher(lg_unkey(best), p.temperature);
-        // those with a weight are a prefix
-        lg_u64 mine = 0;
-        for (int i = t; i < n; i += LG_SAMPLE_WG) mine += lg_weigh(wg, lg_unkey(~(uint32_t)(s.cand[i] >> 32))) != 0;
-        n = (int)lg_block_sum(mine, s.part);
-        limit = p.top_k > 0 && p.top_k < n ? p.top_k : n;
-        open = n;
+        uint32_t key = 0;
+        float x[PT];
+        #pragma unroll
+        for (int i = 0; i < PT; ++i) { const int at = t * PT + i; x[i] = at < n_vocab ? row[at] : -INFINITY; const uint32_t k = lg_key(x[i]); if (k > key) key = k; }
+        key = lg_block_max<LG_SAMPLE_WG>(key, s.key);        // (its barriers: the table's too)
+        span.key = key; span.top = lg_unkey(key);
+        span.wg = lg_weigher(span.top, p.temperature, s.tab);
+        #pragma unroll
+        for (int i = 0; i < PT; ++i) {
+            const uint32_t k = lg_key(x[i]);
+            c[i] = (lg_u64)~k << 32 | (uint32_t)(t * PT + i);
+            m[i] = kind != LG_ROW_FIRST && key != 0x007FFFFFu ? lg_weigh(span.wg, x[i]) : 0;
+            if (kind == LG_ROW_FIRST && k == key && t * PT + i < n_vocab) atomicMin(&s.at, t * PT + i);
+        }
     } else {
-        const SampleSpan span = lg_sample_span(p, w, g, s.s_key, s.s_min);
-        if (span.none) { if (t == 0) answer(-1, 0, 0); return; }
-        wg = span.wg;
-        const uint32_t best = lg_key(span.top);
-        if (kind == LG_ROW_FIRST) {
-            if (t == 0) s.at = n_vocab;
+        if (kind == LG_ROW_ALONE) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
+        // what the launches before left, all requested at once
+        uint32_t gk[LG_SAMPLE_GROUPS / LG_SAMPLE_WG];
+        #pragma unroll
+        for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) { const int at = t + i * LG_SAMPLE_WG; gk[i] = at < g.groups ? w.gmax[at] : 0; }
+        if (kind == LG_ROW_BORDER) {
+            #pragma unroll
+            for (int i = 0; i < PT; ++i) c[i] = w.cand[t + i * LG_SAMPLE_WG];
+            n = (int)*w.ncand;
+        }
+        if (kind == LG_ROW_BORDER || kind == LG_ROW_FREE) {
+            lg_u64 part[3] = { 0, 0, 0 };
+            if (t < a.slices) { part[0] = w.part[t * 3]; part[1] = w.part[t * 3 + 1]; part[2] = w.part[t * 3 + 2]; }     // (at most 128 slices)
+            for (int i = t; i < LG_SAMPLE_GROUPS; i += LG_SAMPLE_WG) s.sum[i] = i < g.groups ? w.gsum[i] : 0;
+            above = lg_block_sum<LG_SAMPLE_WG>(part[0], s.part);
+            total = lg_block_sum<LG_SAMPLE_WG>(part[1], s.part);
+            kept = (uint32_t)lg_block_sum<LG_SAMPLE_WG>(part[2], s.part);
+        }
+        span = lg_sample_span<LG_SAMPLE_WG>(p, w, g, s.tab, s.key);
+        if (span.key != 0x007FFFFFu && kind == LG_ROW_FIRST) {
+            #pragma unroll
+            for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) if (gk[i] == span.key) atomicMin(&s.at, t + i * LG_SAMPLE_WG);
             __syncthreads();
-            for (int i = t; i < g.groups; i += LG_SAMPLE_WG) if (w.gmax[i] == best) { atomicMin(&s.at, i); break; }
+            const int grp = s.at;
+            __syncthreads();
+            if (t == 0) s.at = n_vocab;
             __syncthreads();
             if (wave == 0) {
                 float l[4];
-                lg_load4<VEC>(row, n_vocab, s.at, l);
-                int first = 4;
-                #pragma unroll
-                for (int i = 3; i >= 0; --i) if (lg_key(l[i]) == best) first = i;
-                const unsigned long long any = __ballot(first < 4);
-                if (any && lane == (int)__builtin_ctzll(any)) answer(s.at * LG_SAMPLE_GROUP + lane * 4 + first, 1, 1);
-            }
-            return;
-        }
-        if (kind == LG_ROW_SMALL) {
-            // a logit that at least top_k groups reach: the lower edge of one of 1024 equal parts between the groups' smallest and largest maxima
-            if (t == 0) { s.n = 0; s.idx = 0x7FFFFFFF; }
-            s.bin[t] = 0;
-            __syncthreads();
-            uint32_t low = 0xFFFFFFFFu, key[LG_SAMPLE_GROUPS / LG_SAMPLE_WG];
-            #pragma unroll
-            for (int u = 0; u < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++u) {
-                const int i = t + u * LG_SAMPLE_WG;
-                key[u] = i < g.groups ? w.gmax[i] : 0;
-                if (key[u] > 0x007FFFFFu && key[u] < low) low = key[u];
-            }
-            for (int o = 1; o < 64; o <<= 1) { const uint32_t k = __shfl_xor((int)low, o); if (k < low) low = k; }
-            if (lane == 0) s.s_key[wave] = low;
-            __syncthreads();
-            for (int i = 0; i < LG_SAMPLE_WG / 64; ++i) if (s.s_key[i] < low) low = s.s_key[i];
-            const int shift = best - low >= 1024 ? 32 - __builtin_clz(best - low) - 10 : 0;
-            #pragma unroll
-            for (int u = 0; u < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++u) if (key[u] >= low && key[u] > 0x007FFFFFu) atomicAdd(&s.bin[(key[u] - low) >> shift], 1u);
-            __syncthreads();
-            lg_u64 all;
-            const uint32_t mine = s.bin[1023 - t];
-            const lg_u64 run = lg_block_run((lg_u64)mine, s.part, &all);
-            if (run >= (lg_u64)p.top_k && run - mine < (lg_u64)p.top_k) s.idx = 1023 - t;
-            __syncthreads();
-            const uint32_t from = all >= (lg_u64)p.top_k ? low + ((uint32_t)s.idx << shift) : 0;        // (fewer groups than top_k: every token)
-            for (int grp = wave; grp < g.groups; grp += LG_SAMPLE_WG / 64) {
-                if (w.gmax[grp] < from || w.gmax[grp] == 0x007FFFFFu) continue;
-                float l[4];
                 lg_load4<VEC>(row, n_vocab, grp, l);
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t k = lg_key(l[i]);
-                    if (k < from || !lg_weigh(wg, l[i])) continue;
-                    const uint32_t at = atomicAdd(&s.n, 1u);
-                    if (at < LG_SAMPLE_CAND) s.cand[at] = (lg_u64)~k << 32 | (uint32_t)(grp * LG_SAMPLE_GROUP + lane * 4 + i);
+                for (int i = 0; i < 4; ++i) if (lg_key(l[i]) == span.key) atomicMin(&s.at, grp * LG_SAMPLE_GROUP + lane * 4 + i);
+            }
+        } else if (kind == LG_ROW_SMALL) {
+            // a logit that at least top_k groups reach: the lower edge of one of 1024 equal parts between the groups' smallest and largest maxima
+            uint32_t low = 0;                                // as ~key
+            #pragma unroll
+            for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) if (gk[i] > 0x007FFFFFu && ~gk[i] > low) low = ~gk[i];
+            s.bin[t] = 0;
+            low = ~lg_block_max<LG_SAMPLE_WG>(low, s.key);
+            const uint32_t wide = span.key - low;
+            const int shift = wide >= 1024 ? 32 - __builtin_clz(wide) - 10 : 0;
+            #pragma unroll
+            for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) if (gk[i] > 0x007FFFFFu) atomicAdd(&s.bin[(gk[i] - low) >> shift], 1ull);
+            __syncthreads();
+            const lg_u64 mine = s.bin[1023 - t], run = lg_block_run<LG_SAMPLE_WG>(mine, s.part, &all);
+            if (run >= (lg_u64)p.top_k && run - mine < (lg_u64)p.top_k) s.idx = 1023 - t;
+            __syncthreads();
+            const uint32_t from = all >= (lg_u64)p.top_k ? low + ((uint32_t)s.idx << shift) : 0x00800000u;      // (fewer groups than top_k: every token)
+            #pragma unroll
+            for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) if (gk[i] >= from) s.groups[atomicAdd(&s.n_groups, 1u)] = t + i * LG_SAMPLE_WG;
+            __syncthreads();
+            const int n_groups = (int)s.n_groups;
+            for (int at = wave; at < n_groups; at += 4 * (LG_SAMPLE_WG / 64)) {             // four groups of a wavefront on their way together
+                float l[4][4];
+                uint32_t grp[4];
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int b = at + j * (LG_SAMPLE_WG / 64);
+                    grp[j] = b < n_groups ? s.groups[b] : g.groups;                         // (behind the row's end: -inf)
+                    lg_load4<VEC>(row, n_vocab, (int)grp[j], l[j]);
                 }
+                #pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t k = lg_key(l[j][i]);
+                        if (k < from) continue;
+                        const uint32_t to = atomicAdd(&s.n, 1u);
+                        if (to < LG_SAMPLE_CAND) s.cand[to] = (lg_u64)~k << 32 | (grp[j] * LG_SAMPLE_GROUP + lane * 4 + i);
+                    }
             }
             __syncthreads();
             n = (int)s.n;
-            if (n > LG_SAMPLE_CAND) { __syncthreads(); lg_sample_row(a, r, s.alone); return; }
-            lg_sample_sort(s.cand, n);
-            limit = p.top_k < n ? p.top_k : n;
-            open = n;
-        } else {
-            SampleRange q{ LG_SAMPLE_BINS, -1, LG_SAMPLE_BINS, 0 };
-            lg_u64 part[3] = { 0, 0, 0 };
-            for (int i = t; i < g.slices; i += LG_SAMPLE_WG)
-                #pragma unroll
-                for (int u = 0; u < 3; ++u) part[u] += w.part[i * 3 + u];
-            above = lg_block_sum(part[0], s.part);
-            total = lg_block_sum(part[1], s.part);
-            kept = (int)lg_block_sum(part[2], s.part);
-            for (int i = t; i < LG_SAMPLE_GROUPS; i += LG_SAMPLE_WG) s.sum[i] = i < g.groups ? w.gsum[i] : 0;
-            if (kind == LG_ROW_BORDER) {
-                q = lg_sample_range(a, p, w, s.range);
-                const uint32_t found = *w.ncand;
-                if (found > LG_SAMPLE_CAND) { lg_sample_row(a, r, s.alone); return; }
-                n = (int)found;
-                for (int i = t; i < n; i += LG_SAMPLE_WG) s.cand[i] = w.cand[i];
-                __syncthreads();
-                lg_sample_sort(s.cand, n);
-                lg_u64 mine = 0;
-                for (int i = t; i < n; i += LG_SAMPLE_WG) mine += lg_sample_bin(span, lg_unkey(~(uint32_t)(s.cand[i] >> 32))) < q.cut;
-                const int i0 = (int)lg_block_sum(mine, s.part);
-                limit = q.cut < LG_SAMPLE_BINS ? i0 + p.top_k - (int)q.above : n;
-                open = q.cut < LG_SAMPLE_BINS && q.last < q.cut - 1 ? i0 : n;
-                if (limit > n) { lg_sample_row(a, r, s.alone); return; }
-                if (q.cut < LG_SAMPLE_BINS) {
-                    lg_u64 v = 0;
-                    for (int i = i0 + t; i < limit; i += LG_SAMPLE_WG) v += lg_weigh(wg, lg_unkey(~(uint32_t)(s.cand[i] >> 32)));
-                    total += lg_block_sum(v, s.part);
-                }
-            } else limit = 0;
-        }
+            #pragma unroll
+            for (int i = 0; i < PT; ++i) { const int at = t + i * LG_SAMPLE_WG; c[i] = at < n && at < LG_SAMPLE_CAND ? s.cand[at] : 0; }
+        } else if (kind == LG_ROW_BORDER) q = lg_sample_range<LG_SAMPLE_WG>(a, p, w, s.range);
+        if (n > LG_SAMPLE_CAND) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
+        #pragma unroll
+        for (int i = 0; i < PT; ++i) m[i] = t + i * LG_SAMPLE_WG < n ? lg_weigh(span.wg, lg_unkey(~(uint32_t)(c[i] >> 32))) : 0;
     }
-    __syncthreads();
-    // the border among the candidates: this thread's are 4 in a row
-    constexpr int PT = LG_SAMPLE_CAND / LG_SAMPLE_WG;
-    lg_u64 wt[PT], sum = 0, all;
-    #pragma unroll
-    for (int i = 0; i < PT; ++i) { const int at = t * PT + i; wt[i] = at < limit ? lg_weigh(wg, lg_unkey(~(uint32_t)(s.cand[at] >> 32))) : 0; sum += wt[i]; }
-    int keep = limit;                                        // candidates that stay
-    if (p.top_p < 1 && kind != LG_ROW_FREE) {
-        lg_u64 run = above + lg_block_run(sum, s.part, &all) - sum;
-        const lg_u64 W = WHOLE || kind == LG_ROW_SMALL ? all : total;
-        const double want_d = __builtin_ceil((double)p.top_p * (double)W);
-        const lg_u64 want = want_d >= 1 ? (lg_u64)want_d < W ? (lg_u64)want_d : W : 1;
-        if (t == 0) s.before = -1;
+    if (span.key == 0x007FFFFFu) { if (t == 0) answer(-1, 0, 0); return; }
+    if (kind == LG_ROW_FIRST) {
         __syncthreads();
+        if (t == 0) answer(s.at, 1, 1);
+        return;
+    }
+    // top-k, then top-p: `last` is the last token in the order that stays
+    lg_u64 last = ~0ull;
+    bool lost = false;                                       // the candidates do not hold the border after all
+    const bool longer = !WHOLE && kind != LG_ROW_SMALL;      // the candidates are a part of what stays
+    if (WHOLE || kind == LG_ROW_SMALL || q.cut < LG_SAMPLE_BINS) {
+        lg_u64 one[PT], mine = 0;
         #pragma unroll
         for (int i = 0; i < PT; ++i) {
-            if (wt[i] && run < want && run + wt[i] >= want) s.before = t * PT + i;
-            run += wt[i];
+            one[i] = m[i] && (!longer || lg_sample_bin(span, lg_unkey(~(uint32_t)(c[i] >> 32))) == q.cut);
+            mine += one[i];
         }
-        __syncthreads();
-        keep = s.before + 1;
-        if (above >= want || keep == 0 || keep > open) { __syncthreads(); lg_sample_row(a, r, s.alone); return; }
+        const lg_u64 have = lg_block_sum<LG_SAMPLE_WG>(mine, s.part), want = p.top_k > 0 ? (lg_u64)p.top_k - (longer ? q.above : 0) : have + 1;
+        if (want < have) { last = lg_among(c, one, want, s); lost = last == ~0ull; }
+        else lost = longer && want > have;
+        lg_u64 sum = 0;
+        #pragma unroll
+        for (int i = 0; i < PT; ++i) { if (c[i] > last) { m[i] = 0; one[i] = 0; } if (one[i]) sum += m[i]; }
+        if (p.top_p < 1) total += lg_block_sum<LG_SAMPLE_WG>(sum, s.part);
     }
-    const lg_u64 last = keep ? s.cand[keep - 1] : ~0ull;     // tokens up to this one stay
-    lg_u64 S = 0, mine = 0;
+    if (p.top_p < 1 && kind != LG_ROW_FREE && !lost) {
+        const double want_d = __builtin_ceil((double)p.top_p * (double)total);
+        const lg_u64 want = want_d >= 1 ? (lg_u64)want_d < total ? (lg_u64)want_d : total : 1;
+        // (bins between top-p's and top-k's hold tokens that are no candidates: those of top-k's are not counted behind them)
+        const bool gap = longer && q.cut < LG_SAMPLE_BINS && q.last < q.cut - 1;
+        lg_u64 in[PT], sum = 0;
+        #pragma unroll
+        for (int i = 0; i < PT; ++i) { in[i] = gap && lg_sample_bin(span, lg_unkey(~(uint32_t)(c[i] >> 32))) > q.last ? 0 : m[i]; sum += in[i]; }
+        const lg_u64 have = lg_block_sum<LG_SAMPLE_WG>(sum, s.part);
+        if (above >= want || above + have < want) lost = true;
+        else { last = lg_among(c, in, want - above, s); lost = last == ~0ull; }
+    }
+    if (lost) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
+    lg_u64 sum = 0;
+    uint32_t mine = 0;
     #pragma unroll
-    for (int i = 0; i < PT; ++i) {
-        const int at = t * PT + i;
-        if (at >= keep || wt[i] < least) wt[i] = 0;
-        if (wt[i]) { S += wt[i]; ++mine; }
-    }
-    kept += (int)lg_block_sum(mine, s.part);
-    const float u = a.u[r];
-    auto target_of = [&](lg_u64 S_) {
-        lg_u64 x = u > 0 ? (lg_u64)__builtin_floor((u < 1 ? (double)u : 1.0) * (double)S_) : 0;
-        return x > S_ - 1 ? S_ - 1 : x;
+    for (int i = 0; i < PT; ++i) { if (c[i] > last || m[i] < least) m[i] = 0; sum += m[i]; mine += m[i] != 0; }
+    kept += (uint32_t)lg_block_sum<LG_SAMPLE_WG>((lg_u64)mine, s.part);
+    auto target_of = [&](lg_u64 S) {
+        const lg_u64 x = u > 0 ? (lg_u64)__builtin_floor((u < 1 ? (double)u : 1.0) * (double)S) : 0;
+        return x > S - 1 ? S - 1 : x;
     };
-    if (WHOLE || kind == LG_ROW_SMALL) {
-        S = lg_block_sum(S, s.part);
-        const lg_u64 target = target_of(S);
-        if (!WHOLE) {
-            // index order: index << 32 | key
-            __syncthreads();
-            for (int i = t; i < keep; i += LG_SAMPLE_WG) { const lg_u64 c = s.cand[i]; s.cand[i] = c << 32 | (uint32_t)~(c >> 32); }
-            lg_sample_sort(s.cand, keep);
-        }
-        sum = 0;
-        uint32_t idx[PT];
+    if (WHOLE) {                                             // the candidates lie in index order
+        lg_u64 run = lg_block_run<LG_SAMPLE_WG>(sum, s.part, &all) - sum;
+        const lg_u64 target = target_of(all);
         #pragma unroll
         for (int i = 0; i < PT; ++i) {
-            const int at = t * PT + i;
-            wt[i] = 0;
-            if (WHOLE) {
-                idx[i] = at;
-                if (at < n_vocab) { const uint32_t k = lg_key(row[at]); if (((lg_u64)~k << 32 | (uint32_t)at) <= last) wt[i] = lg_weigh(wg, lg_unkey(k)); }
-            } else if (at < keep) { idx[i] = (uint32_t)(s.cand[at] >> 32); wt[i] = lg_weigh(wg, lg_unkey((uint32_t)s.cand[at])); }
-            if (wt[i] < least) wt[i] = 0;
-            sum += wt[i];
+            if (m[i] && run <= target && run + m[i] > target) answer(t * PT + i, (double)m[i] / (double)all, (int)kept);
+            run += m[i];
         }
-        lg_u64 run = lg_block_run(sum, s.part, &all) - sum;
+        return;
+    }
+    if (kind == LG_ROW_SMALL) {
+        // at most LG_SAMPLE_SMALL_K stay: each one's running sum in index order from all of them, by four threads each where there are few
+        all = lg_block_sum<LG_SAMPLE_WG>(sum, s.part);
+        const lg_u64 target = target_of(all);
+        if (t == 0) s.n = 0;
+        __syncthreads();
         #pragma unroll
-        for (int i = 0; i < PT; ++i) {
-            if (wt[i] && run <= target && run + wt[i] > target) answer((int)idx[i], (double)wt[i] / (double)S, kept);
-            run += wt[i];
+        for (int i = 0; i < PT; ++i) if (m[i]) { const uint32_t at = atomicAdd(&s.n, 1u); s.list[at] = (lg_u64)(uint32_t)c[i] << 45 | m[i]; }       // (19 bits of index, 45 of weight)
+        __syncthreads();
+        const uint32_t stay = s.n, ways = stay <= LG_SAMPLE_WG / 4 ? 4 : 1, who = (uint32_t)t / ways;
+        if (who < stay) {
+            const lg_u64 me = s.list[who], weight = me & ((1ull << 45) - 1);
+            lg_u64 upto = 0;
+            for (uint32_t i = (uint32_t)t % ways; i < stay; i += ways) { const lg_u64 x = s.list[i]; if (x >> 45 <= me >> 45) upto += x & ((1ull << 45) - 1); }
+            if (ways == 4) { upto += __shfl_xor(upto, 1); upto += __shfl_xor(upto, 2); }
+            if ((uint32_t)t % ways == 0 && upto > target && upto - weight <= target) answer((int)(me >> 45), (double)weight / (double)all, (int)kept);
         }
         return;
     }
     // the groups' sums with the candidates that stay, the group of the draw, and the token in it
     #pragma unroll
-    for (int i = 0; i < PT; ++i) if (wt[i]) atomicAdd(&s.sum[(uint32_t)s.cand[t * PT + i] / LG_SAMPLE_GROUP], wt[i]);
+    for (int i = 0; i < PT; ++i) if (m[i]) atomicAdd(&s.sum[(uint32_t)c[i] / LG_SAMPLE_GROUP], m[i]);
     __syncthreads();
     constexpr int GT = LG_SAMPLE_GROUPS / LG_SAMPLE_WG;
     lg_u64 gs[GT];
     sum = 0;
     #pragma unroll
     for (int i = 0; i < GT; ++i) { gs[i] = s.sum[t * GT + i]; sum += gs[i]; }
-    lg_u64 run = lg_block_run(sum, s.part, &all) - sum;
-    S = all;
-    const lg_u64 target = target_of(S);
+    lg_u64 run = lg_block_run<LG_SAMPLE_WG>(sum, s.part, &all) - sum;
+    const lg_u64 target = target_of(all);
     #pragma unroll
     for (int i = 0; i < GT; ++i) {
         if (run <= target && run + gs[i] > target) { s.at = t * GT + i; s.rest = target - run; }
@@ -733,22 +753,22 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
     }
     __syncthreads();
     if (wave == 0) {
+        const int grp = s.at;
+        const lg_u64 rest = s.rest;
         float l[4];
-        lg_load4<VEC>(row, n_vocab, s.at, l);
+        lg_load4<VEC>(row, n_vocab, grp, l);
+        lg_u64 wt[4];
         sum = 0;
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t k = lg_key(l[i]), idx = s.at * LG_SAMPLE_GROUP + lane * 4 + i;
-            wt[i] = kind == LG_ROW_FREE || ((lg_u64)~k << 32 | idx) <= last ? lg_weigh(wg, l[i]) : 0;
+            wt[i] = ((lg_u64)~lg_key(l[i]) << 32 | (uint32_t)(grp * LG_SAMPLE_GROUP + lane * 4 + i)) <= last ? lg_weigh(span.wg, l[i]) : 0;
             if (wt[i] < least) wt[i] = 0;
             sum += wt[i];
         }
-        lg_u64 at = sum;
-        for (int o = 1; o < 64; o <<= 1) { const lg_u64 v = __shfl_up(at, o); if (lane >= o) at += v; }
-        at -= sum;
+        lg_u64 at = lg_wave_run(sum) - sum;
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (wt[i] && at <= s.rest && at + wt[i] > s.rest) answer(s.at * LG_SAMPLE_GROUP + lane * 4 + i, (double)wt[i] / (double)S, kept);
+            if (wt[i] && at <= rest && at + wt[i] > rest) answer(grp * LG_SAMPLE_GROUP + lane * 4 + i, (double)wt[i] / (double)all, (int)kept);
             at += wt[i];
         }
     }

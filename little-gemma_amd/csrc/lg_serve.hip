@@ -144,6 +144,8 @@ extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float 
     return 0;
 }
 
+// Groups of 256 logits in a call from which on the passes over them take workgroups of 64 groups instead of 16: fewer of them read a row's bins again
+#define LG_SAMPLE_WIDE 16384
 // ---- sample -----------------------------------------------------------------------------------------------------
 extern "C" size_t lg_hip_sample_workspace(int rows, int n_vocab) {
     if (rows < 0 || n_vocab <= LG_SAMPLE_CAND || n_vocab > LG_SAMPLE_VOCAB) return 0;
@@ -151,12 +153,20 @@ extern "C" size_t lg_hip_sample_workspace(int rows, int n_vocab) {
 }
 
 template <bool VEC>
-static void launch_sample(const SampleArgs &a, int rows, char *work, hipStream_t st) {
+static void launch_sample(SampleArgs a, int rows, char *work, hipStream_t st) {
     if (!work) { hipLaunchKernelGGL((lg_k_sample_finish<VEC, true>), dim3(rows), dim3(LG_SAMPLE_WG), 0, st, a, work); return; }
     const SampleGeo g = lg_sample_geo(a.n_vocab);
-    hipLaunchKernelGGL(lg_k_sample_max<VEC>, dim3((unsigned)rows * g.maxes), dim3(LG_SAMPLE_MAX_WG), 0, st, a, work);
-    hipLaunchKernelGGL(lg_k_sample_bins<VEC>, dim3((unsigned)rows * g.slices), dim3(LG_SAMPLE_WG), 0, st, a, work);
-    hipLaunchKernelGGL(lg_k_sample_sums<VEC>, dim3((unsigned)rows * g.slices), dim3(LG_SAMPLE_WG), 0, st, a, work);
+    const dim3 maxes((unsigned)g.maxes, rows), few((unsigned)(g.groups + 15) / 16, rows), many((unsigned)(g.groups + 63) / 64, rows);
+    hipLaunchKernelGGL(lg_k_sample_max<VEC>, maxes, dim3(LG_SAMPLE_MAX_WG), 0, st, a, work);
+    const bool narrow = (int64_t)rows * g.groups < LG_SAMPLE_WIDE;
+    a.slices = (int)(narrow ? few : many).x;
+    if (narrow) {
+        hipLaunchKernelGGL((lg_k_sample_bins<VEC, 256>), few, dim3(256), 0, st, a, work);
+        hipLaunchKernelGGL((lg_k_sample_sums<VEC, 256>), few, dim3(256), 0, st, a, work);
+    } else {
+        hipLaunchKernelGGL((lg_k_sample_bins<VEC, 1024>), many, dim3(1024), 0, st, a, work);
+        hipLaunchKernelGGL((lg_k_sample_sums<VEC, 1024>), many, dim3(1024), 0, st, a, work);
+    }
     hipLaunchKernelGGL((lg_k_sample_finish<VEC, false>), dim3(rows), dim3(LG_SAMPLE_WG), 0, st, a, work);
 }
 
@@ -171,7 +181,7 @@ extern "C" int lg_hip_sample(const float *d_logits, int64_t stride, int rows, in
     const size_t need = lg_hip_sample_workspace(rows, n_vocab);
     if (need && (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)))
         return lg_fail(-2, "sample: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
-    const SampleArgs a{ d_logits, (long long)stride, (const SampleRow *)d_params, d_u, d_tok, d_prob, d_kept, n_vocab };
+    const SampleArgs a{ d_logits, (long long)stride, (const SampleRow *)d_params, d_u, d_tok, d_prob, d_kept, n_vocab, 0 };
     // loads of 16 bytes where every row is aligned to that
     if (aligned16(d_logits) && stride % 4 == 0) launch_sample<true>(a, rows, need ? (char *)d_work : nullptr, (hipStream_t)stream);
     else launch_sample<false>(a, rows, need ? (char *)d_work : nullptr, (hipStream_t)stream);
