@@ -212,7 +212,8 @@ struct SampleWork {                     // per row, in working memory
     lg_u64 *mass; uint32_t *count;      // [LG_SAMPLE_BINS]
     lg_u64 *gsum;                       // [groups]
     lg_u64 *part;                       // [slices][3]: sum above the candidates, sum that top-p goes by (without the candidates), tokens kept above them
-    uint32_t *ncand; lg_u64 *cand;      // [LG_SAMPLE_CAND] ~key << 32 | index
+    uint32_t *ncand;                    // candidates; behind it the row's SampleRange
+    lg_u64 *cand;                       // [LG_SAMPLE_CAND] ~key << 32 | index
 };
 struct SampleGeo { int groups, maxes, slices; size_t gmax, smin, mass, count, gsum, part, ncand, cand, row; };
 __host__ __device__ inline size_t lg_up64(size_t n) { return (n + 63) & ~(size_t)63; }
@@ -303,12 +304,7 @@ __device__ __forceinline__ SampleSpan lg_sample_span(const SampleRow &p, const S
     uint32_t key = 0, least = 0;
     for (int i = threadIdx.x; i < g.groups; i += NT) { const uint32_t k = w.gmax[i]; if (k > key) key = k; }
     for (int i = threadIdx.x; i < g.maxes; i += NT) { const uint32_t k = w.smin[i]; if (k > least) least = k; }
-    key = lg_wave_max(key); least = lg_wave_max(least);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) { part[threadIdx.x >> 6] = key; part[NT / 64 + (threadIdx.x >> 6)] = least; }
-    __syncthreads();
-    #pragma unroll
-    for (int i = 0; i < NT / 64; ++i) { if (part[i] > key) key = part[i]; if (part[NT / 64 + i] > least) least = part[NT / 64 + i]; }
+    lg_block_max2<NT>(key, least, part);
     SampleSpan s;
     s.key = key;
     s.top = lg_unkey(key);
@@ -324,9 +320,10 @@ __device__ __forceinline__ int lg_sample_bin(const SampleSpan &s, float l) {
     return b >= 0 ? b < (float)(LG_SAMPLE_BINS - 1) ? (int)b : LG_SAMPLE_BINS - 1 : 0;
 }
 
-// NT threads read 16 (256) or 64 (1024) groups
-template <bool VEC, int NT>
-__global__ __launch_bounds__(NT) void lg_k_sample_bins(SampleArgs a, char *base) {
+// (64 groups to a workgroup: with 16, more workgroups add to the row's bins; 5 rows 7.6 -> 10.3 us)
+template <bool VEC>
+__global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_bins(SampleArgs a, char *base) {
+    constexpr int NT = LG_SAMPLE_WG;
     __shared__ lg_u64 mass[LG_SAMPLE_BINS];
     __shared__ uint32_t count[LG_SAMPLE_BINS], part[NT / 32];
     __shared__ double tab[32];
@@ -418,6 +415,7 @@ __device__ __forceinline__ SampleRange lg_sample_range(const SampleArgs &a, cons
     return q;
 }
 
+// NT threads read 16 (256) or 64 (1024) groups
 template <bool VEC, int NT>
 __global__ __launch_bounds__(NT) void lg_k_sample_sums(SampleArgs a, char *base) {
     __shared__ uint32_t part[NT / 32], s_n;
@@ -440,7 +438,10 @@ __global__ __launch_bounds__(NT) void lg_k_sample_sums(SampleArgs a, char *base)
     if (threadIdx.x == 3) s_n = 0;
     const bool border = kind == LG_ROW_BORDER, by_mass = border && p.top_p < 1;
     SampleRange q{ LG_SAMPLE_BINS, -1, LG_SAMPLE_BINS, 0 };
-    if (border) q = lg_sample_range<NT>(a, p, w, s_range);
+    if (border) {
+        q = lg_sample_range<NT>(a, p, w, s_range);
+        if (slice == 0 && threadIdx.x == 0) *(SampleRange *)(w.ncand + 4) = q;
+    }
     const SampleSpan s = lg_sample_span<NT>(p, w, g, tab, part);
     if (s.key == 0x007FFFFFu) return;
     const lg_u64 least = lg_least(p);
@@ -484,57 +485,62 @@ __global__ __launch_bounds__(NT) void lg_k_sample_sums(SampleArgs a, char *base)
 }
 
 // One workgroup, one row.  Candidates are ~key << 32 | index: smaller is earlier in the order.  This thread's are in registers, with their measures.
-#define LG_SAMPLE_LIST    1024                   // candidates of one part of 1024 that the border's exact place is sought among
+#define LG_SAMPLE_LIST    512                    // what stays of a small top-k
+#define LG_SAMPLE_FEW     128                    // candidates of a small top-k whose order and sums are taken pair by pair
+static_assert(LG_SAMPLE_LIST >= LG_SAMPLE_SMALL_K && LG_SAMPLE_LIST >= LG_SAMPLE_FEW, "room for what stays");
 constexpr int LG_SAMPLE_PT = LG_SAMPLE_CAND / LG_SAMPLE_WG;
 struct SampleFinishLds {
-    lg_u64 sum[LG_SAMPLE_GROUPS], bin[1024], list[LG_SAMPLE_LIST], size[LG_SAMPLE_LIST], cand[LG_SAMPLE_CAND], part[LG_SAMPLE_WG / 64], last, before, rest;
+    lg_u64 sum[LG_SAMPLE_GROUPS], bin[1024], list[LG_SAMPLE_LIST], size[64], cand[LG_SAMPLE_CAND], part[LG_SAMPLE_WG / 32], part3[3], last, rest, whole;
     double tab[32];
     uint32_t key[LG_SAMPLE_WG / 32], groups[LG_SAMPLE_GROUPS];
     uint32_t n, n_groups;
     int at, idx;
-    SampleRangeLds<LG_SAMPLE_WG> range;
     SampleLds alone;
 };
-// The candidate at which the running sum of measures, in order, reaches `want` (1 .. the sum of all): among 1024 equal parts of the keys first, then
-// in that part.  ~0: the part holds more than LG_SAMPLE_LIST.  Measures of 0 are no candidates.
-__device__ __forceinline__ lg_u64 lg_among(const lg_u64 (&c)[LG_SAMPLE_PT], const lg_u64 (&m)[LG_SAMPLE_PT], lg_u64 want, SampleFinishLds &s) {
+// The candidate at which the running sum of measures, in order, reaches `want` (1 .. the sum of all); measures of 0 are no candidates.  1024 equal parts
+// between the first and the last candidate, the part that holds the border cut again until it has at most 64 of them (once for logits that lie
+// anywhere, again for a group of equal ones, by their index then), and a wavefront over these.
+__device__ __forceinline__ lg_u64 lg_among(const lg_u64 (&c)[LG_SAMPLE_PT], const lg_u64 (&m_in)[LG_SAMPLE_PT], lg_u64 want, SampleFinishLds &s) {
     const int t = threadIdx.x;
-    uint32_t hi = 0, lo = 0;
+    lg_u64 m[LG_SAMPLE_PT];
     #pragma unroll
-    for (int i = 0; i < LG_SAMPLE_PT; ++i) if (m[i]) { const uint32_t nk = (uint32_t)(c[i] >> 32); if (~nk > hi) hi = ~nk; if (nk > lo) lo = nk; }
-    hi = lg_wave_max(hi); lo = lg_wave_max(lo);
-    __syncthreads();
-    if ((t & 63) == 0) { s.key[t >> 6] = hi; s.key[LG_SAMPLE_WG / 64 + (t >> 6)] = lo; }
-    s.bin[t] = 0;
-    if (t == 0) { s.n = 0; s.last = ~0ull; }
-    __syncthreads();
-    #pragma unroll
-    for (int i = 0; i < LG_SAMPLE_WG / 64; ++i) { if (s.key[i] > hi) hi = s.key[i]; if (s.key[LG_SAMPLE_WG / 64 + i] > lo) lo = s.key[LG_SAMPLE_WG / 64 + i]; }
-    const uint32_t from = ~hi, span = lo - from;                             // in ~key, largest logit first
-    const int shift = span >= 1024 ? 32 - __builtin_clz(span) - 10 : 0;
-    #pragma unroll
-    for (int i = 0; i < LG_SAMPLE_PT; ++i) if (m[i]) atomicAdd(&s.bin[((uint32_t)(c[i] >> 32) - from) >> shift], m[i]);
-    __syncthreads();
-    lg_u64 all;
-    const lg_u64 mine = s.bin[t], run = lg_block_run<LG_SAMPLE_WG>(mine, s.part, &all);
-    if (run >= want && run - mine < want) { s.at = t; s.before = run - mine; }
-    __syncthreads();
-    const uint32_t part = (uint32_t)s.at;
-    const lg_u64 before = s.before;
-    #pragma unroll
-    for (int i = 0; i < LG_SAMPLE_PT; ++i)
-        if (m[i] && ((uint32_t)(c[i] >> 32) - from) >> shift == part) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < LG_SAMPLE_LIST) { s.list[at] = c[i]; s.size[at] = m[i]; } }
-    __syncthreads();
-    const uint32_t n = s.n;
-    if (n > LG_SAMPLE_LIST) return ~0ull;
-    if ((uint32_t)t < n) {
-        const lg_u64 me = s.list[t], own = s.size[t];
-        lg_u64 upto = before;
-        for (uint32_t i = 0; i < n; ++i) if (s.list[i] <= me) upto += s.size[i];
-        if (upto >= want && upto - own < want) s.last = me;
+    for (int i = 0; i < LG_SAMPLE_PT; ++i) m[i] = m_in[i];
+    for (;;) {                                               // (every round but the last leaves out a candidate: the first and the last lie in different parts)
+        lg_u64 from = 0, to = 0;                             // from as its complement
+        #pragma unroll
+        for (int i = 0; i < LG_SAMPLE_PT; ++i) if (m[i]) { if (~c[i] > from) from = ~c[i]; if (c[i] > to) to = c[i]; }
+        s.bin[t] = 0;
+        if (t == 0) s.n = 0;
+        lg_block_max2<LG_SAMPLE_WG>(from, to, s.part);       // (its barriers: the clearing's too)
+        from = ~from;
+        const lg_u64 span = to - from;
+        const int shift = span >= 1024 ? 64 - __builtin_clzll(span) - 10 : 0;
+        #pragma unroll
+        for (int i = 0; i < LG_SAMPLE_PT; ++i) if (m[i]) atomicAdd(&s.bin[(c[i] - from) >> shift], m[i]);
+        __syncthreads();
+        lg_u64 all;
+        const lg_u64 mine = s.bin[t], run = lg_block_run<LG_SAMPLE_WG>(mine, s.part, &all);
+        if (run >= want && run - mine < want) { s.at = t; s.rest = run - mine; }
+        __syncthreads();
+        const lg_u64 part = (lg_u64)s.at;
+        want -= s.rest;
+        #pragma unroll
+        for (int i = 0; i < LG_SAMPLE_PT; ++i) {
+            if (m[i] && (c[i] - from) >> shift != part) m[i] = 0;
+            if (m[i]) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < 64) { s.list[at] = c[i]; s.size[at] = m[i]; } }
+        }
+        __syncthreads();
+        const uint32_t n = s.n;
+        if (n > 64) { __syncthreads(); continue; }
+        if (t < 64) {
+            const lg_u64 me = (uint32_t)t < n ? s.list[t] : ~0ull, own = (uint32_t)t < n ? s.size[t] : 0;
+            lg_u64 upto = 0;
+            for (uint32_t i = 0; i < n; ++i) { const lg_u64 x = lg_lane(me, i), y = lg_lane(own, i); if (x <= me) upto += y; }
+            if (own && upto >= want && upto - own < want) s.last = me;
+        }
+        __syncthreads();
+        return s.last;
     }
-    __syncthreads();
-    return s.last;
 }
 
 // Whole rows of up to LG_SAMPLE_CAND tokens (WHOLE: no launch came before), or what the launches before left of longer ones
@@ -587,16 +593,19 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             #pragma unroll
             for (int i = 0; i < PT; ++i) c[i] = w.cand[t + i * LG_SAMPLE_WG];
             n = (int)*w.ncand;
+            q = *(const SampleRange *)(w.ncand + 4);
         }
         if (kind == LG_ROW_BORDER || kind == LG_ROW_FREE) {
-            lg_u64 part[3] = { 0, 0, 0 };
-            if (t < a.slices) { part[0] = w.part[t * 3]; part[1] = w.part[t * 3 + 1]; part[2] = w.part[t * 3 + 2]; }     // (at most 128 slices)
+            if (wave < 3) {                                  // (at most 128 slices: a wavefront for each sum)
+                lg_u64 x = 0;
+                for (int i = lane; i < a.slices; i += 64) x += w.part[i * 3 + wave];
+                x = lg_wave_total(x);
+                if (lane == 0) s.part3[wave] = x;
+            }
             for (int i = t; i < LG_SAMPLE_GROUPS; i += LG_SAMPLE_WG) s.sum[i] = i < g.groups ? w.gsum[i] : 0;
-            above = lg_block_sum<LG_SAMPLE_WG>(part[0], s.part);
-            total = lg_block_sum<LG_SAMPLE_WG>(part[1], s.part);
-            kept = (uint32_t)lg_block_sum<LG_SAMPLE_WG>(part[2], s.part);
         }
-        span = lg_sample_span<LG_SAMPLE_WG>(p, w, g, s.tab, s.key);
+        span = lg_sample_span<LG_SAMPLE_WG>(p, w, g, s.tab, s.key);          // (its barriers are the sums' too)
+        if (kind == LG_ROW_BORDER || kind == LG_ROW_FREE) { above = s.part3[0]; total = s.part3[1]; kept = (uint32_t)s.part3[2]; }
         if (span.key != 0x007FFFFFu && kind == LG_ROW_FIRST) {
             #pragma unroll
             for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) if (gk[i] == span.key) atomicMin(&s.at, t + i * LG_SAMPLE_WG);
@@ -640,21 +649,31 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
                     grp[j] = b < n_groups ? s.groups[b] : g.groups;                         // (behind the row's end: -inf)
                     lg_load4<VEC>(row, n_vocab, (int)grp[j], l[j]);
                 }
+                uint32_t found = 0;
+                #pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) found += lg_key(l[j][i]) >= from;
+                uint32_t to = lg_wave_run(found);
+                const uint32_t of_all = lg_last_lane(to);
+                uint32_t first = 0;
+                if (lane == 0) first = atomicAdd(&s.n, of_all);
+                to += lg_lane(first, 0) - found;
                 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t k = lg_key(l[j][i]);
                         if (k < from) continue;
-                        const uint32_t to = atomicAdd(&s.n, 1u);
                         if (to < LG_SAMPLE_CAND) s.cand[to] = (lg_u64)~k << 32 | (grp[j] * LG_SAMPLE_GROUP + lane * 4 + i);
+                        ++to;
                     }
             }
             __syncthreads();
             n = (int)s.n;
             #pragma unroll
             for (int i = 0; i < PT; ++i) { const int at = t + i * LG_SAMPLE_WG; c[i] = at < n && at < LG_SAMPLE_CAND ? s.cand[at] : 0; }
-        } else if (kind == LG_ROW_BORDER) q = lg_sample_range<LG_SAMPLE_WG>(a, p, w, s.range);
+        }
         if (n > LG_SAMPLE_CAND) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
         #pragma unroll
         for (int i = 0; i < PT; ++i) m[i] = t + i * LG_SAMPLE_WG < n ? lg_weigh(span.wg, lg_unkey(~(uint32_t)(c[i] >> 32))) : 0;
@@ -663,6 +682,47 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
     if (kind == LG_ROW_FIRST) {
         __syncthreads();
         if (t == 0) answer(s.at, 1, 1);
+        return;
+    }
+    auto target_of = [&](lg_u64 S) {
+        const lg_u64 x = u > 0 ? (lg_u64)__builtin_floor((u < 1 ? (double)u : 1.0) * (double)S) : 0;
+        return x > S - 1 ? S - 1 : x;
+    };
+    if (!WHOLE && kind == LG_ROW_SMALL && n <= LG_SAMPLE_FEW) {
+        // few candidates: each one's place in the order and the sum up to it from all of them, by eight threads each; then the same in index order among
+        // what stays (three barriers; the way below takes 25)
+        const uint32_t who = (uint32_t)t >> 3, sub = t & 7;
+        const bool on = (int)who < n;
+        if (t < n) { s.list[t] = c[0]; s.sum[t] = m[0]; }
+        if (t == 0) s.last = ~0ull;
+        __syncthreads();
+        const lg_u64 me = on ? s.list[who] : ~0ull, own = on ? s.sum[who] : 0;
+        lg_u64 upto = 0;
+        uint32_t place = 0;
+        if (on) for (uint32_t i = sub; (int)i < n; i += 8) { const lg_u64 x = s.sum[i]; if (x && s.list[i] <= me) { upto += x; ++place; } }
+        for (int o = 1; o < 8; o <<= 1) { upto += __shfl_xor(upto, o); place += (uint32_t)__shfl_xor((int)place, o); }
+        // (a weight of 0 is the end of the order: no candidate)
+        if (t == 0) { s.whole = 0; s.n = 0; }
+        __syncthreads();
+        if (own && sub == 0 && place <= (uint32_t)p.top_k) atomicMax(&s.whole, upto);
+        __syncthreads();
+        const lg_u64 W = s.whole;
+        lg_u64 want = W;
+        if (p.top_p < 1) { const double want_d = __builtin_ceil((double)p.top_p * (double)W); want = want_d >= 1 ? (lg_u64)want_d < W ? (lg_u64)want_d : W : 1; }
+        if (own && sub == 0 && upto >= want && upto - own < want) s.last = me;
+        __syncthreads();
+        const lg_u64 last = s.last;
+        lg_u64 S = 0, run = 0;
+        uint32_t stay = 0;
+        if (on) for (uint32_t i = sub; (int)i < n; i += 8) {
+            const lg_u64 x = s.list[i], y = s.sum[i];
+            if (x <= last && y >= least) { S += y; ++stay; if ((uint32_t)x <= (uint32_t)me) run += y; }
+        }
+        for (int o = 1; o < 8; o <<= 1) { S += __shfl_xor(S, o); run += __shfl_xor(run, o); stay += (uint32_t)__shfl_xor((int)stay, o); }
+        if (own >= least && me <= last && sub == 0) {
+            const lg_u64 target = target_of(S);
+            if (run > target && run - own <= target) answer((int)(uint32_t)me, (double)own / (double)S, (int)stay);
+        }
         return;
     }
     // top-k, then top-p: `last` is the last token in the order that stays
@@ -677,7 +737,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             mine += one[i];
         }
         const lg_u64 have = lg_block_sum<LG_SAMPLE_WG>(mine, s.part), want = p.top_k > 0 ? (lg_u64)p.top_k - (longer ? q.above : 0) : have + 1;
-        if (want < have) { last = lg_among(c, one, want, s); lost = last == ~0ull; }
+        if (want < have) last = lg_among(c, one, want, s);
         else lost = longer && want > have;
         lg_u64 sum = 0;
         #pragma unroll
@@ -694,7 +754,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         for (int i = 0; i < PT; ++i) { in[i] = gap && lg_sample_bin(span, lg_unkey(~(uint32_t)(c[i] >> 32))) > q.last ? 0 : m[i]; sum += in[i]; }
         const lg_u64 have = lg_block_sum<LG_SAMPLE_WG>(sum, s.part);
         if (above >= want || above + have < want) lost = true;
-        else { last = lg_among(c, in, want - above, s); lost = last == ~0ull; }
+        else last = lg_among(c, in, want - above, s);
     }
     if (lost) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
     lg_u64 sum = 0;
@@ -702,10 +762,6 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
     #pragma unroll
     for (int i = 0; i < PT; ++i) { if (c[i] > last || m[i] < least) m[i] = 0; sum += m[i]; mine += m[i] != 0; }
     kept += (uint32_t)lg_block_sum<LG_SAMPLE_WG>((lg_u64)mine, s.part);
-    auto target_of = [&](lg_u64 S) {
-        const lg_u64 x = u > 0 ? (lg_u64)__builtin_floor((u < 1 ? (double)u : 1.0) * (double)S) : 0;
-        return x > S - 1 ? S - 1 : x;
-    };
     if (WHOLE) {                                             // the candidates lie in index order
         lg_u64 run = lg_block_run<LG_SAMPLE_WG>(sum, s.part, &all) - sum;
         const lg_u64 target = target_of(all);

@@ -158,15 +158,11 @@ static void launch_sample(SampleArgs a, int rows, char *work, hipStream_t st) {
     const SampleGeo g = lg_sample_geo(a.n_vocab);
     const dim3 maxes((unsigned)g.maxes, rows), few((unsigned)(g.groups + 15) / 16, rows), many((unsigned)(g.groups + 63) / 64, rows);
     hipLaunchKernelGGL(lg_k_sample_max<VEC>, maxes, dim3(LG_SAMPLE_MAX_WG), 0, st, a, work);
+    hipLaunchKernelGGL(lg_k_sample_bins<VEC>, many, dim3(LG_SAMPLE_WG), 0, st, a, work);
     const bool narrow = (int64_t)rows * g.groups < LG_SAMPLE_WIDE;
     a.slices = (int)(narrow ? few : many).x;
-    if (narrow) {
-        hipLaunchKernelGGL((lg_k_sample_bins<VEC, 256>), few, dim3(256), 0, st, a, work);
-        hipLaunchKernelGGL((lg_k_sample_sums<VEC, 256>), few, dim3(256), 0, st, a, work);
-    } else {
-        hipLaunchKernelGGL((lg_k_sample_bins<VEC, 1024>), many, dim3(1024), 0, st, a, work);
-        hipLaunchKernelGGL((lg_k_sample_sums<VEC, 1024>), many, dim3(1024), 0, st, a, work);
-    }
+    if (narrow) hipLaunchKernelGGL((lg_k_sample_sums<VEC, 256>), few, dim3(256), 0, st, a, work);
+    else hipLaunchKernelGGL((lg_k_sample_sums<VEC, 1024>), many, dim3(1024), 0, st, a, work);
     hipLaunchKernelGGL((lg_k_sample_finish<VEC, false>), dim3(rows), dim3(LG_SAMPLE_WG), 0, st, a, work);
 }
 
