@@ -185,7 +185,7 @@ struct PageAttn {
     float *out; long long out_stride;
     float *pm, *pl, *pacc;              // [n_seq][H][splits], [..][hd]: partials of more than one split
     float scale;
-    int H, nkv, max_blocks, max_len, window, chunk, splits;
+    int H, nkv, units, max_blocks, max_len, window, chunk, splits;      // units: sequences x key heads
 };
 // The keys a sequence sees: [lo, len)
 __device__ __forceinline__ void lg_pa_range(const PageAttn &a, int seq, int &lo, int &len) {
@@ -201,15 +201,34 @@ __device__ __forceinline__ int lg_pa_splits(const PageAttn &a, int lo, int len) 
     return len > lo ? (len - first + a.chunk - 1) / a.chunk : 0;
 }
 
+// Where the rows of a tile's two halves lie: the page's first value, or page 0's where there is no such page
+struct PageTile { long long row[2]; bool ok[2]; };
+__device__ __forceinline__ PageTile lg_pa_tile(const PageAttn &a, const int32_t *table, int t0, long long head) {
+    PageTile p;
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int t = t0 + 16 * h, b = t >> a.g.shift;
+        const int page = b < a.max_blocks ? table[b] : -1;
+        p.ok[h] = page >= 0 && page < a.g.n_pages;
+        p.row[h] = (p.ok[h] ? page : 0) * a.g.page_stride + (t & ((1 << a.g.shift) - 1)) * a.g.row_stride + head;
+    }
+    return p;
+}
+
+// Two wavefronts on a SIMD at heads of up to 256: registers for both have to be asked for
+constexpr int lg_pa_per_simd(int hd) { return hd == 512 ? 1 : hd == 256 ? 2 : hd == 128 ? 3 : 4; }
 template <int HD>
-__global__ __launch_bounds__(LG_PA_WAVES * 64) void lg_k_page_attn(PageAttn a) {
+__global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_page_attn(PageAttn a) {
+    constexpr bool AHEAD = HD <= 256;               // a tile's values and the next one's keys are on their way while it is worked on; at 512 the registers do not hold both
     constexpr int KS = HD / 32;                     // score steps
     constexpr int DL = HD >= 128 ? 8 : HD / 16;     // dimensions of a value load
     constexpr int CH = HD / (16 * DL);              // value loads of a key row
     constexpr int NT = HD / 16;                     // output tiles
     __shared__ float s_m[LG_PA_WAVES][8], s_l[LG_PA_WAVES][8];
-    __shared__ float s_o[LG_PA_WAVES][8][HD];
-    const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
+    __shared__ __align__(16) union { lg_h8 q[KS][64]; float o[LG_PA_WAVES][8][HD]; } s;
+    // (all first splits, then all second ones: short sequences have only those, and with a sequence's splits side by side 8 of them would put every first one on
+    // the same XCD: 61 sequences of up to 8192 keys 80 -> 120 us)
+    const int split = blockIdx.x / a.units, unit = blockIdx.x % a.units;
     const int seq = unit / a.nkv, kvh = unit % a.nkv, G = a.H / a.nkv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
@@ -218,17 +237,35 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64) void lg_k_page_attn(PageAttn a) {
     const int n_split = lg_pa_splits(a, lo, len);
     if (split >= n_split && !(a.splits == 1)) return;
     const int first = (lo & ~(LG_PA_TILE - 1)) + split * a.chunk, end = len < first + a.chunk ? len : first + a.chunk;
+    const int32_t *table = a.table + (long long)seq * a.max_blocks;
+    constexpr int STEP = LG_PA_WAVES * LG_PA_TILE;
+    int t0 = first + wave * LG_PA_TILE;
 
-    // queries: operand B of the scores, column c = query head c % 8, high part for c < 8
-    lg_h8 qf[KS];
-    float qs = 0;                                   // factor of the raw scores, in powers of two (base 2 exponent of the softmax)
+    lg_h8 kf[2][KS];
+    PageTile now{}, next{};
+    auto load_keys = [&](const PageTile &p) {
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint16_t *kp = a.g.k + p.row[h] + c * a.g.row_stride + g * 8;
+            #pragma unroll
+            for (int i = 0; i < KS; ++i) kf[h][i] = *(const lg_h8 *)(kp + i * 32);
+        }
+    };
+    if (t0 < end) {
+        now = lg_pa_tile(a, table, t0, kvh * HD);
+        if constexpr (AHEAD) load_keys(now);
+        if (t0 + STEP < end) next = lg_pa_tile(a, table, t0 + STEP, kvh * HD);
+    }
+
+    // queries: operand B of the scores, column c = query head c % 8, high part for c < 8; a quarter of the steps from each wavefront
+    float qs;                                       // factor of the raw scores: base-2 exponents
     {
         const int h = c & 7;
-        const float *q = a.q + seq * a.q_stride + (long long)(kvh * G + (h < G ? h : 0)) * HD;
+        const float *q = a.q + seq * a.q_stride + (long long)(kvh * G + (h < G ? h : 0)) * HD + g * 8;
         float top = 0;
         #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const float4 x = *(const float4 *)(q + s * 32 + g * 8), y = *(const float4 *)(q + s * 32 + g * 8 + 4);
+        for (int i = 0; i < KS; ++i) {
+            const float4 x = *(const float4 *)(q + i * 32), y = *(const float4 *)(q + i * 32 + 4);
             top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
         }
         top = fmaxf(top, __shfl_xor(top, 16));
@@ -236,51 +273,67 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64) void lg_k_page_attn(PageAttn a) {
         int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;       // top * 2^-e in [2^14, 2^15)
         if (e < -100) e = -100;                                     // (zero and tiny rows; 2^-e stays a float)
         const float up = __uint_as_float((unsigned)(127 - e) << 23);
-        #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const float4 x = *(const float4 *)(q + s * 32 + g * 8), y = *(const float4 *)(q + s * 32 + g * 8 + 4);
+        for (int i = wave; i < KS; i += LG_PA_WAVES) {
+            const float4 x = *(const float4 *)(q + i * 32), y = *(const float4 *)(q + i * 32 + 4);
             const float v[8] = { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w };
+            lg_h8 part;
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float z = v[j] * up;
                 const _Float16 hi = (_Float16)z;
-                qf[s][j] = c < 8 ? hi : (_Float16)(z - (float)hi);
+                part[j] = c < 8 ? hi : (_Float16)(z - (float)hi);
             }
+            s.q[i][lane] = part;
         }
         qs = a.scale * 1.44269504088896341f * __uint_as_float((unsigned)(127 + e) << 23);
     }
+    __syncthreads();
     lg_f4 acc[NT];
     #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i] = (lg_f4){ 0, 0, 0, 0 };
     float m = -INFINITY, l = 0;                     // of query row c; l of this lane's keys alone
 
-    const int32_t *table = a.table + (long long)seq * a.max_blocks;
-    const int mask = (1 << a.g.shift) - 1;
-    for (int t0 = first + wave * LG_PA_TILE; t0 < end; t0 += LG_PA_WAVES * LG_PA_TILE) {
-        bool ok[2]; long long row[2];               // of the half tiles
-        #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int t = t0 + 16 * h, b = t >> a.g.shift;
-            const int page = b < a.max_blocks ? table[b] : -1;
-            ok[h] = page >= 0 && page < a.g.n_pages;
-            row[h] = (ok[h] ? page : 0) * a.g.page_stride + (t & mask) * a.g.row_stride + kvh * HD;
-        }
-        lg_f4 s[2] = { { 0, 0, 0, 0 }, { 0, 0, 0, 0 } };
-        #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint16_t *kp = a.g.k + row[h] + c * a.g.row_stride + g * 8;
+    // One tile: its values are requested before its scores are made, the next tile's keys before its values are used
+    for (; t0 < end; t0 += STEP) {
+        uint32_t w[CH][8][DL / 2];
+        auto load_values = [&](const PageTile &p) {
             #pragma unroll
-            for (int i = 0; i < KS; ++i) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const lg_h8 *)(kp + i * 32), qf[i], s[h], 0, 0, 0);
+            for (int ch = 0; ch < CH; ++ch)
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint16_t *vp = a.g.v + p.row[j >> 2] + (4 * g + (j & 3)) * a.g.row_stride + ch * 128 + c * DL;
+                    if constexpr (DL == 8) { const uint4 u = *(const uint4 *)vp; w[ch][j][0] = u.x; w[ch][j][1] = u.y; w[ch][j][2] = u.z; w[ch][j][3] = u.w; }
+                    else { const uint2 u = *(const uint2 *)vp; w[ch][j][0] = u.x; w[ch][j][1] = u.y; }
+                }
+        };
+        const PageTile here = now;
+        if constexpr (AHEAD) load_values(here);
+        else load_keys(here);
+        __builtin_amdgcn_sched_barrier(0);
+        lg_f4 sc[2] = { { 0, 0, 0, 0 }, { 0, 0, 0, 0 } };
+        #pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            const lg_h8 q = s.q[i][lane];
+            sc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][i], q, sc[0], 0, 0, 0);
+            sc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][i], q, sc[1], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!AHEAD) load_values(here);
+        if (t0 + STEP < end) {
+            now = next;
+            if constexpr (AHEAD) load_keys(now);
+            if (t0 + 2 * STEP < end) next = lg_pa_tile(a, table, t0 + 2 * STEP, kvh * HD);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         // base-2 exponents; rows c and c + 8 hold the two parts of a query's score
         float x[2][4], top = -INFINITY;
         #pragma unroll
         for (int h = 0; h < 2; ++h)
             #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float both = s[h][r] + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(s[h][r]), 0x128, 0xF, 0xF, true));   // row_ror:8
+                const float both = sc[h][r] + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(sc[h][r]), 0x128, 0xF, 0xF, true));   // row_ror:8
                 const int t = t0 + 16 * h + 4 * g + r;
-                x[h][r] = ok[h] && t >= lo && t < end ? both * qs : -INFINITY;
+                x[h][r] = here.ok[h] && t >= lo && t < end ? both * qs : -INFINITY;
                 top = fmaxf(top, x[h][r]);
             }
         top = fmaxf(top, __shfl_xor(top, 16));
@@ -307,57 +360,54 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64) void lg_k_page_attn(PageAttn a) {
                 const _Float16 hi = (_Float16)p;
                 pf[4 * h + r] = c < 8 ? hi : (_Float16)(p - (float)hi);
             }
-        // values; a masked key's may be anything (0 * inf is not 0): zeros in its place
-        const bool whole = t0 >= lo && t0 + LG_PA_TILE <= end && ok[0] && ok[1];
-        #pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-            uint32_t w[8][DL / 2];
+        // a masked key's values may be anything (0 * inf is not 0): zeros in their place
+        if (!(t0 >= lo && t0 + LG_PA_TILE <= end && here.ok[0] && here.ok[1])) {
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int kk = 4 * g + (j & 3), h = j >> 2;
-                const uint16_t *vp = a.g.v + row[h] + kk * a.g.row_stride + ch * 128 + c * DL;
-                if constexpr (DL == 8) { const uint4 u = *(const uint4 *)vp; w[j][0] = u.x; w[j][1] = u.y; w[j][2] = u.z; w[j][3] = u.w; }
-                else { const uint2 u = *(const uint2 *)vp; w[j][0] = u.x; w[j][1] = u.y; }
-                if (!whole) {
-                    const int t = t0 + 16 * h + kk;
-                    if (!(ok[h] && t >= lo && t < end)) {
+                const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                if (!(here.ok[j >> 2] && t >= lo && t < end)) {
+                    #pragma unroll
+                    for (int ch = 0; ch < CH; ++ch)
                         #pragma unroll
-                        for (int i = 0; i < DL / 2; ++i) w[j][i] = 0;
-                    }
+                        for (int i = 0; i < DL / 2; ++i) w[ch][j][i] = 0;
                 }
             }
+        }
+        #pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
             #pragma unroll
             for (int i = 0; i < DL; ++i) {
                 union { uint32_t u[4]; lg_h8 h; } b;
                 #pragma unroll
-                for (int k2 = 0; k2 < 4; ++k2) b.u[k2] = __builtin_amdgcn_perm(w[2 * k2 + 1][i >> 1], w[2 * k2][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
+                for (int k2 = 0; k2 < 4; ++k2) b.u[k2] = __builtin_amdgcn_perm(w[ch][2 * k2 + 1][i >> 1], w[ch][2 * k2][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
                 acc[ch * DL + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, b.h, acc[ch * DL + i], 0, 0, 0);
             }
-        }
     }
     // the wavefronts' parts: sums over the quarters of a tile, then the four together
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (lane < 8) { s_m[wave][lane] = m; s_l[wave][lane] = l; }
+    __syncthreads();                                // (the queries' last reader)
+    // the two parts of a probability: rows 4 g + r of the lower and the upper half of the lanes.  One exchange joins two registers' halves
     #pragma unroll
     for (int i = 0; i < NT; ++i)
         #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float both = acc[i][r] + __shfl_xor(acc[i][r], 32);
-            if (lane < 32) s_o[wave][4 * g + r][(i / DL) * 128 + c * DL + i % DL] = both;
+        for (int r = 0; r < 4; r += 2) {
+            const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][r]), __float_as_uint(acc[i][r + 1]), false, false);
+            s.o[wave][4 * (g & 1) + r + (g >> 1)][(i / DL) * 128 + c * DL + i % DL] = __uint_as_float(u[0]) + __uint_as_float(u[1]);
         }
     __syncthreads();
     for (int id = threadIdx.x; id < G * HD; id += LG_PA_WAVES * 64) {
         const int h = id / HD, d = id % HD;
         float M = -INFINITY, L = 0, o = 0;
         #pragma unroll
-        for (int w = 0; w < LG_PA_WAVES; ++w) M = fmaxf(M, s_m[w][h]);
+        for (int v = 0; v < LG_PA_WAVES; ++v) M = fmaxf(M, s_m[v][h]);
         #pragma unroll
-        for (int w = 0; w < LG_PA_WAVES; ++w) {
-            if (s_l[w][h] == 0.0f) continue;                        // no key; a score of NaN leaves its mark in the sum
-            const float f = __builtin_amdgcn_exp2f(s_m[w][h] - M);
-            L += f * s_l[w][h];
-            o += f * s_o[w][h][d];
+        for (int v = 0; v < LG_PA_WAVES; ++v) {
+            if (s_l[v][h] == 0.0f) continue;                        // no key; a score of NaN leaves its mark in the sum
+            const float f = __builtin_amdgcn_exp2f(s_m[v][h] - M);
+            L += f * s_l[v][h];
+            o += f * s.o[v][h][d];
         }
         const int head = kvh * G + h;
         if (a.splits == 1) a.out[seq * a.out_stride + (long long)head * HD + d] = L == 0.0f ? 0.0f : o / L;
@@ -369,22 +419,57 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64) void lg_k_page_attn(PageAttn a) {
     }
 }
 
-// The splits of a sequence, joined: a workgroup per (sequence, head), a thread per dimension.
+// The splits of a sequence, joined: a workgroup per (sequence, head).  A split's factor is computed once, by one thread; then the wavefronts take splits in
+// turn, a lane HD / 64 dimensions, and their sums are added in order.
+#define LG_PM_WAVES 4
 template <int HD>
-__global__ __launch_bounds__(HD) void lg_k_page_merge(PageAttn a) {
-    const int unit = blockIdx.x, seq = unit / a.H, head = unit % a.H, d = threadIdx.x;
+__global__ __launch_bounds__(LG_PM_WAVES * 64) void lg_k_page_merge(PageAttn a) {
+    constexpr int NT = LG_PM_WAVES * 64, D = HD / 64;
+    __shared__ float s_f[NT], s_w[LG_PM_WAVES], s_o[LG_PM_WAVES][HD];
+    const int head = blockIdx.x, seq = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     int lo, len;
     lg_pa_range(a, seq, lo, len);
     const int n = lg_pa_splits(a, lo, len);
-    const long long at = (long long)unit * a.splits;
-    float M = -INFINITY, L = 0, o = 0;
-    for (int s = 0; s < n; ++s) M = fmaxf(M, a.pm[at + s]);
-    for (int s = 0; s < n; ++s) {
-        const float ls = a.pl[at + s];
-        if (ls == 0.0f) continue;                               // no key: its pages are left out
-        const float f = __builtin_amdgcn_exp2f(a.pm[at + s] - M);
-        L += f * ls;
-        o += f * a.pacc[(at + s) * HD + d];
+    const long long at = ((long long)seq * a.H + head) * a.splits;
+    float M = -INFINITY;
+    for (int i = t; i < n; i += NT) M = fmaxf(M, a.pm[at + i]);
+    for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
+    if (lane == 0) s_w[wave] = M;
+    __syncthreads();
+    #pragma unroll
+    for (int v = 0; v < LG_PM_WAVES; ++v) M = fmaxf(M, s_w[v]);
+    float L = 0, o[D];
+    #pragma unroll
+    for (int i = 0; i < D; ++i) o[i] = 0;
+    for (int base = 0; base < n; base += NT) {
+        const int i = base + t;
+        const float ls = i < n ? a.pl[at + i] : 0.0f, f = ls == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(a.pm[at + i] - M);     // (0: no key, its pages are left out)
+        L += ls == 0.0f ? 0.0f : f * ls;
+        __syncthreads();
+        s_f[t] = f;
+        __syncthreads();
+        const int m = n - base < NT ? n - base : NT;
+        #pragma unroll 4
+        for (int k = wave; k < m; k += LG_PM_WAVES) {
+            const float *p = a.pacc + (at + base + k) * HD + lane * D;
+            const float fk = s_f[k];
+            #pragma unroll
+            for (int d = 0; d < D; ++d) o[d] += fk * p[d];
+        }
     }
-    a.out[seq * a.out_stride + (long long)head * HD + d] = L == 0.0f ? 0.0f : o / L;
+    for (int x = 1; x < 64; x <<= 1) L += __shfl_xor(L, x);
+    __syncthreads();
+    if (lane == 0) s_w[wave] = L;
+    #pragma unroll
+    for (int d = 0; d < D; ++d) s_o[wave][lane * D + d] = o[d];
+    __syncthreads();
+    L = 0;
+    #pragma unroll
+    for (int v = 0; v < LG_PM_WAVES; ++v) L += s_w[v];
+    for (int d = t; d < HD; d += NT) {
+        float x = 0;
+        #pragma unroll
+        for (int v = 0; v < LG_PM_WAVES; ++v) x += s_o[v][d];
+        a.out[seq * a.out_stride + (long long)head * HD + d] = L == 0.0f ? 0.0f : x / L;
+    }
 }

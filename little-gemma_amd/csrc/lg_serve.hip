@@ -84,7 +84,7 @@ extern "C" int lg_hip_paged_write(const struct lg_hip_pages *p, const float *d_k
 // Keys of a split: as many as give the chip about four workgroups per CU were every sequence at its longest, 128 (a tile for each wavefront) to 1024.
 struct AttnSplit { int chunk, splits; };
 static AttnSplit split_of(int n_seq, int n_head_kv, int max_len, int window) {
-    const int64_t span = (window > 0 && window < max_len ? window : max_len) + LG_PA_TILE - 1;
+    const int64_t span = window > 0 && window < max_len ? window + LG_PA_TILE - 1 : max_len > 1 ? max_len : 1;     // (a window need not start with a tile)
     int64_t chunk = span * n_seq * n_head_kv / 1024;
     chunk = (chunk + 127) / 128 * 128;
     chunk = chunk < 128 ? 128 : chunk > 1024 ? 1024 : chunk;
@@ -104,8 +104,8 @@ extern "C" size_t lg_hip_paged_attention_workspace(int n_seq, int n_head, int n_
 
 template <int HD>
 static void launch_attn(const PageAttn &a, int n_seq, hipStream_t st) {
-    hipLaunchKernelGGL(lg_k_page_attn<HD>, dim3((unsigned)((int64_t)n_seq * a.nkv * a.splits)), dim3(LG_PA_WAVES * 64), 0, st, a);
-    if (a.splits > 1) hipLaunchKernelGGL(lg_k_page_merge<HD>, dim3((unsigned)((int64_t)n_seq * a.H)), dim3(HD), 0, st, a);
+    hipLaunchKernelGGL(lg_k_page_attn<HD>, dim3((unsigned)((int64_t)a.units * a.splits)), dim3(LG_PA_WAVES * 64), 0, st, a);
+    if (a.splits > 1) hipLaunchKernelGGL(lg_k_page_merge<HD>, dim3(a.H, n_seq), dim3(LG_PM_WAVES * 64), 0, st, a);
 }
 
 extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float *d_q, int64_t q_stride, int n_seq, int n_head, const int32_t *d_table,
@@ -125,14 +125,14 @@ extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float 
     if (q_stride < qd || q_stride % 4 || !aligned16(d_q)) return lg_fail(-2, "paged_attention: query rows of %lld values, %lld apart (aligned to 16 bytes)", (long long)qd, (long long)q_stride);
     if (out_stride < qd || ((uintptr_t)d_out & 3)) return lg_fail(-2, "paged_attention: output rows of %lld values, %lld apart", (long long)qd, (long long)out_stride);
     const AttnSplit s = split_of(n_seq, p->n_head_kv, max_len, window);
-    if ((int64_t)n_seq * n_head * s.splits > INT32_MAX / 2) return lg_fail(-2, "paged_attention: %d sequences of %d splits in one call", n_seq, s.splits);
+    if (n_seq > 65535 || (int64_t)n_seq * p->n_head_kv * s.splits > INT32_MAX) return lg_fail(-2, "paged_attention: %d sequences of %d key heads in %d splits in one call", n_seq, p->n_head_kv, s.splits);
     const size_t need = lg_hip_paged_attention_workspace(n_seq, n_head, p->n_head_kv, hd, max_len, window);
     if (need && (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)))
         return lg_fail(-2, "paged_attention: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
     const size_t part = up256((size_t)n_seq * n_head * s.splits * 4);
     float *const w = (float *)d_work;
     const PageAttn a{ g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, w, need ? (float *)((char *)d_work + part) : nullptr,
-                      need ? (float *)((char *)d_work + 2 * part) : nullptr, scale, n_head, p->n_head_kv, max_blocks, max_len, window, s.chunk, s.splits };
+                      need ? (float *)((char *)d_work + 2 * part) : nullptr, scale, n_head, p->n_head_kv, n_seq * p->n_head_kv, max_blocks, max_len, window, s.chunk, s.splits };
     hipStream_t st = (hipStream_t)stream;
     switch (hd) {
         case 64:  launch_attn<64>(a, n_seq, st); break;
