@@ -175,6 +175,8 @@ __global__ __launch_bounds__(256) void lg_k_page_write(PageGeo g, const float *k
 // K and V never pass through LDS.  Maximum and sum run in f32; the sum is of the unsplit probabilities.
 #define LG_PA_WAVES 4
 #define LG_PA_TILE  32
+// A barrier for what went through LDS: loads from memory stay on their way, which the barrier of __syncthreads waits for as well
+__device__ __forceinline__ void lg_barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 typedef _Float16 lg_h8 __attribute__((ext_vector_type(8)));
 typedef float lg_f4 __attribute__((ext_vector_type(4)));
 
@@ -201,16 +203,24 @@ __device__ __forceinline__ int lg_pa_splits(const PageAttn &a, int lo, int len) 
     return len > lo ? (len - first + a.chunk - 1) / a.chunk : 0;
 }
 
-// Where the rows of a tile's two halves lie: the page's first value, or page 0's where there is no such page
+// The pages of a tile's two halves, and where their rows lie: page 0's first value where there is no such page
 struct PageTile { long long row[2]; bool ok[2]; };
-__device__ __forceinline__ PageTile lg_pa_tile(const PageAttn &a, const int32_t *table, int t0, long long head) {
+struct PageIds { int id[2]; };
+__device__ __forceinline__ PageIds lg_pa_ids(const PageAttn &a, const int32_t *table, int t0) {
+    PageIds p;
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int b = (t0 + 16 * h) >> a.g.shift, id = table[b < a.max_blocks ? b : a.max_blocks - 1];
+        p.id[h] = b < a.max_blocks ? id : -1;
+    }
+    return p;
+}
+__device__ __forceinline__ PageTile lg_pa_tile(const PageAttn &a, const PageIds &ids, int t0, int head) {
     PageTile p;
     #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int t = t0 + 16 * h, b = t >> a.g.shift;
-        const int page = b < a.max_blocks ? table[b] : -1;
-        p.ok[h] = page >= 0 && page < a.g.n_pages;
-        p.row[h] = (p.ok[h] ? page : 0) * a.g.page_stride + (t & ((1 << a.g.shift) - 1)) * a.g.row_stride + head;
+        p.ok[h] = ids.id[h] >= 0 && ids.id[h] < a.g.n_pages;
+        p.row[h] = (p.ok[h] ? ids.id[h] : 0) * a.g.page_stride + ((t0 + 16 * h) & ((1 << a.g.shift) - 1)) * a.g.row_stride + head;
     }
     return p;
 }
@@ -232,17 +242,28 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     const int seq = unit / a.nkv, kvh = unit % a.nkv, G = a.H / a.nkv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
+    constexpr int STEP = LG_PA_WAVES * LG_PA_TILE;
+    const int32_t *table = a.table + (long long)seq * a.max_blocks;
+    // Queries are asked for first: what is asked for later arrives later, and behind the keys they would hold the first scores up.  Without a window the
+    // first tile's place does not depend on the length either, and its pages' ids come together with that.
+    float4 qv[KS][2];
+    {
+        const int h = c & 7;
+        const float *q = a.q + seq * a.q_stride + (long long)(kvh * G + (h < G ? h : 0)) * HD + g * 8;
+        #pragma unroll
+        for (int i = 0; i < KS; ++i) { qv[i][0] = *(const float4 *)(q + i * 32); qv[i][1] = *(const float4 *)(q + i * 32 + 4); }
+    }
+    PageIds ids = lg_pa_ids(a, table, split * a.chunk + wave * LG_PA_TILE);
     int lo, len;
     lg_pa_range(a, seq, lo, len);
     const int n_split = lg_pa_splits(a, lo, len);
     if (split >= n_split && !(a.splits == 1)) return;
     const int first = (lo & ~(LG_PA_TILE - 1)) + split * a.chunk, end = len < first + a.chunk ? len : first + a.chunk;
-    const int32_t *table = a.table + (long long)seq * a.max_blocks;
-    constexpr int STEP = LG_PA_WAVES * LG_PA_TILE;
     int t0 = first + wave * LG_PA_TILE;
+    if (lo) ids = lg_pa_ids(a, table, t0);
 
     lg_h8 kf[2][KS];
-    PageTile now{}, next{};
+    PageTile now = lg_pa_tile(a, ids, t0, kvh * HD);
     auto load_keys = [&](const PageTile &p) {
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -251,31 +272,30 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
             for (int i = 0; i < KS; ++i) kf[h][i] = *(const lg_h8 *)(kp + i * 32);
         }
     };
+    __builtin_amdgcn_sched_barrier(0);
     if (t0 < end) {
-        now = lg_pa_tile(a, table, t0, kvh * HD);
         if constexpr (AHEAD) load_keys(now);
-        if (t0 + STEP < end) next = lg_pa_tile(a, table, t0 + STEP, kvh * HD);
+        if (t0 + STEP < end) ids = lg_pa_ids(a, table, t0 + STEP);
     }
+    __builtin_amdgcn_sched_barrier(0);
 
     // queries: operand B of the scores, column c = query head c % 8, high part for c < 8; a quarter of the steps from each wavefront
     float qs;                                       // factor of the raw scores: base-2 exponents
     {
-        const int h = c & 7;
-        const float *q = a.q + seq * a.q_stride + (long long)(kvh * G + (h < G ? h : 0)) * HD + g * 8;
         float top = 0;
         #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            const float4 x = *(const float4 *)(q + i * 32), y = *(const float4 *)(q + i * 32 + 4);
-            top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
-        }
+        for (int i = 0; i < KS; ++i)
+            #pragma unroll
+            for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fmaxf(fabsf(qv[i][j].x), fabsf(qv[i][j].y)), fmaxf(fabsf(qv[i][j].z), fabsf(qv[i][j].w))));
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;       // top * 2^-e in [2^14, 2^15)
         if (e < -100) e = -100;                                     // (zero and tiny rows; 2^-e stays a float)
         const float up = __uint_as_float((unsigned)(127 - e) << 23);
-        for (int i = wave; i < KS; i += LG_PA_WAVES) {
-            const float4 x = *(const float4 *)(q + i * 32), y = *(const float4 *)(q + i * 32 + 4);
-            const float v[8] = { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w };
+        #pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            if (i % LG_PA_WAVES != wave) continue;
+            const float v[8] = { qv[i][0].x, qv[i][0].y, qv[i][0].z, qv[i][0].w, qv[i][1].x, qv[i][1].y, qv[i][1].z, qv[i][1].w };
             lg_h8 part;
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -287,7 +307,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
         }
         qs = a.scale * 1.44269504088896341f * __uint_as_float((unsigned)(127 + e) << 23);
     }
-    __syncthreads();
+    lg_barrier_lds();
     lg_f4 acc[NT];
     #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i] = (lg_f4){ 0, 0, 0, 0 };
@@ -320,9 +340,9 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (!AHEAD) load_values(here);
         if (t0 + STEP < end) {
-            now = next;
+            now = lg_pa_tile(a, ids, t0 + STEP, kvh * HD);
             if constexpr (AHEAD) load_keys(now);
-            if (t0 + 2 * STEP < end) next = lg_pa_tile(a, table, t0 + 2 * STEP, kvh * HD);
+            if (t0 + 2 * STEP < end) ids = lg_pa_ids(a, table, t0 + 2 * STEP);
         }
         __builtin_amdgcn_sched_barrier(0);
         // base-2 exponents; rows c and c + 8 hold the two parts of a query's score
@@ -390,30 +410,43 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     __syncthreads();                                // (the queries' last reader)
     // the two parts of a probability: rows 4 g + r of the lower and the upper half of the lanes.  One exchange joins two registers' halves
     #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int ch = 0; ch < CH; ++ch)
         #pragma unroll
         for (int r = 0; r < 4; r += 2) {
-            const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][r]), __float_as_uint(acc[i][r + 1]), false, false);
-            s.o[wave][4 * (g & 1) + r + (g >> 1)][(i / DL) * 128 + c * DL + i % DL] = __uint_as_float(u[0]) + __uint_as_float(u[1]);
+            float o[DL];
+            #pragma unroll
+            for (int i = 0; i < DL; ++i) {
+                const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[ch * DL + i][r]), __float_as_uint(acc[ch * DL + i][r + 1]), false, false);
+                o[i] = __uint_as_float(u[0]) + __uint_as_float(u[1]);
+            }
+            #pragma unroll
+            for (int i = 0; i < DL; i += 4) *(float4 *)&s.o[wave][4 * (g & 1) + r + (g >> 1)][ch * 128 + c * DL + i] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
     __syncthreads();
-    for (int id = threadIdx.x; id < G * HD; id += LG_PA_WAVES * 64) {
-        const int h = id / HD, d = id % HD;
-        float M = -INFINITY, L = 0, o = 0;
+    for (int id = threadIdx.x; id < G * (HD / 4); id += LG_PA_WAVES * 64) {
+        const int h = id / (HD / 4), d = id % (HD / 4) * 4;
+        float M = -INFINITY, L = 0;
+        float4 o = make_float4(0, 0, 0, 0);
         #pragma unroll
         for (int v = 0; v < LG_PA_WAVES; ++v) M = fmaxf(M, s_m[v][h]);
         #pragma unroll
         for (int v = 0; v < LG_PA_WAVES; ++v) {
-            if (s_l[v][h] == 0.0f) continue;                        // no key; a score of NaN leaves its mark in the sum
+            const float lv = s_l[v][h];
+            if (lv == 0.0f) continue;                               // no key; a score of NaN leaves its mark in the sum
             const float f = __builtin_amdgcn_exp2f(s_m[v][h] - M);
-            L += f * s_l[v][h];
-            o += f * s.o[v][h][d];
+            const float4 x = *(const float4 *)&s.o[v][h][d];
+            L += f * lv;
+            o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
         }
         const int head = kvh * G + h;
-        if (a.splits == 1) a.out[seq * a.out_stride + (long long)head * HD + d] = L == 0.0f ? 0.0f : o / L;
-        else {
+        if (a.splits == 1) {
+            float *const p = a.out + seq * a.out_stride + (long long)head * HD + d;       // (rows may start anywhere)
+            const float x[4] = { o.x, o.y, o.z, o.w };
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = L == 0.0f ? 0.0f : x[i] / L;
+        } else {
             const long long at = ((long long)seq * a.H + head) * a.splits + split;
-            a.pacc[at * HD + d] = o;
+            *(float4 *)(a.pacc + at * HD + d) = o;
             if (d == 0) { a.pm[at] = M; a.pl[at] = L; }
         }
     }
@@ -431,31 +464,38 @@ __global__ __launch_bounds__(LG_PM_WAVES * 64) void lg_k_page_merge(PageAttn a) 
     lg_pa_range(a, seq, lo, len);
     const int n = lg_pa_splits(a, lo, len);
     const long long at = ((long long)seq * a.H + head) * a.splits;
-    float M = -INFINITY;
-    for (int i = t; i < n; i += NT) M = fmaxf(M, a.pm[at + i]);
+    // what the first NT splits need is asked for at once: a wavefront's first four sums with the maxima
+    typedef float vec __attribute__((ext_vector_type(D)));
+    constexpr int FIRST = 4;
+    auto sums = [&](int k) { return *(const vec *)(a.pacc + (at + k) * HD + lane * D); };
+    vec ahead[FIRST];
+    const float m0 = t < n ? a.pm[at + t] : -INFINITY, l0 = t < n ? a.pl[at + t] : 0.0f;
+    #pragma unroll
+    for (int j = 0; j < FIRST; ++j) if (wave + j * LG_PM_WAVES < n) ahead[j] = sums(wave + j * LG_PM_WAVES);
+    float M = m0;
+    for (int i = t + NT; i < n; i += NT) M = fmaxf(M, a.pm[at + i]);
     for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
     if (lane == 0) s_w[wave] = M;
     __syncthreads();
     #pragma unroll
     for (int v = 0; v < LG_PM_WAVES; ++v) M = fmaxf(M, s_w[v]);
-    float L = 0, o[D];
-    #pragma unroll
-    for (int i = 0; i < D; ++i) o[i] = 0;
+    float L = 0;
+    vec o = 0;
     for (int base = 0; base < n; base += NT) {
         const int i = base + t;
-        const float ls = i < n ? a.pl[at + i] : 0.0f, f = ls == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(a.pm[at + i] - M);     // (0: no key, its pages are left out)
+        const float mi = base ? i < n ? a.pm[at + i] : 0.0f : m0, ls = base ? i < n ? a.pl[at + i] : 0.0f : l0;
+        const float f = ls == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mi - M);                 // (0: no key, its pages are left out)
         L += ls == 0.0f ? 0.0f : f * ls;
         __syncthreads();
         s_f[t] = f;
         __syncthreads();
         const int m = n - base < NT ? n - base : NT;
-        #pragma unroll 4
-        for (int k = wave; k < m; k += LG_PM_WAVES) {
-            const float *p = a.pacc + (at + base + k) * HD + lane * D;
-            const float fk = s_f[k];
+        int k = wave;
+        if (!base)
             #pragma unroll
-            for (int d = 0; d < D; ++d) o[d] += fk * p[d];
-        }
+            for (int j = 0; j < FIRST; ++j, k += LG_PM_WAVES) if (k < m) o += s_f[k] * ahead[j];
+        #pragma unroll 4
+        for (; k < m; k += LG_PM_WAVES) o += s_f[k] * sums(base + k);
     }
     for (int x = 1; x < 64; x <<= 1) L += __shfl_xor(L, x);
     __syncthreads();
