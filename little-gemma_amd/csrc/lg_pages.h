@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
+#include <type_traits>
 
 #define LG_PLAN_SEQS 4096           // sequences of a plan: their running sums lie in LDS
 #define LG_PLAN_WG   1024
@@ -175,6 +176,7 @@ __global__ __launch_bounds__(256) void lg_k_page_write(PageGeo g, const float *k
 // K and V never pass through LDS.  Maximum and sum run in f32; the sum is of the unsplit probabilities.
 #define LG_PA_WAVES 4
 #define LG_PA_TILE  32
+#define LG_PA_CHUNK 2048            // keys of a split at most: their page ids lie in LDS
 // A barrier for what went through LDS: loads from memory stay on their way, which the barrier of __syncthreads waits for as well
 __device__ __forceinline__ void lg_barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 typedef _Float16 lg_h8 __attribute__((ext_vector_type(8)));
@@ -236,6 +238,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     constexpr int NT = HD / 16;                     // output tiles
     __shared__ float s_m[LG_PA_WAVES][8], s_l[LG_PA_WAVES][8];
     __shared__ __align__(16) union { lg_h8 q[KS][64]; float o[LG_PA_WAVES][8][HD]; } s;
+    __shared__ int32_t s_ids[LG_PA_CHUNK / 16 + 1];
     // (all first splits, then all second ones: short sequences have only those, and with a sequence's splits side by side 8 of them would put every first one on
     // the same XCD: 61 sequences of up to 8192 keys 80 -> 120 us)
     const int split = blockIdx.x / a.units, unit = blockIdx.x % a.units;
@@ -261,9 +264,24 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     const int first = (lo & ~(LG_PA_TILE - 1)) + split * a.chunk, end = len < first + a.chunk ? len : first + a.chunk;
     int t0 = first + wave * LG_PA_TILE;
     if (lo) ids = lg_pa_ids(a, table, t0);
+    // the later tiles' ids through LDS: a load of them inside the loop would be waited for together with the keys that are on their way
+    const int b0 = first >> a.g.shift;
+    static_assert(LG_PA_CHUNK / 16 + 1 <= LG_PA_WAVES * 64, "an id for each thread");
+    const bool has_id = (int)threadIdx.x <= ((end - 1) >> a.g.shift) - b0;
+    const int my_id = has_id && b0 + (int)threadIdx.x < a.max_blocks ? table[b0 + threadIdx.x] : -1;
+    auto tile_at = [&](int t) {
+        PageIds p;
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int i = ((t + 16 * h < end ? t + 16 * h : t) >> a.g.shift) - b0;             // (a half behind the end is masked)
+            p.id[h] = __builtin_amdgcn_readfirstlane(s_ids[i]);
+        }
+        return lg_pa_tile(a, p, t, kvh * HD);
+    };
 
     lg_h8 kf[2][KS];
     PageTile now = lg_pa_tile(a, ids, t0, kvh * HD);
+    if (t0 >= end) now.row[0] = now.row[1] = kvh * HD;          // (no tile: page 0's rows, so that the loads need no branch, after which everything would be waited for)
     auto load_keys = [&](const PageTile &p) {
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -273,11 +291,9 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
         }
     };
     __builtin_amdgcn_sched_barrier(0);
-    if (t0 < end) {
-        if constexpr (AHEAD) load_keys(now);
-        if (t0 + STEP < end) ids = lg_pa_ids(a, table, t0 + STEP);
-    }
+    if constexpr (AHEAD) load_keys(now);
     __builtin_amdgcn_sched_barrier(0);
+    if (has_id) s_ids[threadIdx.x] = my_id;
 
     // queries: operand B of the scores, column c = query head c % 8, high part for c < 8; a quarter of the steps from each wavefront
     float qs;                                       // factor of the raw scores: base-2 exponents
@@ -314,7 +330,8 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     float m = -INFINITY, l = 0;                     // of query row c; l of this lane's keys alone
 
     // One tile: its values are requested before its scores are made, the next tile's keys before its values are used
-    for (; t0 < end; t0 += STEP) {
+    auto work = [&](auto more) {                    // more: a tile follows (a branch around its loads would have them waited for with this tile's)
+        constexpr bool MORE = decltype(more)::value;
         uint32_t w[CH][8][DL / 2];
         auto load_values = [&](const PageTile &p) {
             #pragma unroll
@@ -327,6 +344,8 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
                 }
         };
         const PageTile here = now;
+        PageTile coming = now;
+        if constexpr (MORE) coming = tile_at(t0 + STEP);
         if constexpr (AHEAD) load_values(here);
         else load_keys(here);
         __builtin_amdgcn_sched_barrier(0);
@@ -339,10 +358,9 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
         }
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (!AHEAD) load_values(here);
-        if (t0 + STEP < end) {
-            now = lg_pa_tile(a, ids, t0 + STEP, kvh * HD);
+        if constexpr (MORE) {
+            now = coming;
             if constexpr (AHEAD) load_keys(now);
-            if (t0 + 2 * STEP < end) ids = lg_pa_ids(a, table, t0 + 2 * STEP);
         }
         __builtin_amdgcn_sched_barrier(0);
         // base-2 exponents; rows c and c + 8 hold the two parts of a query's score
@@ -402,7 +420,9 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
                 for (int k2 = 0; k2 < 4; ++k2) b.u[k2] = __builtin_amdgcn_perm(w[ch][2 * k2 + 1][i >> 1], w[ch][2 * k2][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
                 acc[ch * DL + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, b.h, acc[ch * DL + i], 0, 0, 0);
             }
-    }
+    };
+    for (; t0 + STEP < end; t0 += STEP) work(std::true_type{});
+    if (t0 < end) work(std::false_type{});
     // the wavefronts' parts: sums over the quarters of a tile, then the four together
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
