@@ -8,6 +8,8 @@
 #include <stdint.h>
 #include <type_traits>
 
+#include "lg_block.h"
+
 #define LG_PLAN_SEQS 4096           // sequences of a plan: their running sums lie in LDS
 #define LG_PLAN_WG   1024
 
@@ -24,19 +26,6 @@ struct PlanArgs {
     int n_seq, shift, n_pages, max_blocks, n_slots;
 };
 
-// Inclusive sum over the workgroup of one value per thread; `part`: [waves] of LDS.  *total = the sum of all.
-template <typename T>
-__device__ __forceinline__ T lg_block_scan(T v, T *part, T *total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    for (int o = 1; o < 64; o <<= 1) { const T u = __shfl_up(v, o); if (lane >= o) v += u; }
-    __syncthreads();                                        // (part may still be read from a call before)
-    if (lane == 63) part[wave] = v;
-    __syncthreads();
-    T before = 0, all = 0;
-    for (int w = 0; w < waves; ++w) { const T p = part[w]; if (w < wave) before += p; all += p; }
-    *total = all;
-    return v + before;
-}
 // The sequence that entry e belongs to: sums[i] <= e < sums[i + 1]
 __device__ __forceinline__ int lg_owner(const int32_t *sums, int n, int e) {
     int lo = 0, hi = n;
@@ -51,7 +40,7 @@ __device__ __forceinline__ int lg_owner(const int32_t *sums, int n, int e) {
 // memory round trips, which a grid would lengthen by a launch per phase.
 __global__ __launch_bounds__(LG_PLAN_WG) void lg_k_plan(PlanArgs a) {
     __shared__ int32_t tok[LG_PLAN_SEQS + 1], need[LG_PLAN_SEQS + 1], freed[LG_PLAN_SEQS + 1];
-    __shared__ long long part[LG_PLAN_WG / 64];
+    __shared__ lg_u64 part[LG_PLAN_WG / 64];
     __shared__ int bad;
     const int t = threadIdx.x, P = 1 << a.shift, n = a.n_seq;
     const long long most = (long long)a.max_blocks << a.shift;
@@ -60,7 +49,7 @@ __global__ __launch_bounds__(LG_PLAN_WG) void lg_k_plan(PlanArgs a) {
     __syncthreads();
     auto blocks = [&](int len) { return (int)(((long long)len + P - 1) >> a.shift); };
     // running sums: sequences t * CH .. t * CH + CH - 1 are this thread's
-    long long v[3][CH], sum[3] = { 0, 0, 0 };
+    lg_u64 v[3][CH], sum[3] = { 0, 0, 0 };
     #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int i = t * CH + c;
@@ -71,11 +60,11 @@ __global__ __launch_bounds__(LG_PLAN_WG) void lg_k_plan(PlanArgs a) {
         #pragma unroll
         for (int k = 0; k < 3; ++k) sum[k] += v[k][c];
     }
-    long long all[3];
+    lg_u64 all[3];
     int32_t *const dst[3] = { tok, need, freed };
     #pragma unroll
     for (int k = 0; k < 3; ++k) {
-        long long run = lg_block_scan(sum[k], part, &all[k]) - sum[k];
+        lg_u64 run = lg_block_run<LG_PLAN_WG>(sum[k], part, &all[k]) - sum[k];
         #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int i = t * CH + c;
@@ -86,9 +75,9 @@ __global__ __launch_bounds__(LG_PLAN_WG) void lg_k_plan(PlanArgs a) {
     }
     const int nf = *a.n_free;
     if (t == 0) {
-        if (nf < 0 || nf > a.n_pages || all[2] + nf > a.n_pages) atomicOr(&bad, LG_PLAN_BAD_STACK);
+        if (nf < 0 || nf > a.n_pages || all[2] + nf > (lg_u64)a.n_pages) atomicOr(&bad, LG_PLAN_BAD_STACK);
         else if (all[1] > nf + all[2]) atomicOr(&bad, LG_PLAN_NO_PAGES);
-        if (all[0] > a.n_slots) atomicOr(&bad, LG_PLAN_NO_SLOTS);
+        if (all[0] > (lg_u64)a.n_slots) atomicOr(&bad, LG_PLAN_NO_SLOTS);
     }
     __syncthreads();
     int st = bad;
@@ -187,9 +176,9 @@ struct PageAttn {
     const float *q; long long q_stride;
     const int32_t *table, *len;
     float *out; long long out_stride;
-    float *pm, *pl, *pacc;              // [n_seq][H][splits], [..][hd]: partials of more than one split
+    float *pm, *pl, *pacc;              // [splits of all][H], [..][hd]: partials of sequences of more than one split
     float scale;
-    int H, nkv, units, max_blocks, max_len, window, chunk, splits;      // units: sequences x key heads
+    int H, nkv, n_seq, max_blocks, max_len, window, slots;       // slots: workgroups that the chip holds at a time
 };
 // The keys a sequence sees: [lo, len)
 __device__ __forceinline__ void lg_pa_range(const PageAttn &a, int seq, int &lo, int &len) {
@@ -200,11 +189,54 @@ __device__ __forceinline__ void lg_pa_range(const PageAttn &a, int seq, int &lo,
     if (len < 0) len = 0;
     lo = a.window > 0 && len > a.window ? len - a.window : 0;
 }
-__device__ __forceinline__ int lg_pa_splits(const PageAttn &a, int lo, int len) {       // of a sequence: those with keys
-    const int first = lo & ~(LG_PA_TILE - 1);
-    return len > lo ? (len - first + a.chunk - 1) / a.chunk : 0;
+__device__ __forceinline__ int lg_pa_tiles(const PageAttn &a, int seq) {
+    int lo, len;
+    lg_pa_range(a, seq, lo, len);
+    return (len + LG_PA_TILE - 1) / LG_PA_TILE - lo / LG_PA_TILE;
 }
-
+// How the call is cut: every workgroup works it out from the lengths.  A compute unit draws a fixed share of what memory gives (it keeps about 32 KB
+// of misses on their way), so the call takes as long as the unit with the most keys: splits of one size, chosen so that their number is what the
+// chip holds at a time, not splits of a fixed size that the lengths fill unevenly.
+// A sequence without keys has one split too: it writes the zeros.
+struct PageCut { int tiles; int seq, index, first, n; };       // tiles of a split; of split number `at`: its sequence, its place there, the number of the sequence's first, how many it has
+struct PageCutLds { uint32_t part[16]; PageCut c; };
+// `total` tiles of `some` sequences that have any: the full splits and one more of each sequence are to be a whole number of rounds of a.slots workgroups, as few as
+// leave half of them to the full ones
+__device__ __forceinline__ uint32_t lg_pa_split_tiles(const PageAttn &a, uint32_t total, uint32_t some) {
+    const uint32_t units = some * a.nkv, half = (uint32_t)a.slots / 2, rounds = units > half ? (units + half - 1) / half : 1, full = rounds * a.slots - units;
+    const lg_u64 tiles = ((lg_u64)total * a.nkv + full - 1) / full;
+    return tiles < 4 ? 4 : tiles > LG_PA_CHUNK / LG_PA_TILE ? LG_PA_CHUNK / LG_PA_TILE : (uint32_t)tiles;
+}
+__device__ __forceinline__ uint32_t lg_pa_splits(uint32_t of, uint32_t tiles) { const uint32_t x = (of + tiles - 1) / tiles; return x ? x : 1u; }
+template <int NT>
+__device__ __forceinline__ PageCut lg_pa_cut(const PageAttn &a, int at, int seq, PageCutLds &s) {      // seq >= 0: of that sequence instead
+    if (a.n_seq <= 64) {                                       // a lane for each, in every wavefront: no barrier
+        const int i = threadIdx.x & 63;
+        const uint32_t mine = i < a.n_seq ? lg_pa_tiles(a, i) : 0, some = (uint32_t)__popcll(__ballot(mine != 0));
+        const uint32_t tiles = lg_pa_split_tiles(a, lg_wave_total(mine), some), n = i < a.n_seq ? lg_pa_splits(mine, tiles) : 0, run = lg_wave_run(n) - n;
+        const lg_u64 it = __ballot(seq < 0 ? (uint32_t)at - run < n : i == seq);
+        if (!it) return { (int)tiles, -1, 0, 0, 0 };
+        const int lane = (int)__builtin_ctzll(it), first = (int)lg_lane(run, lane);
+        return { (int)tiles, lane, at - first, first, (int)lg_lane(n, lane) };
+    }
+    const int per = (a.n_seq + NT - 1) / NT, i0 = threadIdx.x * per;
+    uint32_t mine = 0, some = 0, all;
+    for (int i = i0; i < i0 + per && i < a.n_seq; ++i) { const uint32_t x = lg_pa_tiles(a, i); mine += x; some += x != 0; }
+    mine = lg_block_sum<NT>(mine, s.part);
+    some = lg_block_sum<NT>(some, s.part);
+    const uint32_t tiles = lg_pa_split_tiles(a, mine, some);
+    if (threadIdx.x == 0) s.c.seq = -1;
+    uint32_t n = 0;
+    for (int i = i0; i < i0 + per && i < a.n_seq; ++i) n += lg_pa_splits(lg_pa_tiles(a, i), tiles);
+    uint32_t run = lg_block_run<NT>(n, s.part, &all) - n;      // (its barriers: seq = -1 comes first)
+    for (int i = i0; i < i0 + per && i < a.n_seq; ++i) {
+        const uint32_t x = lg_pa_splits(lg_pa_tiles(a, i), tiles);
+        if (seq < 0 ? (uint32_t)at - run < x : i == seq) s.c = { (int)tiles, i, at - (int)run, (int)run, (int)x };
+        run += x;
+    }
+    __syncthreads();
+    return s.c;
+}
 // The pages of a tile's two halves, and where their rows lie: page 0's first value where there is no such page
 struct PageTile { long long row[2]; bool ok[2]; };
 struct PageIds { int id[2]; };
@@ -239,16 +271,16 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     __shared__ float s_m[LG_PA_WAVES][8], s_l[LG_PA_WAVES][8];
     __shared__ __align__(16) union { lg_h8 q[KS][64]; float o[LG_PA_WAVES][8][HD]; } s;
     __shared__ int32_t s_ids[LG_PA_CHUNK / 16 + 1];
-    // (all first splits, then all second ones: short sequences have only those, and with a sequence's splits side by side 8 of them would put every first one on
-    // the same XCD: 61 sequences of up to 8192 keys 80 -> 120 us)
-    const int split = blockIdx.x / a.units, unit = blockIdx.x % a.units;
-    const int seq = unit / a.nkv, kvh = unit % a.nkv, G = a.H / a.nkv;
+    __shared__ PageCutLds s_cut;
+    const int kvh = blockIdx.x % a.nkv, G = a.H / a.nkv;
+    const PageCut cut = lg_pa_cut<LG_PA_WAVES * 64>(a, blockIdx.x / a.nkv, -1, s_cut);
+    const int seq = __builtin_amdgcn_readfirstlane(cut.seq);
+    if (seq < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     constexpr int STEP = LG_PA_WAVES * LG_PA_TILE;
     const int32_t *table = a.table + (long long)seq * a.max_blocks;
-    // Queries are asked for first: what is asked for later arrives later, and behind the keys they would hold the first scores up.  Without a window the
-    // first tile's place does not depend on the length either, and its pages' ids come together with that.
+    // queries are asked for first: what is asked for later arrives later, and behind the keys they would hold the first scores up
     float4 qv[KS][2];
     {
         const int h = c & 7;
@@ -256,14 +288,12 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
         #pragma unroll
         for (int i = 0; i < KS; ++i) { qv[i][0] = *(const float4 *)(q + i * 32); qv[i][1] = *(const float4 *)(q + i * 32 + 4); }
     }
-    PageIds ids = lg_pa_ids(a, table, split * a.chunk + wave * LG_PA_TILE);
     int lo, len;
     lg_pa_range(a, seq, lo, len);
-    const int n_split = lg_pa_splits(a, lo, len);
-    if (split >= n_split && !(a.splits == 1)) return;
-    const int first = (lo & ~(LG_PA_TILE - 1)) + split * a.chunk, end = len < first + a.chunk ? len : first + a.chunk;
+    const int chunk = __builtin_amdgcn_readfirstlane(cut.tiles) * LG_PA_TILE, n_split = __builtin_amdgcn_readfirstlane(cut.n);
+    const int first = (lo & ~(LG_PA_TILE - 1)) + __builtin_amdgcn_readfirstlane(cut.index) * chunk, end = len < first + chunk ? len : first + chunk;
     int t0 = first + wave * LG_PA_TILE;
-    if (lo) ids = lg_pa_ids(a, table, t0);
+    const PageIds ids = lg_pa_ids(a, table, t0);
     // the later tiles' ids through LDS: a load of them inside the loop would be waited for together with the keys that are on their way
     const int b0 = first >> a.g.shift;
     static_assert(LG_PA_CHUNK / 16 + 1 <= LG_PA_WAVES * 64, "an id for each thread");
@@ -459,13 +489,13 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
             o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
         }
         const int head = kvh * G + h;
-        if (a.splits == 1) {
+        if (n_split == 1) {
             float *const p = a.out + seq * a.out_stride + (long long)head * HD + d;       // (rows may start anywhere)
             const float x[4] = { o.x, o.y, o.z, o.w };
             #pragma unroll
             for (int i = 0; i < 4; ++i) p[i] = L == 0.0f ? 0.0f : x[i] / L;
         } else {
-            const long long at = ((long long)seq * a.H + head) * a.splits + split;
+            const long long at = (long long)(blockIdx.x / a.nkv) * a.H + head;
             *(float4 *)(a.pacc + at * HD + d) = o;
             if (d == 0) { a.pm[at] = M; a.pl[at] = L; }
         }
@@ -474,26 +504,27 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
 
 // The splits of a sequence, joined: a workgroup per (sequence, head).  A split's factor is computed once, by one thread; then the wavefronts take splits in
 // turn, a lane HD / 64 dimensions, and their sums are added in order.
-#define LG_PM_WAVES 4
+#define LG_PM_WAVES 8
 template <int HD>
 __global__ __launch_bounds__(LG_PM_WAVES * 64) void lg_k_page_merge(PageAttn a) {
     constexpr int NT = LG_PM_WAVES * 64, D = HD / 64;
     __shared__ float s_f[NT], s_w[LG_PM_WAVES], s_o[LG_PM_WAVES][HD];
-    const int head = blockIdx.x, seq = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    int lo, len;
-    lg_pa_range(a, seq, lo, len);
-    const int n = lg_pa_splits(a, lo, len);
-    const long long at = ((long long)seq * a.H + head) * a.splits;
-    // what the first NT splits need is asked for at once: a wavefront's first four sums with the maxima
+    __shared__ PageCutLds s_cut;
+    const int head = blockIdx.x, seq = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const PageCut cut = lg_pa_cut<NT>(a, 0, seq, s_cut);
+    const int n = __builtin_amdgcn_readfirstlane(cut.n), from = __builtin_amdgcn_readfirstlane(cut.first);
+    if (n < 2) return;                                       // (its one split has written the output)
+    // what the first NT splits need is asked for at once: a wavefront's first eight sums with the maxima
     typedef float vec __attribute__((ext_vector_type(D)));
-    constexpr int FIRST = 4;
-    auto sums = [&](int k) { return *(const vec *)(a.pacc + (at + k) * HD + lane * D); };
+    constexpr int FIRST = HD == 512 ? 4 : 8;
+    auto place = [&](int k) { return (long long)(from + k) * a.H + head; };
+    auto sums = [&](int k) { return *(const vec *)(a.pacc + place(k) * HD + lane * D); };
     vec ahead[FIRST];
-    const float m0 = t < n ? a.pm[at + t] : -INFINITY, l0 = t < n ? a.pl[at + t] : 0.0f;
+    const float m0 = t < n ? a.pm[place(t)] : -INFINITY, l0 = t < n ? a.pl[place(t)] : 0.0f;
     #pragma unroll
-    for (int j = 0; j < FIRST; ++j) if (wave + j * LG_PM_WAVES < n) ahead[j] = sums(wave + j * LG_PM_WAVES);
+    for (int j = 0; j < FIRST; ++j) { const int k = wave + j * LG_PM_WAVES; ahead[j] = sums(k < n ? k : n - 1); }
     float M = m0;
-    for (int i = t + NT; i < n; i += NT) M = fmaxf(M, a.pm[at + i]);
+    for (int i = t + NT; i < n; i += NT) M = fmaxf(M, a.pm[place(i)]);
     for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
     if (lane == 0) s_w[wave] = M;
     __syncthreads();
@@ -503,7 +534,7 @@ __global__ __launch_bounds__(LG_PM_WAVES * 64) void lg_k_page_merge(PageAttn a) 
     vec o = 0;
     for (int base = 0; base < n; base += NT) {
         const int i = base + t;
-        const float mi = base ? i < n ? a.pm[at + i] : 0.0f : m0, ls = base ? i < n ? a.pl[at + i] : 0.0f : l0;
+        const float mi = base ? i < n ? a.pm[place(i)] : 0.0f : m0, ls = base ? i < n ? a.pl[place(i)] : 0.0f : l0;
         const float f = ls == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mi - M);                 // (0: no key, its pages are left out)
         L += ls == 0.0f ? 0.0f : f * ls;
         __syncthreads();

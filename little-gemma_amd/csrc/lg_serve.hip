@@ -4,6 +4,7 @@
 // capture can take it.  What the host can see is checked here; what lies in device memory (lengths, page ids, slots) is checked by the kernels.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <algorithm>
 
 #include "../../include/lg_hip.h"
 #include "lg_host.h"
@@ -81,14 +82,18 @@ extern "C" int lg_hip_paged_write(const struct lg_hip_pages *p, const float *d_k
 }
 
 // ---- attend -----------------------------------------------------------------------------------------------------
-// Keys of a split: as many as give the chip about four workgroups per CU were every sequence at its longest, 128 (a tile for each wavefront) to 1024.
-struct AttnSplit { int chunk, splits; };
-static AttnSplit split_of(int n_seq, int n_head_kv, int max_len, int window) {
-    const int64_t span = window > 0 && window < max_len ? window + LG_PA_TILE - 1 : max_len > 1 ? max_len : 1;     // (a window need not start with a tile)
-    int64_t chunk = span * n_seq * n_head_kv / 1024;
-    chunk = (chunk + 127) / 128 * 128;
-    chunk = chunk < 128 ? 128 : chunk > 1024 ? 1024 : chunk;
-    return { (int)chunk, (int)((span + chunk - 1) / chunk) };
+#define LG_PA_SEQS   4096            // sequences of a call: every workgroup goes over their lengths
+// Workgroups of lg_k_page_attn at a time: lg_pa_per_simd on each of 256 compute units
+static int slots_of(int hd) { return 256 * lg_pa_per_simd(hd); }
+// Splits of all sequences together, at most.  lg_pa_split_tiles makes the full ones of a key head slots / n_head_kv or fewer for every round, the rounds one or 2 units / slots rounded
+// up, where splits of 4 tiles to LG_PA_CHUNK keys allow; every sequence has one that is not full besides
+struct AttnCut { int64_t splits; bool join; };
+static AttnCut cut_of(int n_seq, int n_head_kv, int hd, int max_len, int window) {
+    // (a window need not start with a tile)
+    const int64_t span = window > 0 && window < max_len ? (int64_t)window + LG_PA_TILE - 1 : max_len, tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
+    const int64_t least = (tiles + 3) / 4, slots = slots_of(hd), units = (int64_t)n_seq * n_head_kv, rounds = std::max<int64_t>(1, (units + slots / 2 - 1) / (slots / 2));
+    const int64_t full = std::max<int64_t>(rounds * slots / n_head_kv, n_seq * tiles / (LG_PA_CHUNK / LG_PA_TILE));
+    return { std::min<int64_t>(n_seq * std::max<int64_t>(least, 1), full + n_seq), least > 1 };
 }
 static bool attn_shape(int n_seq, int n_head, int n_head_kv, int hd, int max_len) {
     return n_seq >= 0 && n_head_kv >= 1 && n_head_kv <= 1024 && n_head >= 1 && n_head % n_head_kv == 0 && n_head / n_head_kv <= 8 &&
@@ -96,16 +101,16 @@ static bool attn_shape(int n_seq, int n_head, int n_head_kv, int hd, int max_len
 }
 extern "C" size_t lg_hip_paged_attention_workspace(int n_seq, int n_head, int n_head_kv, int hd, int max_len, int window) {
     if (!attn_shape(n_seq, n_head, n_head_kv, hd, max_len)) return 0;
-    const AttnSplit s = split_of(n_seq, n_head_kv, max_len, window);
-    if (s.splits == 1) return 0;
-    const size_t slots = (size_t)n_seq * n_head * s.splits;
+    const AttnCut c = cut_of(n_seq, n_head_kv, hd, max_len, window);
+    if (!c.join) return 0;
+    const size_t slots = (size_t)c.splits * n_head;
     return 2 * up256(slots * 4) + slots * hd * 4;
 }
 
 template <int HD>
-static void launch_attn(const PageAttn &a, int n_seq, hipStream_t st) {
-    hipLaunchKernelGGL(lg_k_page_attn<HD>, dim3((unsigned)((int64_t)a.units * a.splits)), dim3(LG_PA_WAVES * 64), 0, st, a);
-    if (a.splits > 1) hipLaunchKernelGGL(lg_k_page_merge<HD>, dim3(a.H, n_seq), dim3(LG_PM_WAVES * 64), 0, st, a);
+static void launch_attn(const PageAttn &a, const AttnCut &c, hipStream_t st) {
+    hipLaunchKernelGGL(lg_k_page_attn<HD>, dim3((unsigned)(c.splits * a.nkv)), dim3(LG_PA_WAVES * 64), 0, st, a);
+    if (c.join) hipLaunchKernelGGL(lg_k_page_merge<HD>, dim3(a.H, a.n_seq), dim3(LG_PM_WAVES * 64), 0, st, a);
 }
 
 extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float *d_q, int64_t q_stride, int n_seq, int n_head, const int32_t *d_table,
@@ -124,21 +129,22 @@ extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float 
     const int64_t qd = (int64_t)n_head * hd;
     if (q_stride < qd || q_stride % 4 || !aligned16(d_q)) return lg_fail(-2, "paged_attention: query rows of %lld values, %lld apart (aligned to 16 bytes)", (long long)qd, (long long)q_stride);
     if (out_stride < qd || ((uintptr_t)d_out & 3)) return lg_fail(-2, "paged_attention: output rows of %lld values, %lld apart", (long long)qd, (long long)out_stride);
-    const AttnSplit s = split_of(n_seq, p->n_head_kv, max_len, window);
-    if (n_seq > 65535 || (int64_t)n_seq * p->n_head_kv * s.splits > INT32_MAX) return lg_fail(-2, "paged_attention: %d sequences of %d key heads in %d splits in one call", n_seq, p->n_head_kv, s.splits);
+    const AttnCut c = cut_of(n_seq, p->n_head_kv, hd, max_len, window);
+    if (n_seq > LG_PA_SEQS || c.splits * n_head > INT32_MAX)
+        return lg_fail(-2, "paged_attention: %d sequences of %d heads in %lld splits in one call (at most %d sequences)", n_seq, n_head, (long long)c.splits, LG_PA_SEQS);
     const size_t need = lg_hip_paged_attention_workspace(n_seq, n_head, p->n_head_kv, hd, max_len, window);
     if (need && (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)))
         return lg_fail(-2, "paged_attention: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
-    const size_t part = up256((size_t)n_seq * n_head * s.splits * 4);
+    const size_t part = up256((size_t)c.splits * n_head * 4);
     float *const w = (float *)d_work;
     const PageAttn a{ g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, w, need ? (float *)((char *)d_work + part) : nullptr,
-                      need ? (float *)((char *)d_work + 2 * part) : nullptr, scale, n_head, p->n_head_kv, n_seq * p->n_head_kv, max_blocks, max_len, window, s.chunk, s.splits };
+                      need ? (float *)((char *)d_work + 2 * part) : nullptr, scale, n_head, p->n_head_kv, n_seq, max_blocks, max_len, window, slots_of(hd) };
     hipStream_t st = (hipStream_t)stream;
     switch (hd) {
-        case 64:  launch_attn<64>(a, n_seq, st); break;
-        case 128: launch_attn<128>(a, n_seq, st); break;
-        case 256: launch_attn<256>(a, n_seq, st); break;
-        default:  launch_attn<512>(a, n_seq, st); break;
+        case 64:  launch_attn<64>(a, c, st); break;
+        case 128: launch_attn<128>(a, c, st); break;
+        case 256: launch_attn<256>(a, c, st); break;
+        default:  launch_attn<512>(a, c, st); break;
     }
     LG_TRY(hipGetLastError());
     return 0;
