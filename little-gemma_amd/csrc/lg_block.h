@@ -83,3 +83,23 @@ __device__ __forceinline__ void lg_block_max2(T &u, T &v, T *part) {          //
     u = lg_wave_max(lane < NW ? part[lane] : 0);
     v = lg_wave_max(lane < NW ? part[NW + lane] : 0);
 }
+// Three running sums at once (exclusive), their totals in `all`; part: 3 NT / 64 words
+template <int NT>
+__device__ __forceinline__ void lg_block_run3(lg_u64 (&v)[3], lg_u64 (&all)[3], lg_u64 *part) {
+    constexpr int NW = NT / 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    lg_u64 own[3];
+    #pragma unroll
+    for (int k = 0; k < 3; ++k) { own[k] = v[k]; v[k] = lg_wave_run(v[k]); }
+    __syncthreads();
+    if (lane == 63)
+        #pragma unroll
+        for (int k = 0; k < 3; ++k) part[k * NW + wave] = v[k];
+    __syncthreads();
+    #pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        const lg_u64 x = lg_wave_run(lane < NW ? part[k * NW + lane] : 0);
+        all[k] = lg_lane(x, NW - 1);
+        v[k] += (wave ? lg_lane(x, wave - 1) : 0) - own[k];
+    }
+}

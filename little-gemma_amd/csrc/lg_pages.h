@@ -11,7 +11,6 @@
 #include "lg_block.h"
 
 #define LG_PLAN_SEQS 4096           // sequences of a plan: their running sums lie in LDS
-#define LG_PLAN_WG   1024
 
 // ---- plan ------------------------------------------------------------------------------------------------------------
 enum { LG_PLAN_BAD_LEN = 1, LG_PLAN_NO_PAGES = 2, LG_PLAN_NO_SLOTS = 4, LG_PLAN_BAD_STACK = 8, LG_PLAN_BAD_PAGE = 16 };   // LG_HIP_PLAN_* of lg_hip.h
@@ -35,46 +34,48 @@ __device__ __forceinline__ int lg_owner(const int32_t *sums, int n, int e) {
 
 // Lengths before and after a step -> pages and slots.  With nb(l) = ceil(l / P), sequence i returns max(0, nb(old) - nb(new)) pages and takes
 // max(0, nb(new) - nb(old)); all returned pages go on the stack first, the first one topmost, then the needed ones are taken from its top in
-// order, so that the plan with the lengths exchanged undoes this one exactly.  All or nothing: whatever *status reports leaves table and stack alone.
-// One workgroup: the whole step is a few thousand words (64 sequences, one new token each: 2 KB), its time is launch and a chain of
-// memory round trips, which a grid would lengthen by a launch per phase.
-__global__ __launch_bounds__(LG_PLAN_WG) void lg_k_plan(PlanArgs a) {
-    __shared__ int32_t tok[LG_PLAN_SEQS + 1], need[LG_PLAN_SEQS + 1], freed[LG_PLAN_SEQS + 1];
-    __shared__ lg_u64 part[LG_PLAN_WG / 64];
+// order, so that the plan with the lengths exchanged undoes this one exactly: needed page e is returned page e as long as there are those.  All or
+// nothing: whatever *status reports leaves table and stack alone.
+// One workgroup, of NT threads: the step is a few thousand words (64 sequences, one new token each: 2 KB), its time a chain of memory round trips.  Where
+// every thread has one page and one token at most the chain is lengths, pages, stores: 64 sequences @PD@.  Slots of many tokens are left to
+// lg_k_plan_slots (`slots` null).
+template <int NT>
+__global__ __launch_bounds__(NT) void lg_k_plan(PlanArgs a) {
+    __shared__ int32_t tok[LG_PLAN_SEQS + 1], need[LG_PLAN_SEQS + 1], freed[LG_PLAN_SEQS + 1], olds[LG_PLAN_SEQS], news[LG_PLAN_SEQS];
+    __shared__ lg_u64 part[3 * NT / 64];
+    __shared__ int32_t taken[NT];
     __shared__ int bad;
-    const int t = threadIdx.x, P = 1 << a.shift, n = a.n_seq;
+    const int t = threadIdx.x, P = 1 << a.shift, n = a.n_seq, n_slots = a.slots ? a.n_slots : 0;
     const long long most = (long long)a.max_blocks << a.shift;
-    constexpr int CH = LG_PLAN_SEQS / LG_PLAN_WG;
-    if (t == 0) bad = 0;
-    __syncthreads();
-    auto blocks = [&](int len) { return (int)(((long long)len + P - 1) >> a.shift); };
-    // running sums: sequences t * CH .. t * CH + CH - 1 are this thread's
-    lg_u64 v[3][CH], sum[3] = { 0, 0, 0 };
-    #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int i = t * CH + c;
-        int lo = i < n ? a.len_old[i] : 0, ln = i < n ? a.len_new[i] : 0;
-        if (lo < 0 || ln < 0 || lo > most || ln > most) { atomicOr(&bad, LG_PLAN_BAD_LEN); lo = ln = 0; }
-        const int d = blocks(ln) - blocks(lo);
-        v[0][c] = ln > lo ? ln - lo : 0; v[1][c] = d > 0 ? d : 0; v[2][c] = d < 0 ? -d : 0;
-        #pragma unroll
-        for (int k = 0; k < 3; ++k) sum[k] += v[k][c];
-    }
-    lg_u64 all[3];
-    int32_t *const dst[3] = { tok, need, freed };
-    #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        lg_u64 run = lg_block_run<LG_PLAN_WG>(sum[k], part, &all[k]) - sum[k];
-        #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int i = t * CH + c;
-            if (i <= n) dst[k][i] = (int32_t)run;             // (used only where the total fits, below)
-            run += v[k][c];
-        }
-        if (t == 0 && n == LG_PLAN_SEQS) dst[k][n] = (int32_t)all[k];
-    }
+    const int per = (n + NT - 1) / NT, i0 = t * per;
     const int nf = *a.n_free;
+    if (t == 0) bad = 0;
+    auto blocks = [&](int len) { return (int)(((long long)len + P - 1) >> a.shift); };
+    auto parts = [&](int i, lg_u64 (&v)[3]) {
+        const int lo = olds[i], ln = news[i], d = blocks(ln) - blocks(lo);
+        v[0] = ln > lo ? ln - lo : 0; v[1] = d > 0 ? d : 0; v[2] = d < 0 ? -d : 0;
+    };
+    // running sums: sequences i0 .. i0 + per - 1 are this thread's
+    lg_u64 run[3] = { 0, 0, 0 }, all[3], v[3];
+    bool wrong = false;
+    for (int i = i0; i < i0 + per && i < n; ++i) {
+        int lo = a.len_old[i], ln = a.len_new[i];
+        if (lo < 0 || ln < 0 || lo > most || ln > most) { wrong = true; lo = ln = 0; }
+        olds[i] = lo; news[i] = ln;
+        parts(i, v);
+        #pragma unroll
+        for (int k = 0; k < 3; ++k) run[k] += v[k];
+    }
+    lg_block_run3<NT>(run, all, part);
+    if (wrong) atomicOr(&bad, LG_PLAN_BAD_LEN);
+    for (int i = i0; i < i0 + per && i < n; ++i) {            // (used only where the totals fit, below)
+        tok[i] = (int32_t)run[0]; need[i] = (int32_t)run[1]; freed[i] = (int32_t)run[2];
+        parts(i, v);
+        #pragma unroll
+        for (int k = 0; k < 3; ++k) run[k] += v[k];
+    }
     if (t == 0) {
+        tok[n] = (int32_t)all[0]; need[n] = (int32_t)all[1]; freed[n] = (int32_t)all[2];
         if (nf < 0 || nf > a.n_pages || all[2] + nf > (lg_u64)a.n_pages) atomicOr(&bad, LG_PLAN_BAD_STACK);
         else if (all[1] > nf + all[2]) atomicOr(&bad, LG_PLAN_NO_PAGES);
         if (all[0] > (lg_u64)a.n_slots) atomicOr(&bad, LG_PLAN_NO_SLOTS);
@@ -82,47 +83,80 @@ __global__ __launch_bounds__(LG_PLAN_WG) void lg_k_plan(PlanArgs a) {
     __syncthreads();
     int st = bad;
     const int nt = (int)all[0], nn = (int)all[1], ng = (int)all[2], top = nf + ng;
-    if (!st) {
-        // every page id that the step would move or write into, before anything moves
-        int ids = 0;
-        for (int e = t; e < ng; e += LG_PLAN_WG) {
-            const int i = lg_owner(freed, n, e);
-            const int id = a.table[(size_t)i * a.max_blocks + blocks(a.len_new[i]) + e - freed[i]];
-            ids |= id < 0 || id >= a.n_pages;
+    auto place = [&](int i, int block) { return a.table + (size_t)i * a.max_blocks + block; };
+    auto leaves = [&](int e) { const int i = lg_owner(freed, n, e); return place(i, blocks(news[i]) + e - freed[i]); };      // where the e-th returned page stands
+    auto comes = [&](int e) { const int i = lg_owner(need, n, e); return place(i, blocks(olds[i]) + e - need[i]); };          // where the e-th needed one goes
+    auto outside = [&](int id) { return id < 0 || id >= a.n_pages; };
+    if (!st && ng <= NT && nn <= NT && n_slots && n_slots <= NT) {
+        // everything is read, then everything is written
+        int32_t *from = nullptr, page = 0, slot = -1, later = -1;
+        if (t < ng) { from = leaves(t); page = *from; }
+        else if (t < nn) page = a.stack[top - 1 - t];
+        int here = 0, pos = 0;
+        if (t < nt) {
+            const int i = lg_owner(tok, n, t);
+            pos = olds[i] + t - tok[i];
+            const int block = pos >> a.shift, nb = blocks(olds[i]);
+            if (block < nb) here = *place(i, block); else later = need[i] + block - nb;
         }
-        for (int e = ng + t; e < nn; e += LG_PLAN_WG) { const int id = a.stack[top - 1 - e]; ids |= id < 0 || id >= a.n_pages; }
-        for (int i = t; i < n; i += LG_PLAN_WG) {
-            const int lo = a.len_old[i];
-            if (a.len_new[i] > lo && (lo & (P - 1))) { const int id = a.table[(size_t)i * a.max_blocks + (lo >> a.shift)]; ids |= id < 0 || id >= a.n_pages; }
-        }
-        if (ids) atomicOr(&bad, LG_PLAN_BAD_PAGE);
+        if (outside(page) || outside(here)) atomicOr(&bad, LG_PLAN_BAD_PAGE);
+        taken[t] = page;
         __syncthreads();
         st = bad;
-    }
-    if (!st) {
-        for (int e = t; e < ng; e += LG_PLAN_WG) {
-            const int i = lg_owner(freed, n, e);
-            int32_t *const p = a.table + (size_t)i * a.max_blocks + blocks(a.len_new[i]) + e - freed[i];
-            a.stack[top - 1 - e] = *p;
-            *p = -1;
+        if (!st) {
+            if (from) { *from = -1; a.stack[top - 1 - t] = page; }
+            if (t < nn) *comes(t) = page;
+            if (t < nt) slot = (later < 0 ? here : taken[later]) * P + (pos & (P - 1));
         }
-        __syncthreads();
-        for (int e = t; e < nn; e += LG_PLAN_WG) {
-            const int i = lg_owner(need, n, e);
-            a.table[(size_t)i * a.max_blocks + blocks(a.len_old[i]) + e - need[i]] = a.stack[top - 1 - e];
+        if (t < n_slots) a.slots[t] = slot;
+    } else {
+        if (!st) {
+            bool ids = false;
+            for (int e = t; e < ng; e += NT) ids |= outside(*leaves(e));
+            for (int e = ng + t; e < nn; e += NT) ids |= outside(a.stack[top - 1 - e]);
+            for (int i = t; i < n; i += NT) if (news[i] > olds[i] && (olds[i] & (P - 1))) ids |= outside(*place(i, olds[i] >> a.shift));
+            if (ids) atomicOr(&bad, LG_PLAN_BAD_PAGE);
+            __syncthreads();
+            st = bad;
         }
-        __syncthreads();
-    }
-    for (int s = t; s < a.n_slots; s += LG_PLAN_WG) {
-        int slot = -1;
-        if (!st && s < nt) {
-            const int i = lg_owner(tok, n, s), pos = a.len_old[i] + s - tok[i];
-            slot = a.table[(size_t)i * a.max_blocks + (pos >> a.shift)] * P + (pos & (P - 1));
+        if (!st) {
+            for (int e = t; e < ng; e += NT) { int32_t *const p = leaves(e); a.stack[top - 1 - e] = *p; *p = -1; }
+            __syncthreads();
+            for (int e = t; e < nn; e += NT) *comes(e) = a.stack[top - 1 - e];
+            __syncthreads();
         }
-        a.slots[s] = slot;
+        for (int s = t; s < n_slots; s += NT) {
+            int slot = -1;
+            if (!st && s < nt) {
+                const int i = lg_owner(tok, n, s), pos = olds[i] + s - tok[i];
+                slot = *place(i, pos >> a.shift) * P + (pos & (P - 1));
+            }
+            a.slots[s] = slot;
+        }
     }
-    for (int i = t; i <= n; i += LG_PLAN_WG) a.start[i] = st ? 0 : tok[i];
+    for (int i = t; i <= n; i += NT) a.start[i] = st ? 0 : tok[i];
     if (t == 0) { *a.status = st; if (!st) *a.n_free = top - nn; }
+}
+// Slots of many tokens, behind the plan (start of what it refused is 0: no token).  Four in a row to a thread: one search each, then along the sequences.
+__global__ __launch_bounds__(256) void lg_k_plan_slots(PlanArgs a) {
+    __shared__ int32_t tok[LG_PLAN_SEQS + 1];
+    const int n = a.n_seq, P = 1 << a.shift;
+    for (int i = threadIdx.x; i <= n; i += 256) tok[i] = a.start[i];
+    __syncthreads();
+    const int s0 = (int)(blockIdx.x * 256 + threadIdx.x) * 4, nt = tok[n];
+    if (s0 >= a.n_slots) return;
+    int out[4] = { -1, -1, -1, -1 };
+    int i = s0 < nt ? lg_owner(tok, n, s0) : 0;
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int s = s0 + k;
+        if (s >= nt) continue;
+        while (tok[i + 1] <= s) ++i;
+        const int pos = a.len_old[i] + s - tok[i];
+        out[k] = a.table[(size_t)i * a.max_blocks + (pos >> a.shift)] * P + (pos & (P - 1));
+    }
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) if (s0 + k < a.n_slots) a.slots[s0 + k] = out[k];
 }
 
 // ---- write -----------------------------------------------------------------------------------------------------------

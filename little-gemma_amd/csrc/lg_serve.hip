@@ -22,6 +22,7 @@ static int shift_of(int page_size) {                 // page_size = 1 << shift; 
 }
 static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
+#define LG_PLAN_APART 2048           // slots
 // ---- plan -------------------------------------------------------------------------------------------------------
 extern "C" size_t lg_hip_paged_plan_workspace(int n_seq) { (void)n_seq; return 0; }
 
@@ -37,8 +38,17 @@ extern "C" int lg_hip_paged_plan(int n_seq, int page_size, int n_pages, int max_
     if (n_slots < 0) return lg_fail(-2, "paged_plan: %d slots", n_slots);
     if (!d_free || !d_n_free || !d_start || !d_status || (n_seq && (!d_len_old || !d_len_new || !d_table)) || (n_slots && !d_slots))
         return lg_fail(-1, "paged_plan: null argument");
-    const PlanArgs a{ d_len_old, d_len_new, d_table, d_free, d_n_free, d_start, d_slots, d_status, n_seq, shift, n_pages, max_blocks, n_slots };
-    hipLaunchKernelGGL(lg_k_plan, dim3(1), dim3(LG_PLAN_WG), 0, (hipStream_t)stream, a);
+    PlanArgs a{ d_len_old, d_len_new, d_table, d_free, d_n_free, d_start, d_slots, d_status, n_seq, shift, n_pages, max_blocks, n_slots };
+    hipStream_t st = (hipStream_t)stream;
+    // four wavefronts where they have a thread for every sequence and token: their barriers are shorter; slots that 1024 threads would go over more than twice by a launch of their own
+    const bool apart = n_slots > LG_PLAN_APART;
+    if (apart) a.slots = nullptr;
+    if (n_seq <= 256 && n_slots <= 256) hipLaunchKernelGGL(lg_k_plan<256>, dim3(1), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(lg_k_plan<1024>, dim3(1), dim3(1024), 0, st, a);
+    if (apart) {
+        a.slots = d_slots;
+        hipLaunchKernelGGL(lg_k_plan_slots, dim3((unsigned)(((int64_t)n_slots + 1023) / 1024)), dim3(256), 0, st, a);
+    }
     LG_TRY(hipGetLastError());
     return 0;
 }

@@ -39,7 +39,7 @@ def same(got, want):
 # ---- plan
 @pytest.mark.parametrize("n, page, most, grow, shrink", [
     (1, 16, 1, 1, 0), (1, 256, 3000, 5, 0), (7, 16, 40, 1, 0), (64, 32, 2000, 1, 0), (65, 64, 500, 700, 0), (130, 16, 300, 3, 40), (1000, 16, 100, 17, 100),
-    (1025, 128, 400, 1, 1), (4096, 16, 33, 2, 3), (3, 16, 100, 20000, 0)])
+    (1025, 128, 400, 1, 1), (4096, 16, 33, 2, 3), (3, 16, 100, 20000, 0), (256, 16, 700, 1, 3), (257, 16, 64, 1, 0), (9, 16, 2000, 2000, 2000), (40, 64, 3, 60, 3)])
 def test_plan_of_a_step_and_its_undoing(dev, n, page, most, grow, shrink):
     rng = np.random.default_rng(n * 1000 + page)
     old = rng.integers(0, most + 1, n)
@@ -217,6 +217,19 @@ def test_attention_of_one_token_per_sequence(lg, dev, H, kv, hd, page, window, l
     assert (got[empty] == 0).all()
 
 
+@pytest.mark.parametrize("n, H, kv, hd, window", [(63, 2, 2, 64, 0), (64, 2, 1, 64, 40), (65, 2, 2, 64, 0), (300, 4, 2, 64, 0), (1025, 1, 1, 64, 33), (4096, 1, 1, 64, 0)])
+def test_attention_of_many_sequences(lg, dev, n, H, kv, hd, window):
+    """A lane, a thread or several of one for the lengths; sequences of one split beside such of many; most free places of a batch."""
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, 40, n)
+    lens[rng.integers(0, n, 3)] = 1500
+    lens[rng.random(n) < 0.3] = 0
+    q, k, v, table = case(rng, H, kv, hd, 16, lens)
+    print(f"attend {n} sequences", flush=True)
+    want, bound = attend_ref(q, k, v, table, lens, 16, k.shape[0], kv, window, 1.0, 1500)
+    within(attend(lg, dev, q, k, v, table, lens, 16, kv, window, 1.0, 1500), want, bound)
+
+
 def test_attention_of_large_and_tiny_queries_and_scales(lg, dev):
     """Scores from almost equal to one key far above the rest, queries near the ends of f32's range, a negative scale, rows of zeros."""
     rng = np.random.default_rng(3)
@@ -243,7 +256,7 @@ def test_attention_clamps_lengths_and_leaves_out_bad_pages(lg, dev):
 
 
 def test_rows_of_a_verify_block_are_sequences_that_share_pages(lg, dev):
-    """Five rows of one sequence: the same table row, lengths one apart; row j is what a call with that row alone gives, bit for bit."""
+    """Five rows of one sequence: the same table row, lengths one apart."""
     rng = np.random.default_rng(12)
     _, k, v, table = case(rng, 8, 2, 256, 32, [1003])
     q = (rng.normal(0, 2, (5, 8, 256)) / 16).astype(np.float32)

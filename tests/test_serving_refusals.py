@@ -55,7 +55,7 @@ def test_write_refuses(lg, k, v, stride, slots, n, code, words):
 
 
 @pytest.mark.parametrize("change, code, words", [
-    (dict(n_seq=-1), -2, "-1 sequences"), (dict(heads=7), -2, "7 query heads"), (dict(heads=18), -2, "18 query heads"), (dict(heads=0), -2, "0 query heads"),
+    (dict(n_seq=-1), -2, "-1 sequences"), (dict(n_seq=4097), -2, "4097 sequences"), (dict(heads=7), -2, "7 query heads"), (dict(heads=18), -2, "18 query heads"), (dict(heads=0), -2, "0 query heads"),
     (dict(max_len=-1), -2, "lengths up to -1"), (dict(max_len=(1 << 30) + 1), -2, "lengths up to"), (dict(blocks=0), -2, "0 blocks"), (dict(blocks=1 << 27), -2, "blocks"),
     (dict(window=-5), -2, "window"), (dict(q=None), -1, "null"), (dict(table=None), -1, "null"), (dict(lens=None), -1, "null"), (dict(out=None), -1, "null"),
     (dict(q_stride=508), -2, "508 apart"), (dict(q_stride=513), -2, "513 apart"), (dict(out_stride=511), -2, "511 apart"),
