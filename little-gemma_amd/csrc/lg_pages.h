@@ -212,7 +212,7 @@ struct PageAttn {
     float *out; long long out_stride;
     float *pm, *pl, *pacc;              // [splits of all][H], [..][hd]: partials of sequences of more than one split
     float scale;
-    int H, nkv, n_seq, max_blocks, max_len, window, slots;       // slots: workgroups that the chip holds at a time
+    int H, nkv, n_seq, max_blocks, max_len, window, slots, least;       // slots: workgroups that the chip holds at a time; least: tiles of a split
 };
 // The keys a sequence sees: [lo, len)
 __device__ __forceinline__ void lg_pa_range(const PageAttn &a, int seq, int &lo, int &len) {
@@ -239,7 +239,7 @@ struct PageCutLds { uint32_t part[16]; PageCut c; };
 __device__ __forceinline__ uint32_t lg_pa_split_tiles(const PageAttn &a, uint32_t total, uint32_t some) {
     const uint32_t units = some * a.nkv, half = (uint32_t)a.slots / 2, rounds = units > half ? (units + half - 1) / half : 1, full = rounds * a.slots - units;
     const lg_u64 tiles = ((lg_u64)total * a.nkv + full - 1) / full;
-    return tiles < 4 ? 4 : tiles > LG_PA_CHUNK / LG_PA_TILE ? LG_PA_CHUNK / LG_PA_TILE : (uint32_t)tiles;
+    return tiles < (uint32_t)a.least ? a.least : tiles > LG_PA_CHUNK / LG_PA_TILE ? LG_PA_CHUNK / LG_PA_TILE : (uint32_t)tiles;
 }
 __device__ __forceinline__ uint32_t lg_pa_splits(uint32_t of, uint32_t tiles) { const uint32_t x = (of + tiles - 1) / tiles; return x ? x : 1u; }
 template <int NT>
@@ -297,11 +297,11 @@ __device__ __forceinline__ PageTile lg_pa_tile(const PageAttn &a, const PageIds 
 constexpr int lg_pa_per_simd(int hd) { return hd == 512 ? 1 : hd == 256 ? 2 : hd == 128 ? 3 : 4; }
 template <int HD>
 __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_page_attn(PageAttn a) {
-    constexpr bool AHEAD = HD <= 256;               // a tile's values and the next one's keys are on their way while it is worked on; at 512 the registers do not hold both
     constexpr int KS = HD / 32;                     // score steps
     constexpr int DL = HD >= 128 ? 8 : HD / 16;     // dimensions of a value load
     constexpr int CH = HD / (16 * DL);              // value loads of a key row
     constexpr int NT = HD / 16;                     // output tiles
+    constexpr int PIECES = HD > 256 ? 2 : 1, KP = KS / PIECES, CP = CH / PIECES;       // rows of 512 in two halves: two pieces of keys or values are in registers at a time
     __shared__ float s_m[LG_PA_WAVES][8], s_l[LG_PA_WAVES][8];
     __shared__ __align__(16) union { lg_h8 q[KS][64]; float o[LG_PA_WAVES][8][HD]; } s;
     __shared__ int32_t s_ids[LG_PA_CHUNK / 16 + 1];
@@ -316,12 +316,12 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     const int32_t *table = a.table + (long long)seq * a.max_blocks;
     // queries are asked for first: what is asked for later arrives later, and behind the keys they would hold the first scores up
     float4 qv[KS][2];
-    {
-        const int h = c & 7;
-        const float *q = a.q + seq * a.q_stride + (long long)(kvh * G + (h < G ? h : 0)) * HD + g * 8;
+    const float *qrow = a.q + seq * a.q_stride + (long long)(kvh * G + ((c & 7) < G ? c & 7 : 0)) * HD + g * 8;
+    auto query = [&](int i, int j) { return *(const float4 *)(qrow + i * 32 + j * 4); };
+    #pragma unroll
+    for (int i = 0; i < KS; ++i)
         #pragma unroll
-        for (int i = 0; i < KS; ++i) { qv[i][0] = *(const float4 *)(q + i * 32); qv[i][1] = *(const float4 *)(q + i * 32 + 4); }
-    }
+        for (int j = 0; j < 2; ++j) qv[i][j] = query(i, j);
     int lo, len;
     lg_pa_range(a, seq, lo, len);
     const int chunk = __builtin_amdgcn_readfirstlane(cut.tiles) * LG_PA_TILE, n_split = __builtin_amdgcn_readfirstlane(cut.n);
@@ -343,19 +343,19 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
         return lg_pa_tile(a, p, t, kvh * HD);
     };
 
-    lg_h8 kf[2][KS];
+    lg_h8 kf[2][KP], kg[PIECES > 1 ? 2 : 1][PIECES > 1 ? KP : 1];          // the keys' first piece, and the second
     PageTile now = lg_pa_tile(a, ids, t0, kvh * HD);
     if (t0 >= end) now.row[0] = now.row[1] = kvh * HD;          // (no tile: page 0's rows, so that the loads need no branch, after which everything would be waited for)
-    auto load_keys = [&](const PageTile &p) {
+    auto load_keys = [&](const PageTile &p, auto &to, int piece) {
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint16_t *kp = a.g.k + p.row[h] + c * a.g.row_stride + g * 8;
+            const uint16_t *kp = a.g.k + p.row[h] + c * a.g.row_stride + g * 8 + piece * KP * 32;
             #pragma unroll
-            for (int i = 0; i < KS; ++i) kf[h][i] = *(const lg_h8 *)(kp + i * 32);
+            for (int i = 0; i < KP; ++i) to[h][i] = *(const lg_h8 *)(kp + i * 32);
         }
     };
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (AHEAD) load_keys(now);
+    load_keys(now, kf, 0);
     __builtin_amdgcn_sched_barrier(0);
     if (has_id) s_ids[threadIdx.x] = my_id;
 
@@ -375,7 +375,9 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
         #pragma unroll
         for (int i = 0; i < KS; ++i) {
             if (i % LG_PA_WAVES != wave) continue;
-            const float v[8] = { qv[i][0].x, qv[i][0].y, qv[i][0].z, qv[i][0].w, qv[i][1].x, qv[i][1].y, qv[i][1].z, qv[i][1].w };
+            // (rows of 512 are read again: beside the keys they do not stay in registers)
+            const float4 x = PIECES > 1 ? query(i, 0) : qv[i][0], y = PIECES > 1 ? query(i, 1) : qv[i][1];
+            const float v[8] = { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w };
             lg_h8 part;
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -393,39 +395,50 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     for (int i = 0; i < NT; ++i) acc[i] = (lg_f4){ 0, 0, 0, 0 };
     float m = -INFINITY, l = 0;                     // of query row c; l of this lane's keys alone
 
-    // One tile: its values are requested before its scores are made, the next tile's keys before its values are used
+    // One tile: its values are requested before its scores are made, the next tile's keys before its values are used.  (In two pieces: each a stage ahead.)
     auto work = [&](auto more) {                    // more: a tile follows (a branch around its loads would have them waited for with this tile's)
         constexpr bool MORE = decltype(more)::value;
-        uint32_t w[CH][8][DL / 2];
-        auto load_values = [&](const PageTile &p) {
-            #pragma unroll
-            for (int ch = 0; ch < CH; ++ch)
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint16_t *vp = a.g.v + p.row[j >> 2] + (4 * g + (j & 3)) * a.g.row_stride + ch * 128 + c * DL;
-                    if constexpr (DL == 8) { const uint4 u = *(const uint4 *)vp; w[ch][j][0] = u.x; w[ch][j][1] = u.y; w[ch][j][2] = u.z; w[ch][j][3] = u.w; }
-                    else { const uint2 u = *(const uint2 *)vp; w[ch][j][0] = u.x; w[ch][j][1] = u.y; }
-                }
-        };
         const PageTile here = now;
         PageTile coming = now;
         if constexpr (MORE) coming = tile_at(t0 + STEP);
-        if constexpr (AHEAD) load_values(here);
-        else load_keys(here);
-        __builtin_amdgcn_sched_barrier(0);
+        uint32_t w[CP][8][DL / 2], w2[PIECES > 1 ? CP : 1][8][DL / 2];
+        auto load_values = [&](auto &to, int piece) {
+            #pragma unroll
+            for (int ch = 0; ch < CP; ++ch)
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint16_t *vp = a.g.v + here.row[j >> 2] + (4 * g + (j & 3)) * a.g.row_stride + (piece * CP + ch) * 128 + c * DL;
+                    if constexpr (DL == 8) { const uint4 u = *(const uint4 *)vp; to[ch][j][0] = u.x; to[ch][j][1] = u.y; to[ch][j][2] = u.z; to[ch][j][3] = u.w; }
+                    else { const uint2 u = *(const uint2 *)vp; to[ch][j][0] = u.x; to[ch][j][1] = u.y; }
+                }
+        };
         lg_f4 sc[2] = { { 0, 0, 0, 0 }, { 0, 0, 0, 0 } };
-        #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            const lg_h8 q = s.q[i][lane];
-            sc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][i], q, sc[0], 0, 0, 0);
-            sc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][i], q, sc[1], 0, 0, 0);
+        auto scores = [&](const auto &k, int piece) {
+            #pragma unroll
+            for (int i = 0; i < KP; ++i) {
+                const lg_h8 q = s.q[piece * KP + i][lane];
+                sc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][i], q, sc[0], 0, 0, 0);
+                sc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][i], q, sc[1], 0, 0, 0);
+            }
+        };
+        if constexpr (PIECES > 1) {
+            load_keys(here, kg, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            scores(kf, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            load_values(w, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            scores(kg, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            load_values(w2, 1);
+        } else {
+            load_values(w, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            scores(kf, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (MORE) load_keys(coming, kf, 0);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (!AHEAD) load_values(here);
-        if constexpr (MORE) {
-            now = coming;
-            if constexpr (AHEAD) load_keys(now);
-        }
+        now = coming;
         __builtin_amdgcn_sched_barrier(0);
         // base-2 exponents; rows c and c + 8 hold the two parts of a query's score
         float x[2][4], top = -INFINITY;
@@ -463,27 +476,38 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
                 pf[4 * h + r] = c < 8 ? hi : (_Float16)(p - (float)hi);
             }
         // a masked key's values may be anything (0 * inf is not 0): zeros in their place
-        if (!(t0 >= lo && t0 + LG_PA_TILE <= end && here.ok[0] && here.ok[1])) {
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                if (!(here.ok[j >> 2] && t >= lo && t < end)) {
-                    #pragma unroll
-                    for (int ch = 0; ch < CH; ++ch)
+        const bool whole = t0 >= lo && t0 + LG_PA_TILE <= end && here.ok[0] && here.ok[1];
+        auto values = [&](auto &v, int piece) {
+            if (!whole) {
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                    if (!(here.ok[j >> 2] && t >= lo && t < end)) {
                         #pragma unroll
-                        for (int i = 0; i < DL / 2; ++i) w[ch][j][i] = 0;
+                        for (int ch = 0; ch < CP; ++ch)
+                            #pragma unroll
+                            for (int i = 0; i < DL / 2; ++i) v[ch][j][i] = 0;
+                    }
                 }
             }
-        }
-        #pragma unroll
-        for (int ch = 0; ch < CH; ++ch)
             #pragma unroll
-            for (int i = 0; i < DL; ++i) {
-                union { uint32_t u[4]; lg_h8 h; } b;
+            for (int ch = 0; ch < CP; ++ch)
                 #pragma unroll
-                for (int k2 = 0; k2 < 4; ++k2) b.u[k2] = __builtin_amdgcn_perm(w[ch][2 * k2 + 1][i >> 1], w[ch][2 * k2][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
-                acc[ch * DL + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, b.h, acc[ch * DL + i], 0, 0, 0);
-            }
+                for (int i = 0; i < DL; ++i) {
+                    union { uint32_t u[4]; lg_h8 h; } b;
+                    #pragma unroll
+                    for (int k2 = 0; k2 < 4; ++k2) b.u[k2] = __builtin_amdgcn_perm(v[ch][2 * k2 + 1][i >> 1], v[ch][2 * k2][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
+                    lg_f4 &to = acc[(piece * CP + ch) * DL + i];
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, b.h, to, 0, 0, 0);
+                }
+        };
+        values(w, 0);
+        if constexpr (PIECES > 1) {
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (MORE) load_keys(coming, kf, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            values(w2, 1);
+        }
     };
     for (; t0 + STEP < end; t0 += STEP) work(std::true_type{});
     if (t0 < end) work(std::false_type{});

@@ -9,7 +9,7 @@
 //   S = sum of the kept, r = min(floor(u S), S - 1); the token is the first in index order whose running sum of kept weights passes r.
 // Rows of up to 2^19 tokens: a sum is at most 2^63.
 //
-// A row is read by many workgroups and finished by one, in four launches (one for rows of at most LG_SAMPLE_CAND tokens):
+// A row is read by many workgroups and finished by one, in four launches (one for rows of at most LG_SAMPLE_WHOLE tokens):
 //   lg_k_sample_max     the largest logit of every group of 256
 //   lg_k_sample_bins    rows whose border is to be found: 2048 bins of equal width from the largest logit down, how many tokens and about what sum each holds
 //   lg_k_sample_sums    the exact sum of every group above the bins that can hold the border, and the tokens in those (candidates)
@@ -202,8 +202,10 @@ __device__ void lg_sample_row(const SampleArgs &a, int r, const double *tab, Sam
 #define LG_SAMPLE_MAX_WG  256                    // lg_k_sample_max: 16 groups to a workgroup
 #define LG_SAMPLE_BINS    2048
 #define LG_SAMPLE_CAND    4096                   // candidates that a row may have
-#define LG_SAMPLE_SMALL_K 512                    // top-k up to which the groups' maxima bound the candidates well: with 1024 groups the tokens not below the
-                                                 // k-th largest maximum are 1.15 k at k = 256 and 1.39 k at 512 where large logits lie anywhere in the row
+#define LG_SAMPLE_WHOLE   8192                   // tokens of a row that one workgroup takes by itself: 8 to a thread (16 do not fit its registers)
+#define LG_SAMPLE_SMALL_K 512                    // top-k up to which, and up to half as many as there are groups, the groups' maxima bound the candidates well: with
+                                                 // 1024 groups the tokens not below the k-th largest maximum are 1.15 k at k = 256 and 1.39 k at 512 where large
+                                                 // logits lie anywhere in the row
 #define LG_SAMPLE_SLACK   2048                   // the estimated sum of a row's bins is trusted to 1 / 2048: four times what the comment at lg_k_sample_bins allows
 
 struct SampleWork {                     // per row, in working memory
@@ -244,7 +246,7 @@ enum { LG_ROW_FIRST, LG_ROW_SMALL, LG_ROW_FREE, LG_ROW_BORDER, LG_ROW_ALONE };
 __device__ __forceinline__ int lg_row_kind(const SampleRow &p, int n_vocab) {
     if (!(p.temperature > 0)) return LG_ROW_FIRST;
     const bool k = p.top_k > 0 && p.top_k < n_vocab;
-    if (k && p.top_k <= LG_SAMPLE_SMALL_K) return LG_ROW_SMALL;
+    if (k && p.top_k <= LG_SAMPLE_SMALL_K && p.top_k <= n_vocab / (2 * LG_SAMPLE_GROUP)) return LG_ROW_SMALL;
     if (!(p.temperature > 1e-20f)) return LG_ROW_ALONE;
     return k || p.top_p < 1 ? LG_ROW_BORDER : LG_ROW_FREE;
 }
@@ -299,12 +301,7 @@ __global__ __launch_bounds__(LG_SAMPLE_MAX_WG) void lg_k_sample_max(SampleArgs a
 
 // The row's largest logit and the width of its bins, in every workgroup anew (1024 keys and 64 minima: less than a launch of their own)
 struct SampleSpan { Weigh wg; float top, scale, c; uint32_t key; };      // key: of the largest logit, 0x007FFFFF: none; scale: bins per unit of logit; c: base-2 exponents per unit
-template <int NT>
-__device__ __forceinline__ SampleSpan lg_sample_span(const SampleRow &p, const SampleWork &w, const SampleGeo &g, const double *tab, uint32_t *part) {
-    uint32_t key = 0, least = 0;
-    for (int i = threadIdx.x; i < g.groups; i += NT) { const uint32_t k = w.gmax[i]; if (k > key) key = k; }
-    for (int i = threadIdx.x; i < g.maxes; i += NT) { const uint32_t k = w.smin[i]; if (k > least) least = k; }
-    lg_block_max2<NT>(key, least, part);
+__device__ __forceinline__ SampleSpan lg_sample_span_of(const SampleRow &p, uint32_t key, uint32_t least, const double *tab) {       // least: ~key of the smallest
     SampleSpan s;
     s.key = key;
     s.top = lg_unkey(key);
@@ -313,6 +310,14 @@ __device__ __forceinline__ SampleSpan lg_sample_span(const SampleRow &p, const S
     const float reach = (float)LG_SAMPLE_REACH * p.temperature, width = fminf(s.top - lg_unkey(~least), reach);
     s.scale = width > 0 && width < INFINITY ? (float)LG_SAMPLE_BINS / width : 0;      // (0: all in the first bin)
     return s;
+}
+template <int NT>
+__device__ __forceinline__ SampleSpan lg_sample_span(const SampleRow &p, const SampleWork &w, const SampleGeo &g, const double *tab, uint32_t *part) {
+    uint32_t key = 0, least = 0;
+    for (int i = threadIdx.x; i < g.groups; i += NT) { const uint32_t k = w.gmax[i]; if (k > key) key = k; }
+    for (int i = threadIdx.x; i < g.maxes; i += NT) { const uint32_t k = w.smin[i]; if (k > least) least = k; }
+    lg_block_max2<NT>(key, least, part);
+    return lg_sample_span_of(p, key, least, tab);
 }
 // Monotone in the logit, also as rounded: a larger logit never has a larger bin
 __device__ __forceinline__ int lg_sample_bin(const SampleSpan &s, float l) {
@@ -488,7 +493,6 @@ __global__ __launch_bounds__(NT) void lg_k_sample_sums(SampleArgs a, char *base)
 #define LG_SAMPLE_LIST    512                    // what stays of a small top-k
 #define LG_SAMPLE_FEW     128                    // candidates of a small top-k whose order and sums are taken pair by pair
 static_assert(LG_SAMPLE_LIST >= LG_SAMPLE_SMALL_K && LG_SAMPLE_LIST >= LG_SAMPLE_FEW, "room for what stays");
-constexpr int LG_SAMPLE_PT = LG_SAMPLE_CAND / LG_SAMPLE_WG;
 struct SampleFinishLds {
     lg_u64 sum[LG_SAMPLE_GROUPS], bin[1024], list[LG_SAMPLE_LIST], size[64], cand[LG_SAMPLE_CAND], part[LG_SAMPLE_WG / 32], part3[3], last, rest, whole;
     double tab[32];
@@ -499,54 +503,69 @@ struct SampleFinishLds {
 };
 // The candidate at which the running sum of measures, in order, reaches `want` (1 .. the sum of all); measures of 0 are no candidates.  1024 equal parts
 // between the first and the last candidate, the part that holds the border cut again until it has at most 64 of them (once for logits that lie
-// anywhere, again for a group of equal ones, by their index then), and a wavefront over these.
-__device__ __forceinline__ lg_u64 lg_among(const lg_u64 (&c)[LG_SAMPLE_PT], const lg_u64 (&m_in)[LG_SAMPLE_PT], lg_u64 want, SampleFinishLds &s) {
+// anywhere, again for a group of equal ones, by their index then), and a wavefront over these.  The parts are of the candidates as numbers, whose keys are
+// logarithms of logits; BINS: the first ones are bins of logits (`bin`, 0..1023), where the candidates are on both sides of 0 and most of the numbers between
+// them the keys of tiny logits.
+template <int PT, bool BINS, typename C, typename M, typename B>
+__device__ __forceinline__ lg_u64 lg_among(C c, M measure, B bin, lg_u64 want, SampleFinishLds &s) {          // c(i), measure(i): of this thread's PT tokens
     const int t = threadIdx.x;
-    lg_u64 m[LG_SAMPLE_PT];
-    #pragma unroll
-    for (int i = 0; i < LG_SAMPLE_PT; ++i) m[i] = m_in[i];
-    for (;;) {                                               // (every round but the last leaves out a candidate: the first and the last lie in different parts)
-        lg_u64 from = 0, to = 0;                             // from as its complement
+    uint32_t out = 0;                                        // bit i: token i is in none of the parts any more
+    auto m = [&](int i) { return out >> i & 1 ? (lg_u64)0 : measure(i); };
+    auto round = [&](auto part_of) {                         // false: the part of the border has more than 64
         #pragma unroll
-        for (int i = 0; i < LG_SAMPLE_PT; ++i) if (m[i]) { if (~c[i] > from) from = ~c[i]; if (c[i] > to) to = c[i]; }
-        s.bin[t] = 0;
-        if (t == 0) s.n = 0;
-        lg_block_max2<LG_SAMPLE_WG>(from, to, s.part);       // (its barriers: the clearing's too)
-        from = ~from;
-        const lg_u64 span = to - from;
-        const int shift = span >= 1024 ? 64 - __builtin_clzll(span) - 10 : 0;
-        #pragma unroll
-        for (int i = 0; i < LG_SAMPLE_PT; ++i) if (m[i]) atomicAdd(&s.bin[(c[i] - from) >> shift], m[i]);
+        for (int i = 0; i < PT; ++i) { const lg_u64 x = m(i); if (x) atomicAdd(&s.bin[part_of(i)], x); }
         __syncthreads();
         lg_u64 all;
         const lg_u64 mine = s.bin[t], run = lg_block_run<LG_SAMPLE_WG>(mine, s.part, &all);
         if (run >= want && run - mine < want) { s.at = t; s.rest = run - mine; }
         __syncthreads();
-        const lg_u64 part = (lg_u64)s.at;
+        const uint32_t part = (uint32_t)s.at;
         want -= s.rest;
         #pragma unroll
-        for (int i = 0; i < LG_SAMPLE_PT; ++i) {
-            if (m[i] && (c[i] - from) >> shift != part) m[i] = 0;
-            if (m[i]) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < 64) { s.list[at] = c[i]; s.size[at] = m[i]; } }
+        for (int i = 0; i < PT; ++i) {
+            const lg_u64 x = m(i);
+            if (!x) continue;
+            if (part_of(i) != part) { out |= 1u << i; continue; }
+            const uint32_t at = atomicAdd(&s.n, 1u);
+            if (at < 64) { s.list[at] = c(i); s.size[at] = x; }
         }
         __syncthreads();
-        const uint32_t n = s.n;
-        if (n > 64) { __syncthreads(); continue; }
-        if (t < 64) {
-            const lg_u64 me = (uint32_t)t < n ? s.list[t] : ~0ull, own = (uint32_t)t < n ? s.size[t] : 0;
-            lg_u64 upto = 0;
-            for (uint32_t i = 0; i < n; ++i) { const lg_u64 x = lg_lane(me, i), y = lg_lane(own, i); if (x <= me) upto += y; }
-            if (own && upto >= want && upto - own < want) s.last = me;
-        }
+        return s.n <= 64;
+    };
+    bool done = false;
+    if constexpr (BINS) {
+        s.bin[t] = 0;
+        if (t == 0) s.n = 0;
         __syncthreads();
-        return s.last;
+        done = round([&](int i) { return (uint32_t)bin(i); });
     }
+    while (!done) {                                          // (every round but the last leaves out a candidate: the first and the last lie in different parts)
+        lg_u64 from = 0, to = 0;                             // from as its complement
+        #pragma unroll
+        for (int i = 0; i < PT; ++i) if (m(i)) { const lg_u64 x = c(i); if (~x > from) from = ~x; if (x > to) to = x; }
+        lg_block_max2<LG_SAMPLE_WG>(from, to, s.part);       // (its first barrier: s.n and the bins are no longer read)
+        s.bin[t] = 0;
+        if (t == 0) s.n = 0;
+        __syncthreads();
+        from = ~from;
+        const lg_u64 span = to - from;
+        const int shift = span >= 1024 ? 64 - __builtin_clzll(span) - 10 : 0;
+        done = round([&](int i) { return (uint32_t)((c(i) - from) >> shift); });
+    }
+    if (t < 64) {
+        const uint32_t n = s.n;
+        const lg_u64 me = (uint32_t)t < n ? s.list[t] : ~0ull, own = (uint32_t)t < n ? s.size[t] : 0;
+        lg_u64 upto = 0;
+        for (uint32_t i = 0; i < n; ++i) { const lg_u64 x = lg_lane(me, i), y = lg_lane(own, i); if (x <= me) upto += y; }
+        if (own && upto >= want && upto - own < want) s.last = me;
+    }
+    __syncthreads();
+    return s.last;
 }
 
-// Whole rows of up to LG_SAMPLE_CAND tokens (WHOLE: no launch came before), or what the launches before left of longer ones
-template <bool VEC, bool WHOLE>
+// Whole rows of up to PT * 1024 tokens (WHOLE: no launch came before), or what the launches before left of longer ones (PT * 1024 = LG_SAMPLE_CAND)
+template <bool VEC, bool WHOLE, int PT>
 __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a, char *base) {
-    constexpr int PT = LG_SAMPLE_PT;
     __shared__ SampleFinishLds s;
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, n_vocab = a.n_vocab;
     const SampleRow p = a.params[r];
@@ -562,26 +581,32 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
     };
     lg_weigh_table(s.tab);
     if (t == 0) { s.n = 0; s.n_groups = 0; s.at = n_vocab; s.idx = 0; }
-    lg_u64 c[PT], m[PT];                                     // this thread's candidates and their weights
+    lg_u64 kept_c[WHOLE ? 1 : PT], m[PT];                    // this thread's candidates and their weights
+    float x[WHOLE ? PT : 1];                                 // (of a whole row its tokens: PT in a row to a thread)
+    auto c = [&](int i) { if constexpr (WHOLE) return (lg_u64)~lg_key(x[i]) << 32 | (uint32_t)(t * PT + i); else return kept_c[i]; };
     lg_u64 above = 0, total = 0, all;                        // sum of the tokens before the candidates; what top-p goes by
     SampleSpan span;
     SampleRange q{ LG_SAMPLE_BINS, -1, LG_SAMPLE_BINS, 0 };
     uint32_t kept = 0;
     int n = 0;
     if (WHOLE) {
-        uint32_t key = 0;
-        float x[PT];
+        uint32_t key = 0, least_key = 0;
         #pragma unroll
-        for (int i = 0; i < PT; ++i) { const int at = t * PT + i; x[i] = at < n_vocab ? row[at] : -INFINITY; const uint32_t k = lg_key(x[i]); if (k > key) key = k; }
-        key = lg_block_max<LG_SAMPLE_WG>(key, s.key);        // (its barriers: the table's too)
-        span.key = key; span.top = lg_unkey(key);
-        span.wg = lg_weigher(span.top, p.temperature, s.tab);
+        for (int i = 0; i < PT; i += 4) {
+            const int at = t * PT + i;
+            if (VEC && at + 3 < n_vocab) { const float4 v = *(const float4 *)(row + at); x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w; }
+            else
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) x[i + j] = at + j < n_vocab ? row[at + j] : -INFINITY;
+        }
+        #pragma unroll
+        for (int i = 0; i < PT; ++i) { const uint32_t k = lg_key(x[i]); if (k > key) key = k; if (k > 0x007FFFFFu && ~k > least_key) least_key = ~k; }
+        lg_block_max2<LG_SAMPLE_WG>(key, least_key, s.key);  // (its barriers: the table's too)
+        span = lg_sample_span_of(p, key, least_key, s.tab);
         #pragma unroll
         for (int i = 0; i < PT; ++i) {
-            const uint32_t k = lg_key(x[i]);
-            c[i] = (lg_u64)~k << 32 | (uint32_t)(t * PT + i);
             m[i] = kind != LG_ROW_FIRST && key != 0x007FFFFFu ? lg_weigh(span.wg, x[i]) : 0;
-            if (kind == LG_ROW_FIRST && k == key && t * PT + i < n_vocab) atomicMin(&s.at, t * PT + i);
+            if (kind == LG_ROW_FIRST && lg_key(x[i]) == key && t * PT + i < n_vocab) atomicMin(&s.at, t * PT + i);
         }
     } else {
         if (kind == LG_ROW_ALONE) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
@@ -591,7 +616,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) { const int at = t + i * LG_SAMPLE_WG; gk[i] = at < g.groups ? w.gmax[at] : 0; }
         if (kind == LG_ROW_BORDER) {
             #pragma unroll
-            for (int i = 0; i < PT; ++i) c[i] = w.cand[t + i * LG_SAMPLE_WG];
+            for (int i = 0; i < PT; ++i) if constexpr (!WHOLE) kept_c[i] = w.cand[t + i * LG_SAMPLE_WG];
             n = (int)*w.ncand;
             q = *(const SampleRange *)(w.ncand + 4);
         }
@@ -672,11 +697,11 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             __syncthreads();
             n = (int)s.n;
             #pragma unroll
-            for (int i = 0; i < PT; ++i) { const int at = t + i * LG_SAMPLE_WG; c[i] = at < n && at < LG_SAMPLE_CAND ? s.cand[at] : 0; }
+            for (int i = 0; i < PT; ++i) if constexpr (!WHOLE) { const int at = t + i * LG_SAMPLE_WG; kept_c[i] = at < n && at < LG_SAMPLE_CAND ? s.cand[at] : 0; }
         }
         if (n > LG_SAMPLE_CAND) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
         #pragma unroll
-        for (int i = 0; i < PT; ++i) m[i] = t + i * LG_SAMPLE_WG < n ? lg_weigh(span.wg, lg_unkey(~(uint32_t)(c[i] >> 32))) : 0;
+        for (int i = 0; i < PT; ++i) m[i] = t + i * LG_SAMPLE_WG < n ? lg_weigh(span.wg, lg_unkey(~(uint32_t)(c(i) >> 32))) : 0;
     }
     if (span.key == 0x007FFFFFu) { if (t == 0) answer(-1, 0, 0); return; }
     if (kind == LG_ROW_FIRST) {
@@ -693,7 +718,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         // what stays (three barriers; the way below takes 25)
         const uint32_t who = (uint32_t)t >> 3, sub = t & 7;
         const bool on = (int)who < n;
-        if (t < n) { s.list[t] = c[0]; s.sum[t] = m[0]; }
+        if (t < n) { s.list[t] = c(0); s.sum[t] = m[0]; }
         if (t == 0) s.last = ~0ull;
         __syncthreads();
         const lg_u64 me = on ? s.list[who] : ~0ull, own = on ? s.sum[who] : 0;
@@ -725,23 +750,23 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         }
         return;
     }
+    auto bin = [&](int i) { if constexpr (WHOLE) return lg_sample_bin(span, x[i]) * 1024 / LG_SAMPLE_BINS; else return 0; };
     // top-k, then top-p: `last` is the last token in the order that stays
     lg_u64 last = ~0ull;
     bool lost = false;                                       // the candidates do not hold the border after all
     const bool longer = !WHOLE && kind != LG_ROW_SMALL;      // the candidates are a part of what stays
     if (WHOLE || kind == LG_ROW_SMALL || q.cut < LG_SAMPLE_BINS) {
-        lg_u64 one[PT], mine = 0;
+        // (top-k counts tokens; of a longer row those of its bin)
+        auto one = [&](int i) { return (lg_u64)(m[i] && (!longer || lg_sample_bin(span, lg_unkey(~(uint32_t)(c(i) >> 32))) == q.cut)); };
+        lg_u64 mine = 0;
         #pragma unroll
-        for (int i = 0; i < PT; ++i) {
-            one[i] = m[i] && (!longer || lg_sample_bin(span, lg_unkey(~(uint32_t)(c[i] >> 32))) == q.cut);
-            mine += one[i];
-        }
+        for (int i = 0; i < PT; ++i) mine += one(i);
         const lg_u64 have = lg_block_sum<LG_SAMPLE_WG>(mine, s.part), want = p.top_k > 0 ? (lg_u64)p.top_k - (longer ? q.above : 0) : have + 1;
-        if (want < have) last = lg_among(c, one, want, s);
-        else lost = longer && want > have;
+        if (want <= have) last = lg_among<PT, WHOLE>(c, one, bin, want, s);         // (also where all of them stay: what comes behind them does not)
+        else lost = longer;
         lg_u64 sum = 0;
         #pragma unroll
-        for (int i = 0; i < PT; ++i) { if (c[i] > last) { m[i] = 0; one[i] = 0; } if (one[i]) sum += m[i]; }
+        for (int i = 0; i < PT; ++i) { if (c(i) > last) m[i] = 0; else if (one(i)) sum += m[i]; }
         if (p.top_p < 1) total += lg_block_sum<LG_SAMPLE_WG>(sum, s.part);
     }
     if (p.top_p < 1 && kind != LG_ROW_FREE && !lost) {
@@ -749,18 +774,19 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         const lg_u64 want = want_d >= 1 ? (lg_u64)want_d < total ? (lg_u64)want_d : total : 1;
         // (bins between top-p's and top-k's hold tokens that are no candidates: those of top-k's are not counted behind them)
         const bool gap = longer && q.cut < LG_SAMPLE_BINS && q.last < q.cut - 1;
-        lg_u64 in[PT], sum = 0;
+        auto in = [&](int i) { return gap && lg_sample_bin(span, lg_unkey(~(uint32_t)(c(i) >> 32))) > q.last ? (lg_u64)0 : m[i]; };
+        lg_u64 sum = 0;
         #pragma unroll
-        for (int i = 0; i < PT; ++i) { in[i] = gap && lg_sample_bin(span, lg_unkey(~(uint32_t)(c[i] >> 32))) > q.last ? 0 : m[i]; sum += in[i]; }
+        for (int i = 0; i < PT; ++i) sum += in(i);
         const lg_u64 have = lg_block_sum<LG_SAMPLE_WG>(sum, s.part);
         if (above >= want || above + have < want) lost = true;
-        else last = lg_among(c, in, want - above, s);
+        else last = lg_among<PT, WHOLE>(c, in, bin, want - above, s);
     }
     if (lost) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
     lg_u64 sum = 0;
     uint32_t mine = 0;
     #pragma unroll
-    for (int i = 0; i < PT; ++i) { if (c[i] > last || m[i] < least) m[i] = 0; sum += m[i]; mine += m[i] != 0; }
+    for (int i = 0; i < PT; ++i) { if (c(i) > last || m[i] < least) m[i] = 0; sum += m[i]; mine += m[i] != 0; }
     kept += (uint32_t)lg_block_sum<LG_SAMPLE_WG>((lg_u64)mine, s.part);
     if (WHOLE) {                                             // the candidates lie in index order
         lg_u64 run = lg_block_run<LG_SAMPLE_WG>(sum, s.part, &all) - sum;
@@ -779,7 +805,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         if (t == 0) s.n = 0;
         __syncthreads();
         #pragma unroll
-        for (int i = 0; i < PT; ++i) if (m[i]) { const uint32_t at = atomicAdd(&s.n, 1u); s.list[at] = (lg_u64)(uint32_t)c[i] << 45 | m[i]; }       // (19 bits of index, 45 of weight)
+        for (int i = 0; i < PT; ++i) if (m[i]) { const uint32_t at = atomicAdd(&s.n, 1u); s.list[at] = (lg_u64)(uint32_t)c(i) << 45 | m[i]; }       // (19 bits of index, 45 of weight)
         __syncthreads();
         const uint32_t stay = s.n, ways = stay <= LG_SAMPLE_WG / 4 ? 4 : 1, who = (uint32_t)t / ways;
         if (who < stay) {
@@ -793,7 +819,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
     }
     // the groups' sums with the candidates that stay, the group of the draw, and the token in it
     #pragma unroll
-    for (int i = 0; i < PT; ++i) if (m[i]) atomicAdd(&s.sum[(uint32_t)c[i] / LG_SAMPLE_GROUP], m[i]);
+    for (int i = 0; i < PT; ++i) if (m[i]) atomicAdd(&s.sum[(uint32_t)c(i) / LG_SAMPLE_GROUP], m[i]);
     __syncthreads();
     constexpr int GT = LG_SAMPLE_GROUPS / LG_SAMPLE_WG;
     lg_u64 gs[GT];

@@ -96,14 +96,19 @@ extern "C" int lg_hip_paged_write(const struct lg_hip_pages *p, const float *d_k
 // Workgroups of lg_k_page_attn at a time: lg_pa_per_simd on each of 256 compute units
 static int slots_of(int hd) { return 256 * lg_pa_per_simd(hd); }
 // Splits of all sequences together, at most.  lg_pa_split_tiles makes the full ones of a key head slots / n_head_kv or fewer for every round, the rounds one or 2 units / slots rounded
-// up, where splits of 4 tiles to LG_PA_CHUNK keys allow; every sequence has one that is not full besides
-struct AttnCut { int64_t splits; bool join; };
+// up, where splits of `tiles` tiles to LG_PA_CHUNK keys allow; every sequence has one that is not full besides
+// Sequences of up to so many tiles are left whole where none is longer: the launch that joins splits takes longer than what a split saves.  One sequence of 512 keys, whole
+// and in splits: heads of 64 7.5 and 8.8 us, 128 8.5 and 9.5, 256 13.9 and 11.2 (384 keys: 11.7 and 11.3); 64 sequences, 2 key heads of 256: 16.4 and 20.2; of
+// 512 (256 keys): 20.7 and 19.4 (192: 19.0 and 19.1).  128 workgroups and more are a half of the compute units at work already
+static int alone_of(int hd, int64_t units) { return hd <= 128 ? 16 : hd == 256 ? (units >= 128 ? 20 : 12) : 6; }
+struct AttnCut { int64_t splits; bool join; int least; };
 static AttnCut cut_of(int n_seq, int n_head_kv, int hd, int max_len, int window) {
     // (a window need not start with a tile)
     const int64_t span = window > 0 && window < max_len ? (int64_t)window + LG_PA_TILE - 1 : max_len, tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
-    const int64_t least = (tiles + 3) / 4, slots = slots_of(hd), units = (int64_t)n_seq * n_head_kv, rounds = std::max<int64_t>(1, (units + slots / 2 - 1) / (slots / 2));
+    const int alone = alone_of(hd, (int64_t)n_seq * n_head_kv), min_tiles = tiles <= alone ? alone : 4;
+    const int64_t least = (tiles + min_tiles - 1) / min_tiles, slots = slots_of(hd), units = (int64_t)n_seq * n_head_kv, rounds = std::max<int64_t>(1, (units + slots / 2 - 1) / (slots / 2));
     const int64_t full = std::max<int64_t>(rounds * slots / n_head_kv, n_seq * tiles / (LG_PA_CHUNK / LG_PA_TILE));
-    return { std::min<int64_t>(n_seq * std::max<int64_t>(least, 1), full + n_seq), least > 1 };
+    return { std::min<int64_t>(n_seq * std::max<int64_t>(least, 1), full + n_seq), least > 1, min_tiles };
 }
 static bool attn_shape(int n_seq, int n_head, int n_head_kv, int hd, int max_len) {
     return n_seq >= 0 && n_head_kv >= 1 && n_head_kv <= 1024 && n_head >= 1 && n_head % n_head_kv == 0 && n_head / n_head_kv <= 8 &&
@@ -148,7 +153,7 @@ extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float 
     const size_t part = up256((size_t)c.splits * n_head * 4);
     float *const w = (float *)d_work;
     const PageAttn a{ g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, w, need ? (float *)((char *)d_work + part) : nullptr,
-                      need ? (float *)((char *)d_work + 2 * part) : nullptr, scale, n_head, p->n_head_kv, n_seq, max_blocks, max_len, window, slots_of(hd) };
+                      need ? (float *)((char *)d_work + 2 * part) : nullptr, scale, n_head, p->n_head_kv, n_seq, max_blocks, max_len, window, slots_of(hd), c.least };
     hipStream_t st = (hipStream_t)stream;
     switch (hd) {
         case 64:  launch_attn<64>(a, c, st); break;
@@ -164,13 +169,17 @@ extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float 
 #define LG_SAMPLE_WIDE 16384
 // ---- sample -----------------------------------------------------------------------------------------------------
 extern "C" size_t lg_hip_sample_workspace(int rows, int n_vocab) {
-    if (rows < 0 || n_vocab <= LG_SAMPLE_CAND || n_vocab > LG_SAMPLE_VOCAB) return 0;
+    if (rows < 0 || n_vocab <= LG_SAMPLE_WHOLE || n_vocab > LG_SAMPLE_VOCAB) return 0;
     return (size_t)rows * lg_sample_geo(n_vocab).row;
 }
 
 template <bool VEC>
 static void launch_sample(SampleArgs a, int rows, char *work, hipStream_t st) {
-    if (!work) { hipLaunchKernelGGL((lg_k_sample_finish<VEC, true>), dim3(rows), dim3(LG_SAMPLE_WG), 0, st, a, work); return; }
+    if (!work) {
+        if (a.n_vocab <= 4 * LG_SAMPLE_WG) hipLaunchKernelGGL((lg_k_sample_finish<VEC, true, 4>), dim3(rows), dim3(LG_SAMPLE_WG), 0, st, a, work);
+        else hipLaunchKernelGGL((lg_k_sample_finish<VEC, true, LG_SAMPLE_WHOLE / LG_SAMPLE_WG>), dim3(rows), dim3(LG_SAMPLE_WG), 0, st, a, work);
+        return;
+    }
     const SampleGeo g = lg_sample_geo(a.n_vocab);
     const dim3 maxes((unsigned)g.maxes, rows), few((unsigned)(g.groups + 15) / 16, rows), many((unsigned)(g.groups + 63) / 64, rows);
     hipLaunchKernelGGL(lg_k_sample_max<VEC>, maxes, dim3(LG_SAMPLE_MAX_WG), 0, st, a, work);
@@ -179,7 +188,7 @@ static void launch_sample(SampleArgs a, int rows, char *work, hipStream_t st) {
     a.slices = (int)(narrow ? few : many).x;
     if (narrow) hipLaunchKernelGGL((lg_k_sample_sums<VEC, 256>), few, dim3(256), 0, st, a, work);
     else hipLaunchKernelGGL((lg_k_sample_sums<VEC, 1024>), many, dim3(1024), 0, st, a, work);
-    hipLaunchKernelGGL((lg_k_sample_finish<VEC, false>), dim3(rows), dim3(LG_SAMPLE_WG), 0, st, a, work);
+    hipLaunchKernelGGL((lg_k_sample_finish<VEC, false, LG_SAMPLE_CAND / LG_SAMPLE_WG>), dim3(rows), dim3(LG_SAMPLE_WG), 0, st, a, work);
 }
 
 extern "C" int lg_hip_sample(const float *d_logits, int64_t stride, int rows, int n_vocab, const struct lg_hip_sampling *d_params, const float *d_u,
