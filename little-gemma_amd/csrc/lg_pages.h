@@ -301,7 +301,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     constexpr int DL = HD >= 128 ? 8 : HD / 16;     // dimensions of a value load
     constexpr int CH = HD / (16 * DL);              // value loads of a key row
     constexpr int NT = HD / 16;                     // output tiles
-    constexpr int PIECES = HD > 256 ? 2 : 1, KP = KS / PIECES, CP = CH / PIECES;       // rows of 512 in two halves: two pieces of keys or values are in registers at a time
+    constexpr int HALVES = HD > 256 ? 1 : 2, TILE = 16 * HALVES;       // keys of a step: rows of 512 leave registers for a half tile (a whole one spills: one key of 512, 15.4 -> 12.4 us)
     __shared__ float s_m[LG_PA_WAVES][8], s_l[LG_PA_WAVES][8];
     __shared__ __align__(16) union { lg_h8 q[KS][64]; float o[LG_PA_WAVES][8][HD]; } s;
     __shared__ int32_t s_ids[LG_PA_CHUNK / 16 + 1];
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     if (seq < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
-    constexpr int STEP = LG_PA_WAVES * LG_PA_TILE;
+    constexpr int STEP = LG_PA_WAVES * TILE;
     const int32_t *table = a.table + (long long)seq * a.max_blocks;
     // queries are asked for first: what is asked for later arrives later, and behind the keys they would hold the first scores up
     float4 qv[KS][2];
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     lg_pa_range(a, seq, lo, len);
     const int chunk = __builtin_amdgcn_readfirstlane(cut.tiles) * LG_PA_TILE, n_split = __builtin_amdgcn_readfirstlane(cut.n);
     const int first = (lo & ~(LG_PA_TILE - 1)) + __builtin_amdgcn_readfirstlane(cut.index) * chunk, end = len < first + chunk ? len : first + chunk;
-    int t0 = first + wave * LG_PA_TILE;
+    int t0 = first + wave * TILE;
     const PageIds ids = lg_pa_ids(a, table, t0);
     // the later tiles' ids through LDS: a load of them inside the loop would be waited for together with the keys that are on their way
     const int b0 = first >> a.g.shift;
@@ -343,19 +343,19 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
         return lg_pa_tile(a, p, t, kvh * HD);
     };
 
-    lg_h8 kf[2][KP], kg[PIECES > 1 ? 2 : 1][PIECES > 1 ? KP : 1];          // the keys' first piece, and the second
+    lg_h8 kf[HALVES][KS];
     PageTile now = lg_pa_tile(a, ids, t0, kvh * HD);
     if (t0 >= end) now.row[0] = now.row[1] = kvh * HD;          // (no tile: page 0's rows, so that the loads need no branch, after which everything would be waited for)
-    auto load_keys = [&](const PageTile &p, auto &to, int piece) {
+    auto load_keys = [&](const PageTile &p) {
         #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint16_t *kp = a.g.k + p.row[h] + c * a.g.row_stride + g * 8 + piece * KP * 32;
+        for (int h = 0; h < HALVES; ++h) {
+            const uint16_t *kp = a.g.k + p.row[h] + c * a.g.row_stride + g * 8;
             #pragma unroll
-            for (int i = 0; i < KP; ++i) to[h][i] = *(const lg_h8 *)(kp + i * 32);
+            for (int i = 0; i < KS; ++i) kf[h][i] = *(const lg_h8 *)(kp + i * 32);
         }
     };
     __builtin_amdgcn_sched_barrier(0);
-    load_keys(now, kf, 0);
+    load_keys(now);
     __builtin_amdgcn_sched_barrier(0);
     if (has_id) s_ids[threadIdx.x] = my_id;
 
@@ -375,9 +375,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
         #pragma unroll
         for (int i = 0; i < KS; ++i) {
             if (i % LG_PA_WAVES != wave) continue;
-            // (rows of 512 are read again: beside the keys they do not stay in registers)
-            const float4 x = PIECES > 1 ? query(i, 0) : qv[i][0], y = PIECES > 1 ? query(i, 1) : qv[i][1];
-            const float v[8] = { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w };
+            const float v[8] = { qv[i][0].x, qv[i][0].y, qv[i][0].z, qv[i][0].w, qv[i][1].x, qv[i][1].y, qv[i][1].z, qv[i][1].w };
             lg_h8 part;
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -395,55 +393,37 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     for (int i = 0; i < NT; ++i) acc[i] = (lg_f4){ 0, 0, 0, 0 };
     float m = -INFINITY, l = 0;                     // of query row c; l of this lane's keys alone
 
-    // One tile: its values are requested before its scores are made, the next tile's keys before its values are used.  (In two pieces: each a stage ahead.)
+    // One tile: its values are requested before its scores are made, the next tile's keys before its values are used
     auto work = [&](auto more) {                    // more: a tile follows (a branch around its loads would have them waited for with this tile's)
         constexpr bool MORE = decltype(more)::value;
         const PageTile here = now;
-        PageTile coming = now;
-        if constexpr (MORE) coming = tile_at(t0 + STEP);
-        uint32_t w[CP][8][DL / 2], w2[PIECES > 1 ? CP : 1][8][DL / 2];
-        auto load_values = [&](auto &to, int piece) {
+        if constexpr (MORE) now = tile_at(t0 + STEP);
+        uint32_t w[CH][4 * HALVES][DL / 2];
+        #pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
             #pragma unroll
-            for (int ch = 0; ch < CP; ++ch)
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint16_t *vp = a.g.v + here.row[j >> 2] + (4 * g + (j & 3)) * a.g.row_stride + (piece * CP + ch) * 128 + c * DL;
-                    if constexpr (DL == 8) { const uint4 u = *(const uint4 *)vp; to[ch][j][0] = u.x; to[ch][j][1] = u.y; to[ch][j][2] = u.z; to[ch][j][3] = u.w; }
-                    else { const uint2 u = *(const uint2 *)vp; to[ch][j][0] = u.x; to[ch][j][1] = u.y; }
-                }
-        };
-        lg_f4 sc[2] = { { 0, 0, 0, 0 }, { 0, 0, 0, 0 } };
-        auto scores = [&](const auto &k, int piece) {
-            #pragma unroll
-            for (int i = 0; i < KP; ++i) {
-                const lg_h8 q = s.q[piece * KP + i][lane];
-                sc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][i], q, sc[0], 0, 0, 0);
-                sc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][i], q, sc[1], 0, 0, 0);
+            for (int j = 0; j < 4 * HALVES; ++j) {
+                const uint16_t *vp = a.g.v + here.row[j >> 2] + (4 * g + (j & 3)) * a.g.row_stride + ch * 128 + c * DL;
+                if constexpr (DL == 8) { const uint4 u = *(const uint4 *)vp; w[ch][j][0] = u.x; w[ch][j][1] = u.y; w[ch][j][2] = u.z; w[ch][j][3] = u.w; }
+                else { const uint2 u = *(const uint2 *)vp; w[ch][j][0] = u.x; w[ch][j][1] = u.y; }
             }
-        };
-        if constexpr (PIECES > 1) {
-            load_keys(here, kg, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            scores(kf, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            load_values(w, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            scores(kg, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            load_values(w2, 1);
-        } else {
-            load_values(w, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            scores(kf, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (MORE) load_keys(coming, kf, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        lg_f4 sc[HALVES];
+        #pragma unroll
+        for (int h = 0; h < HALVES; ++h) sc[h] = (lg_f4){ 0, 0, 0, 0 };
+        #pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            const lg_h8 q = s.q[i][lane];
+            #pragma unroll
+            for (int h = 0; h < HALVES; ++h) sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][i], q, sc[h], 0, 0, 0);
         }
-        now = coming;
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (MORE) load_keys(now);
         __builtin_amdgcn_sched_barrier(0);
         // base-2 exponents; rows c and c + 8 hold the two parts of a query's score
-        float x[2][4], top = -INFINITY;
+        float x[HALVES][4], top = -INFINITY;
         #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < HALVES; ++h)
             #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float both = sc[h][r] + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(sc[h][r]), 0x128, 0xF, 0xF, true));   // row_ror:8
@@ -465,9 +445,10 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
                 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[i][r] *= fr[r];
         }
-        lg_h8 pf;
+        typedef _Float16 part __attribute__((ext_vector_type(4 * HALVES)));
+        part pf;
         #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < HALVES; ++h)
             #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float p = x[h][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[h][r] - m + 14.0f);
@@ -476,38 +457,29 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
                 pf[4 * h + r] = c < 8 ? hi : (_Float16)(p - (float)hi);
             }
         // a masked key's values may be anything (0 * inf is not 0): zeros in their place
-        const bool whole = t0 >= lo && t0 + LG_PA_TILE <= end && here.ok[0] && here.ok[1];
-        auto values = [&](auto &v, int piece) {
-            if (!whole) {
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                    if (!(here.ok[j >> 2] && t >= lo && t < end)) {
+        if (!(t0 >= lo && t0 + TILE <= end && here.ok[0] && here.ok[HALVES - 1])) {
+            #pragma unroll
+            for (int j = 0; j < 4 * HALVES; ++j) {
+                const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                if (!(here.ok[j >> 2] && t >= lo && t < end)) {
+                    #pragma unroll
+                    for (int ch = 0; ch < CH; ++ch)
                         #pragma unroll
-                        for (int ch = 0; ch < CP; ++ch)
-                            #pragma unroll
-                            for (int i = 0; i < DL / 2; ++i) v[ch][j][i] = 0;
-                    }
+                        for (int i = 0; i < DL / 2; ++i) w[ch][j][i] = 0;
                 }
             }
-            #pragma unroll
-            for (int ch = 0; ch < CP; ++ch)
-                #pragma unroll
-                for (int i = 0; i < DL; ++i) {
-                    union { uint32_t u[4]; lg_h8 h; } b;
-                    #pragma unroll
-                    for (int k2 = 0; k2 < 4; ++k2) b.u[k2] = __builtin_amdgcn_perm(v[ch][2 * k2 + 1][i >> 1], v[ch][2 * k2][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
-                    lg_f4 &to = acc[(piece * CP + ch) * DL + i];
-                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, b.h, to, 0, 0, 0);
-                }
-        };
-        values(w, 0);
-        if constexpr (PIECES > 1) {
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (MORE) load_keys(coming, kf, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            values(w2, 1);
         }
+        #pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
+            #pragma unroll
+            for (int i = 0; i < DL; ++i) {
+                union { uint32_t u[2 * HALVES]; part h; } b;
+                #pragma unroll
+                for (int k2 = 0; k2 < 2 * HALVES; ++k2) b.u[k2] = __builtin_amdgcn_perm(w[ch][2 * k2 + 1][i >> 1], w[ch][2 * k2][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
+                lg_f4 &to = acc[ch * DL + i];
+                if constexpr (HALVES == 2) to = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, b.h, to, 0, 0, 0);
+                else to = __builtin_amdgcn_mfma_f32_16x16x16f16(pf, b.h, to, 0, 0, 0);
+            }
     };
     for (; t0 + STEP < end; t0 += STEP) work(std::true_type{});
     if (t0 < end) work(std::false_type{});

@@ -59,9 +59,7 @@ struct Weigh { double top, inv; const double *tab; };
 // comes after r^5 is 2e-15).  Adding 1.5 2^52 leaves n in the low bits, adding 2^52 the result.  Beyond LG_SAMPLE_REACH it is 0.  (The series of e^r to r^12
 // without the table is 25 operations in place of 14: lg_k_sample_sums of 5 rows of 262144 21.0 -> @SUMS@ us with it.)
 #define LG_SAMPLE_REACH   31.5
-__device__ __forceinline__ lg_u64 lg_weigh(const Weigh &w, float l) {
-    const double y = l == (float)w.top ? 0.0 : ((double)l - w.top) * w.inv;
-    if (!(y >= -LG_SAMPLE_REACH * 46.166241308446828384) || l == -INFINITY) return 0;
+__device__ __forceinline__ lg_u64 lg_weight_at(const Weigh &w, double y) {          // y of -LG_SAMPLE_REACH 32 / ln 2 .. 0
     const double t = y + 6755399441055744.0, r = y - (t - 6755399441055744.0);
     const int n = (int)(uint32_t)(lg_u64)__double_as_longlong(t);
     double p = 3.9737099845494161e-11;
@@ -73,9 +71,17 @@ __device__ __forceinline__ lg_u64 lg_weigh(const Weigh &w, float l) {
     const double scale = __longlong_as_double(__double_as_longlong(w.tab[n & 31]) + ((long long)(44 + (n >> 5)) << 52));
     return (lg_u64)__double_as_longlong(__builtin_fma(p, scale, 4503599627370496.0)) & 0x000FFFFFFFFFFFFFull;
 }
+__device__ __forceinline__ lg_u64 lg_weigh(const Weigh &w, float l) {
+    const double y = l == (float)w.top ? 0.0 : ((double)l - w.top) * w.inv;
+    return y >= -LG_SAMPLE_REACH * 46.166241308446828384 && l != -INFINITY ? lg_weight_at(w, y) : 0;
+}
+// The same for a finite maximum and a logit whose exponent is known to be above LG_SAMPLE_FLOOR (in base 2, to an f32's accuracy; a weight is 0 below -45)
+#define LG_SAMPLE_FLOOR   -45.2f
+__device__ __forceinline__ lg_u64 lg_weight(const Weigh &w, float l) { return lg_weight_at(w, ((double)l - w.top) * w.inv); }
 __device__ __forceinline__ Weigh lg_weigher(float top, float T, const double *tab) { return { (double)top, T > 0 ? 46.166241308446828384 / (double)T : 0.0, tab }; }
-// (the caller's next barrier is the table's)
-__device__ __forceinline__ void lg_weigh_table(double *tab) { if (threadIdx.x < 32) tab[threadIdx.x] = lg_exp2_32nds[threadIdx.x]; }
+// The table on its way: asked for first, stored once the kernel's other loads are asked for (the caller's next barrier is the table's)
+__device__ __forceinline__ double lg_table_entry() { return lg_exp2_32nds[threadIdx.x & 31]; }
+__device__ __forceinline__ void lg_table_store(double *tab, double entry) { if (threadIdx.x < 32) tab[threadIdx.x] = entry; }
 
 // One workgroup, one row: the border by digits of the key (4 passes of 8 bits each for top-k and top-p), then the draw.
 struct SampleLds { lg_u64 bin[256]; lg_u64 part[LG_SAMPLE_WG / 64]; uint32_t key; int idx; lg_u64 rest; };    // (tab: the caller's)
@@ -83,7 +89,7 @@ struct SampleLds { lg_u64 bin[256]; lg_u64 part[LG_SAMPLE_WG / 64]; uint32_t key
 // The key at which a running sum from the largest key down reaches `want` (1..sum of all), among the tokens in question with keys >= low (of key `low`
 // itself the first `ties` count); *before = the sum of the tokens with larger keys.  BY_COUNT: every token counts 1, else its weight.
 template <bool BY_COUNT>
-__device__ uint32_t lg_border(const SampleArgs &a, const float *row, const Weigh &wg, uint32_t low, int ties, lg_u64 want, lg_u64 *before, SampleLds &s) {
+__device__ __forceinline__ uint32_t lg_border(const SampleArgs &a, const float *row, const Weigh &wg, uint32_t low, int ties, lg_u64 want, lg_u64 *before, SampleLds &s) {
     uint32_t prefix = 0, mask = 0;
     lg_u64 above = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
@@ -113,9 +119,8 @@ __device__ uint32_t lg_border(const SampleArgs &a, const float *row, const Weigh
     return prefix;
 }
 
-__device__ void lg_sample_row(const SampleArgs &a, int r, const double *tab, SampleLds &s) {
+__device__ __forceinline__ void lg_sample_row(const SampleArgs &a, int r, const SampleRow &p, const double *tab, SampleLds &s) {
     const float *row = a.logits + r * a.stride;
-    const SampleRow p = a.params[r];
     const int n = a.n_vocab, t = threadIdx.x;
     // the largest logit, and the first token that has it
     uint32_t key = 0; int at = n;
@@ -338,13 +343,14 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_bins(SampleArgs a, c
     if (lg_row_kind(p, a.n_vocab) != LG_ROW_BORDER) return;
     const SampleWork w = lg_sample_work(base, g, r);
     const float *row = a.logits + r * a.stride;
+    const double entry = lg_table_entry();
     float l[4][4];
     #pragma unroll
     for (int j = 0; j < 4; ++j) lg_load4<VEC>(row, a.n_vocab, slice * (NT / 16) + j * (NT / 64) + wave, l[j]);
-    lg_weigh_table(tab);
+    lg_table_store(tab, entry);
     for (int i = threadIdx.x; i < LG_SAMPLE_BINS; i += NT) { mass[i] = 0; count[i] = 0; }
     const SampleSpan s = lg_sample_span<NT>(p, w, g, tab, part);                      // (its barriers are the clearing's too)
-    if (s.key == 0x007FFFFFu) return;
+    if (s.key == 0x007FFFFFu || s.top == INFINITY) return;
     const bool by_count = p.top_k > 0 && p.top_k < a.n_vocab, by_mass = p.top_p < 1;
     #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -435,49 +441,61 @@ __global__ __launch_bounds__(NT) void lg_k_sample_sums(SampleArgs a, char *base)
     if (kind != LG_ROW_BORDER && kind != LG_ROW_FREE) return;
     const SampleWork w = lg_sample_work(base, g, r);
     const float *row = a.logits + r * a.stride;
+    const double entry = lg_table_entry();
     float l[4][4];
     #pragma unroll
     for (int j = 0; j < 4; ++j) lg_load4<VEC>(row, a.n_vocab, slice * (NT / 16) + j * (NT / 64) + wave, l[j]);
-    lg_weigh_table(tab);
+    lg_table_store(tab, entry);
     if (threadIdx.x < 3) s_sum[threadIdx.x] = 0;
     if (threadIdx.x == 3) s_n = 0;
-    const bool border = kind == LG_ROW_BORDER, by_mass = border && p.top_p < 1;
+    const bool border = kind == LG_ROW_BORDER;
     SampleRange q{ LG_SAMPLE_BINS, -1, LG_SAMPLE_BINS, 0 };
     if (border) {
         q = lg_sample_range<NT>(a, p, w, s_range);
         if (slice == 0 && threadIdx.x == 0) *(SampleRange *)(w.ncand + 4) = q;
     }
     const SampleSpan s = lg_sample_span<NT>(p, w, g, tab, part);
-    if (s.key == 0x007FFFFFu) return;
+    if (s.key == 0x007FFFFFu || s.top == INFINITY) return;
     const lg_u64 least = lg_least(p);
-    const float floor_ = !border && least > 1 ? __builtin_amdgcn_logf((float)least * 5.684341886080802e-14f) - 0.01f : -46.0f;       // (2^-44; in base 2)
-    lg_u64 above = 0, total = 0;
+    // What is behind top-k's bin, or below min-p where nothing else is asked, needs no weight (a little more than that gets one); a wavefront without such a
+    // token goes on, one with some does all of its lanes without branches
+    float floor_ = LG_SAMPLE_FLOOR;
+    if (border && q.cut < LG_SAMPLE_BINS && s.scale > 0) floor_ = fmaxf(floor_, s.c * ((float)(q.cut + 1) / s.scale) * 1.0001f - 0.01f);
+    if (!border && least > 1) floor_ = fmaxf(floor_, __builtin_amdgcn_logf((float)least * 5.684341886080802e-14f) - 0.01f);       // (2^-44; in base 2)
+    lg_u64 whole = 0, above = 0;                               // sums of all before top-k's bin and of those above the candidates
     uint32_t kept = 0;
     #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int grp = slice * (NT / 16) + j * (NT / 64) + wave;
-        lg_u64 sum = 0;
+        lg_u64 sum = 0, of_group = 0;
+        uint32_t cands = 0;
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float x = l[j][i], e = x == s.top ? 0.0f : (s.top - x) * s.c;
-            if (!(e > floor_)) continue;
+            const float x = l[j][i];
+            const bool needed = (s.top - x) * s.c > floor_;
+            if (!__any(needed)) continue;
+            const lg_u64 wt = needed ? lg_weight(s.wg, x) : 0;
             const int b = border ? lg_sample_bin(s, x) : 0;
-            const bool cand = border && ((b >= q.first && b <= q.last) || b == q.cut);
-            if (!(b < q.first || cand || (by_mass && b < q.cut))) continue;
-            const lg_u64 wt = lg_weigh(s.wg, x);
-            if (by_mass && b < q.cut) total += wt;
-            if (b < q.first) { above += wt; if (wt >= least) { sum += wt; ++kept; } }
-            if (cand && wt) {
-                const uint32_t at = atomicAdd(&s_n, 1u);
-                const lg_u64 c = (lg_u64)~lg_key(x) << 32 | (uint32_t)(grp * LG_SAMPLE_GROUP + lane * 4 + i);
-                if (at < ROOM) s_cand[at] = c;
-            }
+            const bool in = b < q.first, stays = in && wt >= least;
+            whole += b < q.cut ? wt : 0;
+            of_group += in ? wt : 0;
+            sum += stays ? wt : 0;
+            kept += stays;
+            cands |= (uint32_t)(border && !in && wt && (b <= q.last || b == q.cut)) << i;
         }
+        above += of_group;
+        if (cands)
+            #pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (cands >> i & 1) {
+                    const uint32_t at = atomicAdd(&s_n, 1u);
+                    if (at < ROOM) s_cand[at] = (lg_u64)~lg_key(l[j][i]) << 32 | (uint32_t)(grp * LG_SAMPLE_GROUP + lane * 4 + i);
+                }
         sum = lg_wave_total(sum);
         if (lane == 0 && grp < g.groups) w.gsum[grp] = sum;
     }
-    above = lg_wave_total(above); total = lg_wave_total(total); kept = lg_wave_total(kept);
-    if (lane == 0) { atomicAdd(&s_sum[0], above); atomicAdd(&s_sum[1], total); atomicAdd(&s_sum[2], (lg_u64)kept); }
+    above = lg_wave_total(above); whole = lg_wave_total(whole); kept = lg_wave_total(kept);
+    if (lane == 0) { atomicAdd(&s_sum[0], above); atomicAdd(&s_sum[1], whole); atomicAdd(&s_sum[2], (lg_u64)kept); }
     __syncthreads();
     if (threadIdx.x < 3) w.part[slice * 3 + threadIdx.x] = s_sum[threadIdx.x];
     if (border && s_n) {
@@ -532,14 +550,25 @@ __device__ __forceinline__ lg_u64 lg_among(C c, M measure, B bin, lg_u64 want, S
         __syncthreads();
         return s.n <= 64;
     };
-    bool done = false;
+    bool done;
     if constexpr (BINS) {
         s.bin[t] = 0;
         if (t == 0) s.n = 0;
         __syncthreads();
         done = round([&](int i) { return (uint32_t)bin(i); });
+    } else {                                                 // by the keys alone
+        uint32_t from = 0, to = 0;
+        #pragma unroll
+        for (int i = 0; i < PT; ++i) if (measure(i)) { const uint32_t x = (uint32_t)(c(i) >> 32); if (~x > from) from = ~x; if (x > to) to = x; }
+        s.bin[t] = 0;
+        if (t == 0) s.n = 0;
+        lg_block_max2<LG_SAMPLE_WG>(from, to, s.key);        // (its barriers are the clearing's too)
+        from = ~from;
+        const uint32_t span = to - from;
+        const int shift = span >= 1024 ? 32 - __builtin_clz(span) - 10 : 0;
+        done = round([&](int i) { return ((uint32_t)(c(i) >> 32) - from) >> shift; });
     }
-    while (!done) {                                          // (every round but the last leaves out a candidate: the first and the last lie in different parts)
+    while (!done) {                                          // by key and index (every round but the last leaves out a candidate: the first and the last lie in different parts)
         lg_u64 from = 0, to = 0;                             // from as its complement
         #pragma unroll
         for (int i = 0; i < PT; ++i) if (m(i)) { const lg_u64 x = c(i); if (~x > from) from = ~x; if (x > to) to = x; }
@@ -564,11 +593,11 @@ __device__ __forceinline__ lg_u64 lg_among(C c, M measure, B bin, lg_u64 want, S
 }
 
 // Whole rows of up to PT * 1024 tokens (WHOLE: no launch came before), or what the launches before left of longer ones (PT * 1024 = LG_SAMPLE_CAND)
+// False: the row is to be taken from its logits alone
 template <bool VEC, bool WHOLE, int PT>
-__global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a, char *base) {
-    __shared__ SampleFinishLds s;
+__device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base, const SampleRow &p, SampleFinishLds &s) {
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, n_vocab = a.n_vocab;
-    const SampleRow p = a.params[r];
+    const double entry = lg_table_entry();
     const float *row = a.logits + r * a.stride, u = a.u[r];
     const SampleGeo g = lg_sample_geo(n_vocab);
     const SampleWork w = WHOLE ? SampleWork{} : lg_sample_work(base, g, r);
@@ -579,7 +608,6 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         if (a.prob) a.prob[r] = (float)prob;
         if (a.kept) a.kept[r] = kept;
     };
-    lg_weigh_table(s.tab);
     if (t == 0) { s.n = 0; s.n_groups = 0; s.at = n_vocab; s.idx = 0; }
     lg_u64 kept_c[WHOLE ? 1 : PT], m[PT];                    // this thread's candidates and their weights
     float x[WHOLE ? PT : 1];                                 // (of a whole row its tokens: PT in a row to a thread)
@@ -601,6 +629,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         }
         #pragma unroll
         for (int i = 0; i < PT; ++i) { const uint32_t k = lg_key(x[i]); if (k > key) key = k; if (k > 0x007FFFFFu && ~k > least_key) least_key = ~k; }
+        lg_table_store(s.tab, entry);
         lg_block_max2<LG_SAMPLE_WG>(key, least_key, s.key);  // (its barriers: the table's too)
         span = lg_sample_span_of(p, key, least_key, s.tab);
         #pragma unroll
@@ -609,11 +638,11 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             if (kind == LG_ROW_FIRST && lg_key(x[i]) == key && t * PT + i < n_vocab) atomicMin(&s.at, t * PT + i);
         }
     } else {
-        if (kind == LG_ROW_ALONE) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
+        if (kind == LG_ROW_ALONE) { lg_table_store(s.tab, entry); return false; }
         // what the launches before left, all requested at once
         uint32_t gk[LG_SAMPLE_GROUPS / LG_SAMPLE_WG];
         #pragma unroll
-        for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) { const int at = t + i * LG_SAMPLE_WG; gk[i] = at < g.groups ? w.gmax[at] : 0; }
+        for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) { const int at = t + i * LG_SAMPLE_WG; gk[i] = w.gmax[at < g.groups ? at : 0]; if (at >= g.groups) gk[i] = 0; }
         if (kind == LG_ROW_BORDER) {
             #pragma unroll
             for (int i = 0; i < PT; ++i) if constexpr (!WHOLE) kept_c[i] = w.cand[t + i * LG_SAMPLE_WG];
@@ -629,8 +658,19 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             }
             for (int i = t; i < LG_SAMPLE_GROUPS; i += LG_SAMPLE_WG) s.sum[i] = i < g.groups ? w.gsum[i] : 0;
         }
-        span = lg_sample_span<LG_SAMPLE_WG>(p, w, g, s.tab, s.key);          // (its barriers are the sums' too)
+        lg_table_store(s.tab, entry);
+        uint32_t low = 0;                                    // ~key of the smallest of the groups' largest logits
+        if (kind == LG_ROW_SMALL) {
+            uint32_t key = 0;
+            #pragma unroll
+            for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) { if (gk[i] > key) key = gk[i]; if (gk[i] > 0x007FFFFFu && ~gk[i] > low) low = ~gk[i]; }
+            s.bin[t] = 0;
+            lg_block_max2<LG_SAMPLE_WG>(key, low, s.key);
+            span = lg_sample_span_of(p, key, low, s.tab);
+            low = ~low;
+        } else span = lg_sample_span<LG_SAMPLE_WG>(p, w, g, s.tab, s.key);   // (its barriers are the sums' too)
         if (kind == LG_ROW_BORDER || kind == LG_ROW_FREE) { above = s.part3[0]; total = s.part3[1]; kept = (uint32_t)s.part3[2]; }
+        if (span.top == INFINITY && (kind == LG_ROW_BORDER || kind == LG_ROW_FREE)) return false;      // (the launches before left nothing)
         if (span.key != 0x007FFFFFu && kind == LG_ROW_FIRST) {
             #pragma unroll
             for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) if (gk[i] == span.key) atomicMin(&s.at, t + i * LG_SAMPLE_WG);
@@ -647,11 +687,6 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             }
         } else if (kind == LG_ROW_SMALL) {
             // a logit that at least top_k groups reach: the lower edge of one of 1024 equal parts between the groups' smallest and largest maxima
-            uint32_t low = 0;                                // as ~key
-            #pragma unroll
-            for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) if (gk[i] > 0x007FFFFFu && ~gk[i] > low) low = ~gk[i];
-            s.bin[t] = 0;
-            low = ~lg_block_max<LG_SAMPLE_WG>(low, s.key);
             const uint32_t wide = span.key - low;
             const int shift = wide >= 1024 ? 32 - __builtin_clz(wide) - 10 : 0;
             #pragma unroll
@@ -665,18 +700,19 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) if (gk[i] >= from) s.groups[atomicAdd(&s.n_groups, 1u)] = t + i * LG_SAMPLE_WG;
             __syncthreads();
             const int n_groups = (int)s.n_groups;
-            for (int at = wave; at < n_groups; at += 4 * (LG_SAMPLE_WG / 64)) {             // four groups of a wavefront on their way together
-                float l[4][4];
-                uint32_t grp[4];
+            constexpr int AT_ONCE = 6;
+            for (int at = wave; at < n_groups; at += AT_ONCE * (LG_SAMPLE_WG / 64)) {      // groups of a wavefront on their way together: k = 64 takes 66 to 80 in all
+                float l[AT_ONCE][4];
+                uint32_t grp[AT_ONCE];
                 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < AT_ONCE; ++j) {
                     const int b = at + j * (LG_SAMPLE_WG / 64);
                     grp[j] = b < n_groups ? s.groups[b] : g.groups;                         // (behind the row's end: -inf)
                     lg_load4<VEC>(row, n_vocab, (int)grp[j], l[j]);
                 }
                 uint32_t found = 0;
                 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < AT_ONCE; ++j)
                     #pragma unroll
                     for (int i = 0; i < 4; ++i) found += lg_key(l[j][i]) >= from;
                 uint32_t to = lg_wave_run(found);
@@ -685,7 +721,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
                 if (lane == 0) first = atomicAdd(&s.n, of_all);
                 to += lg_lane(first, 0) - found;
                 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < AT_ONCE; ++j)
                     #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t k = lg_key(l[j][i]);
@@ -699,15 +735,15 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             #pragma unroll
             for (int i = 0; i < PT; ++i) if constexpr (!WHOLE) { const int at = t + i * LG_SAMPLE_WG; kept_c[i] = at < n && at < LG_SAMPLE_CAND ? s.cand[at] : 0; }
         }
-        if (n > LG_SAMPLE_CAND) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
+        if (n > LG_SAMPLE_CAND) return false;
         #pragma unroll
         for (int i = 0; i < PT; ++i) m[i] = t + i * LG_SAMPLE_WG < n ? lg_weigh(span.wg, lg_unkey(~(uint32_t)(c(i) >> 32))) : 0;
     }
-    if (span.key == 0x007FFFFFu) { if (t == 0) answer(-1, 0, 0); return; }
+    if (span.key == 0x007FFFFFu) { if (t == 0) answer(-1, 0, 0); return true; }
     if (kind == LG_ROW_FIRST) {
         __syncthreads();
         if (t == 0) answer(s.at, 1, 1);
-        return;
+        return true;
     }
     auto target_of = [&](lg_u64 S) {
         const lg_u64 x = u > 0 ? (lg_u64)__builtin_floor((u < 1 ? (double)u : 1.0) * (double)S) : 0;
@@ -724,8 +760,9 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         const lg_u64 me = on ? s.list[who] : ~0ull, own = on ? s.sum[who] : 0;
         lg_u64 upto = 0;
         uint32_t place = 0;
-        if (on) for (uint32_t i = sub; (int)i < n; i += 8) { const lg_u64 x = s.sum[i]; if (x && s.list[i] <= me) { upto += x; ++place; } }
-        for (int o = 1; o < 8; o <<= 1) { upto += __shfl_xor(upto, o); place += (uint32_t)__shfl_xor((int)place, o); }
+        #pragma unroll 4
+        for (uint32_t i = sub; on && (int)i < n; i += 8) { const lg_u64 x = s.sum[i]; if (x && s.list[i] <= me) { upto += x; ++place; } }
+        upto = lg_eight_total(upto); place = lg_eight_total(place);
         // (a weight of 0 is the end of the order: no candidate)
         if (t == 0) { s.whole = 0; s.n = 0; }
         __syncthreads();
@@ -739,16 +776,17 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         const lg_u64 last = s.last;
         lg_u64 S = 0, run = 0;
         uint32_t stay = 0;
-        if (on) for (uint32_t i = sub; (int)i < n; i += 8) {
+        #pragma unroll 4
+        for (uint32_t i = sub; on && (int)i < n; i += 8) {
             const lg_u64 x = s.list[i], y = s.sum[i];
             if (x <= last && y >= least) { S += y; ++stay; if ((uint32_t)x <= (uint32_t)me) run += y; }
         }
-        for (int o = 1; o < 8; o <<= 1) { S += __shfl_xor(S, o); run += __shfl_xor(run, o); stay += (uint32_t)__shfl_xor((int)stay, o); }
+        S = lg_eight_total(S); run = lg_eight_total(run); stay = lg_eight_total(stay);
         if (own >= least && me <= last && sub == 0) {
             const lg_u64 target = target_of(S);
             if (run > target && run - own <= target) answer((int)(uint32_t)me, (double)own / (double)S, (int)stay);
         }
-        return;
+        return true;
     }
     auto bin = [&](int i) { if constexpr (WHOLE) return lg_sample_bin(span, x[i]) * 1024 / LG_SAMPLE_BINS; else return 0; };
     // top-k, then top-p: `last` is the last token in the order that stays
@@ -782,7 +820,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
         if (above >= want || above + have < want) lost = true;
         else last = lg_among<PT, WHOLE>(c, in, bin, want - above, s);
     }
-    if (lost) { __syncthreads(); lg_sample_row(a, r, s.tab, s.alone); return; }
+    if (lost) return false;
     lg_u64 sum = 0;
     uint32_t mine = 0;
     #pragma unroll
@@ -796,7 +834,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             if (m[i] && run <= target && run + m[i] > target) answer(t * PT + i, (double)m[i] / (double)all, (int)kept);
             run += m[i];
         }
-        return;
+        return true;
     }
     if (kind == LG_ROW_SMALL) {
         // at most LG_SAMPLE_SMALL_K stay: each one's running sum in index order from all of them, by four threads each where there are few
@@ -815,7 +853,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             if (ways == 4) { upto += __shfl_xor(upto, 1); upto += __shfl_xor(upto, 2); }
             if ((uint32_t)t % ways == 0 && upto > target && upto - weight <= target) answer((int)(me >> 45), (double)weight / (double)all, (int)kept);
         }
-        return;
+        return true;
     }
     // the groups' sums with the candidates that stay, the group of the draw, and the token in it
     #pragma unroll
@@ -854,4 +892,13 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a,
             at += wt[i];
         }
     }
+    return true;
+}
+template <bool VEC, bool WHOLE, int PT>
+__global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_finish(SampleArgs a, char *base) {
+    __shared__ SampleFinishLds s;
+    const SampleRow p = a.params[blockIdx.x];
+    if (lg_sample_finish<VEC, WHOLE, PT>(a, base, p, s)) return;
+    __syncthreads();
+    lg_sample_row(a, blockIdx.x, p, s.tab, s.alone);
 }

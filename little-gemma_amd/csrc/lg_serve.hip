@@ -99,7 +99,7 @@ static int slots_of(int hd) { return 256 * lg_pa_per_simd(hd); }
 // up, where splits of `tiles` tiles to LG_PA_CHUNK keys allow; every sequence has one that is not full besides
 // Sequences of up to so many tiles are left whole where none is longer: the launch that joins splits takes longer than what a split saves.  One sequence of 512 keys, whole
 // and in splits: heads of 64 7.5 and 8.8 us, 128 8.5 and 9.5, 256 13.9 and 11.2 (384 keys: 11.7 and 11.3); 64 sequences, 2 key heads of 256: 16.4 and 20.2; of
-// 512 (256 keys): 20.7 and 19.4 (192: 19.0 and 19.1).  128 workgroups and more are a half of the compute units at work already
+// 512 192 keys 18.0 and 19.7, 256 20.2 and 19.8.  128 workgroups and more are a half of the compute units at work already
 static int alone_of(int hd, int64_t units) { return hd <= 128 ? 16 : hd == 256 ? (units >= 128 ? 20 : 12) : 6; }
 struct AttnCut { int64_t splits; bool join; int least; };
 static AttnCut cut_of(int n_seq, int n_head_kv, int hd, int max_len, int window) {
