@@ -331,6 +331,14 @@ size_t lg_hip_sample_workspace(int rows, int n_vocab);
 int    lg_hip_sample(const float *d_logits, int64_t stride, int rows, int n_vocab, const struct lg_hip_sampling *d_params, const float *d_u,
                      int32_t *d_tok, float *d_prob, int32_t *d_kept, void *d_work, size_t work_bytes, void *stream);
 
+/* lg_hip_forward_spec with drawn tokens in place of greedy ones: out[j] = the token that lg_hip_sample draws from row j's logits by u[j], all
+ * rows with the parameters *how (host memory, like u), *adv = 1 + number of leading drafts that equal the token drawn before them, the hidden state
+ * that of row *adv - 1.  Numbers that belong to positions (u[j] that of position pos + j, whatever the block) make a generation the same with and
+ * without drafts.  Needs the "store_logits" option; the logits stay on the device (the reference's sampling hook reads every row,
+ * src/cuda/mtp-kernel.cuh:103-118).  A row without a token (lg_hip_sample) gives -1. */
+int    lg_hip_forward_sample(lg_hip_model *m, lg_hip_kv *kv, const int32_t *toks, int n_rows, int pos, const struct lg_hip_sampling *how,
+                             const float *u, int32_t *out, int32_t *adv);
+
 /* ffn_down of a verify block of 4..8 rows on the matrix cores (lg_k_down_m), in isolation: act = rows x FF floats (quantized
  * to q8 on the device, as the gate/up kernel's epilogue does), down = FF-wide q4_0 rows of the E outputs; out = rows x E,
  * the four K-quarter slabs added by the four workgroups of a row group themselves (join = 1: a hand-over inside their XCD)

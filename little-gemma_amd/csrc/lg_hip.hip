@@ -253,6 +253,11 @@ struct lg_hip_model {
     int last_rows = 0, last_adv = 0;
     float *lstage = nullptr;           // pinned: two rows of logits on their way to a caller (lg_hip_get_logits), row j in half j % 2
     int lread = -1, lcoming = -1;      // the row of the latest step read last, and the one whose copy has been started
+    // drawing tokens from a step's logits (lg_hip_forward_sample), made on first use: parameters and numbers of its rows, their tokens, working memory
+    struct lg_hip_sampling *how = nullptr;
+    float *draw_u = nullptr;
+    int32_t *drawn = nullptr;
+    uint8_t *draw_work = nullptr;
     int store_logits = 0, use_graph = 1, wide_prefill = 1, fuse_rows = 1, attn_rows = 1, attn_rows_fq = 1, head_mfma = 1, down_kq = 1, tail_spread = 1, rows_geglu = 0, narrow = 1, attn_out = 1, tail_qkv = 1, attn_geglu = 2, mid = 2;
     uint32_t mid_rows = 0;             // bit r: blocks of r rows have launches of lg_mid.h while mid is 2
     // the feed-forward half of a layer as one XCD-partitioned launch (lg_xffn.h): built when the shape and the chip fit
@@ -2356,6 +2361,53 @@ extern "C" int lg_hip_forward_spec(lg_hip_model *m, lg_hip_kv *kv, const int32_t
     if ((rc = load_block(m, toks, rows, pos, true))) return rc;
     if ((rc = launch_step(m, kv, rows, true))) return rc;
     if ((rc = wait_report(m, "forward_spec", rows, out, adv))) return rc;
+    m->last_rows = rows; m->last_adv = *adv;
+    return 0;
+}
+
+// ---- a step whose tokens are drawn --------------------------------------------------------------------
+// Parameters and numbers arrive as kernel arguments (a copy ahead of the step would be waited for), the results leave as a greedy step's do: the
+// accept rule on the drawn tokens, the accepted row's hidden state, and the report that the host polls for.
+struct DrawArgs { struct lg_hip_sampling how; float u[LG_HIP_MAX_ROWS]; int32_t tok[LG_HIP_MAX_ROWS]; };
+__global__ void lg_k_draw_load(DrawArgs a, int rows, struct lg_hip_sampling *how, float *u) {
+    if ((int)threadIdx.x < rows) { how[threadIdx.x] = a.how; u[threadIdx.x] = a.u[threadIdx.x]; }
+}
+__global__ __launch_bounds__(LG_WG) void lg_k_draw_accept(DrawArgs a, int rows, const int32_t *drawn, const float *hidden_rows, float *hidden, int E, const StepCtl *ctl,
+                                                          int32_t *host, int report) {
+    int adv = 1;
+    while (adv < rows && drawn[adv - 1] == a.tok[adv]) ++adv;
+    for (int i = threadIdx.x; i < E; i += LG_WG) hidden[i] = hidden_rows[(size_t)(adv - 1) * E + i];
+    if (threadIdx.x == 0) {
+        for (int j = 0; j < rows; ++j) host[LG_REPORT_OUT + j] = drawn[j];
+        host[LG_REPORT_ADV] = adv;
+        host[LG_REPORT_ERR] = ctl->err;
+        __hip_atomic_store(host + LG_REPORT_SEQ, report, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
+    }
+}
+extern "C" int lg_hip_forward_sample(lg_hip_model *m, lg_hip_kv *kv, const int32_t *toks, int rows, int pos, const struct lg_hip_sampling *how,
+                                     const float *u, int32_t *out, int32_t *adv) {
+    int rc = check_block(m, kv, toks, rows, rows, pos);
+    if (rc) return rc;
+    if (!how || !u || !out || !adv) return fail(-1, "forward_sample: null argument");
+    if (!m->store_logits) return fail(-4, "forward_sample: the store_logits option is off");
+    if (m->n_vocab > 524288) return fail(-2, "forward_sample: a vocabulary of %d (at most 524288)", m->n_vocab);
+    HIP_TRY(hipSetDevice(m->device));
+    const size_t work = lg_hip_sample_workspace(m->max_rows, m->n_vocab);
+    if (!m->drawn && (dev_alloc(m, &m->how, (size_t)LG_HIP_MAX_ROWS) || dev_alloc(m, &m->draw_u, (size_t)LG_HIP_MAX_ROWS) || dev_alloc(m, &m->draw_work, work ? work : 256) ||
+                      dev_alloc(m, &m->drawn, (size_t)LG_HIP_MAX_ROWS)))
+        return -7;
+    DrawArgs a{};
+    a.how = *how;
+    memcpy(a.u, u, (size_t)rows * 4);
+    memcpy(a.tok, toks, (size_t)rows * 4);
+    if ((rc = load_block(m, toks, rows, pos, false))) return rc;
+    if ((rc = launch_step(m, kv, rows, true))) return rc;
+    if (++m->reports == INT32_MAX) m->reports = 1;
+    hipLaunchKernelGGL(lg_k_draw_load, dim3(1), dim3(64), 0, m->stream, a, rows, m->how, m->draw_u);
+    if ((rc = lg_hip_sample(m->logits, m->n_vocab, rows, m->n_vocab, m->how, m->draw_u, m->drawn, nullptr, nullptr, m->draw_work, work, m->stream))) return rc;
+    hipLaunchKernelGGL(lg_k_draw_accept, dim3(1), dim3(LG_WG), 0, m->stream, a, rows, m->drawn, m->hidden_rows, m->g_hidden, m->E, m->ctl, m->pin + 32, m->reports);
+    HIP_TRY(hipGetLastError());
+    if ((rc = wait_report(m, "forward_sample", rows, out, adv))) return rc;
     m->last_rows = rows; m->last_adv = *adv;
     return 0;
 }

@@ -105,6 +105,7 @@ def load_hip():
     L.lg_hip_sample_workspace.argtypes = [I, I]
     L.lg_hip_sample_workspace.restype = Z
     L.lg_hip_sample.argtypes = [P, Q, I, I] + [P] * 6 + [Z, P]
+    L.lg_hip_forward_sample.argtypes = [P, P, i32p, I, I, C.POINTER(Sampling), f32p, i32p, C.POINTER(C.c_int32)]
     _hip = L
     return L
 
@@ -149,6 +150,8 @@ def load_backend():
     B.lg_model_device_kv.restype = C.c_void_p
     B.lg_model_last_hidden.argtypes = [C.c_void_p, f32p]
     B.lg_model_release.restype = None
+    B.lg_session_sampling.argtypes = [C.c_float, C.c_int, C.c_float, C.c_float, C.c_uint64]
+    B.lg_session_sampling.restype = None
     B.lg_session_mtp_open.argtypes = [C.c_void_p, C.c_char_p]
     B.lg_session_mtp_open.restype = C.c_void_p
     B.lg_session_mtp_close.argtypes = [C.c_void_p]
@@ -221,6 +224,21 @@ class HipBackend:
         out = np.full(len(t), -1, np.int32)
         adv = self.B.lg_session_forward_spec(self.s, t, len(t), int(pos), out)
         return adv, out
+
+    def forward_sample(self, toks, pos, how, u):
+        """A step whose tokens are drawn: how = (temperature, top_k, top_p, min_p), u = a number of [0, 1) per row; (adv, tokens)."""
+        t = np.ascontiguousarray(toks, np.int32)
+        u = np.ascontiguousarray(u, np.float32)
+        if u.size != t.size:
+            raise HipError("forward_sample: a random number per row")
+        out = np.full(len(t), -1, np.int32)
+        adv = C.c_int32(0)
+        hip_check(self.H.lg_hip_forward_sample(self.dev, self.dkv, t, len(t), int(pos), C.byref(Sampling(*how)), u, out, C.byref(adv)), "forward_sample")
+        return adv.value, out
+
+    def sampling(self, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, seed=0):
+        """Every generation and step through the model.h calls from here on draws its tokens; temperature 0: takes the likeliest again."""
+        self.B.lg_session_sampling(temperature, top_k, top_p, min_p, seed)
 
     def generate(self, prompt, n_gen, rows=1, drafts=None):
         p = np.ascontiguousarray(prompt, np.int32)

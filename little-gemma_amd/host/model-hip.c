@@ -113,11 +113,35 @@ static void want_logits(lg_hip_model *d, int on) {
     g_logits_on = on;
 }
 
+/* Drawn tokens instead of greedy ones, for every step from here on (how = NULL: greedy again).  The number that draws a row's token comes from the seed and
+ * the row's position alone, so a generation is the same with and without drafts. */
+static struct lg_hip_sampling g_how;
+static int g_sampling;
+static uint64_t g_seed;
+void lg_model_set_sampling(const struct lg_hip_sampling *how, uint64_t seed) {
+    g_sampling = how != NULL;
+    if (how) g_how = *how;
+    g_seed = seed;
+}
+static float uniform_at(uint64_t seed, int pos) {               /* splitmix64's finalizer, 24 bits of [0, 1) */
+    uint64_t z = seed + 0x9E3779B97F4A7C15ull * ((uint64_t)pos + 1);
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    return (float)((z ^ (z >> 31)) >> 40) * 0x1p-24f;
+}
+
 /* The block form with a run-time width; model_forward_spec below pins it to LG_MTP_N. */
 int lg_model_forward_spec_n(struct model *m, struct kvcache *kv, const int *toks, int rows, int pos, int *out) {
     lg_hip_model *d = device_model(m);
     int adv = 0;
-    want_logits(d, model_pick != NULL);
+    want_logits(d, model_pick != NULL || g_sampling);
+    if (g_sampling && !model_pick) {
+        float u[LG_HIP_MAX_ROWS];
+        for (int j = 0; j < rows && j < LG_HIP_MAX_ROWS; j++) u[j] = uniform_at(g_seed, pos + j);
+        if (lg_hip_forward_sample(d, device_kv(kv), toks, rows, pos, &g_how, u, out, &adv) != 0) die("forward_sample");
+        for (int j = 0; j < adv; j++) if (out[j] < 0) { fprintf(stderr, "run-hip: no token to draw at position %d\n", pos + j); exit(1); }
+        return adv;
+    }
     if (lg_hip_forward_spec(d, device_kv(kv), toks, rows, pos, out, &adv) != 0) die("forward_spec");
     if (model_pick) {
         /* sampling hook: pick from every row's logits, accept while the pick agrees
@@ -237,9 +261,10 @@ int  mtp_draft_chain_device(struct mtp *t, const struct model *m, const struct k
 }
 /* n_rounds speculative rounds with no host round trip in between (draft, chained drafts, verify, accept, next
  * chosen token: the body of the reference's loop, src/run.c:54-71 and :559-574, kept on the device).  Returns 0,
- * or -1 when the head is unavailable or cannot chain: the caller then drives the loop itself. */
+ * or -1 when the head is unavailable or cannot chain, or tokens are drawn: the caller then drives the loop itself. */
 int lg_model_mtp_rounds(struct mtp *t, const struct model *m, struct kvcache *kv, int token, int pos, int rows,
                         int n_rounds, int *blocks, int *out, int *adv) {
+    if (g_sampling) return -1;                     /* rounds on the device are greedy */
     lg_hip_model *d = draft_model(t, m);
     if (!d) return -1;
     int rc = lg_hip_mtp_rounds(d, device_kv(kv), token, pos, rows, n_rounds, blocks, out, adv, NULL);

@@ -5,14 +5,18 @@
  * flags and the loop (prefill, first token, plain or block-LG_MTP_N speculative greedy steps, the
  * same stderr statistics lines) but takes the prompt as token ids and prints token ids:
  *
- *   run-hip -m model.gguf -p 12,7,99,4 [-n 256] [-mtp assistant.gguf [-rounds R] | -mtp drafts.txt | -mtp self]
+ *   run-hip -m model.gguf -p 12,7,99,4 [-n 256] [-temp T [-top-k K] [-top-p P] [-min-p M] [-seed S]]
+ *           [-mtp assistant.gguf [-rounds R] | -mtp drafts.txt | -mtp self]
  *
  * -mtp assistant.gguf drafts with a gemma4-assistant head on the device, like the reference's -mtp
- * (src/run.c:719), after a plain greedy run of the same prompt: the two outputs must be
+ * (src/run.c:719), after a plain run of the same prompt: the two outputs must be
  * byte-identical (docs/mtp.md:16-19) and the exit status says whether they were.  -rounds R keeps R
  * speculative rounds on the device between host waits (default 8); 0 waits after every draft and
  * every verify step, as the reference's loop does.  -mtp drafts.txt replays a file of draft token
  * ids instead of a head; -mtp self replays the plain run's own output as (perfect) drafts.
+ * -temp T (above 0) draws the tokens instead of taking the likeliest one, on the device (lg_hip_sample); -top-k, -top-p and -min-p
+ * narrow the choice.  A token's random number comes from the seed and its position, so the outputs with and without -mtp are the same here
+ * too (and -rounds counts as 0: rounds on the device are greedy).
  * Output: generated token ids on stdout, one line.
  */
 #include <stdio.h>
@@ -44,21 +48,29 @@ static int parse_ids(const char *s, int *out, int cap) {
 
 int main(int argc, char **argv) {
     const char *model = NULL, *prompt = NULL, *mtp = NULL;
-    int n_gen = 256, rounds = 8;
+    int n_gen = 256, rounds = 8, top_k = 0;
+    float temp = 0.0f, top_p = 1.0f, min_p = 0.0f;
+    unsigned long long seed = 0;
     for (int i = 1; i < argc; i++) {
         if (!strcmp(argv[i], "-m") && i + 1 < argc) model = argv[++i];
         else if (!strcmp(argv[i], "-p") && i + 1 < argc) prompt = argv[++i];
         else if (!strcmp(argv[i], "-mtp") && i + 1 < argc) mtp = argv[++i];
         else if (!strcmp(argv[i], "-n") && i + 1 < argc) n_gen = atoi(argv[++i]);
         else if (!strcmp(argv[i], "-rounds") && i + 1 < argc) rounds = atoi(argv[++i]);
+        else if (!strcmp(argv[i], "-temp") && i + 1 < argc) temp = strtof(argv[++i], NULL);
+        else if (!strcmp(argv[i], "-top-k") && i + 1 < argc) top_k = atoi(argv[++i]);
+        else if (!strcmp(argv[i], "-top-p") && i + 1 < argc) top_p = strtof(argv[++i], NULL);
+        else if (!strcmp(argv[i], "-min-p") && i + 1 < argc) min_p = strtof(argv[++i], NULL);
+        else if (!strcmp(argv[i], "-seed") && i + 1 < argc) seed = strtoull(argv[++i], NULL, 10);
     }
     if (!model || !prompt) {
-        printf("Usage: %s -m <model.gguf> -p <id,id,...> [-n N] [-mtp <assistant.gguf> [-rounds R] | -mtp <draft-ids.txt> | -mtp self]\n"
+        printf("Usage: %s -m <model.gguf> -p <id,id,...> [-n N] [-temp T [-top-k K] [-top-p P] [-min-p M] [-seed S]] [-mtp <assistant.gguf> [-rounds R] | -mtp <draft-ids.txt> | -mtp self]\n"
                "       -rounds R: speculative rounds kept on the device between host waits (default 8; 0 = one wait per draft\n"
                "       and per verify step, like the reference's loop)\n"
                "       (built with LG_MTP_N=%d: speculative blocks verify %d tokens per step)\n", argv[0], LG_MTP_N, LG_MTP_N);
         return 1;
     }
+    lg_session_sampling(temp, top_k, top_p, min_p, seed);
     static int ids[8192];
     int n_prompt = parse_ids(prompt, ids, 8192);
     if (n_prompt < 1 || n_gen < 1) { fprintf(stderr, "run-hip: empty prompt\n"); return 1; }
@@ -93,7 +105,7 @@ int main(int argc, char **argv) {
             fprintf(stderr, "gen:    %d tokens in %.2fs (%.2f tok/s)\n", g, dt, g / (dt > 0 ? dt : 1e-9));
             fprintf(stderr, "mtp:    %d steps, %d drafts, %d accepted (%.0f%%), block %d\n", steps, nd, na, nd ? 100.0 * na / nd : 0.0, LG_MTP_N);
             int bad = g != n_gen || memcmp(plain, emitted, (size_t)g * sizeof(int)) != 0;
-            fprintf(stderr, "check:  -mtp output %s plain greedy output\n", bad ? "DIFFERS FROM" : "is byte-identical to");
+            fprintf(stderr, "check:  -mtp output %s plain %s output\n", bad ? "DIFFERS FROM" : "is byte-identical to", temp > 0 ? "sampled" : "greedy");
             lg_session_mtp_close(head);
             free(emitted); free(drafts); free(plain);
             lg_session_close(s);
@@ -130,7 +142,7 @@ int main(int argc, char **argv) {
     int rc = 0;
     if (plain) {
         rc = memcmp(plain, emitted, (size_t)g * sizeof(int)) != 0;
-        fprintf(stderr, "check:  -mtp output %s plain greedy output\n", rc ? "DIFFERS FROM" : "is byte-identical to");
+        fprintf(stderr, "check:  -mtp output %s plain %s output\n", rc ? "DIFFERS FROM" : "is byte-identical to", temp > 0 ? "sampled" : "greedy");
     }
     free(emitted); free(drafts); free(plain);
     lg_session_close(s);

@@ -8,6 +8,7 @@
 int lg_model_forward_spec_n(struct model *m, struct kvcache *kv, const int *toks, int rows, int pos, int *out);
 lg_hip_model *lg_mtp_device(struct mtp *t, const struct model *m);
 void lg_model_release(void);
+void lg_model_set_sampling(const struct lg_hip_sampling *how, uint64_t seed);
 int lg_model_mtp_rounds(struct mtp *t, const struct model *m, struct kvcache *kv, int token, int pos, int rows,
                         int n_rounds, int *blocks, int *out, int *adv);
 
@@ -53,6 +54,11 @@ int  lg_session_forward_next(struct lg_session *s, int token, int pos) { return 
 void lg_session_forward(struct lg_session *s, int token, int pos, float *logits) { model_forward(&s->m, &s->kv, token, pos, logits); }
 int  lg_session_forward_spec(struct lg_session *s, const int *toks, int rows, int pos, int *out) {
     return lg_model_forward_spec_n(&s->m, &s->kv, toks, rows, pos, out);
+}
+
+void lg_session_sampling(float temperature, int top_k, float top_p, float min_p, uint64_t seed) {
+    const struct lg_hip_sampling how = { temperature, top_k, top_p, min_p };
+    lg_model_set_sampling(temperature > 0 ? &how : NULL, seed);
 }
 
 /* The generation loop of the reference (src/run.c:737-768) on token ids: prefill all but the last

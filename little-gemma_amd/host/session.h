@@ -6,6 +6,7 @@
  */
 #ifndef LG_SESSION_H
 #define LG_SESSION_H
+#include <stdint.h>
 #include "model.h"
 
 struct lg_session;
@@ -28,6 +29,9 @@ int  lg_session_forward_spec(struct lg_session *s, const int *toks, int rows, in
  * Returns tokens emitted; *steps = target forwards/verify steps run. */
 int  lg_session_generate(struct lg_session *s, const int *prompt, int n_prompt, int n_gen, int rows,
                          const int *drafts, int *emitted, int *steps);
+/* Tokens drawn by temperature, top-k, top-p and min-p (lg_hip_sample) in every generation and step of this process from here on, the same ones
+ * with and without drafts; temperature not above 0: greedy ones again. */
+void lg_session_sampling(float temperature, int top_k, float top_p, float min_p, uint64_t seed);
 /* Draft head (include/model.h:156-178): open a gemma4-assistant file for this session's model,
  * one draft (chain = 0: from the target's hidden; 1: chained on the head's own), the head's
  * post-norm hidden, its logits (dst NULL: switch storing on/off), and the reference's
