@@ -219,7 +219,7 @@ struct SampleWork {                     // per row, in working memory
     lg_u64 *mass; uint32_t *count;      // [LG_SAMPLE_BINS]
     lg_u64 *gsum;                       // [groups]
     lg_u64 *part;                       // [slices][3]: sum above the candidates, sum that top-p goes by (without the candidates), tokens kept above them
-    uint32_t *ncand;                    // candidates; behind it the row's SampleRange
+    uint32_t *ncand;                    // candidates; behind it, from word 4 on, the row's SampleRange, from word 8 its largest key and ~key of its smallest logit
     lg_u64 *cand;                       // [LG_SAMPLE_CAND] ~key << 32 | index
 };
 struct SampleGeo { int groups, maxes, slices; size_t gmax, smin, mass, count, gsum, part, ncand, cand, row; };
@@ -304,11 +304,11 @@ __global__ __launch_bounds__(LG_SAMPLE_MAX_WG) void lg_k_sample_max(SampleArgs a
     if (threadIdx.x == 0) w.smin[part] = least;
 }
 
-// The row's largest logit and the width of its bins, in every workgroup anew (1024 keys and 64 minima: less than a launch of their own)
-struct SampleSpan { Weigh wg; float top, scale, c; uint32_t key; };      // key: of the largest logit, 0x007FFFFF: none; scale: bins per unit of logit; c: base-2 exponents per unit
-__device__ __forceinline__ SampleSpan lg_sample_span_of(const SampleRow &p, uint32_t key, uint32_t least, const double *tab) {       // least: ~key of the smallest
+// The row's largest logit and the width of its bins
+struct SampleSpan { Weigh wg; float top, scale, c; uint32_t key, least; };      // key: of the largest logit, 0x007FFFFF: none; least: ~key of the smallest; scale: bins per unit of logit; c: base-2 exponents per unit
+__device__ __forceinline__ SampleSpan lg_sample_span_of(const SampleRow &p, uint32_t key, uint32_t least, const double *tab) {
     SampleSpan s;
-    s.key = key;
+    s.key = key; s.least = least;
     s.top = lg_unkey(key);
     s.wg = lg_weigher(s.top, p.temperature, tab);
     s.c = -(float)(1.4426950408889634 / (double)p.temperature);
@@ -316,13 +316,21 @@ __device__ __forceinline__ SampleSpan lg_sample_span_of(const SampleRow &p, uint
     s.scale = width > 0 && width < INFINITY ? (float)LG_SAMPLE_BINS / width : 0;      // (0: all in the first bin)
     return s;
 }
+// From what lg_k_sample_max left: this thread's share, asked for early, and all of it
+struct SampleEnds { uint32_t key, least; };
 template <int NT>
-__device__ __forceinline__ SampleSpan lg_sample_span(const SampleRow &p, const SampleWork &w, const SampleGeo &g, const double *tab, uint32_t *part) {
-    uint32_t key = 0, least = 0;
-    for (int i = threadIdx.x; i < g.groups; i += NT) { const uint32_t k = w.gmax[i]; if (k > key) key = k; }
-    for (int i = threadIdx.x; i < g.maxes; i += NT) { const uint32_t k = w.smin[i]; if (k > least) least = k; }
-    lg_block_max2<NT>(key, least, part);
-    return lg_sample_span_of(p, key, least, tab);
+__device__ __forceinline__ SampleEnds lg_sample_ends(const SampleWork &w, const SampleGeo &g) {
+    SampleEnds e{ 0, 0 };
+    #pragma unroll
+    for (int i = 0; i < LG_SAMPLE_GROUPS / NT; ++i) { const int at = threadIdx.x + i * NT; const uint32_t k = w.gmax[at < g.groups ? at : 0]; if (k > e.key) e.key = k; }
+    const uint32_t k = w.smin[(int)threadIdx.x < g.maxes ? threadIdx.x : 0];          // (at most 128)
+    e.least = k;
+    return e;
+}
+template <int NT>
+__device__ __forceinline__ SampleSpan lg_sample_span(const SampleRow &p, SampleEnds e, const double *tab, uint32_t *part) {
+    lg_block_max2<NT>(e.key, e.least, part);
+    return lg_sample_span_of(p, e.key, e.least, tab);
 }
 // Monotone in the logit, also as rounded: a larger logit never has a larger bin
 __device__ __forceinline__ int lg_sample_bin(const SampleSpan &s, float l) {
@@ -340,17 +348,20 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_bins(SampleArgs a, c
     const SampleGeo g = lg_sample_geo(a.n_vocab);
     const int r = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
     const SampleRow p = a.params[r];
-    if (lg_row_kind(p, a.n_vocab) != LG_ROW_BORDER) return;
+    const int kind = lg_row_kind(p, a.n_vocab);
+    if (kind != LG_ROW_BORDER && !(kind == LG_ROW_FREE && slice == 0)) return;
     const SampleWork w = lg_sample_work(base, g, r);
     const float *row = a.logits + r * a.stride;
     const double entry = lg_table_entry();
+    const SampleEnds ends = lg_sample_ends<NT>(w, g);
     float l[4][4];
     #pragma unroll
     for (int j = 0; j < 4; ++j) lg_load4<VEC>(row, a.n_vocab, slice * (NT / 16) + j * (NT / 64) + wave, l[j]);
     lg_table_store(tab, entry);
     for (int i = threadIdx.x; i < LG_SAMPLE_BINS; i += NT) { mass[i] = 0; count[i] = 0; }
-    const SampleSpan s = lg_sample_span<NT>(p, w, g, tab, part);                      // (its barriers are the clearing's too)
-    if (s.key == 0x007FFFFFu || s.top == INFINITY) return;
+    const SampleSpan s = lg_sample_span<NT>(p, ends, tab, part);                      // (its barriers are the clearing's too)
+    if (slice == 0 && threadIdx.x == 0) { w.ncand[8] = s.key; w.ncand[9] = s.least; }        // for the launches behind this one
+    if (kind != LG_ROW_BORDER || s.key == 0x007FFFFFu || s.top == INFINITY) return;
     const bool by_count = p.top_k > 0 && p.top_k < a.n_vocab, by_mass = p.top_p < 1;
     #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -376,19 +387,27 @@ struct SampleRange { int first, last, cut; uint32_t above; };        // top-p's 
 template <int NT>
 struct SampleRangeLds { lg_u64 part[NT / 64]; SampleRange r; lg_u64 lo, hi; };
 template <int NT>
-__device__ __forceinline__ SampleRange lg_sample_range(const SampleArgs &a, const SampleRow &p, const SampleWork &w, SampleRangeLds<NT> &s) {
+struct SampleBins { lg_u64 m[LG_SAMPLE_BINS / NT]; uint32_t c[LG_SAMPLE_BINS / NT]; };           // this thread's, asked for early
+template <int NT>
+__device__ __forceinline__ SampleBins<NT> lg_sample_bins(const SampleWork &w) {
+    constexpr int PT = LG_SAMPLE_BINS / NT;
+    SampleBins<NT> b;
+    #pragma unroll
+    for (int i = 0; i < PT; ++i) { b.m[i] = w.mass[threadIdx.x * PT + i]; b.c[i] = w.count[threadIdx.x * PT + i]; }
+    return b;
+}
+template <int NT>
+__device__ __forceinline__ SampleRange lg_sample_range(const SampleArgs &a, const SampleRow &p, const SampleBins<NT> &bins, SampleRangeLds<NT> &s) {
     constexpr int PT = LG_SAMPLE_BINS / NT;
     const int b0 = threadIdx.x * PT;
     const bool by_count = p.top_k > 0 && p.top_k < a.n_vocab, by_mass = p.top_p < 1;
     if (threadIdx.x == 0) s.r = { 0, LG_SAMPLE_BINS - 1, LG_SAMPLE_BINS, 0 };
-    lg_u64 m[PT];
-    if (by_mass)
-        #pragma unroll
-        for (int i = 0; i < PT; ++i) m[i] = w.mass[b0 + i];
+    const lg_u64 (&m)[PT] = bins.m;
     if (by_count) {
-        lg_u64 c[PT], sum = 0, all;
+        const uint32_t (&c)[PT] = bins.c;
+        lg_u64 sum = 0, all;
         #pragma unroll
-        for (int i = 0; i < PT; ++i) { c[i] = w.count[b0 + i]; sum += c[i]; }
+        for (int i = 0; i < PT; ++i) sum += c[i];
         lg_u64 run = lg_block_run<NT>(sum, s.part, &all) - sum;
         #pragma unroll
         for (int i = 0; i < PT; ++i) {
@@ -441,20 +460,22 @@ __global__ __launch_bounds__(NT) void lg_k_sample_sums(SampleArgs a, char *base)
     if (kind != LG_ROW_BORDER && kind != LG_ROW_FREE) return;
     const SampleWork w = lg_sample_work(base, g, r);
     const float *row = a.logits + r * a.stride;
+    const bool border = kind == LG_ROW_BORDER;
     const double entry = lg_table_entry();
+    const SampleBins<NT> bins = border ? lg_sample_bins<NT>(w) : SampleBins<NT>{};
     float l[4][4];
     #pragma unroll
     for (int j = 0; j < 4; ++j) lg_load4<VEC>(row, a.n_vocab, slice * (NT / 16) + j * (NT / 64) + wave, l[j]);
+    const uint32_t key = w.ncand[8], least_key = w.ncand[9];
     lg_table_store(tab, entry);
     if (threadIdx.x < 3) s_sum[threadIdx.x] = 0;
     if (threadIdx.x == 3) s_n = 0;
-    const bool border = kind == LG_ROW_BORDER;
     SampleRange q{ LG_SAMPLE_BINS, -1, LG_SAMPLE_BINS, 0 };
     if (border) {
-        q = lg_sample_range<NT>(a, p, w, s_range);
+        q = lg_sample_range<NT>(a, p, bins, s_range);
         if (slice == 0 && threadIdx.x == 0) *(SampleRange *)(w.ncand + 4) = q;
-    }
-    const SampleSpan s = lg_sample_span<NT>(p, w, g, tab, part);
+    } else __syncthreads();
+    const SampleSpan s = lg_sample_span_of(p, key, least_key, tab);
     if (s.key == 0x007FFFFFu || s.top == INFINITY) return;
     const lg_u64 least = lg_least(p);
     // What is behind top-k's bin, or below min-p where nothing else is asked, needs no weight (a little more than that gets one); a wavefront without such a
@@ -668,7 +689,11 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
             lg_block_max2<LG_SAMPLE_WG>(key, low, s.key);
             span = lg_sample_span_of(p, key, low, s.tab);
             low = ~low;
-        } else span = lg_sample_span<LG_SAMPLE_WG>(p, w, g, s.tab, s.key);   // (its barriers are the sums' too)
+        } else if (kind == LG_ROW_FIRST) span = lg_sample_span<LG_SAMPLE_WG>(p, lg_sample_ends<LG_SAMPLE_WG>(w, g), s.tab, s.key);
+        else {
+            span = lg_sample_span_of(p, w.ncand[8], w.ncand[9], s.tab);
+            __syncthreads();                                 // (the sums and the table)
+        }
         if (kind == LG_ROW_BORDER || kind == LG_ROW_FREE) { above = s.part3[0]; total = s.part3[1]; kept = (uint32_t)s.part3[2]; }
         if (span.top == INFINITY && (kind == LG_ROW_BORDER || kind == LG_ROW_FREE)) return false;      // (the launches before left nothing)
         if (span.key != 0x007FFFFFu && kind == LG_ROW_FIRST) {
