@@ -76,8 +76,8 @@ def test_attention_refuses(lg, change, code, words):
 @pytest.mark.parametrize("change, code, words", [
     (dict(rows=-1), -2, "-1 rows"), (dict(rows=65536), -2, "rows"), (dict(vocab=0), -2, "vocabulary of 0"), (dict(vocab=524289), -2, "vocabulary"),
     (dict(stride=99), -2, "99 apart"), (dict(logits=None), -1, "null"), (dict(params=None), -1, "null"), (dict(u=None), -1, "null"), (dict(tok=None), -1, "null"),
-    (dict(logits=C.c_void_p((1 << 20) + 2)), -2, "aligned"), (dict(vocab=8192, work=None), -2, "working memory"), (dict(vocab=8192, short=1), -2, "working memory"),
-    (dict(vocab=8192, work=C.c_void_p((1 << 20) + 16)), -2, "working memory")])
+    (dict(logits=C.c_void_p((1 << 20) + 2)), -2, "aligned"), (dict(vocab=8193, work=None), -2, "working memory"), (dict(vocab=8193, short=1), -2, "working memory"),
+    (dict(vocab=8193, work=C.c_void_p((1 << 20) + 16)), -2, "working memory")])
 def test_sample_refuses(lg, change, code, words):
     H = lg.hiplib.load_hip()
     a = dict(logits=P16, stride=524289, rows=3, vocab=100, params=P16, u=P16, tok=P16, work=P16, short=0)
