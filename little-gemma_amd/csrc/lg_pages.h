@@ -44,12 +44,12 @@ __global__ __launch_bounds__(NT) void lg_k_plan(PlanArgs a) {
     __shared__ int32_t tok[LG_PLAN_SEQS + 1], need[LG_PLAN_SEQS + 1], freed[LG_PLAN_SEQS + 1], olds[LG_PLAN_SEQS], news[LG_PLAN_SEQS];
     __shared__ lg_u64 part[3 * NT / 64];
     __shared__ int32_t taken[NT];
-    __shared__ int bad;
+    __shared__ int bad, bad_page;                             // (a word of its own: wavefronts may find pages while others still read the first)
     const int t = threadIdx.x, P = 1 << a.shift, n = a.n_seq, n_slots = a.slots ? a.n_slots : 0;
     const long long most = (long long)a.max_blocks << a.shift;
     const int per = (n + NT - 1) / NT, i0 = t * per;
     const int nf = *a.n_free;
-    if (t == 0) bad = 0;
+    if (t == 0) { bad = 0; bad_page = 0; }
     auto blocks = [&](int len) { return (int)(((long long)len + P - 1) >> a.shift); };
     auto parts = [&](int i, lg_u64 (&v)[3]) {
         const int lo = olds[i], ln = news[i], d = blocks(ln) - blocks(lo);
@@ -99,10 +99,10 @@ __global__ __launch_bounds__(NT) void lg_k_plan(PlanArgs a) {
             const int block = pos >> a.shift, nb = blocks(olds[i]);
             if (block < nb) here = *place(i, block); else later = need[i] + block - nb;
         }
-        if (outside(page) || outside(here)) atomicOr(&bad, LG_PLAN_BAD_PAGE);
+        if (outside(page) || outside(here)) atomicOr(&bad_page, LG_PLAN_BAD_PAGE);
         taken[t] = page;
         __syncthreads();
-        st = bad;
+        st = bad_page;
         if (!st) {
             if (from) { *from = -1; a.stack[top - 1 - t] = page; }
             if (t < nn) *comes(t) = page;
@@ -115,9 +115,9 @@ __global__ __launch_bounds__(NT) void lg_k_plan(PlanArgs a) {
             for (int e = t; e < ng; e += NT) ids |= outside(*leaves(e));
             for (int e = ng + t; e < nn; e += NT) ids |= outside(a.stack[top - 1 - e]);
             for (int i = t; i < n; i += NT) if (news[i] > olds[i] && (olds[i] & (P - 1))) ids |= outside(*place(i, olds[i] >> a.shift));
-            if (ids) atomicOr(&bad, LG_PLAN_BAD_PAGE);
+            if (ids) atomicOr(&bad_page, LG_PLAN_BAD_PAGE);
             __syncthreads();
-            st = bad;
+            st = bad_page;
         }
         if (!st) {
             for (int e = t; e < ng; e += NT) { int32_t *const p = leaves(e); a.stack[top - 1 - e] = *p; *p = -1; }

@@ -94,6 +94,29 @@ def test_plan_reports_and_leaves_everything_as_it_was(dev, old, new, nf, n_slots
     assert np.array_equal(t2, table) and np.array_equal(s2, stack) and nf2 == nf
 
 
+@pytest.mark.parametrize("n, grow", [(200, 1), (900, 1), (300, 40)])
+def test_plan_of_many_sequences_refuses_one_bad_page(dev, n, grow):
+    """Whichever wavefront finds it, all of them refuse: a page outside the cache in the first, the last and another sequence, and on the stack."""
+    rng = np.random.default_rng(n)
+    old = rng.integers(1, 120, n)
+    old[[0, n // 2, n - 1]] = 21                             # (a page that is written into; and one that is taken)
+    old[1] = 32
+    new = old + grow
+    n_pages = int(pages_of(new, 16).sum()) + 2
+    table, stack, nf = pool_of(rng, old, 16, n_pages, 12)
+    n_slots = n * grow
+    for i in (0, n // 2, n - 1, None):
+        t, s = table.copy(), stack.copy()
+        if i is None:
+            s[nf - 1] = n_pages
+        else:
+            t[i, pages_of(old[i], 16) - 1] = -5
+        want = plan_ref(16, old.tolist(), new.tolist(), t, s, nf, n_slots)
+        assert want[2] == 16
+        for _ in range(5):
+            same(plan(dev, 16, old, new, t, s, nf, n_slots), want)
+
+
 def test_plan_through_many_steps_keeps_every_page_once(dev):
     rng = np.random.default_rng(5)
     page, n, n_pages, blocks = 16, 23, 150, 12
