@@ -311,8 +311,9 @@ int    lg_hip_paged_write(const struct lg_hip_pages *pages, const float *d_k, co
  * row, q_stride (a multiple of 4; d_q aligned to 16 bytes) and out_stride floats apart.  d_len [n_seq] is read on the device; lengths above
  * max_len or max_blocks * page_size count as that, a sequence of length 0 or less gets zeros, positions whose page is outside 0..n_pages-1
  * are left out.  max_len bounds the lengths that a captured call will see, and the working memory.  The rows of a verify block are
- * sequences with the same table row and lengths one apart.  What masked positions hold does not matter; infinities and NaN in positions
- * that are seen give outputs that are not finite in the heads that read them. */
+ * sequences with the same table row and lengths one apart.  At most 4096 sequences in a call, and 2^31 tiles of 32 keys in all
+ * of them together.  What masked positions hold does not matter; infinities and NaN in positions that are seen, or in a query, spoil the heads that read
+ * them (NaN as a rule) and no others. */
 size_t lg_hip_paged_attention_workspace(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, int window);
 int    lg_hip_paged_attention(const struct lg_hip_pages *pages, const float *d_q, int64_t q_stride, int n_seq, int n_head, const int32_t *d_table,
                               int max_blocks, const int32_t *d_len, int max_len, int window, float scale, float *d_out, int64_t out_stride,

@@ -20,6 +20,7 @@ static int shift_of(int page_size) {                 // page_size = 1 << shift; 
     if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) return -1;
     return __builtin_ctz((unsigned)page_size);
 }
+#define LG_MOST_GROUPS ((1 << 24) - 1)                // workgroups of 256 threads in a launch
 static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 #define LG_PLAN_APART 2048           // slots
@@ -85,7 +86,7 @@ extern "C" int lg_hip_paged_write(const struct lg_hip_pages *p, const float *d_k
     if (stride < width || stride % 4 || !aligned16(d_k) || !aligned16(d_v))
         return lg_fail(-2, "paged_write: rows of %d values, %lld apart (aligned to 16 bytes)", width, (long long)stride);
     const int64_t groups = ((int64_t)n_tok * (width / 4) + 255) / 256;
-    if (groups > INT32_MAX) return lg_fail(-2, "paged_write: %d tokens of %d values in one call", n_tok, width);
+    if (groups > LG_MOST_GROUPS) return lg_fail(-2, "paged_write: %d tokens of %d values in one call", n_tok, width);
     hipLaunchKernelGGL(lg_k_page_write, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, g, d_k, d_v, (long long)stride, d_slots, n_tok, width / 8);
     LG_TRY(hipGetLastError());
     return 0;
@@ -101,14 +102,14 @@ static int slots_of(int hd) { return 256 * lg_pa_per_simd(hd); }
 // and in splits: heads of 64 7.5 and 8.8 us, 128 8.5 and 9.5, 256 13.9 and 11.2 (384 keys: 11.7 and 11.3); 64 sequences, 2 key heads of 256: 16.4 and 20.2; of
 // 512 192 keys 18.0 and 19.7, 256 20.2 and 19.8.  128 workgroups and more are a half of the compute units at work already
 static int alone_of(int hd, int64_t units) { return hd <= 128 ? 16 : hd == 256 ? (units >= 128 ? 20 : 12) : 6; }
-struct AttnCut { int64_t splits; bool join; int least; };
+struct AttnCut { int64_t splits, tiles; bool join; int least; };        // tiles: of all sequences, at most
 static AttnCut cut_of(int n_seq, int n_head_kv, int hd, int max_len, int window) {
     // (a window need not start with a tile)
     const int64_t span = window > 0 && window < max_len ? (int64_t)window + LG_PA_TILE - 1 : max_len, tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
     const int alone = alone_of(hd, (int64_t)n_seq * n_head_kv), min_tiles = tiles <= alone ? alone : 4;
     const int64_t least = (tiles + min_tiles - 1) / min_tiles, slots = slots_of(hd), units = (int64_t)n_seq * n_head_kv, rounds = std::max<int64_t>(1, (units + slots / 2 - 1) / (slots / 2));
     const int64_t full = std::max<int64_t>(rounds * slots / n_head_kv, n_seq * tiles / (LG_PA_CHUNK / LG_PA_TILE));
-    return { std::min<int64_t>(n_seq * std::max<int64_t>(least, 1), full + n_seq), least > 1, min_tiles };
+    return { std::min<int64_t>(n_seq * std::max<int64_t>(least, 1), full + n_seq), n_seq * tiles, least > 1, min_tiles };
 }
 static bool attn_shape(int n_seq, int n_head, int n_head_kv, int hd, int max_len) {
     return n_seq >= 0 && n_head_kv >= 1 && n_head_kv <= 1024 && n_head >= 1 && n_head % n_head_kv == 0 && n_head / n_head_kv <= 8 &&
@@ -145,7 +146,8 @@ extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float 
     if (q_stride < qd || q_stride % 4 || !aligned16(d_q)) return lg_fail(-2, "paged_attention: query rows of %lld values, %lld apart (aligned to 16 bytes)", (long long)qd, (long long)q_stride);
     if (out_stride < qd || ((uintptr_t)d_out & 3)) return lg_fail(-2, "paged_attention: output rows of %lld values, %lld apart", (long long)qd, (long long)out_stride);
     const AttnCut c = cut_of(n_seq, p->n_head_kv, hd, max_len, window);
-    if (n_seq > LG_PA_SEQS || c.splits * n_head > INT32_MAX)
+    // (sums over the sequences are 32 bits on the device, and so are a launch's threads)
+    if (n_seq > LG_PA_SEQS || c.tiles > INT32_MAX || c.splits * n_head > LG_MOST_GROUPS)
         return lg_fail(-2, "paged_attention: %d sequences of %d heads in %lld splits in one call (at most %d sequences)", n_seq, n_head, (long long)c.splits, LG_PA_SEQS);
     const size_t need = lg_hip_paged_attention_workspace(n_seq, n_head, p->n_head_kv, hd, max_len, window);
     if (need && (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)))

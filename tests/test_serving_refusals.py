@@ -54,6 +54,14 @@ def test_write_refuses(lg, k, v, stride, slots, n, code, words):
     assert H.lg_hip_paged_write(C.byref(p), k, v, stride, slots, 0, None) == 0                    # nothing to write
 
 
+def test_calls_beyond_what_a_launch_holds_are_refused(lg):
+    H, p = lg.hiplib.load_hip(), pages(lg, {})
+    refused(lg, H.lg_hip_paged_write(C.byref(p), P16, P16, 128, P16, 1 << 27, None), -2, "tokens of 128 values in one call")
+    for seqs, heads, kv in ((4096, 2, 1), (128, 2, 1), (4096, 16, 2)):           # tiles of all sequences, splits of all heads
+        q = pages(lg, dict(n_head_kv=kv))
+        refused(lg, H.lg_hip_paged_attention(C.byref(q), P16, 64 * heads, seqs, heads, P16, 1 << 26, P16, 1 << 30, 0, 1.0, P16, 64 * heads, P16, 1 << 62, None), -2, "in one call")
+
+
 @pytest.mark.parametrize("change, code, words", [
     (dict(n_seq=-1), -2, "-1 sequences"), (dict(n_seq=4097), -2, "4097 sequences"), (dict(heads=7), -2, "7 query heads"), (dict(heads=18), -2, "18 query heads"), (dict(heads=0), -2, "0 query heads"),
     (dict(max_len=-1), -2, "lengths up to -1"), (dict(max_len=(1 << 30) + 1), -2, "lengths up to"), (dict(blocks=0), -2, "0 blocks"), (dict(blocks=1 << 27), -2, "blocks"),
