@@ -636,7 +636,7 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
     lg_u64 above = 0, total = 0, all;                        // sum of the tokens before the candidates; what top-p goes by
     SampleSpan span;
     SampleRange q{ LG_SAMPLE_BINS, -1, LG_SAMPLE_BINS, 0 };
-    uint32_t kept = 0;
+    uint32_t kept = 0, from = 0;                             // from: a small top-k's candidates are the tokens with this key and larger ones
     int n = 0;
     if (WHOLE) {
         uint32_t key = 0, least_key = 0;
@@ -720,7 +720,8 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
             const lg_u64 mine = s.bin[1023 - t], run = lg_block_run<LG_SAMPLE_WG>(mine, s.part, &all);
             if (run >= (lg_u64)p.top_k && run - mine < (lg_u64)p.top_k) s.idx = 1023 - t;
             __syncthreads();
-            const uint32_t from = all >= (lg_u64)p.top_k ? low + ((uint32_t)s.idx << shift) : 0x00800000u;      // (fewer groups than top_k: every token)
+            s.bin[t] = 0;
+            from = all >= (lg_u64)p.top_k ? low + ((uint32_t)s.idx << shift) : 0x00800000u;      // (fewer groups than top_k: every token)
             #pragma unroll
             for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) if (gk[i] >= from) s.groups[atomicAdd(&s.n_groups, 1u)] = t + i * LG_SAMPLE_WG;
             __syncthreads();
@@ -810,6 +811,55 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
         if (own >= least && me <= last && sub == 0) {
             const lg_u64 target = target_of(S);
             if (run > target && run - own <= target) answer((int)(uint32_t)me, (double)own / (double)S, (int)stay);
+        }
+        return true;
+    }
+    if (!WHOLE && kind == LG_ROW_SMALL && n <= LG_SAMPLE_LIST) {
+        // a few hundred: each one's place in the order and the sum up to it from 1024 equal parts of the keys, and pair by pair within its part; then the same in index
+        // order among what stays.  A part has its count above 54 bits of sum: 512 weights of 2^44 are 2^53
+        const lg_u64 me = c(0), own = m[0], low54 = (1ull << 54) - 1;
+        const uint32_t wide = span.key - from;
+        const int shift = wide >= 1024 ? 32 - __builtin_clz(wide) - 10 : 0;
+        const uint32_t part = (span.key - ~(uint32_t)(me >> 32)) >> shift;
+        if (own) atomicAdd(&s.bin[part], 1ull << 54 | own);
+        __syncthreads();
+        const lg_u64 mine = s.bin[t], before = lg_block_run<LG_SAMPLE_WG>(mine, s.part, &all) - mine;
+        s.sum[t] = before;
+        s.groups[t] = (uint32_t)(before >> 54);              // where the next one of the part goes
+        __syncthreads();
+        if (own) { const uint32_t at = atomicAdd(&s.groups[part], 1u); s.list[at] = me; s.cand[at] = own; }
+        __syncthreads();
+        lg_u64 upto = 0;
+        uint32_t place = 0;
+        if (own) {
+            const lg_u64 first = s.sum[part];
+            place = (uint32_t)(first >> 54); upto = first & low54;
+            for (uint32_t i = place, to = place + (uint32_t)(s.bin[part] >> 54); i < to; ++i) if (s.list[i] <= me) { upto += s.cand[i]; ++place; }
+        }
+        const uint32_t count = (uint32_t)(all >> 54), k = (uint32_t)p.top_k < count ? (uint32_t)p.top_k : count;
+        if (own && place == k) s.whole = upto;
+        __syncthreads();
+        s.bin[t] = 0;
+        const lg_u64 W = s.whole;
+        lg_u64 want = W;
+        if (p.top_p < 1) { const double want_d = __builtin_ceil((double)p.top_p * (double)W); want = want_d >= 1 ? (lg_u64)want_d < W ? (lg_u64)want_d : W : 1; }
+        if (own && upto >= want && upto - own < want) s.last = me;
+        if (t == 0) s.n = 0;
+        __syncthreads();
+        const bool stays = own >= least && me <= s.last;
+        const uint32_t piece = (uint32_t)me / (LG_SAMPLE_VOCAB / 1024);
+        if (stays) atomicAdd(&s.bin[piece], 1ull << 54 | own);
+        __syncthreads();
+        const lg_u64 here = s.bin[t], run = lg_block_run<LG_SAMPLE_WG>(here, s.part, &all), S = all & low54, target = target_of(S);
+        if ((run & low54) > target && ((run - here) & low54) <= target) { s.at = t; s.rest = (run - here) & low54; }
+        __syncthreads();
+        const bool in = stays && (int)piece == s.at;
+        if (in) { const uint32_t at = atomicAdd(&s.n, 1u); s.list[at] = me; s.cand[at] = own; }
+        __syncthreads();
+        if (in) {
+            lg_u64 to = s.rest;
+            for (uint32_t i = 0; i < s.n; ++i) if ((uint32_t)s.list[i] <= (uint32_t)me) to += s.cand[i];
+            if (to > target && to - own <= target) answer((int)(uint32_t)me, (double)own / (double)S, (int)(all >> 54));
         }
         return true;
     }
