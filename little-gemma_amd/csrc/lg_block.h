@@ -38,18 +38,6 @@ __device__ __forceinline__ T lg_wave_max(T v) {
 __device__ __forceinline__ uint32_t lg_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
 __device__ __forceinline__ lg_u64 lg_lane(lg_u64 v, int lane) { return (lg_u64)lg_lane((uint32_t)(v >> 32), lane) << 32 | lg_lane((uint32_t)v, lane); }
 
-// The sum of each eight lanes, in all of them: the neighbour, the pair beside, the other half's mirror image
-template <int CTRL>
-__device__ __forceinline__ uint32_t lg_move(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true); }
-template <int CTRL>
-__device__ __forceinline__ lg_u64 lg_move(lg_u64 v) { return (lg_u64)lg_move<CTRL>((uint32_t)(v >> 32)) << 32 | lg_move<CTRL>((uint32_t)v); }
-template <typename T>
-__device__ __forceinline__ T lg_eight_total(T v) {
-    v += lg_move<0xB1>(v);
-    v += lg_move<0x4E>(v);
-    return v + lg_move<0x141>(v);
-}
-
 // Over a workgroup of NT <= 1024 threads; `part` is LDS of NT / 64 words.  A barrier before its first use, for the caller's earlier reads, is in here.
 // A wavefront reads the others' parts with one load, a lane each, and runs over them by primitives: with a load per part from every wavefront the LDS is
 // what 16 of them wait for (one workgroup's running sum 0.5 -> 0.2 us).

@@ -529,9 +529,8 @@ __global__ __launch_bounds__(NT) void lg_k_sample_sums(SampleArgs a, char *base)
 }
 
 // One workgroup, one row.  Candidates are ~key << 32 | index: smaller is earlier in the order.  This thread's are in registers, with their measures.
-#define LG_SAMPLE_LIST    512                    // what stays of a small top-k
-#define LG_SAMPLE_FEW     128                    // candidates of a small top-k whose order and sums are taken pair by pair
-static_assert(LG_SAMPLE_LIST >= LG_SAMPLE_SMALL_K && LG_SAMPLE_LIST >= LG_SAMPLE_FEW, "room for what stays");
+#define LG_SAMPLE_LIST    512                    // what stays of a small top-k, and its candidates that are ordered by parts of their keys
+static_assert(LG_SAMPLE_LIST >= LG_SAMPLE_SMALL_K && LG_SAMPLE_LIST <= 512, "room for what stays; sums of 54 bits");
 struct SampleFinishLds {
     lg_u64 sum[LG_SAMPLE_GROUPS], bin[1024], list[LG_SAMPLE_LIST], size[64], cand[LG_SAMPLE_CAND], part[LG_SAMPLE_WG / 32], part3[3], last, rest, whole;
     double tab[32];
@@ -775,48 +774,9 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
         const lg_u64 x = u > 0 ? (lg_u64)__builtin_floor((u < 1 ? (double)u : 1.0) * (double)S) : 0;
         return x > S - 1 ? S - 1 : x;
     };
-    if (!WHOLE && kind == LG_ROW_SMALL && n <= LG_SAMPLE_FEW) {
-        // few candidates: each one's place in the order and the sum up to it from all of them, by eight threads each; then the same in index order among
-        // what stays (three barriers; the way below takes 25)
-        const uint32_t who = (uint32_t)t >> 3, sub = t & 7;
-        const bool on = (int)who < n;
-        if (t < n) { s.list[t] = c(0); s.sum[t] = m[0]; }
-        if (t == 0) s.last = ~0ull;
-        __syncthreads();
-        const lg_u64 me = on ? s.list[who] : ~0ull, own = on ? s.sum[who] : 0;
-        lg_u64 upto = 0;
-        uint32_t place = 0;
-        #pragma unroll 4
-        for (uint32_t i = sub; on && (int)i < n; i += 8) { const lg_u64 x = s.sum[i]; if (x && s.list[i] <= me) { upto += x; ++place; } }
-        upto = lg_eight_total(upto); place = lg_eight_total(place);
-        // (a weight of 0 is the end of the order: no candidate)
-        if (t == 0) { s.whole = 0; s.n = 0; }
-        __syncthreads();
-        if (own && sub == 0 && place <= (uint32_t)p.top_k) atomicMax(&s.whole, upto);
-        __syncthreads();
-        const lg_u64 W = s.whole;
-        lg_u64 want = W;
-        if (p.top_p < 1) { const double want_d = __builtin_ceil((double)p.top_p * (double)W); want = want_d >= 1 ? (lg_u64)want_d < W ? (lg_u64)want_d : W : 1; }
-        if (own && sub == 0 && upto >= want && upto - own < want) s.last = me;
-        __syncthreads();
-        const lg_u64 last = s.last;
-        lg_u64 S = 0, run = 0;
-        uint32_t stay = 0;
-        #pragma unroll 4
-        for (uint32_t i = sub; on && (int)i < n; i += 8) {
-            const lg_u64 x = s.list[i], y = s.sum[i];
-            if (x <= last && y >= least) { S += y; ++stay; if ((uint32_t)x <= (uint32_t)me) run += y; }
-        }
-        S = lg_eight_total(S); run = lg_eight_total(run); stay = lg_eight_total(stay);
-        if (own >= least && me <= last && sub == 0) {
-            const lg_u64 target = target_of(S);
-            if (run > target && run - own <= target) answer((int)(uint32_t)me, (double)own / (double)S, (int)stay);
-        }
-        return true;
-    }
     if (!WHOLE && kind == LG_ROW_SMALL && n <= LG_SAMPLE_LIST) {
         // a few hundred: each one's place in the order and the sum up to it from 1024 equal parts of the keys, and pair by pair within its part; then the same in index
-        // order among what stays.  A part has its count above 54 bits of sum: 512 weights of 2^44 are 2^53
+        // order among what stays.  (All pairs instead, in a third of the barriers: 16.6 and 17.2 us at top-k 20, even at 40, 21.1 and 18.7 at 100.)  A part has its count above 54 bits of sum: 512 weights of 2^44 are 2^53
         const lg_u64 me = c(0), own = m[0], low54 = (1ull << 54) - 1;
         const uint32_t wide = span.key - from;
         const int shift = wide >= 1024 ? 32 - __builtin_clz(wide) - 10 : 0;
