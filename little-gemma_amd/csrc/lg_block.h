@@ -26,12 +26,18 @@ __device__ __forceinline__ uint32_t lg_last_lane(uint32_t v) { return (uint32_t)
 __device__ __forceinline__ lg_u64 lg_last_lane(lg_u64 v) { return (lg_u64)lg_last_lane((uint32_t)(v >> 32)) << 32 | lg_last_lane((uint32_t)v); }
 template <typename T>
 __device__ __forceinline__ T lg_wave_total(T v) { return lg_last_lane(lg_wave_run(v)); }
-// The largest of the lanes' numbers (0 and up)
+// The largest of the lanes' numbers (0 and up): of each sixteen in the last of them, and of all
+template <typename T>
+__device__ __forceinline__ T lg_row_max(T v) {
+    auto top = [&](T u) { if (u > v) v = u; };
+    top(lg_shift<0x111, 0xF>(v)); top(lg_shift<0x112, 0xF>(v)); top(lg_shift<0x114, 0xF>(v)); top(lg_shift<0x118, 0xF>(v));
+    return v;
+}
 template <typename T>
 __device__ __forceinline__ T lg_wave_max(T v) {
     auto top = [&](T u) { if (u > v) v = u; };
-    top(lg_shift<0x111, 0xF>(v)); top(lg_shift<0x112, 0xF>(v)); top(lg_shift<0x114, 0xF>(v));
-    top(lg_shift<0x118, 0xF>(v)); top(lg_shift<0x142, 0xA>(v)); top(lg_shift<0x143, 0xC>(v));
+    v = lg_row_max(v);
+    top(lg_shift<0x142, 0xA>(v)); top(lg_shift<0x143, 0xC>(v));
     return lg_last_lane(v);
 }
 // A lane's number, the same lane for the whole wavefront

@@ -213,8 +213,11 @@ __device__ __forceinline__ void lg_sample_row(const SampleArgs &a, int r, const 
                                                  // logits lie anywhere in the row
 #define LG_SAMPLE_SLACK   2048                   // the estimated sum of a row's bins is trusted to 1 / 2048: four times what the comment at lg_k_sample_bins allows
 
+// Tokens whose largest logit lg_k_sample_max keeps: a group's, a quarter's where these are no more than LG_SAMPLE_GROUPS (a small top-k is to be half of their number
+// at most, and its candidates lie in fewer tokens: a row of 32000, top-k 64, 31.1 -> 17.4 us; of 128000, top-k 200, 22.5 -> 18.2)
+__host__ __device__ constexpr int lg_top_shift(int n_vocab) { return n_vocab <= LG_SAMPLE_GROUPS * 64 ? 6 : 8; }
 struct SampleWork {                     // per row, in working memory
-    uint32_t *gmax;                     // [groups] keys
+    uint32_t *gmax;                     // [tops] keys
     uint32_t *smin;                     // [workgroups of lg_k_sample_max] ~key of the smallest logit above -inf, 0: none
     lg_u64 *mass; uint32_t *count;      // [LG_SAMPLE_BINS]
     lg_u64 *gsum;                       // [groups]
@@ -222,15 +225,16 @@ struct SampleWork {                     // per row, in working memory
     uint32_t *ncand;                    // candidates; behind it, from word 4 on, the row's SampleRange, from word 8 its largest key and ~key of its smallest logit
     lg_u64 *cand;                       // [LG_SAMPLE_CAND] ~key << 32 | index
 };
-struct SampleGeo { int groups, maxes, slices; size_t gmax, smin, mass, count, gsum, part, ncand, cand, row; };
+struct SampleGeo { int groups, tops, maxes, slices; size_t gmax, smin, mass, count, gsum, part, ncand, cand, row; };
 __host__ __device__ inline size_t lg_up64(size_t n) { return (n + 63) & ~(size_t)63; }
 __host__ __device__ inline SampleGeo lg_sample_geo(int n_vocab) {
     SampleGeo g;
     g.groups = (n_vocab + LG_SAMPLE_GROUP - 1) / LG_SAMPLE_GROUP;
+    g.tops = (n_vocab + (1 << lg_top_shift(n_vocab)) - 1) >> lg_top_shift(n_vocab);
     g.maxes = (g.groups + 15) / 16;
     g.slices = (g.groups + 15) / 16;                 // of the passes after it at most: 16 groups or 64 each, as lg_hip_sample chooses
     size_t at = 0;
-    g.gmax = at;  at += lg_up64((size_t)g.groups * 4);
+    g.gmax = at;  at += lg_up64((size_t)g.tops * 4);
     g.smin = at;  at += lg_up64((size_t)g.maxes * 4);
     g.mass = at;  at += LG_SAMPLE_BINS * 8;
     g.count = at; at += LG_SAMPLE_BINS * 4;
@@ -251,7 +255,7 @@ enum { LG_ROW_FIRST, LG_ROW_SMALL, LG_ROW_FREE, LG_ROW_BORDER, LG_ROW_ALONE };
 __device__ __forceinline__ int lg_row_kind(const SampleRow &p, int n_vocab) {
     if (!(p.temperature > 0)) return LG_ROW_FIRST;
     const bool k = p.top_k > 0 && p.top_k < n_vocab;
-    if (k && p.top_k <= LG_SAMPLE_SMALL_K && p.top_k <= n_vocab / (2 * LG_SAMPLE_GROUP)) return LG_ROW_SMALL;
+    if (k && p.top_k <= LG_SAMPLE_SMALL_K && p.top_k <= n_vocab >> (lg_top_shift(n_vocab) + 1)) return LG_ROW_SMALL;
     if (!(p.temperature > 1e-20f)) return LG_ROW_ALONE;
     return k || p.top_p < 1 ? LG_ROW_BORDER : LG_ROW_FREE;
 }
@@ -260,16 +264,17 @@ __device__ __forceinline__ lg_u64 lg_least(const SampleRow &p) {      // the sma
     const double m = __builtin_ceil((double)p.min_p * LG_SAMPLE_ONE);
     return m >= 1 ? m < LG_SAMPLE_ONE ? (lg_u64)m : (lg_u64)LG_SAMPLE_ONE : 1;
 }
-// Four tokens of a lane in group `grp`; -inf behind the row's end.  VEC: rows aligned to 16 bytes
+// Tokens i .. i + 3; -inf behind the row's end.  VEC: rows aligned to 16 bytes
 template <bool VEC>
-__device__ __forceinline__ void lg_load4(const float *row, int n, int grp, float (&l)[4]) {
-    const int i = grp * LG_SAMPLE_GROUP + (threadIdx.x & 63) * 4;
+__device__ __forceinline__ void lg_load4_at(const float *row, int n, int i, float (&l)[4]) {
     if (VEC && i + 3 < n) { const float4 x = *(const float4 *)(row + i); l[0] = x.x; l[1] = x.y; l[2] = x.z; l[3] = x.w; }
     else
         #pragma unroll
         for (int j = 0; j < 4; ++j) l[j] = i + j < n ? row[i + j] : -INFINITY;
 }
-
+// Four tokens of a lane in group `grp`
+template <bool VEC>
+__device__ __forceinline__ void lg_load4(const float *row, int n, int grp, float (&l)[4]) { lg_load4_at<VEC>(row, n, grp * LG_SAMPLE_GROUP + (threadIdx.x & 63) * 4, l); }
 
 template <bool VEC>
 __global__ __launch_bounds__(LG_SAMPLE_MAX_WG) void lg_k_sample_max(SampleArgs a, char *base) {
@@ -286,6 +291,7 @@ __global__ __launch_bounds__(LG_SAMPLE_MAX_WG) void lg_k_sample_max(SampleArgs a
     if (lg_row_kind(p, a.n_vocab) == LG_ROW_BORDER)
         for (int i = part * LG_SAMPLE_MAX_WG + threadIdx.x; i < LG_SAMPLE_BINS; i += g.maxes * LG_SAMPLE_MAX_WG) { w.mass[i] = 0; w.count[i] = 0; }
     if (part == 0 && threadIdx.x == 0) *w.ncand = 0;
+    const bool quarters = lg_top_shift(a.n_vocab) == 6;
     uint32_t least = 0;                                      // as ~key: the largest is the smallest logit
     #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -296,9 +302,15 @@ __global__ __launch_bounds__(LG_SAMPLE_MAX_WG) void lg_k_sample_max(SampleArgs a
             if (k > m) m = k;
             if (k > 0x007FFFFFu && ~k > least) least = ~k;
         }
-        m = lg_wave_max(m);
         const int grp = part * 16 + wave * 4 + j;
-        if (lane == 0 && grp < g.groups) w.gmax[grp] = m;
+        if (quarters) {
+            m = lg_row_max(m);
+            const int at = grp * 4 + (lane >> 4);
+            if ((lane & 15) == 15 && at < g.tops) w.gmax[at] = m;
+        } else {
+            m = lg_wave_max(m);
+            if (lane == 0 && grp < g.tops) w.gmax[grp] = m;
+        }
     }
     least = lg_block_max<LG_SAMPLE_MAX_WG>(least, s_min);
     if (threadIdx.x == 0) w.smin[part] = least;
@@ -322,7 +334,7 @@ template <int NT>
 __device__ __forceinline__ SampleEnds lg_sample_ends(const SampleWork &w, const SampleGeo &g) {
     SampleEnds e{ 0, 0 };
     #pragma unroll
-    for (int i = 0; i < LG_SAMPLE_GROUPS / NT; ++i) { const int at = threadIdx.x + i * NT; const uint32_t k = w.gmax[at < g.groups ? at : 0]; if (k > e.key) e.key = k; }
+    for (int i = 0; i < LG_SAMPLE_GROUPS / NT; ++i) { const int at = threadIdx.x + i * NT; const uint32_t k = w.gmax[at < g.tops ? at : 0]; if (k > e.key) e.key = k; }
     const uint32_t k = w.smin[(int)threadIdx.x < g.maxes ? threadIdx.x : 0];          // (at most 128)
     e.least = k;
     return e;
@@ -621,7 +633,7 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
     const float *row = a.logits + r * a.stride, u = a.u[r];
     const SampleGeo g = lg_sample_geo(n_vocab);
     const SampleWork w = WHOLE ? SampleWork{} : lg_sample_work(base, g, r);
-    const int kind = lg_row_kind(p, n_vocab);
+    const int kind = lg_row_kind(p, n_vocab), top_shift = lg_top_shift(n_vocab);
     const lg_u64 least = lg_least(p);
     auto answer = [&](int tok, double prob, int kept) {
         a.tok[r] = tok;
@@ -662,7 +674,7 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
         // what the launches before left, all requested at once
         uint32_t gk[LG_SAMPLE_GROUPS / LG_SAMPLE_WG];
         #pragma unroll
-        for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) { const int at = t + i * LG_SAMPLE_WG; gk[i] = w.gmax[at < g.groups ? at : 0]; if (at >= g.groups) gk[i] = 0; }
+        for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) { const int at = t + i * LG_SAMPLE_WG; gk[i] = w.gmax[at < g.tops ? at : 0]; if (at >= g.tops) gk[i] = 0; }
         if (kind == LG_ROW_BORDER) {
             #pragma unroll
             for (int i = 0; i < PT; ++i) if constexpr (!WHOLE) kept_c[i] = w.cand[t + i * LG_SAMPLE_WG];
@@ -703,11 +715,12 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
             __syncthreads();
             if (t == 0) s.at = n_vocab;
             __syncthreads();
-            if (wave == 0) {
+            const int first = (grp << top_shift) + lane * 4;
+            if (wave == 0 && lane < 1 << (top_shift - 2)) {
                 float l[4];
-                lg_load4<VEC>(row, n_vocab, grp, l);
+                lg_load4_at<VEC>(row, n_vocab, first, l);
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) if (lg_key(l[i]) == span.key) atomicMin(&s.at, grp * LG_SAMPLE_GROUP + lane * 4 + i);
+                for (int i = 0; i < 4; ++i) if (lg_key(l[i]) == span.key) atomicMin(&s.at, first + i);
             }
         } else if (kind == LG_ROW_SMALL) {
             // a logit that at least top_k groups reach: the lower edge of one of 1024 equal parts between the groups' smallest and largest maxima
@@ -726,14 +739,15 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
             __syncthreads();
             const int n_groups = (int)s.n_groups;
             constexpr int AT_ONCE = 6;
-            for (int at = wave; at < n_groups; at += AT_ONCE * (LG_SAMPLE_WG / 64)) {      // groups of a wavefront on their way together: k = 64 takes 66 to 80 in all
+            const int each = 8 - top_shift;                          // a wavefront's load is one group, or four quarters
+            for (int at = wave; at << each < n_groups; at += AT_ONCE * (LG_SAMPLE_WG / 64)) {      // groups of a wavefront on their way together: k = 64 takes 66 to 80 in all
                 float l[AT_ONCE][4];
-                uint32_t grp[AT_ONCE];
+                int tok[AT_ONCE];
                 #pragma unroll
                 for (int j = 0; j < AT_ONCE; ++j) {
-                    const int b = at + j * (LG_SAMPLE_WG / 64);
-                    grp[j] = b < n_groups ? s.groups[b] : g.groups;                         // (behind the row's end: -inf)
-                    lg_load4<VEC>(row, n_vocab, (int)grp[j], l[j]);
+                    const int b = ((at + j * (LG_SAMPLE_WG / 64)) << each) + (lane >> (top_shift - 2));
+                    tok[j] = b < n_groups ? (int)(s.groups[b] << top_shift) + (lane & ((1 << (top_shift - 2)) - 1)) * 4 : n_vocab;         // (behind the row's end: -inf)
+                    lg_load4_at<VEC>(row, n_vocab, tok[j], l[j]);
                 }
                 uint32_t found = 0;
                 #pragma unroll
@@ -751,7 +765,7 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t k = lg_key(l[j][i]);
                         if (k < from) continue;
-                        if (to < LG_SAMPLE_CAND) s.cand[to] = (lg_u64)~k << 32 | (grp[j] * LG_SAMPLE_GROUP + lane * 4 + i);
+                        if (to < LG_SAMPLE_CAND) s.cand[to] = (lg_u64)~k << 32 | (uint32_t)(tok[j] + i);
                         ++to;
                     }
             }

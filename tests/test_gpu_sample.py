@@ -173,3 +173,20 @@ def test_the_same_row_gives_the_same_token_wherever_it_stands(dev):
     many = sample(dev, np.repeat(one, 12, 0), p * 4, np.full(12, 0.37, np.float32))
     for i in range(12):
         assert [int(many[j][i]) for j in (0, 2)] == [int(alone[i % 3][j][0]) for j in (0, 2)] and many[1][i] == alone[i % 3][1][0]
+
+
+@pytest.mark.parametrize("V, k", [(8193, 64), (8193, 65), (8321, 65), (33001, 257), (131072, 512), (131073, 256), (131073, 257), (262144, 513), (200003, 128)])
+def test_a_small_top_k_and_the_next_larger_one(dev, V, k):
+    """Rows by their groups' maxima up to a top-k of half as many as there are groups: of any distribution, of few tokens, of many equal ones, of likely ones
+    that lie together, of tiny weights."""
+    rng = np.random.default_rng(V + k)
+    l = rows_like_logits(rng, 7, V)
+    few = rng.choice(V, 30, replace=False)
+    l[1] = np.where(np.isin(np.arange(V), few), l[1], -np.inf)
+    l[2] = np.round(l[2] * 2) / 2                            # hundreds of equal ones at the border
+    l[3, V - 700:] += np.float32(9.0)
+    l[4] = np.float32(1.0); l[4, V // 2:V // 2 + 300] = np.float32(1.25)
+    l[5] *= np.float32(30.0)
+    print(f"sample V={V} k={k}", flush=True)
+    for rest in ((0.95, 0.0), (1.0, 0.0), (0.3, 0.02)):
+        check(dev, l, [(1.0, k, *rest)] * 6 + [(0.4, k - 7, *rest)], rng.random(7))
