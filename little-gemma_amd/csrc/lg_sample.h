@@ -22,6 +22,7 @@
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "lg_block.h"
 
@@ -788,14 +789,43 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
         const lg_u64 x = u > 0 ? (lg_u64)__builtin_floor((u < 1 ? (double)u : 1.0) * (double)S) : 0;
         return x > S - 1 ? S - 1 : x;
     };
-    if (!WHOLE && kind == LG_ROW_SMALL && n <= LG_SAMPLE_LIST) {
-        // a few hundred: each one's place in the order and the sum up to it from 1024 equal parts of the keys, and pair by pair within its part; then the same in index
-        // order among what stays.  (All pairs instead, in a third of the barriers: 16.6 and 17.2 us at top-k 20, even at 40, 21.1 and 18.7 at 100.)  A part has its count above 54 bits of sum: 512 weights of 2^44 are 2^53
-        const lg_u64 me = c(0), own = m[0], low54 = (1ull << 54) - 1;
+    auto bin = [&](int i) { if constexpr (WHOLE) return lg_sample_bin(span, x[i]) * 1024 / LG_SAMPLE_BINS; else return 0; };
+    // top-k, then top-p: `last` is the last token in the order that stays
+    lg_u64 last = ~0ull;
+    bool lost = false;                                       // the candidates do not hold the border after all
+    const bool small = !WHOLE && kind == LG_ROW_SMALL;
+    constexpr lg_u64 one_more = 1ull << 54, sum_of = one_more - 1;                           // a count above 54 bits of sum: 512 weights of 2^44 are 2^53
+    // At most LG_SAMPLE_SMALL_K of R candidates a thread stay: the part of the draw among 1024 of the vocabulary, and pair by pair those in it (one row, top-k 512 and
+    // top-p 0.95: each one's running sum from all that stay 58.0 us, so 36.5).  The parts and s.n are 0
+    auto small_draw = [&](auto regs, lg_u64 last) {
+        constexpr int R = decltype(regs)::value;
+        auto stays = [&](int i) { return m[i] >= least && c(i) <= last; };
+        auto piece = [&](int i) { return (int)((uint32_t)c(i) / (LG_SAMPLE_VOCAB / 1024)); };
+        #pragma unroll
+        for (int i = 0; i < R; ++i) if (stays(i)) atomicAdd(&s.bin[piece(i)], one_more | m[i]);
+        __syncthreads();
+        const lg_u64 here = s.bin[t], upto = lg_block_run<LG_SAMPLE_WG>(here, s.part, &all), S = all & sum_of, target = target_of(S), before = (upto - here) & sum_of;
+        if ((upto & sum_of) > target && before <= target) { s.at = t; s.rest = before; }
+        __syncthreads();
+        #pragma unroll
+        for (int i = 0; i < R; ++i) if (stays(i) && piece(i) == s.at) { const uint32_t at = atomicAdd(&s.n, 1u); s.list[at] = c(i); s.cand[at] = m[i]; }
+        __syncthreads();
+        const uint32_t in = s.n;
+        if ((uint32_t)t >= in) return;
+        const uint32_t me = (uint32_t)s.list[t];
+        const lg_u64 own = s.cand[t];
+        lg_u64 to = s.rest;
+        for (uint32_t i = 0; i < in; ++i) if ((uint32_t)s.list[i] <= me) to += s.cand[i];
+        if (to > target && to - own <= target) answer((int)me, (double)own / (double)S, (int)(all >> 54));
+    };
+    if (small && n <= LG_SAMPLE_LIST) {
+        // a few hundred: each one's place in the order and the sum up to it from 1024 equal parts of the keys, and pair by pair within its part.
+        // (All pairs instead, in a third of the barriers: 16.6 and 17.2 us at top-k 20, even at 40, 21.1 and 18.7 at 100.)
+        const lg_u64 me = c(0), own = m[0];
         const uint32_t wide = span.key - from;
         const int shift = wide >= 1024 ? 32 - __builtin_clz(wide) - 10 : 0;
         const uint32_t part = (span.key - ~(uint32_t)(me >> 32)) >> shift;
-        if (own) atomicAdd(&s.bin[part], 1ull << 54 | own);
+        if (own) atomicAdd(&s.bin[part], one_more | own);
         __syncthreads();
         const lg_u64 mine = s.bin[t], before = lg_block_run<LG_SAMPLE_WG>(mine, s.part, &all) - mine;
         s.sum[t] = before;
@@ -807,42 +837,24 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
         uint32_t place = 0;
         if (own) {
             const lg_u64 first = s.sum[part];
-            place = (uint32_t)(first >> 54); upto = first & low54;
+            place = (uint32_t)(first >> 54); upto = first & sum_of;
             for (uint32_t i = place, to = place + (uint32_t)(s.bin[part] >> 54); i < to; ++i) if (s.list[i] <= me) { upto += s.cand[i]; ++place; }
         }
         const uint32_t count = (uint32_t)(all >> 54), k = (uint32_t)p.top_k < count ? (uint32_t)p.top_k : count;
         if (own && place == k) s.whole = upto;
         __syncthreads();
-        s.bin[t] = 0;
         const lg_u64 W = s.whole;
+        s.bin[t] = 0;
+        if (t == 0) s.n = 0;
         lg_u64 want = W;
         if (p.top_p < 1) { const double want_d = __builtin_ceil((double)p.top_p * (double)W); want = want_d >= 1 ? (lg_u64)want_d < W ? (lg_u64)want_d : W : 1; }
         if (own && upto >= want && upto - own < want) s.last = me;
-        if (t == 0) s.n = 0;
         __syncthreads();
-        const bool stays = own >= least && me <= s.last;
-        const uint32_t piece = (uint32_t)me / (LG_SAMPLE_VOCAB / 1024);
-        if (stays) atomicAdd(&s.bin[piece], 1ull << 54 | own);
-        __syncthreads();
-        const lg_u64 here = s.bin[t], run = lg_block_run<LG_SAMPLE_WG>(here, s.part, &all), S = all & low54, target = target_of(S);
-        if ((run & low54) > target && ((run - here) & low54) <= target) { s.at = t; s.rest = (run - here) & low54; }
-        __syncthreads();
-        const bool in = stays && (int)piece == s.at;
-        if (in) { const uint32_t at = atomicAdd(&s.n, 1u); s.list[at] = me; s.cand[at] = own; }
-        __syncthreads();
-        if (in) {
-            lg_u64 to = s.rest;
-            for (uint32_t i = 0; i < s.n; ++i) if ((uint32_t)s.list[i] <= (uint32_t)me) to += s.cand[i];
-            if (to > target && to - own <= target) answer((int)(uint32_t)me, (double)own / (double)S, (int)(all >> 54));
-        }
+        small_draw(std::integral_constant<int, 1>{}, s.last);
         return true;
     }
-    auto bin = [&](int i) { if constexpr (WHOLE) return lg_sample_bin(span, x[i]) * 1024 / LG_SAMPLE_BINS; else return 0; };
-    // top-k, then top-p: `last` is the last token in the order that stays
-    lg_u64 last = ~0ull;
-    bool lost = false;                                       // the candidates do not hold the border after all
-    const bool longer = !WHOLE && kind != LG_ROW_SMALL;      // the candidates are a part of what stays
-    if (WHOLE || kind == LG_ROW_SMALL || q.cut < LG_SAMPLE_BINS) {
+    const bool longer = !WHOLE && !small;      // the candidates are a part of what stays
+    if (WHOLE || small || q.cut < LG_SAMPLE_BINS) {
         // (top-k counts tokens; of a longer row those of its bin)
         auto one = [&](int i) { return (lg_u64)(m[i] && (!longer || lg_sample_bin(span, lg_unkey(~(uint32_t)(c(i) >> 32))) == q.cut)); };
         lg_u64 mine = 0;
@@ -874,7 +886,7 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
     uint32_t mine = 0;
     #pragma unroll
     for (int i = 0; i < PT; ++i) { if (c(i) > last || m[i] < least) m[i] = 0; sum += m[i]; mine += m[i] != 0; }
-    kept += (uint32_t)lg_block_sum<LG_SAMPLE_WG>((lg_u64)mine, s.part);
+    if (!small) kept += (uint32_t)lg_block_sum<LG_SAMPLE_WG>((lg_u64)mine, s.part);
     if (WHOLE) {                                             // the candidates lie in index order
         lg_u64 run = lg_block_run<LG_SAMPLE_WG>(sum, s.part, &all) - sum;
         const lg_u64 target = target_of(all);
@@ -885,23 +897,11 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
         }
         return true;
     }
-    if (kind == LG_ROW_SMALL) {
-        // at most LG_SAMPLE_SMALL_K stay: each one's running sum in index order from all of them, by four threads each where there are few
-        all = lg_block_sum<LG_SAMPLE_WG>(sum, s.part);
-        const lg_u64 target = target_of(all);
+    if (small) {
+        s.bin[t] = 0;
         if (t == 0) s.n = 0;
         __syncthreads();
-        #pragma unroll
-        for (int i = 0; i < PT; ++i) if (m[i]) { const uint32_t at = atomicAdd(&s.n, 1u); s.list[at] = (lg_u64)(uint32_t)c(i) << 45 | m[i]; }       // (19 bits of index, 45 of weight)
-        __syncthreads();
-        const uint32_t stay = s.n, ways = stay <= LG_SAMPLE_WG / 4 ? 4 : 1, who = (uint32_t)t / ways;
-        if (who < stay) {
-            const lg_u64 me = s.list[who], weight = me & ((1ull << 45) - 1);
-            lg_u64 upto = 0;
-            for (uint32_t i = (uint32_t)t % ways; i < stay; i += ways) { const lg_u64 x = s.list[i]; if (x >> 45 <= me >> 45) upto += x & ((1ull << 45) - 1); }
-            if (ways == 4) { upto += __shfl_xor(upto, 1); upto += __shfl_xor(upto, 2); }
-            if ((uint32_t)t % ways == 0 && upto > target && upto - weight <= target) answer((int)(me >> 45), (double)weight / (double)all, (int)kept);
-        }
+        small_draw(std::integral_constant<int, PT>{}, last);
         return true;
     }
     // the groups' sums with the candidates that stay, the group of the draw, and the token in it
