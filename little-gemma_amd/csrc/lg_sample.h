@@ -58,7 +58,7 @@ __device__ const double lg_exp2_32nds[32] = {
 struct Weigh { double top, inv; const double *tab; };
 // 2^44 e^((l - top) / T), rounded.  With y = 32 (l - top) / (T ln 2) = n + r, n whole, it is 2^(44 + n / 32) times the power series of 2^(r / 32) (|r| <= 1/2: what
 // comes after r^5 is 2e-15).  Adding 1.5 2^52 leaves n in the low bits, adding 2^52 the result.  Beyond LG_SAMPLE_REACH it is 0.  (The series of e^r to r^12
-// without the table is 25 operations in place of 14: lg_k_sample_sums of 5 rows of 262144 21.0 -> @SUMS@ us with it.)
+// without the table would be 25 operations in place of 14.)
 #define LG_SAMPLE_REACH   31.5
 __device__ __forceinline__ lg_u64 lg_weight_at(const Weigh &w, double y) {          // y of -LG_SAMPLE_REACH 32 / ln 2 .. 0
     const double t = y + 6755399441055744.0, r = y - (t - 6755399441055744.0);
@@ -209,9 +209,10 @@ __device__ __forceinline__ void lg_sample_row(const SampleArgs &a, int r, const 
 #define LG_SAMPLE_BINS    2048
 #define LG_SAMPLE_CAND    4096                   // candidates that a row may have
 #define LG_SAMPLE_WHOLE   8192                   // tokens of a row that one workgroup takes by itself: 8 to a thread (16 do not fit its registers)
-#define LG_SAMPLE_SMALL_K 512                    // top-k up to which, and up to half as many as there are groups, the groups' maxima bound the candidates well: with
-                                                 // 1024 groups the tokens not below the k-th largest maximum are 1.15 k at k = 256 and 1.39 k at 512 where large
-                                                 // logits lie anywhere in the row
+#define LG_SAMPLE_SMALL_K 400                    // top-k up to which, and up to half as many as there are groups, the groups' maxima bound the candidates well: with
+                                                 // 1024 groups the tokens not below the k-th largest maximum are 1.15 k at k = 256 and 1.27 k at 400 where large
+                                                 // logits lie anywhere in the row.  One row of 262144 by maxima and by bins: top-k 200 22 and 32 us, 400 29 and 33,
+                                                 // 512 (more than LG_SAMPLE_LIST candidates) 37 and 32
 #define LG_SAMPLE_SLACK   2048                   // the estimated sum of a row's bins is trusted to 1 / 2048: four times what the comment at lg_k_sample_bins allows
 
 // Tokens whose largest logit lg_k_sample_max keeps: a group's, a quarter's where these are no more than LG_SAMPLE_GROUPS (a small top-k is to be half of their number
@@ -795,8 +796,8 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
     bool lost = false;                                       // the candidates do not hold the border after all
     const bool small = !WHOLE && kind == LG_ROW_SMALL;
     constexpr lg_u64 one_more = 1ull << 54, sum_of = one_more - 1;                           // a count above 54 bits of sum: 512 weights of 2^44 are 2^53
-    // At most LG_SAMPLE_SMALL_K of R candidates a thread stay: the part of the draw among 1024 of the vocabulary, and pair by pair those in it (one row, top-k 512 and
-    // top-p 0.95: each one's running sum from all that stay 58.0 us, so 36.5).  The parts and s.n are 0
+    // At most LG_SAMPLE_SMALL_K of R candidates a thread stay: the part of the draw among 1024 of the vocabulary, and pair by pair those in it (each one's
+    // running sum from all that stay instead: 58.0 and 36.6 us a row where 490 stay).  The parts and s.n are 0
     auto small_draw = [&](auto regs, lg_u64 last) {
         constexpr int R = decltype(regs)::value;
         auto stays = [&](int i) { return m[i] >= least && c(i) <= last; };
