@@ -203,6 +203,8 @@ __global__ __launch_bounds__(256) void lg_k_page_write(PageGeo g, const float *k
 // units, each at what it can draw); one of 100 keys: 4.5 us.
 #define LG_PA_WAVES 4
 #define LG_PA_TILE  32
+#define LG_PA_LANES 64
+#define LG_PA_SEQS  4096            // sequences of a call
 #define LG_PA_CHUNK 2048            // keys of a split at most: their page ids lie in LDS
 // A barrier for what went through LDS: loads from memory stay on their way, which the barrier of __syncthreads waits for as well
 __device__ __forceinline__ void lg_barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -216,7 +218,8 @@ struct PageAttn {
     float *out; long long out_stride;
     float *pm, *pl, *pacc;              // [splits of all][H], [..][hd]: partials of sequences of more than one split
     float scale;
-    int H, nkv, n_seq, max_blocks, max_len, window, slots, least;       // slots: workgroups that the chip holds at a time; least: tiles of a split
+    int32_t *cut;                       // of more than LG_PA_LANES sequences, from lg_k_page_cut: tiles of a split; [n_seq + 1] splits before each sequence; their sequences
+    int H, nkv, n_seq, max_blocks, max_len, window, slots, least;       // slots: workgroups that the chip holds at a time; least: tiles of a split, or all of a sequence's where there are no partials
 };
 // The keys a sequence sees: [lo, len)
 __device__ __forceinline__ void lg_pa_range(const PageAttn &a, int seq, int &lo, int &len) {
@@ -237,7 +240,6 @@ __device__ __forceinline__ int lg_pa_tiles(const PageAttn &a, int seq) {
 // chip holds at a time, not splits of a fixed size that the lengths fill unevenly.
 // A sequence without keys has one split too: it writes the zeros.
 struct PageCut { int tiles; int seq, index, first, n; };       // tiles of a split; of split number `at`: its sequence, its place there, the number of the sequence's first, how many it has
-struct PageCutLds { uint32_t part[16]; PageCut c; };
 // `total` tiles of `some` sequences that have any: the smallest of a few sizes whose splits are at most a whole number of rounds of a.slots workgroups, as few as leave half of
 // them to splits that are full.  Were every sequence's last split a full one, `some` more than total / size would be needed; ragged ones need half as many, and the size
 // for that is tried first (61 sequences of 4..8192 keys, heads of 256: 74.3 -> 72.1 us).  count(t): the splits of size t
@@ -250,6 +252,7 @@ __device__ __forceinline__ uint32_t lg_pa_split_tiles(const PageAttn &a, uint32_
     };
     const uint32_t most = size(some);
     if (some < 2 || most == (uint32_t)a.least) return most;
+    #pragma unroll 1
     for (uint32_t eighths = 4; eighths < 8; ++eighths) {
         const uint32_t tiles = size((some * eighths + 7) / 8);
         if (tiles == most) break;
@@ -258,39 +261,58 @@ __device__ __forceinline__ uint32_t lg_pa_split_tiles(const PageAttn &a, uint32_
     return most;
 }
 __device__ __forceinline__ uint32_t lg_pa_splits(uint32_t of, uint32_t tiles) { const uint32_t x = (of + tiles - 1) / tiles; return x ? x : 1u; }
-template <int NT>
-__device__ __forceinline__ PageCut lg_pa_cut(const PageAttn &a, int at, int seq, PageCutLds &s) {      // seq >= 0: of that sequence instead
-    if (a.n_seq <= 64) {                                       // a lane for each, in every wavefront: no barrier
-        const int i = threadIdx.x & 63;
-        const uint32_t mine = i < a.n_seq ? lg_pa_tiles(a, i) : 0, some = (uint32_t)__popcll(__ballot(mine != 0));
-        const uint32_t tiles = lg_pa_split_tiles(a, lg_wave_total(mine), some, [&](uint32_t t) { return lg_wave_total((mine + t - 1) / t); });
-        const uint32_t n = i < a.n_seq ? lg_pa_splits(mine, tiles) : 0, run = lg_wave_run(n) - n;
-        const lg_u64 it = __ballot(seq < 0 ? (uint32_t)at - run < n : i == seq);
-        if (!it) return { (int)tiles, -1, 0, 0, 0 };
-        const int lane = (int)__builtin_ctzll(it), first = (int)lg_lane(run, lane);
-        return { (int)tiles, lane, at - first, first, (int)lg_lane(n, lane) };
+__device__ __forceinline__ PageCut lg_pa_cut(const PageAttn &a, int at, int seq) {              // seq >= 0: of that sequence instead
+    if (!a.pm) return { a.least, at, 0, at, 1 };
+    if (a.n_seq > LG_PA_LANES) {
+        if (seq < 0) {
+            seq = a.cut[2 + a.n_seq + at];
+            if (at >= a.cut[1 + a.n_seq]) return { 0, -1, 0, 0, 0 };
+        }
+        const int first = a.cut[1 + seq];
+        return { a.cut[0], seq, at - first, first, a.cut[2 + seq] - first };
     }
-    const int per = (a.n_seq + NT - 1) / NT, i0 = threadIdx.x * per;
-    uint32_t mine = 0, some = 0, all;
-    for (int i = i0; i < i0 + per && i < a.n_seq; ++i) { const uint32_t x = lg_pa_tiles(a, i); mine += x; some += x != 0; }
-    mine = lg_block_sum<NT>(mine, s.part);
-    some = lg_block_sum<NT>(some, s.part);
-    const uint32_t tiles = lg_pa_split_tiles(a, mine, some, [&](uint32_t t) {
+    // a lane for each, in every wavefront: no barrier
+    const int i = threadIdx.x & 63;
+    const uint32_t mine = i < a.n_seq ? lg_pa_tiles(a, i) : 0, some = (uint32_t)__popcll(__ballot(mine != 0));
+    const uint32_t tiles = lg_pa_split_tiles(a, lg_wave_total(mine), some, [&](uint32_t t) { return lg_wave_total((mine + t - 1) / t); });
+    const uint32_t n = i < a.n_seq ? lg_pa_splits(mine, tiles) : 0, run = lg_wave_run(n) - n;
+    const lg_u64 it = __ballot(seq < 0 ? (uint32_t)at - run < n : i == seq);
+    if (!it) return { (int)tiles, -1, 0, 0, 0 };
+    const int lane = (int)__builtin_ctzll(it), first = (int)lg_lane(run, lane);
+    return { (int)tiles, lane, at - first, first, (int)lg_lane(n, lane) };
+}
+// The cut of more sequences than a wavefront has lanes, worked out once: in every workgroup it takes several barriers and passes over the
+// lengths.  400 sequences of all lengths up to 1024, heads of 128: 66.8 -> 48.0 us, with the joining launch's workgroups of one wavefront
+#define LG_PC_WG    1024
+__global__ __launch_bounds__(LG_PC_WG) void lg_k_page_cut(PageAttn a) {
+    __shared__ uint32_t part[LG_PC_WG / 64];
+    __shared__ int32_t before[LG_PA_SEQS + 1];
+    constexpr int PER = LG_PA_SEQS / LG_PC_WG;
+    const int per = (a.n_seq + LG_PC_WG - 1) / LG_PC_WG, i0 = threadIdx.x * per;
+    uint32_t x[PER], mine = 0, some = 0, all;
+    #pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        x[k] = k < per && i0 + k < a.n_seq ? lg_pa_tiles(a, i0 + k) : 0;
+        mine += x[k]; some += x[k] != 0;
+    }
+    const uint32_t total = lg_block_sum<LG_PC_WG>(mine, part);
+    some = lg_block_sum<LG_PC_WG>(some, part);
+    const uint32_t tiles = lg_pa_split_tiles(a, total, some, [&](uint32_t t) {
         uint32_t n = 0;
-        for (int i = i0; i < i0 + per && i < a.n_seq; ++i) n += (lg_pa_tiles(a, i) + t - 1) / t;
-        return lg_block_sum<NT>(n, s.part);
+        #pragma unroll
+        for (int k = 0; k < PER; ++k) n += (x[k] + t - 1) / t;
+        return lg_block_sum<LG_PC_WG>(n, part);
     });
-    if (threadIdx.x == 0) s.c.seq = -1;
     uint32_t n = 0;
-    for (int i = i0; i < i0 + per && i < a.n_seq; ++i) n += lg_pa_splits(lg_pa_tiles(a, i), tiles);
-    uint32_t run = lg_block_run<NT>(n, s.part, &all) - n;      // (its barriers: seq = -1 comes first)
-    for (int i = i0; i < i0 + per && i < a.n_seq; ++i) {
-        const uint32_t x = lg_pa_splits(lg_pa_tiles(a, i), tiles);
-        if (seq < 0 ? (uint32_t)at - run < x : i == seq) s.c = { (int)tiles, i, at - (int)run, (int)run, (int)x };
-        run += x;
-    }
+    #pragma unroll
+    for (int k = 0; k < PER; ++k) n += k < per && i0 + k < a.n_seq ? lg_pa_splits(x[k], tiles) : 0;
+    uint32_t run = lg_block_run<LG_PC_WG>(n, part, &all) - n;
+    #pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (k < per && i0 + k < a.n_seq) { before[i0 + k] = (int32_t)run; a.cut[1 + i0 + k] = (int32_t)run; run += lg_pa_splits(x[k], tiles); }
+    if (threadIdx.x == 0) { before[a.n_seq] = (int32_t)all; a.cut[0] = (int32_t)tiles; a.cut[1 + a.n_seq] = (int32_t)all; }
     __syncthreads();
-    return s.c;
+    for (int s = threadIdx.x; s < (int)all; s += LG_PC_WG) a.cut[2 + a.n_seq + s] = lg_owner(before, a.n_seq, s);
 }
 // The pages of a tile's two halves, and where their rows lie: page 0's first value where there is no such page
 struct PageTile { long long row[2]; bool ok[2]; };
@@ -326,9 +348,8 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     __shared__ float s_m[LG_PA_WAVES][8], s_l[LG_PA_WAVES][8];
     __shared__ __align__(16) union { lg_h8 q[KS][64]; float o[LG_PA_WAVES][8][HD]; } s;
     __shared__ int32_t s_ids[LG_PA_CHUNK / 16 + 1];
-    __shared__ PageCutLds s_cut;
     const int kvh = blockIdx.x % a.nkv, G = a.H / a.nkv;
-    const PageCut cut = lg_pa_cut<LG_PA_WAVES * 64>(a, blockIdx.x / a.nkv, -1, s_cut);
+    const PageCut cut = lg_pa_cut(a, blockIdx.x / a.nkv, -1);
     const int seq = __builtin_amdgcn_readfirstlane(cut.seq);
     if (seq < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -336,13 +357,14 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     constexpr int STEP = LG_PA_WAVES * TILE;
     const int32_t *table = a.table + (long long)seq * a.max_blocks;
     // queries are asked for first: what is asked for later arrives later, and behind the keys they would hold the first scores up
-    float4 qv[KS][2];
+    // A wavefront takes every fourth step's (all of them in every wavefront: one key, heads of 512 12.0 -> 9.4 us, of 256 7.1 -> 6.3)
+    constexpr int QS = (KS + LG_PA_WAVES - 1) / LG_PA_WAVES;
+    float4 qv[QS][2];
     const float *qrow = a.q + seq * a.q_stride + (long long)(kvh * G + ((c & 7) < G ? c & 7 : 0)) * HD + g * 8;
-    auto query = [&](int i, int j) { return *(const float4 *)(qrow + i * 32 + j * 4); };
     #pragma unroll
-    for (int i = 0; i < KS; ++i)
+    for (int i = 0; i < QS; ++i)
         #pragma unroll
-        for (int j = 0; j < 2; ++j) qv[i][j] = query(i, j);
+        for (int j = 0; j < 2; ++j) qv[i][j] = *(const float4 *)(qrow + (KS < LG_PA_WAVES ? wave % KS : i * LG_PA_WAVES + wave) * 32 + j * 4);
     int lo, len;
     lg_pa_range(a, seq, lo, len);
     const int chunk = __builtin_amdgcn_readfirstlane(cut.tiles) * LG_PA_TILE, n_split = __builtin_amdgcn_readfirstlane(cut.n);
@@ -366,7 +388,6 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
 
     lg_h8 kf[HALVES][KS];
     PageTile now = lg_pa_tile(a, ids, t0, kvh * HD);
-    if (t0 >= end) now.row[0] = now.row[1] = kvh * HD;          // (no tile: page 0's rows, so that the loads need no branch, after which everything would be waited for)
     auto load_keys = [&](const PageTile &p) {
         #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
@@ -375,27 +396,28 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
             for (int i = 0; i < KS; ++i) kf[h][i] = *(const lg_h8 *)(kp + i * 32);
         }
     };
-    __builtin_amdgcn_sched_barrier(0);
-    load_keys(now);
-    __builtin_amdgcn_sched_barrier(0);
-    if (has_id) s_ids[threadIdx.x] = my_id;
-
-    // queries: operand B of the scores, column c = query head c % 8, high part for c < 8; a quarter of the steps from each wavefront
+    // queries: operand B of the scores, column c = query head c % 8, high part for c < 8
     float qs;                                       // factor of the raw scores: base-2 exponents
-    {
+    auto queries = [&]() {
+        if (has_id) s_ids[threadIdx.x] = my_id;
         float top = 0;
         #pragma unroll
-        for (int i = 0; i < KS; ++i)
+        for (int i = 0; i < QS; ++i)
             #pragma unroll
             for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fmaxf(fabsf(qv[i][j].x), fabsf(qv[i][j].y)), fmaxf(fabsf(qv[i][j].z), fabsf(qv[i][j].w))));
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
+        if (lane < 8) s_m[wave][lane] = top;
+        lg_barrier_lds();
+        #pragma unroll
+        for (int v = 0; v < LG_PA_WAVES; ++v) top = fmaxf(top, s_m[v][c & 7]);
         int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;       // top * 2^-e in [2^14, 2^15)
         if (e < -100) e = -100;                                     // (zero and tiny rows; 2^-e stays a float)
         const float up = __uint_as_float((unsigned)(127 - e) << 23);
         #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            if (i % LG_PA_WAVES != wave) continue;
+        for (int i = 0; i < QS; ++i) {
+            const int step = i * LG_PA_WAVES + wave;
+            if (step >= KS) continue;
             const float v[8] = { qv[i][0].x, qv[i][0].y, qv[i][0].z, qv[i][0].w, qv[i][1].x, qv[i][1].y, qv[i][1].z, qv[i][1].w };
             lg_h8 part;
             #pragma unroll
@@ -404,11 +426,22 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
                 const _Float16 hi = (_Float16)z;
                 part[j] = c < 8 ? hi : (_Float16)(z - (float)hi);
             }
-            s.q[i][lane] = part;
+            s.q[step][lane] = part;
         }
         qs = a.scale * 1.44269504088896341f * __uint_as_float((unsigned)(127 + e) << 23);
+        lg_barrier_lds();
+    };
+    // A wavefront without a tile asks for no keys (84 short sequences of heads of 256: 12.0 -> 9.7 us).  The queries are prepared on either side of that branch: behind it
+    // they would have to wait for everything in flight
+    if (t0 < end) {
+        __builtin_amdgcn_sched_barrier(0);
+        load_keys(now);
+        __builtin_amdgcn_sched_barrier(0);
+        queries();
+    } else {
+        queries();
+        asm volatile("");                           // (so that the two sides stay apart)
     }
-    lg_barrier_lds();
     lg_f4 acc[NT];
     #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i] = (lg_f4){ 0, 0, 0, 0 };
@@ -524,27 +557,30 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
             for (int i = 0; i < DL; i += 4) *(float4 *)&s.o[wave][4 * (g & 1) + r + (g >> 1)][ch * 128 + c * DL + i] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
     __syncthreads();
-    for (int id = threadIdx.x; id < G * (HD / 4); id += LG_PA_WAVES * 64) {
-        const int h = id / (HD / 4), d = id % (HD / 4) * 4;
+    // all eight heads' sums, so that nothing waits for a branch; those there are are stored (rows may start anywhere: four values at a time where they are aligned for that)
+    constexpr int OUT = 8 * HD / 4, ROUNDS = (OUT + LG_PA_WAVES * 64 - 1) / (LG_PA_WAVES * 64);
+    const bool wide = (((uintptr_t)a.out | (uintptr_t)a.out_stride * 4) & 15) == 0;
+    #pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+        const int id = threadIdx.x + k * (LG_PA_WAVES * 64), h = id / (HD / 4) & 7, d = id % (HD / 4) * 4;
         float M = -INFINITY, L = 0;
         float4 o = make_float4(0, 0, 0, 0);
         #pragma unroll
         for (int v = 0; v < LG_PA_WAVES; ++v) M = fmaxf(M, s_m[v][h]);
         #pragma unroll
         for (int v = 0; v < LG_PA_WAVES; ++v) {
-            const float lv = s_l[v][h];
-            if (lv == 0.0f) continue;                               // no key; a score of NaN leaves its mark in the sum
-            const float f = __builtin_amdgcn_exp2f(s_m[v][h] - M);
+            const float lv = s_l[v][h], f = lv == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_m[v][h] - M);       // (0: no key; a score of NaN leaves its mark in the sum)
             const float4 x = *(const float4 *)&s.o[v][h][d];
             L += f * lv;
             o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
         }
+        if (id >= G * (HD / 4)) continue;
         const int head = kvh * G + h;
         if (n_split == 1) {
-            float *const p = a.out + seq * a.out_stride + (long long)head * HD + d;       // (rows may start anywhere)
-            const float x[4] = { o.x, o.y, o.z, o.w };
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = L == 0.0f ? 0.0f : x[i] / L;
+            float *const p = a.out + seq * a.out_stride + (long long)head * HD + d;
+            const float4 x = L == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(o.x / L, o.y / L, o.z / L, o.w / L);
+            if (wide) *(float4 *)p = x;
+            else { p[0] = x.x; p[1] = x.y; p[2] = x.z; p[3] = x.w; }
         } else {
             const long long at = (long long)(blockIdx.x / a.nkv) * a.H + head;
             *(float4 *)(a.pacc + at * HD + d) = o;
@@ -555,14 +591,12 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
 
 // The splits of a sequence, joined: a workgroup per (sequence, head).  A split's factor is computed once, by one thread; then the wavefronts take splits in
 // turn, a lane HD / 64 dimensions, and their sums are added in order.  A chain of cut, maxima, factors and sums: 5 to 6 us for 8 or 16 heads of 256, whether 60 or 500 splits.
-#define LG_PM_WAVES 8
-template <int HD>
-__global__ __launch_bounds__(LG_PM_WAVES * 64) void lg_k_page_merge(PageAttn a) {
-    constexpr int NT = LG_PM_WAVES * 64, D = HD / 64;
-    __shared__ float s_f[NT], s_w[LG_PM_WAVES], s_o[LG_PM_WAVES][HD];
-    __shared__ PageCutLds s_cut;
+template <int HD, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void lg_k_page_merge(PageAttn a) {
+    constexpr int NT = WAVES * 64, D = HD / 64;
+    __shared__ float s_f[NT], s_w[WAVES], s_o[WAVES][HD];
     const int head = blockIdx.x, seq = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const PageCut cut = lg_pa_cut<NT>(a, 0, seq, s_cut);
+    const PageCut cut = lg_pa_cut(a, 0, seq);
     const int n = __builtin_amdgcn_readfirstlane(cut.n), from = __builtin_amdgcn_readfirstlane(cut.first);
     if (n < 2) return;                                       // (its one split has written the output)
     // what the first NT splits need is asked for at once: a wavefront's first eight sums with the maxima
@@ -573,14 +607,14 @@ __global__ __launch_bounds__(LG_PM_WAVES * 64) void lg_k_page_merge(PageAttn a) 
     vec ahead[FIRST];
     const float m0 = t < n ? a.pm[place(t)] : -INFINITY, l0 = t < n ? a.pl[place(t)] : 0.0f;
     #pragma unroll
-    for (int j = 0; j < FIRST; ++j) { const int k = wave + j * LG_PM_WAVES; ahead[j] = sums(k < n ? k : n - 1); }
+    for (int j = 0; j < FIRST; ++j) { const int k = wave + j * WAVES; ahead[j] = sums(k < n ? k : n - 1); }
     float M = m0;
     for (int i = t + NT; i < n; i += NT) M = fmaxf(M, a.pm[place(i)]);
     for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
     if (lane == 0) s_w[wave] = M;
     __syncthreads();
     #pragma unroll
-    for (int v = 0; v < LG_PM_WAVES; ++v) M = fmaxf(M, s_w[v]);
+    for (int v = 0; v < WAVES; ++v) M = fmaxf(M, s_w[v]);
     float L = 0;
     vec o = 0;
     for (int base = 0; base < n; base += NT) {
@@ -595,9 +629,9 @@ __global__ __launch_bounds__(LG_PM_WAVES * 64) void lg_k_page_merge(PageAttn a) 
         int k = wave;
         if (!base)
             #pragma unroll
-            for (int j = 0; j < FIRST; ++j, k += LG_PM_WAVES) if (k < m) o += s_f[k] * ahead[j];
+            for (int j = 0; j < FIRST; ++j, k += WAVES) if (k < m) o += s_f[k] * ahead[j];
         #pragma unroll 4
-        for (; k < m; k += LG_PM_WAVES) o += s_f[k] * sums(base + k);
+        for (; k < m; k += WAVES) o += s_f[k] * sums(base + k);
     }
     for (int x = 1; x < 64; x <<= 1) L += __shfl_xor(L, x);
     __syncthreads();
@@ -607,11 +641,11 @@ __global__ __launch_bounds__(LG_PM_WAVES * 64) void lg_k_page_merge(PageAttn a) 
     __syncthreads();
     L = 0;
     #pragma unroll
-    for (int v = 0; v < LG_PM_WAVES; ++v) L += s_w[v];
+    for (int v = 0; v < WAVES; ++v) L += s_w[v];
     for (int d = t; d < HD; d += NT) {
         float x = 0;
         #pragma unroll
-        for (int v = 0; v < LG_PM_WAVES; ++v) x += s_o[v][d];
+        for (int v = 0; v < WAVES; ++v) x += s_o[v][d];
         a.out[seq * a.out_stride + (long long)head * HD + d] = L == 0.0f ? 0.0f : x / L;
     }
 }

@@ -95,15 +95,20 @@ extern "C" int lg_hip_paged_write(const struct lg_hip_pages *p, const float *d_k
 }
 
 // ---- attend -----------------------------------------------------------------------------------------------------
-#define LG_PA_SEQS   4096            // sequences of a call: every workgroup goes over their lengths
 // Workgroups of lg_k_page_attn at a time: lg_pa_per_simd on each of 256 compute units
 static int slots_of(int hd) { return 256 * lg_pa_per_simd(hd); }
 // Splits of all sequences together, at most.  lg_pa_split_tiles makes the full ones of a key head slots / n_head_kv or fewer for every round, the rounds one or 2 units / slots rounded
 // up, where splits of `tiles` tiles to LG_PA_CHUNK keys allow; every sequence has one that is not full besides
-// Sequences of up to so many tiles are left whole where none is longer: the launch that joins splits takes longer than what a split saves.  One sequence of 512 keys, whole
-// and in splits: heads of 64 7.5 and 8.8 us, 128 8.5 and 9.5, 256 13.9 and 11.2 (384 keys: 11.7 and 11.3); 64 sequences, 2 key heads of 256: 16.4 and 20.2; of
-// 512 192 keys 18.0 and 19.7, 256 20.2 and 19.8.  128 workgroups and more are a half of the compute units at work already
-static int alone_of(int hd, int64_t units) { return hd <= 128 ? 16 : hd == 256 ? (units >= 128 ? 20 : 12) : 6; }
+// Sequences of up to so many tiles are left whole where none is longer: the cut, the partials and the launch that joins them take longer than what splits save, the more so where
+// the sequences' key heads keep the chip at work by themselves.  Whole and in splits, us: one sequence of 512 keys, heads of 64 7.1 and 8.1, 128 8.0 and 9.0, 256 12.7 and 10.3 (320
+// keys: 9.7 and 10.2), 512 24.8 and 16.1 (192: 14.0 and 15.9).  Two key heads, all sequences as long as the longest / of all lengths up to it: 64 sequences of 1024, heads of 128 13.5 and
+// 19.3 / 13.1 and 13.6; of 768, heads of 256 19.9 and 26.0 / 18.9 and 18.1; 128 of 2047, heads of 128 39.6 and 48.9 / 26.7 and 32.5, heads of 256 93.6 and 114 / 55.3 and 57.7;
+// 200 of 2047, heads of 256 152 and 174 / 104 and 91.  One key head of 512: 128 of 512 28.1 and 36.6 / 26.3 and 25.4, 200 of 1024 75.7 and 94.3 / 48.8 and 51.9
+static int alone_of(int hd, int64_t units) {
+    const int tier = units < 128 ? 0 : units < 256 ? 1 : 2;
+    static const int tiles[4][3] = { { 20, 32, 64 }, { 18, 32, 64 }, { 11, 24, 48 }, { 7, 16, 32 } };          // heads of 64, 128, 256, 512
+    return tiles[hd == 64 ? 0 : hd == 128 ? 1 : hd == 256 ? 2 : 3][tier];
+}
 struct AttnCut { int64_t splits, tiles; bool join; int least; };        // tiles: of all sequences, at most
 static AttnCut cut_of(int n_seq, int n_head_kv, int hd, int max_len, int window) {
     // (a window need not start with a tile)
@@ -117,18 +122,22 @@ static bool attn_shape(int n_seq, int n_head, int n_head_kv, int hd, int max_len
     return n_seq >= 0 && n_head_kv >= 1 && n_head_kv <= 1024 && n_head >= 1 && n_head % n_head_kv == 0 && n_head / n_head_kv <= 8 &&
            (hd == 64 || hd == 128 || hd == 256 || hd == 512) && max_len >= 0 && max_len <= (1 << 30);
 }
+static size_t cut_bytes(int n_seq, const AttnCut &c) { return n_seq > LG_PA_LANES ? up256(((size_t)c.splits + n_seq + 2) * 4) : 0; }
 extern "C" size_t lg_hip_paged_attention_workspace(int n_seq, int n_head, int n_head_kv, int hd, int max_len, int window) {
     if (!attn_shape(n_seq, n_head, n_head_kv, hd, max_len)) return 0;
     const AttnCut c = cut_of(n_seq, n_head_kv, hd, max_len, window);
     if (!c.join) return 0;
     const size_t slots = (size_t)c.splits * n_head;
-    return 2 * up256(slots * 4) + slots * hd * 4;
+    return cut_bytes(n_seq, c) + 2 * up256(slots * 4) + slots * hd * 4;
 }
 
 template <int HD>
 static void launch_attn(const PageAttn &a, const AttnCut &c, hipStream_t st) {
     hipLaunchKernelGGL(lg_k_page_attn<HD>, dim3((unsigned)(c.splits * a.nkv)), dim3(LG_PA_WAVES * 64), 0, st, a);
-    if (c.join) hipLaunchKernelGGL(lg_k_page_merge<HD>, dim3(a.H, a.n_seq), dim3(LG_PM_WAVES * 64), 0, st, a);
+    if (!c.join) return;
+    // eight wavefronts to a head, or one where the chip has a head for each
+    if (a.n_seq > LG_PA_LANES) hipLaunchKernelGGL((lg_k_page_merge<HD, 1>), dim3(a.H, a.n_seq), dim3(64), 0, st, a);
+    else hipLaunchKernelGGL((lg_k_page_merge<HD, 8>), dim3(a.H, a.n_seq), dim3(512), 0, st, a);
 }
 
 extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float *d_q, int64_t q_stride, int n_seq, int n_head, const int32_t *d_table,
@@ -155,10 +164,11 @@ extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float 
     if (need && (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)))
         return lg_fail(-2, "paged_attention: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
     const size_t part = up256((size_t)c.splits * n_head * 4);
-    float *const w = (float *)d_work;
-    const PageAttn a{ g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, w, need ? (float *)((char *)d_work + part) : nullptr,
-                      need ? (float *)((char *)d_work + 2 * part) : nullptr, scale, n_head, p->n_head_kv, n_seq, max_blocks, max_len, window, slots_of(hd), c.least };
+    char *const w = need ? (char *)d_work + cut_bytes(n_seq, c) : nullptr;
+    const PageAttn a{ g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, (float *)w, need ? (float *)(w + part) : nullptr,
+                      need ? (float *)(w + 2 * part) : nullptr, scale, need ? (int32_t *)d_work : nullptr, n_head, p->n_head_kv, n_seq, max_blocks, max_len, window, slots_of(hd), c.least };
     hipStream_t st = (hipStream_t)stream;
+    if (c.join && n_seq > LG_PA_LANES) hipLaunchKernelGGL(lg_k_page_cut, dim3(1), dim3(LG_PC_WG), 0, st, a);
     switch (hd) {
         case 64:  launch_attn<64>(a, c, st); break;
         case 128: launch_attn<128>(a, c, st); break;
