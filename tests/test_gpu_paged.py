@@ -253,6 +253,23 @@ def test_attention_of_many_sequences(lg, dev, n, H, kv, hd, window):
     within(attend(lg, dev, q, k, v, table, lens, 16, kv, window, 1.0, 1500), want, bound)
 
 
+@pytest.mark.parametrize("n, H, kv, hd, window, longest", [(65, 8, 2, 64, 0, 2500), (66, 1, 1, 64, 0, 20011), (300, 4, 2, 128, 0, 3000), (70, 8, 2, 256, 2100, 2500),
+                                                           (67, 8, 1, 512, 0, 1500), (1025, 2, 1, 64, 0, 3001), (4096, 1, 1, 64, 0, 2500)])
+def test_attention_of_many_sequences_in_splits(lg, dev, n, H, kv, hd, window, longest):
+    """More sequences than a wavefront has lanes, one of them long and a few of middle length: cut by the launch ahead; more splits of one sequence than a
+    wavefront joins at a time; one length that a captured call would bring later."""
+    rng = np.random.default_rng(n + hd)
+    lens = rng.integers(0, 50, n)
+    lens[rng.integers(0, n, 4)] = 700
+    lens[rng.random(n) < 0.2] = 0
+    lens[n // 3] = longest
+    q, k, v, table = case(rng, H, kv, hd, 16, lens)
+    print(f"attend {n} sequences of up to {longest}, hd={hd}", flush=True)
+    for told in (lens, np.minimum(lens, 40), np.zeros_like(lens)):
+        want, bound = attend_ref(q, k, v, table, told, 16, k.shape[0], kv, window, 1.0, longest)
+        within(attend(lg, dev, q, k, v, table, told, 16, kv, window, 1.0, longest), want, bound)
+
+
 def test_attention_of_large_and_tiny_queries_and_scales(lg, dev):
     """Scores from almost equal to one key far above the rest, queries near the ends of f32's range, a negative scale, rows of zeros."""
     rng = np.random.default_rng(3)
