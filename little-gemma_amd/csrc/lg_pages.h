@@ -218,7 +218,7 @@ struct PageAttn {
     float *out; long long out_stride;
     float *pm, *pl, *pacc;              // [splits of all][H], [..][hd]: partials of sequences of more than one split
     float scale;
-    int32_t *cut;                       // of more than LG_PA_LANES sequences, from lg_k_page_cut: tiles of a split; [n_seq + 1] splits before each sequence; their sequences
+    int32_t *cut;                       // [n_seq + 1] splits before each sequence, for the joining launch; of more than LG_PA_LANES sequences from lg_k_page_cut, and then: tiles of a split; the splits' sequences
     int H, nkv, n_seq, max_blocks, max_len, window, slots, least;       // slots: workgroups that the chip holds at a time; least: tiles of a split, or all of a sequence's where there are no partials
 };
 // The keys a sequence sees: [lo, len)
@@ -261,22 +261,20 @@ __device__ __forceinline__ uint32_t lg_pa_split_tiles(const PageAttn &a, uint32_
     return most;
 }
 __device__ __forceinline__ uint32_t lg_pa_splits(uint32_t of, uint32_t tiles) { const uint32_t x = (of + tiles - 1) / tiles; return x ? x : 1u; }
-__device__ __forceinline__ PageCut lg_pa_cut(const PageAttn &a, int at, int seq) {              // seq >= 0: of that sequence instead
+__device__ __forceinline__ PageCut lg_pa_cut(const PageAttn &a, int at) {
     if (!a.pm) return { a.least, at, 0, at, 1 };
     if (a.n_seq > LG_PA_LANES) {
-        if (seq < 0) {
-            seq = a.cut[2 + a.n_seq + at];
-            if (at >= a.cut[1 + a.n_seq]) return { 0, -1, 0, 0, 0 };
-        }
-        const int first = a.cut[1 + seq];
-        return { a.cut[0], seq, at - first, first, a.cut[2 + seq] - first };
+        const int seq = a.cut[2 + a.n_seq + at];
+        if (at >= a.cut[a.n_seq]) return { 0, -1, 0, 0, 0 };
+        const int first = a.cut[seq];
+        return { a.cut[1 + a.n_seq], seq, at - first, first, a.cut[seq + 1] - first };
     }
     // a lane for each, in every wavefront: no barrier
     const int i = threadIdx.x & 63;
     const uint32_t mine = i < a.n_seq ? lg_pa_tiles(a, i) : 0, some = (uint32_t)__popcll(__ballot(mine != 0));
     const uint32_t tiles = lg_pa_split_tiles(a, lg_wave_total(mine), some, [&](uint32_t t) { return lg_wave_total((mine + t - 1) / t); });
     const uint32_t n = i < a.n_seq ? lg_pa_splits(mine, tiles) : 0, run = lg_wave_run(n) - n;
-    const lg_u64 it = __ballot(seq < 0 ? (uint32_t)at - run < n : i == seq);
+    const lg_u64 it = __ballot((uint32_t)at - run < n);
     if (!it) return { (int)tiles, -1, 0, 0, 0 };
     const int lane = (int)__builtin_ctzll(it), first = (int)lg_lane(run, lane);
     return { (int)tiles, lane, at - first, first, (int)lg_lane(n, lane) };
@@ -309,8 +307,8 @@ __global__ __launch_bounds__(LG_PC_WG) void lg_k_page_cut(PageAttn a) {
     uint32_t run = lg_block_run<LG_PC_WG>(n, part, &all) - n;
     #pragma unroll
     for (int k = 0; k < PER; ++k)
-        if (k < per && i0 + k < a.n_seq) { before[i0 + k] = (int32_t)run; a.cut[1 + i0 + k] = (int32_t)run; run += lg_pa_splits(x[k], tiles); }
-    if (threadIdx.x == 0) { before[a.n_seq] = (int32_t)all; a.cut[0] = (int32_t)tiles; a.cut[1 + a.n_seq] = (int32_t)all; }
+        if (k < per && i0 + k < a.n_seq) { before[i0 + k] = (int32_t)run; a.cut[i0 + k] = (int32_t)run; run += lg_pa_splits(x[k], tiles); }
+    if (threadIdx.x == 0) { before[a.n_seq] = (int32_t)all; a.cut[a.n_seq] = (int32_t)all; a.cut[a.n_seq + 1] = (int32_t)tiles; }
     __syncthreads();
     for (int s = threadIdx.x; s < (int)all; s += LG_PC_WG) a.cut[2 + a.n_seq + s] = lg_owner(before, a.n_seq, s);
 }
@@ -349,7 +347,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
     __shared__ __align__(16) union { lg_h8 q[KS][64]; float o[LG_PA_WAVES][8][HD]; } s;
     __shared__ int32_t s_ids[LG_PA_CHUNK / 16 + 1];
     const int kvh = blockIdx.x % a.nkv, G = a.H / a.nkv;
-    const PageCut cut = lg_pa_cut(a, blockIdx.x / a.nkv, -1);
+    const PageCut cut = lg_pa_cut(a, blockIdx.x / a.nkv);
     const int seq = __builtin_amdgcn_readfirstlane(cut.seq);
     if (seq < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -557,6 +555,11 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
             for (int i = 0; i < DL; i += 4) *(float4 *)&s.o[wave][4 * (g & 1) + r + (g >> 1)][ch * 128 + c * DL + i] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
     __syncthreads();
+    // (behind the loads: lengths and page ids come through the scalar cache as long as nothing has been stored)
+    if (a.pm && a.n_seq <= LG_PA_LANES && kvh == 0 && cut.index == 0 && threadIdx.x == 0) {
+        a.cut[seq] = cut.first;
+        if (seq == a.n_seq - 1) a.cut[a.n_seq] = cut.first + cut.n;
+    }
     // all eight heads' sums, so that nothing waits for a branch; those there are are stored (rows may start anywhere: four values at a time where they are aligned for that)
     constexpr int OUT = 8 * HD / 4, ROUNDS = (OUT + LG_PA_WAVES * 64 - 1) / (LG_PA_WAVES * 64);
     const bool wide = (((uintptr_t)a.out | (uintptr_t)a.out_stride * 4) & 15) == 0;
@@ -596,8 +599,7 @@ __global__ __launch_bounds__(WAVES * 64) void lg_k_page_merge(PageAttn a) {
     constexpr int NT = WAVES * 64, D = HD / 64;
     __shared__ float s_f[NT], s_w[WAVES], s_o[WAVES][HD];
     const int head = blockIdx.x, seq = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const PageCut cut = lg_pa_cut(a, 0, seq);
-    const int n = __builtin_amdgcn_readfirstlane(cut.n), from = __builtin_amdgcn_readfirstlane(cut.first);
+    const int from = a.cut[seq], n = a.cut[seq + 1] - from;
     if (n < 2) return;                                       // (its one split has written the output)
     // what the first NT splits need is asked for at once: a wavefront's first eight sums with the maxima
     typedef float vec __attribute__((ext_vector_type(D)));

@@ -122,7 +122,7 @@ static bool attn_shape(int n_seq, int n_head, int n_head_kv, int hd, int max_len
     return n_seq >= 0 && n_head_kv >= 1 && n_head_kv <= 1024 && n_head >= 1 && n_head % n_head_kv == 0 && n_head / n_head_kv <= 8 &&
            (hd == 64 || hd == 128 || hd == 256 || hd == 512) && max_len >= 0 && max_len <= (1 << 30);
 }
-static size_t cut_bytes(int n_seq, const AttnCut &c) { return n_seq > LG_PA_LANES ? up256(((size_t)c.splits + n_seq + 2) * 4) : 0; }
+static size_t cut_bytes(int n_seq, const AttnCut &c) { return up256(((size_t)n_seq + 1 + (n_seq > LG_PA_LANES ? 1 + c.splits : 0)) * 4); }
 extern "C" size_t lg_hip_paged_attention_workspace(int n_seq, int n_head, int n_head_kv, int hd, int max_len, int window) {
     if (!attn_shape(n_seq, n_head, n_head_kv, hd, max_len)) return 0;
     const AttnCut c = cut_of(n_seq, n_head_kv, hd, max_len, window);
