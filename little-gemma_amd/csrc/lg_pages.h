@@ -198,9 +198,9 @@ __global__ __launch_bounds__(256) void lg_k_page_write(PageGeo g, const float *k
 //   values in registers (v_perm_b32).
 // K and V never pass through LDS.  Maximum and sum run in f32; the sum is of the unsplit probabilities.
 // Bound by memory: a flop for every byte of K and V and query head of a group, where the matrix cores have hundreds.  What remains beside the bytes is the chain at either end
-// (lengths, page ids, first keys; sums of the wavefronts: 5 to 7 us together).  24 sequences of up to 16384 keys, 8 key heads of 256: 503 us, 6.4 TB/s; one of 100003 keys:
-// 136 us, 6.0 TB/s; 61 ragged ones of up to 8192, 2 key heads: 68 us, 5.1 TB/s (what the splits leave uneven); 64 windows of 512: 17.6 us, 3 TB/s (128 of 256 compute
-// units, each at what it can draw); one of 100 keys: 4.5 us.
+// (lengths, page ids, first keys; sums of the wavefronts: 3 to 6 us together).  24 sequences of up to 16384 keys, 8 key heads of 256: 503 us, 6.4 TB/s; one of 100003 keys:
+// 134 us, 6.1 TB/s; 61 ragged ones of up to 8192, 2 key heads: 66 us, 5.2 TB/s (what the splits leave uneven); 64 windows of 512: 16 us, 3.3 TB/s (128 of 256 compute
+// units, each at what it can draw); one of 100 keys: 3.9 us.
 #define LG_PA_WAVES 4
 #define LG_PA_TILE  32
 #define LG_PA_LANES 64
@@ -235,7 +235,7 @@ __device__ __forceinline__ int lg_pa_tiles(const PageAttn &a, int seq) {
     lg_pa_range(a, seq, lo, len);
     return (len + LG_PA_TILE - 1) / LG_PA_TILE - lo / LG_PA_TILE;
 }
-// How the call is cut: every workgroup works it out from the lengths.  A compute unit draws a fixed share of what memory gives (it keeps about 32 KB
+// How the call is cut, from the lengths: by every workgroup for up to LG_PA_LANES sequences, by lg_k_page_cut for more.  A compute unit draws a fixed share of what memory gives (it keeps about 32 KB
 // of misses on their way), so the call takes as long as the unit with the most keys: splits of one size, chosen so that their number is what the
 // chip holds at a time, not splits of a fixed size that the lengths fill unevenly.
 // A sequence without keys has one split too: it writes the zeros.
@@ -593,7 +593,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
 }
 
 // The splits of a sequence, joined: a workgroup per (sequence, head).  A split's factor is computed once, by one thread; then the wavefronts take splits in
-// turn, a lane HD / 64 dimensions, and their sums are added in order.  A chain of cut, maxima, factors and sums: 5 to 6 us for 8 or 16 heads of 256, whether 60 or 500 splits.
+// turn, a lane HD / 64 dimensions, and their sums are added in order.  A chain of maxima, factors and sums: 5 us for 8 or 16 heads of 256, whether 60 or 500 splits.
 template <int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void lg_k_page_merge(PageAttn a) {
     constexpr int NT = WAVES * 64, D = HD / 64;
