@@ -270,6 +270,52 @@ def test_attention_of_many_sequences_in_splits(lg, dev, n, H, kv, hd, window, lo
         within(attend(lg, dev, q, k, v, table, told, 16, kv, window, 1.0, longest), want, bound)
 
 
+@pytest.mark.parametrize("n, H, kv, hd, longest", [(3, 8, 2, 256, 3000), (64, 4, 1, 64, 2500), (70, 8, 2, 128, 2500)])
+def test_split_attention_in_two_graphs_at_once(lg, dev, n, H, kv, hd, longest):
+    """Joined splits recorded into two graphs, each with working memory of its own that holds rubbish; between the replays, which overlap, the lengths change
+    and eager calls run.  Every replay gives to the bit what the call by itself gives, and that is near the plain form."""
+    rng, rt = np.random.default_rng(n), dev.rt
+    most = np.where(np.arange(n) % 7 == 0, longest, 90)
+    q, k, v, table = case(rng, H, kv, hd, 32, most)
+    mem = [dev.up(x.view(np.uint16)) for x in (k, v)]
+    dq, dt, dl, out = dev.up(q), dev.up(table, np.int32), dev.up(most, np.int32), [dev.up(np.zeros((n, H, hd), np.float32)) for _ in range(3)]
+    p = lg.hiplib.Pages(mem[0].value, mem[1].value, k.shape[0], 32, kv, hd, kv * hd, 32 * kv * hd)
+    need = dev.H.lg_hip_paged_attention_workspace(n, H, kv, hd, longest, 0)
+    assert need > 0
+    work = [dev.up(np.full(need, 0xFF, np.uint8)) for _ in range(3)]
+
+    def call(i, stream=None):
+        dev.check(dev.H.lg_hip_paged_attention(C.byref(p), dq, H * hd, n, H, dt, table.shape[1], dl, longest, 0, 1.0, out[i], H * hd, work[i], need, stream), "paged_attention")
+
+    rt.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+    rt.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
+    rt.hipGraphExecDestroy.argtypes = rt.hipGraphDestroy.argtypes = rt.hipStreamDestroy.argtypes = [C.c_void_p]
+    streams, graphs, execs = [[C.c_void_p() for _ in range(2)] for _ in range(3)]
+    for i in range(2):
+        assert rt.hipStreamCreateWithFlags(C.byref(streams[i]), 1) == 0
+        assert rt.hipStreamBeginCapture(streams[i], 0) == 0
+        try:
+            call(i, streams[i])
+        finally:
+            end = rt.hipStreamEndCapture(streams[i], C.byref(graphs[i]))
+        assert end == 0 and rt.hipGraphInstantiate(C.byref(execs[i]), graphs[i], None, None, 0) == 0
+    for replay in range(4):
+        lens = most if replay == 0 else np.where(rng.random(n) < 0.2, 0, rng.integers(1, most + 1))
+        dev.put(dl, lens.astype(np.int32))
+        assert rt.hipDeviceSynchronize() == 0
+        print(f"replay {replay}", flush=True)
+        for i in range(2):
+            assert rt.hipGraphLaunch(execs[i], streams[i]) == 0
+        call(2)
+        assert rt.hipDeviceSynchronize() == 0
+        got = [dev.back(o, (n, H, hd), np.float32) for o in out]
+        assert np.array_equal(got[0], got[2]) and np.array_equal(got[1], got[2])
+        within(got[2], *attend_ref(q, k, v, table, lens, 32, k.shape[0], kv, 0, 1.0, longest), f"replay {replay}")
+    for i in range(2):
+        rt.hipGraphExecDestroy(execs[i]); rt.hipGraphDestroy(graphs[i]); rt.hipStreamDestroy(streams[i])
+    dev.free()
+
+
 def test_attention_of_large_and_tiny_queries_and_scales(lg, dev):
     """Scores from almost equal to one key far above the rest, queries near the ends of f32's range, a negative scale, rows of zeros."""
     rng = np.random.default_rng(3)
