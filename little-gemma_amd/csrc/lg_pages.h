@@ -264,7 +264,7 @@ template <typename Count>
 __device__ __forceinline__ uint32_t lg_pa_split_tiles(const PageAttn &a, uint32_t total, uint32_t some, Count count) {
     const uint32_t units = some * a.nkv, half = (uint32_t)a.slots / 2, rounds = units > half ? (units + half - 1) / half : 1, room = rounds * a.slots / a.nkv;
     auto size = [&](uint32_t spare) {
-        const uint32_t full = room - spare, tiles = (total + full - 1) / full;
+        const uint32_t full = room > spare ? room - spare : 1, tiles = (total + full - 1) / full;
         return tiles < (uint32_t)a.least ? a.least : tiles > LG_PA_CHUNK / LG_PA_TILE ? LG_PA_CHUNK / LG_PA_TILE : tiles;
     };
     const uint32_t most = size(some);

@@ -97,8 +97,6 @@ extern "C" int lg_hip_paged_write(const struct lg_hip_pages *p, const float *d_k
 // ---- attend -----------------------------------------------------------------------------------------------------
 // Workgroups of lg_k_page_attn at a time: lg_pa_per_simd on each of 256 compute units
 static int slots_of(int hd) { return 256 * lg_pa_per_simd(hd); }
-// Splits of all sequences together, at most.  lg_pa_split_tiles makes the full ones of a key head slots / n_head_kv or fewer for every round, the rounds one or 2 units / slots rounded
-// up, where splits of `tiles` tiles to LG_PA_CHUNK keys allow; every sequence has one that is not full besides
 // Sequences of up to so many tiles are left whole where none is longer: the cut, the partials and the launch that joins them take longer than what splits save, the more so where
 // the sequences' key heads keep the chip at work by themselves.  Whole and in splits, us: one sequence of 512 keys, heads of 64 7.1 and 8.1, 128 8.0 and 9.0, 256 12.7 and 10.3 (320
 // keys: 9.7 and 10.2), 512 24.8 and 16.1 (192: 14.0 and 15.9).  Two key heads, all sequences as long as the longest / of all lengths up to it: 64 sequences of 1024, heads of 128 13.5 and
@@ -110,6 +108,8 @@ static int alone_of(int hd, int64_t units) {
     return tiles[hd == 64 ? 0 : hd == 128 ? 1 : hd == 256 ? 2 : 3][tier];
 }
 struct AttnCut { int64_t splits, tiles; bool join; int least; };        // tiles: of all sequences, at most
+// Splits of all sequences together, at most.  lg_pa_split_tiles makes the full ones of a key head slots / n_head_kv or fewer for every round, the rounds one or 2 units / slots rounded
+// up, where splits of min_tiles tiles to LG_PA_CHUNK keys allow; every sequence has one that is not full besides
 static AttnCut cut_of(int n_seq, int n_head_kv, int hd, int max_len, int window) {
     // (a window need not start with a tile)
     const int64_t span = window > 0 && window < max_len ? (int64_t)window + LG_PA_TILE - 1 : max_len, tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
@@ -135,7 +135,7 @@ template <int HD>
 static void launch_attn(const PageAttn &a, const AttnCut &c, hipStream_t st) {
     hipLaunchKernelGGL(lg_k_page_attn<HD>, dim3((unsigned)(c.splits * a.nkv)), dim3(LG_PA_WAVES * 64), 0, st, a);
     if (!c.join) return;
-    // eight wavefronts to a head, or one where the chip has a head for each
+    // eight wavefronts to a head, or one where there are hundreds of heads (two are no faster)
     if (a.n_seq > LG_PA_LANES) hipLaunchKernelGGL((lg_k_page_merge<HD, 1>), dim3(a.H, a.n_seq), dim3(64), 0, st, a);
     else hipLaunchKernelGGL((lg_k_page_merge<HD, 8>), dim3(a.H, a.n_seq), dim3(512), 0, st, a);
 }
