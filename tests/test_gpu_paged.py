@@ -270,6 +270,15 @@ def test_attention_of_many_sequences_in_splits(lg, dev, n, H, kv, hd, window, lo
         within(attend(lg, dev, q, k, v, table, told, 16, kv, window, 1.0, longest), want, bound)
 
 
+@pytest.mark.parametrize("lens", [[0], [0, 0, 0], [1, 0, 31]])
+def test_split_attention_of_more_key_heads_than_workgroups_at_a_time(lg, dev, lens):
+    """A cut of next to nothing among 300 heads of 512, all sequences empty or nearly."""
+    rng = np.random.default_rng(len(lens))
+    q, k, v, table = case(rng, 300, 300, 512, 16, lens)
+    want, bound = attend_ref(q, k, v, table, lens, 16, k.shape[0], 300, 0, 1.0, 1000)
+    within(attend(lg, dev, q, k, v, table, lens, 16, 300, 0, 1.0, 1000), want, bound)
+
+
 @pytest.mark.parametrize("n, H, kv, hd, longest", [(3, 8, 2, 256, 3000), (64, 4, 1, 64, 2500), (70, 8, 2, 128, 2500)])
 def test_split_attention_in_two_graphs_at_once(lg, dev, n, H, kv, hd, longest):
     """Joined splits recorded into two graphs, each with working memory of its own that holds rubbish; between the replays, which overlap, the lengths change
