@@ -17,7 +17,7 @@
 //                       Rows of a small top-k come here at once: the k-th largest of the groups' largest logits is at most the k-th largest logit, so
 //                       the tokens not below it, few more than k, are the candidates.
 // What the second and third find only narrows down: the border is taken from whole-number sums, and where the candidates turn out not to hold
-// it (too many, a bin's sum estimated too far off) lg_sample_row finds it from the row alone.
+// it (too many, a bin's sum estimated too far off) lg_sample_row finds it from the row alone, as it does where f32 does not hold the logits' distances.
 //
 // A row is 4 bytes a token and is read once (a small top-k, greedy), twice (no top-k and no top-p) or three times, from the second time on mostly from caches: 64 rows of 262144
 // have 67 MB, which a bare read takes 11.8 us for.  Launches of them with rows of all kinds: 14.6 us (4.6 TB/s), 10.8, 22.3 and 19.9 us.  Few rows are bound by
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(LG_SAMPLE_MAX_WG) void lg_k_sample_max(SampleArgs a
 }
 
 // The row's largest logit and the width of its bins
-struct SampleSpan { Weigh wg; float top, scale, c; uint32_t key, least; };      // key: of the largest logit, 0x007FFFFF: none; least: ~key of the smallest; scale: bins per unit of logit; c: base-2 exponents per unit
+struct SampleSpan { Weigh wg; float top, scale, c; uint32_t key, least; bool wide; };      // key: of the largest logit, 0x007FFFFF: none; least: ~key of the smallest; scale: bins per unit of logit; c: base-2 exponents per unit
 __device__ __forceinline__ SampleSpan lg_sample_span_of(const SampleRow &p, uint32_t key, uint32_t least, const double *tab) {
     SampleSpan s;
     s.key = key; s.least = least;
@@ -333,6 +333,9 @@ __device__ __forceinline__ SampleSpan lg_sample_span_of(const SampleRow &p, uint
     s.c = -(float)(1.4426950408889634 / (double)p.temperature);
     const float reach = (float)LG_SAMPLE_REACH * p.temperature, width = fminf(s.top - lg_unkey(~least), reach);
     s.scale = width > 0 && width < INFINITY ? (float)LG_SAMPLE_BINS / width : 0;      // (0: all in the first bin)
+    // `wide`: distances from the largest logit that f32 does not hold may have weight: an infinite largest logit, or a smallest one further away than f32 holds at a
+    // temperature that reaches as far (above 1.08e37).  Bins and sums, which take distances in f32, leave such a row to lg_sample_row, which takes them in f64
+    s.wide = s.top == INFINITY || width == INFINITY;
     return s;
 }
 // From what lg_k_sample_max left: this thread's share, asked for early, and all of it
@@ -380,7 +383,7 @@ __global__ __launch_bounds__(LG_SAMPLE_WG) void lg_k_sample_bins(SampleArgs a, c
     for (int i = threadIdx.x; i < LG_SAMPLE_BINS; i += NT) { mass[i] = 0; count[i] = 0; }
     const SampleSpan s = lg_sample_span<NT>(p, ends, tab, part);                      // (its barriers are the clearing's too)
     if (slice == 0 && threadIdx.x == 0) { w.ncand[8] = s.key; w.ncand[9] = s.least; }        // for the launches behind this one
-    if (kind != LG_ROW_BORDER || s.key == 0x007FFFFFu || s.top == INFINITY) return;
+    if (kind != LG_ROW_BORDER || s.key == 0x007FFFFFu || s.wide) return;
     const bool by_count = p.top_k > 0 && p.top_k < a.n_vocab, by_mass = p.top_p < 1;
     #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -495,7 +498,7 @@ __global__ __launch_bounds__(NT) void lg_k_sample_sums(SampleArgs a, char *base)
         if (slice == 0 && threadIdx.x == 0) *(SampleRange *)(w.ncand + 4) = q;
     } else __syncthreads();
     const SampleSpan s = lg_sample_span_of(p, key, least_key, tab);
-    if (s.key == 0x007FFFFFu || s.top == INFINITY) return;
+    if (s.key == 0x007FFFFFu || s.wide) return;
     const lg_u64 least = lg_least(p);
     // What is behind top-k's bin, or below min-p where nothing else is asked, needs no weight (a little more than that gets one); a wavefront without such a
     // token goes on, one with some does all of its lanes without branches
@@ -713,7 +716,7 @@ __device__ __forceinline__ bool lg_sample_finish(const SampleArgs &a, char *base
             __syncthreads();                                 // (the sums and the table)
         }
         if (kind == LG_ROW_BORDER || kind == LG_ROW_FREE) { above = s.part3[0]; total = s.part3[1]; kept = (uint32_t)s.part3[2]; }
-        if (span.top == INFINITY && (kind == LG_ROW_BORDER || kind == LG_ROW_FREE)) return false;      // (the launches before left nothing)
+        if (span.wide && (kind == LG_ROW_BORDER || kind == LG_ROW_FREE)) return false;      // (the launches before left nothing)
         if (span.key != 0x007FFFFFu && kind == LG_ROW_FIRST) {
             #pragma unroll
             for (int i = 0; i < LG_SAMPLE_GROUPS / LG_SAMPLE_WG; ++i) if (gk[i] == span.key) atomicMin(&s.at, t + i * LG_SAMPLE_WG);
