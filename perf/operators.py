@@ -219,7 +219,7 @@ def prepare(case, seed):
         _prepare_attend(s, case, rng, gen)
     else:
         _prepare_sample(s, case, rng, gen)
-    s.call = None
+    s.device, s.calls = torch.cuda.current_device(), {}
     return s
 
 
@@ -242,39 +242,39 @@ def _pool(s):
     return _own().Pages(s.kpool.data_ptr(), s.vpool.data_ptr(), s.n_pages, c["page"], c["kv"], c["hd"], width, width * c["page"])
 
 
-def _bound(s):
-    """The call of a state with its arguments in place, as a serving loop keeps it: pointers, handles, working memory."""
-    L, c = _own(), s.case
-    H, p = L.load_hip(), (lambda t: C.c_void_p(t.data_ptr()))
-    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+def _bound(s, stream):
+    """The call of a state on a stream with its arguments in place, as a serving loop keeps it: pointers, handles, working memory of the stream's own.
+    (call, what it keeps alive, arguments of each call in turn)"""
+    L, c, work = _own(), s.case, []
+    H, p, stream = L.load_hip(), (lambda t: C.c_void_p(t.data_ptr())), C.c_void_p(stream)
 
     def memory(n):
-        s.work = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
-        return p(s.work), C.c_size_t(n)
+        work.append(torch.empty(max(n, 16), dtype=torch.uint8, device="cuda"))
+        return p(work[0]), C.c_size_t(n)
 
     if c["kind"] == "plan":
         w = memory(H.lg_hip_paged_plan_workspace(c["n_seq"]))
         head = (c["n_seq"], c["page"], s.n_pages, s.blocks)
         a = (*head, p(s.len_old), p(s.len_new), p(s.table), p(s.stack), p(s.n_free), p(s.start), p(s.slots), s.n_slots, p(s.status), *w, stream)
         b = (*head, p(s.len_new), p(s.len_old), p(s.table), p(s.stack), p(s.n_free), p(s.start2), p(s.slots2), s.n_slots, p(s.status2), *w, stream)
-        return H.lg_hip_paged_plan, a, b
+        return H.lg_hip_paged_plan, work, a, b
     if c["kind"] == "write":
-        s.pool = _pool(s)
-        return H.lg_hip_paged_write, (C.byref(s.pool), p(s.k), p(s.v), s.x.shape[1], p(s.slots), c["n_tok"], stream)
+        return H.lg_hip_paged_write, work, (C.byref(_pool(s)), p(s.k), p(s.v), s.x.shape[1], p(s.slots), c["n_tok"], stream)
     if c["kind"] == "attend":
-        s.pool = _pool(s)
         w = memory(H.lg_hip_paged_attention_workspace(c["n_seq"], c["heads"], c["kv"], c["hd"], s.max_len, c["window"]))
-        return H.lg_hip_paged_attention, (C.byref(s.pool), p(s.q), s.x.shape[1], c["n_seq"], c["heads"], p(s.table), s.blocks, p(s.lens), s.max_len,
-                                          c["window"], s.scale, p(s.out), s.out.shape[1], *w, stream)
+        return H.lg_hip_paged_attention, work, (C.byref(_pool(s)), p(s.q), s.x.shape[1], c["n_seq"], c["heads"], p(s.table), s.blocks, p(s.lens), s.max_len,
+                                                c["window"], s.scale, p(s.out), s.out.shape[1], *w, stream)
     w = memory(H.lg_hip_sample_workspace(c["rows"], c["vocab"]))
-    return H.lg_hip_sample, (p(s.logits), c["vocab"], c["rows"], c["vocab"], p(s.params), p(s.u), p(s.tok), p(s.prob), p(s.kept), *w, stream)
+    return H.lg_hip_sample, work, (p(s.logits), c["vocab"], c["rows"], c["vocab"], p(s.params), p(s.u), p(s.tok), p(s.prob), p(s.kept), *w, stream)
 
 
 def _run_own(s):
-    if s.call is None:
-        s.call = _bound(s)
-    f = s.call[0]
-    for args in s.call[1:]:
+    # the stream that is current now (its handle alone: 0.1 us, a Stream object 2.8)
+    stream = torch._C._cuda_getCurrentRawStream(s.device)
+    if stream not in s.calls:
+        s.calls[stream] = _bound(s, stream)
+    f, _, *passes = s.calls[stream]
+    for args in passes:
         rc = f(*args)
         if rc:
             _own().hip_check(rc, s.case["kind"])
