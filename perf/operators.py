@@ -244,7 +244,7 @@ def _pool(s):
 
 def _bound(s, stream):
     """The call of a state on a stream with its arguments in place, as a serving loop keeps it: pointers, handles, working memory of the stream's own.
-    (call, what it keeps alive, arguments of each call in turn)"""
+    (call, arguments of each call in turn, the memory)"""
     L, c, work = _own(), s.case, []
     H, p, stream = L.load_hip(), (lambda t: C.c_void_p(t.data_ptr())), C.c_void_p(stream)
 
@@ -257,15 +257,15 @@ def _bound(s, stream):
         head = (c["n_seq"], c["page"], s.n_pages, s.blocks)
         a = (*head, p(s.len_old), p(s.len_new), p(s.table), p(s.stack), p(s.n_free), p(s.start), p(s.slots), s.n_slots, p(s.status), *w, stream)
         b = (*head, p(s.len_new), p(s.len_old), p(s.table), p(s.stack), p(s.n_free), p(s.start2), p(s.slots2), s.n_slots, p(s.status2), *w, stream)
-        return H.lg_hip_paged_plan, work, a, b
+        return H.lg_hip_paged_plan, (a, b), work
     if c["kind"] == "write":
-        return H.lg_hip_paged_write, work, (C.byref(_pool(s)), p(s.k), p(s.v), s.x.shape[1], p(s.slots), c["n_tok"], stream)
+        return H.lg_hip_paged_write, ((C.byref(_pool(s)), p(s.k), p(s.v), s.x.shape[1], p(s.slots), c["n_tok"], stream),), work
     if c["kind"] == "attend":
         w = memory(H.lg_hip_paged_attention_workspace(c["n_seq"], c["heads"], c["kv"], c["hd"], s.max_len, c["window"]))
-        return H.lg_hip_paged_attention, work, (C.byref(_pool(s)), p(s.q), s.x.shape[1], c["n_seq"], c["heads"], p(s.table), s.blocks, p(s.lens), s.max_len,
-                                                c["window"], s.scale, p(s.out), s.out.shape[1], *w, stream)
+        return H.lg_hip_paged_attention, ((C.byref(_pool(s)), p(s.q), s.x.shape[1], c["n_seq"], c["heads"], p(s.table), s.blocks, p(s.lens), s.max_len,
+                                           c["window"], s.scale, p(s.out), s.out.shape[1], *w, stream),), work
     w = memory(H.lg_hip_sample_workspace(c["rows"], c["vocab"]))
-    return H.lg_hip_sample, work, (p(s.logits), c["vocab"], c["rows"], c["vocab"], p(s.params), p(s.u), p(s.tok), p(s.prob), p(s.kept), *w, stream)
+    return H.lg_hip_sample, ((p(s.logits), c["vocab"], c["rows"], c["vocab"], p(s.params), p(s.u), p(s.tok), p(s.prob), p(s.kept), *w, stream),), work
 
 
 def _run_own(s):
@@ -273,7 +273,7 @@ def _run_own(s):
     stream = torch._C._cuda_getCurrentRawStream(s.device)
     if stream not in s.calls:
         s.calls[stream] = _bound(s, stream)
-    f, _, *passes = s.calls[stream]
+    f, passes, _ = s.calls[stream]
     for args in passes:
         rc = f(*args)
         if rc:
