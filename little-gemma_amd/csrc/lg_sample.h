@@ -17,7 +17,7 @@
 //                       Rows of a small top-k come here at once: the k-th largest of the groups' largest logits is at most the k-th largest logit, so
 //                       the tokens not below it, few more than k, are the candidates.
 // What the second and third find only narrows down: the border is taken from whole-number sums, and where the candidates turn out not to hold
-// it (too many, a bin's sum estimated too far off) lg_sample_row finds it from the row alone, as it does where f32 does not hold the logits' distances.
+// it (too many, as with a top-p near 1; a bin's sum estimated too far off) lg_sample_row finds it from the row alone, as it does where f32 does not hold the logits' distances.
 //
 // A row is 4 bytes a token and is read once (a small top-k, greedy), twice (no top-k and no top-p) or three times, from the second time on mostly from caches: 64 rows of 262144
 // have 67 MB, which a bare read takes 11.8 us for.  Launches of them with rows of all kinds: 14.6 us (4.6 TB/s), 10.8, 22.3 and 19.9 us.  Few rows are bound by
@@ -218,7 +218,10 @@ __device__ __forceinline__ void lg_sample_row(const SampleArgs &a, int r, const 
                                                  // 1024 groups the tokens not below the k-th largest maximum are 1.15 k at k = 256 and 1.27 k at 400 where large
                                                  // logits lie anywhere in the row.  One row of 262144 by maxima and by bins: top-k 200 22 and 32 us, 400 29 and 33,
                                                  // 512 (more than LG_SAMPLE_LIST candidates) 37 and 32
-#define LG_SAMPLE_SLACK   2048                   // the estimated sum of a row's bins is trusted to 1 / 2048: four times what the comment at lg_k_sample_bins allows
+#define LG_SAMPLE_SLACK   2048                   // the estimated sum of a row's bins is trusted to 1 / 2048: four times what the comment at lg_k_sample_bins allows, a bound for
+                                                 // half a unit of each of 2^19 tokens.  Of a bell's tail that share is thousands of tokens: near a top-p of 1 there are more
+                                                 // than LG_SAMPLE_CAND of them, and the row is taken alone.  One row of 262144, normal logits of a spread of 3 with some
+                                                 // higher ones, T 1: top-p 0.99 32 us, from 0.995 on 780; of 128000 0.995 33, 0.999 404; of 60000 0.995 31, 0.999 222
 
 // Tokens whose largest logit lg_k_sample_max keeps: a group's, a quarter's where these are no more than LG_SAMPLE_GROUPS (a small top-k is to be half of their number
 // at most, and its candidates lie in fewer tokens: a row of 32000, top-k 64, 31.1 -> 17.4 us; of 128000, top-k 200, 22.5 -> 18.2)

@@ -100,8 +100,11 @@ static int slots_of(int hd) { return 256 * lg_pa_per_simd(hd); }
 // Sequences of up to so many tiles are left whole where none is longer: the cut, the partials and the launch that joins them take longer than what splits save, the more so where
 // the sequences' key heads keep the chip at work by themselves.  Whole and in splits, us: one sequence of 512 keys, heads of 64 7.1 and 8.1, 128 8.0 and 9.0, 256 12.7 and 10.3 (320
 // keys: 9.7 and 10.2), 512 24.8 and 16.1 (192: 14.0 and 15.9).  Two key heads, all sequences as long as the longest / of all lengths up to it: 64 sequences of 1024, heads of 128 13.5 and
-// 19.3 / 13.1 and 13.6; of 768, heads of 256 19.9 and 26.0 / 18.9 and 18.1; 128 of 2047, heads of 128 39.6 and 48.9 / 26.7 and 32.5, heads of 256 93.6 and 114 / 55.3 and 57.7;
-// 200 of 2047, heads of 256 152 and 174 / 104 and 91.  One key head of 512: 128 of 512 28.1 and 36.6 / 26.3 and 25.4, 200 of 1024 75.7 and 94.3 / 48.8 and 51.9
+// 19.3 / 13.1 and 13.6; of 768, heads of 256 19.9 and 26.0 / 18.9 and 18.1; 128 of 2047, heads of 128 39.6 and 48.9 / 26.7 and 32.5, heads of 256 91.1 and 113 / 52.7 and 53.1;
+// 200 of 2047, heads of 256 151 and 169 / 108 and 95.  One key head of 512: 128 of 512 28.1 and 36.4 / 26.7 and 26.1.
+// A limit holds for all numbers of units in its tier and lies where splits begin to gain for some of them; for others, lengths above it take the slower side.  One key head of 512, 1024
+// keys (limit 512): 128 sequences 49.8 and 57.7 / 44.5 and 35.0, but 200 75.7 and 94.1 / 47.1 and 51.7.  Two heads of 256, 2047 keys (limit 1536): 150 sequences 138 and 126 / 94.4 and
+// 67.6, but the 128 above
 static int alone_of(int hd, int64_t units) {
     const int tier = units < 128 ? 0 : units < 256 ? 1 : 2;
     static const int tiles[4][3] = { { 20, 32, 64 }, { 18, 32, 64 }, { 11, 24, 48 }, { 7, 16, 32 } };          // heads of 64, 128, 256, 512
