@@ -332,6 +332,85 @@ size_t lg_hip_sample_workspace(int rows, int n_vocab);
 int    lg_hip_sample(const float *d_logits, int64_t stride, int rows, int n_vocab, const struct lg_hip_sampling *d_params, const float *d_u,
                      int32_t *d_tok, float *d_prob, int32_t *d_kept, void *d_work, size_t work_bytes, void *stream);
 
+/* ---- the same step with trees of drafted tokens -----
+ * Every sequence may bring a tree of up to 64 rows into a step: row 0 the token chosen last, every other row a drafted token that hangs on an earlier row,
+ * its parent.  A step grows each sequence by its tree (lg_hip_paged_plan, whose d_start says where a tree's rows are among the step's: row j of sequence i is row
+ * d_start[i] + j, its K and V at position len - n + j, where len counts the tree's n rows), computes all rows, accepts a path, moves its rows
+ * down, and takes the rest back (lg_hip_paged_plan again, from len to d_len_out).  A chain of drafts is a tree whose parents are 0, 1, 2, ...
+ * n_seq 0..4096, max_tree (1..64) bounds the rows of a tree, n_rows those of the step. */
+
+/* Before the step, from d_parent [n_rows] (a tree's rows count from 0; row 0's parent is not read): d_mask (aligned to 8 bytes), the row and the rows above it up to row 0 as a set of 64 bits; d_pos,
+ * the position that the row stands for, committed positions + rows above it (rotations and windows go by it); d_seq, its sequence.  *d_status [n_seq]: 0, or the
+ * LG_HIP_TREE_ bits of what is wrong with a tree: its rows then get an empty set and position -1 (nothing is written for LG_HIP_TREE_BAD_ROWS). */
+enum { LG_HIP_TREE_BAD_ROWS = 1,       /* d_start falls, a tree has more than max_tree rows, or a row is outside 0..n_rows-1 */
+       LG_HIP_TREE_BAD_PARENT = 2,     /* a parent that is not an earlier row */
+       LG_HIP_TREE_BAD_LENGTH = 4 };   /* a length below the tree's rows */
+int    lg_hip_tree_plan(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_len, uint64_t *d_mask, int32_t *d_pos,
+                        int32_t *d_seq, int32_t *d_status, void *stream);
+/* After it, from d_token [n_rows], the rows' tokens, and d_next [n_rows], the token picked behind each row (lg_hip_sample, or the likeliest): from row 0 on to the first row that hangs on
+ * the current one and holds the token picked behind it, as long as there is one.  d_path [n_seq][max_tree]: the rows passed, the rest -1; d_count: how many (0 for a tree without rows,
+ * or with LG_HIP_TREE_BAD_ROWS); d_len_out: the sequence's length with them alone; d_last: the token picked behind the last one (-1 where there is no row). A picked token below 0 fits no row.  */
+int    lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_token, const int32_t *d_next,
+                          const int32_t *d_len, int32_t *d_path, int32_t *d_count, int32_t *d_len_out, int32_t *d_last, void *stream);
+/* Attention of every row of the trees, as lg_hip_paged_attention: out = softmax(scale * q.k) v over the committed positions t of the row's sequence and the tree's positions committed + k for the rows k
+ * that its set d_mask names, of which only those with t > d_pos[row] - window and d_pos[row k] > d_pos[row] - window where window is not 0.  d_len [n_seq] counts the trees' rows.  Sets need not come from lg_hip_tree_plan: any rows of the
+ * same tree may be named, later ones too; positions are at least the committed length, a row with another one sees nothing.  A row that sees nothing gets
+ * zeros, so do the rows of a sequence whose length is below its rows or above max_len or max_blocks * page_size; rows of a tree with LG_HIP_TREE_BAD_ROWS and rows of no tree are left as they are.
+ * Positions whose page is outside 0..n_pages-1 are left out.  What is not seen by a row does not reach it, whatever it holds, also where other rows of the tree see it; infinities and NaN that are seen
+ * spoil the heads that read them (NaN as a rule) and no others. */
+size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree, int n_head, int n_head_kv, int head_dim, int max_len, int window);
+int    lg_hip_paged_tree_attention(const struct lg_hip_pages *pages, const float *d_q, int64_t q_stride, int n_rows, int n_seq, int max_tree, int n_head,
+                                   const int32_t *d_table, int max_blocks, const int32_t *d_len, const int32_t *d_start, const uint64_t *d_mask, const int32_t *d_pos,
+                                   int max_len, int window, float scale, float *d_out, int64_t out_stride, void *d_work, size_t work_bytes, void *stream);
+/* The rows of accepted paths to where they are accepted, in all layers of a cache at once: the K and V row at position committed + path[k] goes to committed + k, k < d_count.  d_len and d_start are those
+ * of the step; layers [n_layers] (host memory) share one table, so they have the same n_pages and page_size.  Paths rise (those of lg_hip_tree_accept do): from the first row that does not, or is no row of the tree, a path is left alone.
+ * So are rows whose page is outside 0..n_pages-1, and sequences whose length does not fit. */
+int    lg_hip_paged_compact(const struct lg_hip_pages *layers, int n_layers, int n_seq, int max_tree, const int32_t *d_table, int max_blocks, const int32_t *d_len,
+                            const int32_t *d_start, const int32_t *d_path, const int32_t *d_count, void *stream);
+
+/* ---- sequences that share pages -----
+ * Row i of the table holds afterwards the first d_len_new[i] positions of what row d_src[i] held before (i itself: the sequence stays, or is cut; -1 with a new length of 0: it ends; several rows may
+ * name one source, rows may change places).  Whole pages are shared: d_shares [n_pages] counts for each page the rows that hold it beyond the first, 0 at the start and for free pages.  A last page that is not
+ * full belongs to its row alone, so that the row may grow into it: where others hold it too, the row gets a page off the stack, and d_from, d_to, d_rows [n_seq] say what lg_hip_paged_copy has to copy (-1, -1, 0 for the other rows).
+ * Pages that no row holds any longer go on the stack first, row by row, the first one topmost.  *d_status: 0, or the LG_HIP_FORK_ bits of what was wrong; then nothing but d_from, d_to and d_rows (nothing to copy) is written.
+ * lg_hip_paged_plan goes on working on such a table for growth, and for taking back pages that were grown since; pages with shares are given back here. A row holds a page once; that is not looked for. */
+enum { LG_HIP_FORK_BAD_LENGTH = 1,     /* a length below 0 or above max_blocks * page_size, or a new one above the source's old one */
+       LG_HIP_FORK_NO_PAGES = 2,       /* not enough free pages for the copies */
+       LG_HIP_FORK_BAD_SOURCE = 4,     /* a source outside -1..n_seq-1 */
+       LG_HIP_FORK_BAD_STACK = 8,      /* a height outside 0..n_pages, also with the pages that come back */
+       LG_HIP_FORK_BAD_PAGE = 16,      /* a page that moves is outside 0..n_pages-1 */
+       LG_HIP_FORK_BAD_SHARES = 32 };  /* shares of a page that moves are below 0, above 4095 or fewer than its rows */
+size_t lg_hip_paged_fork_workspace(int n_seq, int n_pages, int max_blocks);
+int    lg_hip_paged_fork(int n_seq, int page_size, int n_pages, int max_blocks, const int32_t *d_src, const int32_t *d_len_old, const int32_t *d_len_new, int32_t *d_table,
+                         int32_t *d_shares, int32_t *d_free, int32_t *d_n_free, int32_t *d_from, int32_t *d_to, int32_t *d_rows, int32_t *d_status, void *d_work,
+                         size_t work_bytes, void *stream);
+/* The first d_rows[i] rows (at most page_size) of page d_from[i] to page d_to[i], i < n (0..65535), K and V of all layers (as lg_hip_paged_compact).  Pairs with a page outside 0..n_pages-1 are left out.  A page that is written may
+ * not be read or written by another pair of the call. */
+int    lg_hip_paged_copy(const struct lg_hip_pages *layers, int n_layers, int n, const int32_t *d_from, const int32_t *d_to, const int32_t *d_rows, void *stream);
+
+/* ---- rules for logits, ahead of lg_hip_sample -----
+ * Penalties of a sequence: logits of the tokens of its text are divided by `repetition` where they are above 0 and multiplied by it elsewhere (1, not above 0 or NaN: off); of those that were generated, which
+ * are all but the first `prompt` tokens of the text, `presence` and `frequency` times the token's count are taken off (NaN: off). */
+struct lg_hip_penalty { float repetition, presence, frequency; int32_t prompt; };
+/* Device memory, all of it optional (NULL or a count of 0). */
+struct lg_hip_logit_rules {
+    int32_t n_seq, n_bias, n_allow;
+    const int32_t *seq;                  /* [rows] the sequence of each row (NULL: row i is sequence i); rows of no sequence 0..n_seq-1 have no penalties and biases */
+    const struct lg_hip_penalty *penalty;/* [n_seq] */
+    const int32_t *hist, *hist_len;      /* [n_seq][hist_stride] the texts, [n_seq] how much of them counts (at most hist_stride, at most 2^30); needs penalty */
+    int64_t hist_stride;
+    const uint64_t *tree_mask;           /* [rows] sets of rows of a tree, as lg_hip_tree_plan's: their tokens count as generated too; needs penalty, tree_start, tree_tok */
+    const int32_t *tree_start, *tree_tok;/* [n_seq + 1] the first row of each sequence's tree, [rows] tokens */
+    const int32_t *bias_start, *bias_tok;/* [n_seq + 1], [n_bias]: sequence i adds bias[j] to the logit of bias_tok[j], bias_start[i] <= j < bias_start[i + 1]; of a token named more than once the last counts */
+    const float *bias;                   /* [n_bias] */
+    const uint32_t *allow;               /* [n_allow][allow_stride] sets of tokens, token t bit t % 32 of word t / 32: logits of the others become -inf */
+    const int32_t *allow_row;            /* [rows] the set of each row, outside 0..n_allow-1: none (NULL: row i has set i) */
+    int64_t allow_stride;                /* words */
+};
+/* Penalties, then biases, then sets, on rows of n_vocab (1..524288) logits, stride and out_stride floats apart; d_out may be d_logits (with the same stride), or not overlap it.  Logits that a penalty or
+ * bias changes are computed in 64 bits and rounded once.  Tokens outside the vocabulary count for nothing. */
+int    lg_hip_adjust_logits(const struct lg_hip_logit_rules *rules, const float *d_logits, int64_t stride, int rows, int n_vocab, float *d_out, int64_t out_stride, void *stream);
+
 /* lg_hip_forward_spec with drawn tokens in place of greedy ones: out[j] = the token that lg_hip_sample draws from row j's logits by u[j], all
  * rows with the parameters *how (host memory, like u), *adv = 1 + number of leading drafts that equal the token drawn before them, the hidden state
  * that of row *adv - 1.  Numbers that belong to positions (u[j] that of position pos + j, whatever the block) make a generation the same with and

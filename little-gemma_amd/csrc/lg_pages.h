@@ -247,7 +247,9 @@ __device__ __forceinline__ void lg_pa_range(const PageAttn &a, int seq, int &lo,
     if (len < 0) len = 0;
     lo = a.window > 0 && len > a.window ? len - a.window : 0;
 }
-__device__ __forceinline__ int lg_pa_tiles(const PageAttn &a, int seq) {
+// What follows serves calls of one row a sequence (PageAttn) and of trees (TreeAttn, lg_tree.h): their lg_pa_range and lg_merge_row differ
+template <class A>
+__device__ __forceinline__ int lg_pa_tiles(const A &a, int seq) {
     int lo, len;
     lg_pa_range(a, seq, lo, len);
     return (len + LG_PA_TILE - 1) / LG_PA_TILE - lo / LG_PA_TILE;
@@ -260,8 +262,8 @@ struct PageCut { int tiles; int seq, index, first, n; };       // tiles of a spl
 // `total` tiles of `some` sequences that have any: the smallest of a few sizes whose splits are at most a whole number of rounds of a.slots workgroups, as few as leave half of
 // them to splits that are full.  Were every sequence's last split a full one, `some` more than total / size would be needed; ragged ones need half as many, and the size
 // for that is tried first (61 sequences of 4..8192 keys, heads of 256: 74.3 -> 72.1 us).  count(t): the splits of size t
-template <typename Count>
-__device__ __forceinline__ uint32_t lg_pa_split_tiles(const PageAttn &a, uint32_t total, uint32_t some, Count count) {
+template <class A, typename Count>
+__device__ __forceinline__ uint32_t lg_pa_split_tiles(const A &a, uint32_t total, uint32_t some, Count count) {
     const uint32_t units = some * a.nkv, half = (uint32_t)a.slots / 2, rounds = units > half ? (units + half - 1) / half : 1, room = rounds * a.slots / a.nkv;
     auto size = [&](uint32_t spare) {
         const uint32_t full = room > spare ? room - spare : 1, tiles = (total + full - 1) / full;
@@ -278,7 +280,8 @@ __device__ __forceinline__ uint32_t lg_pa_split_tiles(const PageAttn &a, uint32_
     return most;
 }
 __device__ __forceinline__ uint32_t lg_pa_splits(uint32_t of, uint32_t tiles) { const uint32_t x = (of + tiles - 1) / tiles; return x ? x : 1u; }
-__device__ __forceinline__ PageCut lg_pa_cut(const PageAttn &a, int at) {
+template <class A>
+__device__ __forceinline__ PageCut lg_pa_cut(const A &a, int at) {
     if (!a.pm) return { a.least, at, 0, at, 1 };
     if (a.n_seq > LG_PA_LANES) {
         const int seq = a.cut[2 + a.n_seq + at];
@@ -299,7 +302,8 @@ __device__ __forceinline__ PageCut lg_pa_cut(const PageAttn &a, int at) {
 // The cut of more sequences than a wavefront has lanes, worked out once: in every workgroup it takes several barriers and passes over the
 // lengths.  400 sequences of all lengths up to 1024, heads of 128: 66.8 -> 48.0 us, with the joining launch's workgroups of one wavefront
 #define LG_PC_WG    1024
-__global__ __launch_bounds__(LG_PC_WG) void lg_k_page_cut(PageAttn a) {
+template <class A>
+__global__ __launch_bounds__(LG_PC_WG) void lg_k_page_cut(A a) {
     __shared__ uint32_t part[LG_PC_WG / 64];
     __shared__ int32_t before[LG_PA_SEQS + 1];
     constexpr int PER = LG_PA_SEQS / LG_PC_WG;
@@ -611,17 +615,23 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_pa_per_simd(HD)) void lg_k_pag
 
 // The splits of a sequence, joined: a workgroup per (sequence, head).  A split's factor is computed once, by one thread; then the wavefronts take splits in
 // turn, a lane HD / 64 dimensions, and their sums are added in order.  A chain of maxima, factors and sums: 5 us for 8 or 16 heads of 256, 65 splits of one sequence or 317 of 61; 8 to 9 where one sequence has 250 to 510 of them.
-template <int HD, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void lg_k_page_merge(PageAttn a) {
+struct MergeRow { int seq; long long row, step, off, out; };        // a head's partials of split k: number k * step + off; its output's first value
+__device__ __forceinline__ MergeRow lg_merge_row(const PageAttn &a) {
+    const int head = blockIdx.x, seq = blockIdx.y;
+    return { seq, seq, a.H, head, head };
+}
+template <int HD, int WAVES, class A>
+__global__ __launch_bounds__(WAVES * 64) void lg_k_page_merge(A a) {
     constexpr int NT = WAVES * 64, D = HD / 64;
     __shared__ float s_f[NT], s_w[WAVES], s_o[WAVES][HD];
-    const int head = blockIdx.x, seq = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int from = a.cut[seq], n = a.cut[seq + 1] - from;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const MergeRow w = lg_merge_row(a);
+    const int from = a.cut[w.seq], n = w.row < 0 ? 0 : a.cut[w.seq + 1] - from;
     if (n < 2) return;                                       // (its one split has written the output)
     // what the first NT splits need is asked for at once: a wavefront's first eight sums with the maxima
     typedef float vec __attribute__((ext_vector_type(D)));
     constexpr int FIRST = HD == 512 ? 4 : 8;
-    auto place = [&](int k) { return (long long)(from + k) * a.H + head; };
+    auto place = [&](int k) { return (from + k) * w.step + w.off; };
     auto sums = [&](int k) { return *(const vec *)(a.pacc + place(k) * HD + lane * D); };
     vec ahead[FIRST];
     const float m0 = t < n ? a.pm[place(t)] : -INFINITY, l0 = t < n ? a.pl[place(t)] : 0.0f;
@@ -665,6 +675,6 @@ __global__ __launch_bounds__(WAVES * 64) void lg_k_page_merge(PageAttn a) {
         float x = 0;
         #pragma unroll
         for (int v = 0; v < WAVES; ++v) x += s_o[v][d];
-        a.out[seq * a.out_stride + (long long)head * HD + d] = L == 0.0f ? 0.0f : x / L;
+        a.out[w.row * a.out_stride + w.out * HD + d] = L == 0.0f ? 0.0f : x / L;
     }
 }

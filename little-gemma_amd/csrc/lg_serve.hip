@@ -10,10 +10,17 @@
 #include "lg_host.h"
 #include "lg_pages.h"
 #include "lg_sample.h"
+#include "lg_tree.h"
+#include "lg_share.h"
+#include "lg_rules.h"
 
 static_assert(LG_PLAN_BAD_LEN == LG_HIP_PLAN_BAD_LENGTH && LG_PLAN_NO_PAGES == LG_HIP_PLAN_NO_PAGES && LG_PLAN_NO_SLOTS == LG_HIP_PLAN_NO_SLOTS &&
               LG_PLAN_BAD_STACK == LG_HIP_PLAN_BAD_STACK && LG_PLAN_BAD_PAGE == LG_HIP_PLAN_BAD_PAGE, "status bits of a plan");
 static_assert(sizeof(SampleRow) == sizeof(struct lg_hip_sampling), "parameters of a row");
+static_assert(LG_TREE_BAD_ROWS == LG_HIP_TREE_BAD_ROWS && LG_TREE_BAD_PARENT == LG_HIP_TREE_BAD_PARENT && LG_TREE_BAD_LEN == LG_HIP_TREE_BAD_LENGTH, "status bits of a tree");
+static_assert(LG_FORK_BAD_LEN == LG_HIP_FORK_BAD_LENGTH && LG_FORK_NO_PAGES == LG_HIP_FORK_NO_PAGES && LG_FORK_BAD_SOURCE == LG_HIP_FORK_BAD_SOURCE &&
+              LG_FORK_BAD_STACK == LG_HIP_FORK_BAD_STACK && LG_FORK_BAD_PAGE == LG_HIP_FORK_BAD_PAGE && LG_FORK_BAD_SHARES == LG_HIP_FORK_BAD_SHARES, "status bits of a fork");
+static_assert(sizeof(RulesPenalty) == sizeof(struct lg_hip_penalty), "penalties of a sequence");
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static int shift_of(int page_size) {                 // page_size = 1 << shift; -1: not served
@@ -139,8 +146,8 @@ static void launch_attn(const PageAttn &a, const AttnCut &c, hipStream_t st) {
     hipLaunchKernelGGL(lg_k_page_attn<HD>, dim3((unsigned)(c.splits * a.nkv)), dim3(LG_PA_WAVES * 64), 0, st, a);
     if (!c.join) return;
     // eight wavefronts to a head, or one where there are hundreds of heads (two are no faster)
-    if (a.n_seq > LG_PA_LANES) hipLaunchKernelGGL((lg_k_page_merge<HD, 1>), dim3(a.H, a.n_seq), dim3(64), 0, st, a);
-    else hipLaunchKernelGGL((lg_k_page_merge<HD, 8>), dim3(a.H, a.n_seq), dim3(512), 0, st, a);
+    if (a.n_seq > LG_PA_LANES) hipLaunchKernelGGL((lg_k_page_merge<HD, 1, PageAttn>), dim3(a.H, a.n_seq), dim3(64), 0, st, a);
+    else hipLaunchKernelGGL((lg_k_page_merge<HD, 8, PageAttn>), dim3(a.H, a.n_seq), dim3(512), 0, st, a);
 }
 
 extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float *d_q, int64_t q_stride, int n_seq, int n_head, const int32_t *d_table,
@@ -171,7 +178,7 @@ extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float 
     const PageAttn a{ g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, (float *)w, need ? (float *)(w + part) : nullptr,
                       need ? (float *)(w + 2 * part) : nullptr, scale, need ? (int32_t *)d_work : nullptr, n_head, p->n_head_kv, n_seq, max_blocks, max_len, window, slots_of(hd), c.least };
     hipStream_t st = (hipStream_t)stream;
-    if (c.join && n_seq > LG_PA_LANES) hipLaunchKernelGGL(lg_k_page_cut, dim3(1), dim3(LG_PC_WG), 0, st, a);
+    if (c.join && n_seq > LG_PA_LANES) hipLaunchKernelGGL(lg_k_page_cut<PageAttn>, dim3(1), dim3(LG_PC_WG), 0, st, a);
     switch (hd) {
         case 64:  launch_attn<64>(a, c, st); break;
         case 128: launch_attn<128>(a, c, st); break;
@@ -224,6 +231,230 @@ extern "C" int lg_hip_sample(const float *d_logits, int64_t stride, int rows, in
     // loads of 16 bytes where every row is aligned to that (top-p of 33 rows of 262144: 66.4 us, of rows that are not 75.2)
     if (aligned16(d_logits) && stride % 4 == 0) launch_sample<true>(a, rows, need ? (char *)d_work : nullptr, (hipStream_t)stream);
     else launch_sample<false>(a, rows, need ? (char *)d_work : nullptr, (hipStream_t)stream);
+    LG_TRY(hipGetLastError());
+    return 0;
+}
+
+// ---- trees ------------------------------------------------------------------------------------------------------
+static int check_trees(const char *who, int n_seq, int max_tree, int n_rows) {
+    if (n_seq < 0 || n_seq > LG_PA_SEQS) return lg_fail(-2, "%s: %d sequences (0..%d)", who, n_seq, LG_PA_SEQS);
+    if (max_tree < 1 || max_tree > LG_TREE_ROWS) return lg_fail(-2, "%s: trees of up to %d rows (1..%d)", who, max_tree, LG_TREE_ROWS);
+    if (n_rows < 0) return lg_fail(-2, "%s: %d rows", who, n_rows);
+    return 0;
+}
+static dim3 waves_for(int n_seq) { return dim3((unsigned)((n_seq + LG_TREE_WG / 64 - 1) / (LG_TREE_WG / 64))); }
+
+extern "C" int lg_hip_tree_plan(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_len, uint64_t *d_mask, int32_t *d_pos,
+                                int32_t *d_seq, int32_t *d_status, void *stream) {
+    const int rc = check_trees("tree_plan", n_seq, max_tree, n_rows);
+    if (rc) return rc;
+    if (n_seq == 0) return 0;
+    if (!d_start || !d_len || !d_status || (n_rows && (!d_parent || !d_mask || !d_pos || !d_seq))) return lg_fail(-1, "tree_plan: null argument");
+    if ((uintptr_t)d_mask & 7) return lg_fail(-2, "tree_plan: sets that are not aligned to 8 bytes");
+    hipLaunchKernelGGL(lg_k_tree_plan, waves_for(n_seq), dim3(LG_TREE_WG), 0, (hipStream_t)stream, d_start, d_parent, d_len, (lg_u64 *)d_mask, d_pos, d_seq, d_status, n_seq, n_rows, max_tree);
+    LG_TRY(hipGetLastError());
+    return 0;
+}
+
+extern "C" int lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_token, const int32_t *d_next, const int32_t *d_len,
+                                  int32_t *d_path, int32_t *d_count, int32_t *d_len_out, int32_t *d_last, void *stream) {
+    const int rc = check_trees("tree_accept", n_seq, max_tree, n_rows);
+    if (rc) return rc;
+    if (n_seq == 0) return 0;
+    if (!d_start || !d_len || !d_path || !d_count || !d_len_out || !d_last || (n_rows && (!d_parent || !d_token || !d_next))) return lg_fail(-1, "tree_accept: null argument");
+    hipLaunchKernelGGL(lg_k_tree_accept, waves_for(n_seq), dim3(LG_TREE_WG), 0, (hipStream_t)stream, d_start, d_parent, d_token, d_next, d_len, d_path, d_count, d_len_out, d_last, n_seq, n_rows,
+                       max_tree);
+    LG_TRY(hipGetLastError());
+    return 0;
+}
+
+// 16-pair tiles of a workgroup: as many as a tree has, up to what registers hold of outputs
+static int tree_tiles(int pairs, int hd) { return pairs <= 16 ? 1 : pairs <= 32 || hd == 512 ? 2 : 4; }
+struct TreeCut { AttnCut c; int tiles, groups, slots; };
+// As cut_of, for workgroups of several pairs: those of one stretch of keys share the chip's room
+static TreeCut tree_cut_of(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
+    const int pairs = max_tree * (n_head / n_head_kv), rt = tree_tiles(pairs, hd), groups = (pairs + 16 * rt - 1) / (16 * rt);
+    const int slots = std::max(2, 256 * lg_tree_per_simd(hd, rt) / groups);
+    // (a tree's rows see a window from the first committed position that its row 0 sees to its last row)
+    const int64_t reach = window > 0 ? (int64_t)window + max_tree + LG_PA_TILE : max_len, span = std::min<int64_t>(reach, max_len), tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
+    const int64_t units = (int64_t)n_seq * n_head_kv;
+    const int alone = alone_of(hd, units * groups), min_tiles = tiles <= alone ? alone : 4;
+    const int64_t least = (tiles + min_tiles - 1) / min_tiles, rounds = std::max<int64_t>(1, (units + slots / 2 - 1) / (slots / 2));
+    const int64_t full = std::max<int64_t>(rounds * slots / n_head_kv, n_seq * tiles / (LG_PA_CHUNK / LG_PA_TILE));
+    return { { std::min<int64_t>(n_seq * std::max<int64_t>(least, 1), full + n_seq), n_seq * tiles, least > 1, min_tiles }, rt, groups, slots };
+}
+extern "C" size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
+    if (!attn_shape(n_seq, n_head, n_head_kv, hd, max_len) || max_tree < 1 || max_tree > LG_TREE_ROWS || window < 0) return 0;
+    const AttnCut c = tree_cut_of(n_seq, max_tree, n_head, n_head_kv, hd, max_len, window).c;
+    if (!c.join) return 0;
+    const size_t slots = (size_t)c.splits * max_tree * n_head;
+    return cut_bytes(n_seq, c) + 2 * up256(slots * 4) + slots * hd * 4;
+}
+
+template <int HD>
+static void launch_tree(const TreeAttn &a, const TreeCut &t, hipStream_t st) {
+    const dim3 grid((unsigned)((a.units + 7) / 8 * 8 * t.groups)), wg(LG_PA_WAVES * 64);
+    if (t.tiles == 1) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1>), grid, wg, 0, st, a);
+    else if (t.tiles == 2) hipLaunchKernelGGL((lg_k_tree_attn<HD, 2>), grid, wg, 0, st, a);
+    else if constexpr (HD <= 256) hipLaunchKernelGGL((lg_k_tree_attn<HD, 4>), grid, wg, 0, st, a);
+    if (!t.c.join) return;
+    if (a.n_seq > LG_PA_LANES) hipLaunchKernelGGL((lg_k_page_merge<HD, 1, TreeAttn>), dim3(a.H * a.max_tree, a.n_seq), dim3(64), 0, st, a);
+    else hipLaunchKernelGGL((lg_k_page_merge<HD, 8, TreeAttn>), dim3(a.H * a.max_tree, a.n_seq), dim3(512), 0, st, a);
+}
+
+extern "C" int lg_hip_paged_tree_attention(const struct lg_hip_pages *p, const float *d_q, int64_t q_stride, int n_rows, int n_seq, int max_tree, int n_head, const int32_t *d_table, int max_blocks,
+                                           const int32_t *d_len, const int32_t *d_start, const uint64_t *d_mask, const int32_t *d_pos, int max_len, int window, float scale, float *d_out,
+                                           int64_t out_stride, void *d_work, size_t work_bytes, void *stream) {
+    PageGeo g;
+    int rc = check_pages("paged_tree_attention", p, &g);
+    if (rc || (rc = check_trees("paged_tree_attention", n_seq, max_tree, n_rows))) return rc;
+    const int hd = p->head_dim;
+    if (!attn_shape(n_seq, n_head, p->n_head_kv, hd, max_len))
+        return lg_fail(-2, "paged_tree_attention: %d query heads on %d key heads (at most 8 each), lengths up to %d", n_head, p->n_head_kv, max_len);
+    if (max_blocks < 1 || (int64_t)max_blocks * p->page_size > INT32_MAX) return lg_fail(-2, "paged_tree_attention: %d blocks of %d positions", max_blocks, p->page_size);
+    if (window < 0) return lg_fail(-2, "paged_tree_attention: a window of %d", window);
+    if (n_seq == 0 || n_rows == 0) return 0;
+    if (!d_q || !d_table || !d_len || !d_start || !d_mask || !d_pos || !d_out) return lg_fail(-1, "paged_tree_attention: null argument");
+    const int64_t qd = (int64_t)n_head * hd;
+    if (q_stride < qd || q_stride % 4 || !aligned16(d_q)) return lg_fail(-2, "paged_tree_attention: query rows of %lld values, %lld apart (aligned to 16 bytes)", (long long)qd, (long long)q_stride);
+    if (out_stride < qd || ((uintptr_t)d_out & 3)) return lg_fail(-2, "paged_tree_attention: output rows of %lld values, %lld apart", (long long)qd, (long long)out_stride);
+    if ((uintptr_t)d_mask & 7) return lg_fail(-2, "paged_tree_attention: sets that are not aligned to 8 bytes");
+    const TreeCut t = tree_cut_of(n_seq, max_tree, n_head, p->n_head_kv, hd, max_len, window);
+    const AttnCut &c = t.c;
+    // (sums over the sequences are 32 bits on the device, and so are a launch's threads)
+    if (c.tiles > INT32_MAX || c.splits * n_head * max_tree > LG_MOST_GROUPS || (int64_t)n_head * max_tree * n_seq > LG_MOST_GROUPS / 2)
+        return lg_fail(-2, "paged_tree_attention: %d sequences of up to %d rows of %d heads in %lld splits in one call", n_seq, max_tree, n_head, (long long)c.splits);
+    const size_t need = lg_hip_paged_tree_attention_workspace(n_seq, max_tree, n_head, p->n_head_kv, hd, max_len, window);
+    if (need && (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)))
+        return lg_fail(-2, "paged_tree_attention: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
+    const size_t part = up256((size_t)c.splits * max_tree * n_head * 4);
+    char *const w = need ? (char *)d_work + cut_bytes(n_seq, c) : nullptr;
+    const TreeAttn a{ { g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, (float *)w, need ? (float *)(w + part) : nullptr, need ? (float *)(w + 2 * part) : nullptr, scale,
+                        need ? (int32_t *)d_work : nullptr, n_head, p->n_head_kv, n_seq, max_blocks, max_len, window, t.slots, c.least },
+                      d_start, d_pos, (const lg_u64 *)d_mask, n_rows, max_tree, t.groups, (int)(c.splits * p->n_head_kv) };
+    hipStream_t st = (hipStream_t)stream;
+    if (c.join && n_seq > LG_PA_LANES) hipLaunchKernelGGL(lg_k_page_cut<TreeAttn>, dim3(1), dim3(LG_PC_WG), 0, st, a);
+    switch (hd) {
+        case 64:  launch_tree<64>(a, t, st); break;
+        case 128: launch_tree<128>(a, t, st); break;
+        case 256: launch_tree<256>(a, t, st); break;
+        default:  launch_tree<512>(a, t, st); break;
+    }
+    LG_TRY(hipGetLastError());
+    return 0;
+}
+
+// ---- shared pages -----------------------------------------------------------------------------------------------
+static size_t fork_page_bytes(int n_pages) { return up256((size_t)n_pages * sizeof(ForkPage)); }
+static bool fork_shape(int n_seq, int n_pages, int max_blocks) {
+    // (entries of the table are counted in 31 bits)
+    return n_seq >= 0 && n_seq <= LG_PLAN_SEQS && n_pages >= 1 && max_blocks >= 1 && (int64_t)n_seq * max_blocks < INT32_MAX;
+}
+extern "C" size_t lg_hip_paged_fork_workspace(int n_seq, int n_pages, int max_blocks) {
+    if (!fork_shape(n_seq, n_pages, max_blocks)) return 0;
+    return fork_page_bytes(n_pages) + up256((size_t)n_seq * max_blocks * 4);
+}
+extern "C" int lg_hip_paged_fork(int n_seq, int page_size, int n_pages, int max_blocks, const int32_t *d_src, const int32_t *d_len_old, const int32_t *d_len_new, int32_t *d_table,
+                                 int32_t *d_shares, int32_t *d_free, int32_t *d_n_free, int32_t *d_from, int32_t *d_to, int32_t *d_rows, int32_t *d_status, void *d_work, size_t work_bytes,
+                                 void *stream) {
+    const int shift = shift_of(page_size);
+    if (n_seq < 0 || n_seq > LG_PLAN_SEQS) return lg_fail(-2, "paged_fork: %d sequences (0..%d)", n_seq, LG_PLAN_SEQS);
+    if (shift < 0) return lg_fail(-2, "paged_fork: pages of %d positions (a power of two of 16..256)", page_size);
+    if (n_pages < 1 || (int64_t)n_pages * page_size > INT32_MAX || max_blocks < 1 || (int64_t)max_blocks * page_size > INT32_MAX || !fork_shape(n_seq, n_pages, max_blocks))
+        return lg_fail(-2, "paged_fork: %d pages and %d blocks of %d positions for %d sequences (positions and entries are 31 bits)", n_pages, max_blocks, page_size, n_seq);
+    if (!d_shares || !d_free || !d_n_free || !d_status || (n_seq && (!d_src || !d_len_old || !d_len_new || !d_table || !d_from || !d_to || !d_rows)))
+        return lg_fail(-1, "paged_fork: null argument");
+    const size_t need = lg_hip_paged_fork_workspace(n_seq, n_pages, max_blocks);
+    if (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)) return lg_fail(-2, "paged_fork: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
+    const ForkArgs a{ d_src, d_len_old, d_len_new, d_table, d_shares, d_free, d_n_free, d_from, d_to, d_rows, d_status, (ForkPage *)d_work, (int32_t *)((char *)d_work + fork_page_bytes(n_pages)),
+                      n_seq, shift, n_pages, max_blocks };
+    hipLaunchKernelGGL(lg_k_page_fork<1024>, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
+    LG_TRY(hipGetLastError());
+    return 0;
+}
+
+// The layers of a cache: one table serves them, so pages are alike in size and number; heads and strides are each layer's own
+static int check_layers(const char *who, const struct lg_hip_pages *p, int n_layers) {
+    if (n_layers < 0) return lg_fail(-2, "%s: %d layers", who, n_layers);
+    if (n_layers && !p) return lg_fail(-1, "%s: null argument", who);
+    for (int i = 0; i < n_layers; ++i) {
+        PageGeo g;
+        const int rc = check_pages(who, p + i, &g);
+        if (rc) return rc;
+        if (p[i].page_size != p[0].page_size || p[i].n_pages != p[0].n_pages)
+            return lg_fail(-2, "%s: layer %d has %d pages of %d positions, layer 0 %d of %d", who, i, p[i].n_pages, p[i].page_size, p[0].n_pages, p[0].page_size);
+    }
+    return 0;
+}
+// LG_LAYERS at a time: launch(layers, how many, most units of one)
+template <typename Launch>
+static void each_layers(const struct lg_hip_pages *p, int n_layers, Launch launch) {
+    for (int from = 0; from < n_layers; from += LG_LAYERS) {
+        PageLayers ls = {};
+        const int n = std::min(LG_LAYERS, n_layers - from);
+        int most = 0;
+        for (int i = 0; i < n; ++i) {
+            const struct lg_hip_pages &x = p[from + i];
+            ls.l[i] = PageLayer{ x.k, x.v, x.row_stride, x.page_stride, x.n_head_kv * x.head_dim / 8 };
+            most = std::max(most, ls.l[i].units);
+        }
+        launch(ls, n, most);
+    }
+}
+extern "C" int lg_hip_paged_compact(const struct lg_hip_pages *layers, int n_layers, int n_seq, int max_tree, const int32_t *d_table, int max_blocks, const int32_t *d_len, const int32_t *d_start,
+                                    const int32_t *d_path, const int32_t *d_count, void *stream) {
+    int rc = check_layers("paged_compact", layers, n_layers);
+    if (rc || (rc = check_trees("paged_compact", n_seq, max_tree, 0))) return rc;
+    if (n_layers == 0) return 0;
+    if (max_blocks < 1 || (int64_t)max_blocks * layers->page_size > INT32_MAX) return lg_fail(-2, "paged_compact: %d blocks of %d positions", max_blocks, layers->page_size);
+    if (n_seq == 0) return 0;
+    if (!d_table || !d_len || !d_start || !d_path || !d_count) return lg_fail(-1, "paged_compact: null argument");
+    each_layers(layers, n_layers, [&](const PageLayers &ls, int n, int most) {
+        hipLaunchKernelGGL(lg_k_page_compact, dim3((unsigned)(2 * most + 255) / 256, (unsigned)n, (unsigned)n_seq), dim3(256), 0, (hipStream_t)stream, ls, d_table, d_len, d_start, d_path, d_count,
+                           max_tree, max_blocks, shift_of(layers->page_size), layers->n_pages);
+    });
+    LG_TRY(hipGetLastError());
+    return 0;
+}
+extern "C" int lg_hip_paged_copy(const struct lg_hip_pages *layers, int n_layers, int n, const int32_t *d_from, const int32_t *d_to, const int32_t *d_rows, void *stream) {
+    const int rc = check_layers("paged_copy", layers, n_layers);
+    if (rc) return rc;
+    if (n < 0 || n > 65535) return lg_fail(-2, "paged_copy: %d pages (0..65535)", n);
+    if (n == 0 || n_layers == 0) return 0;
+    if (!d_from || !d_to || !d_rows) return lg_fail(-1, "paged_copy: null argument");
+    each_layers(layers, n_layers, [&](const PageLayers &ls, int k, int most) {
+        // several workgroups to a page where there are few pages
+        const int64_t pages = (int64_t)n * k * 2, whole = ((int64_t)layers->page_size * most + 1023) / 1024;
+        const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(whole, 4096 / pages));
+        hipLaunchKernelGGL(lg_k_page_copy, dim3((unsigned)(2 * parts), (unsigned)k, (unsigned)n), dim3(256), 0, (hipStream_t)stream, ls, d_from, d_to, d_rows, shift_of(layers->page_size),
+                           layers->n_pages, parts);
+    });
+    LG_TRY(hipGetLastError());
+    return 0;
+}
+
+// ---- rules ------------------------------------------------------------------------------------------------------
+extern "C" int lg_hip_adjust_logits(const struct lg_hip_logit_rules *r, const float *d_logits, int64_t stride, int rows, int n_vocab, float *d_out, int64_t out_stride, void *stream) {
+    if (!r) return lg_fail(-1, "adjust_logits: null argument");
+    if (rows < 0 || rows > 65535) return lg_fail(-2, "adjust_logits: %d rows (0..65535)", rows);
+    if (n_vocab < 1 || n_vocab > LG_RULES_VOCAB) return lg_fail(-2, "adjust_logits: a vocabulary of %d (1..%d)", n_vocab, LG_RULES_VOCAB);
+    if (stride < n_vocab || out_stride < n_vocab) return lg_fail(-2, "adjust_logits: rows of %d logits, %lld and %lld apart", n_vocab, (long long)stride, (long long)out_stride);
+    if (r->n_seq < 0 || r->n_bias < 0 || r->n_allow < 0) return lg_fail(-2, "adjust_logits: %d sequences, %d biases, %d grammars", r->n_seq, r->n_bias, r->n_allow);
+    if (r->hist && (r->hist_stride < 1 || r->hist_stride > 1 << 30)) return lg_fail(-2, "adjust_logits: texts %lld tokens apart", (long long)r->hist_stride);
+    if (r->n_allow && r->allow_stride < (n_vocab + 31) / 32) return lg_fail(-2, "adjust_logits: sets of %d tokens, %lld words apart", n_vocab, (long long)r->allow_stride);
+    if (rows == 0) return 0;
+    if (!d_logits || !d_out || (r->hist && (!r->hist_len || !r->penalty)) || (r->tree_mask && (!r->tree_start || !r->tree_tok || !r->penalty)) ||
+        (r->n_bias && (!r->bias_start || !r->bias_tok || !r->bias)) || (r->n_allow && !r->allow))
+        return lg_fail(-1, "adjust_logits: null argument");
+    if ((((uintptr_t)d_logits | (uintptr_t)d_out | (uintptr_t)r->hist) & 3) || ((uintptr_t)r->tree_mask & 7)) return lg_fail(-2, "adjust_logits: arguments that are not aligned");
+    if (d_out == d_logits && stride != out_stride) return lg_fail(-2, "adjust_logits: rows in place, %lld and %lld apart", (long long)stride, (long long)out_stride);
+    const RulesArgs a{ d_logits, (long long)stride, d_out, (long long)out_stride, r->seq, (const RulesPenalty *)r->penalty, r->hist, r->hist_len, (long long)r->hist_stride,
+                       (const lg_u64 *)r->tree_mask, r->tree_start, r->tree_tok, r->n_bias ? r->bias_start : nullptr, r->bias_tok, r->bias, r->allow, r->allow_row, (long long)r->allow_stride,
+                       rows, n_vocab, r->n_seq, r->n_bias, r->n_allow };
+    const dim3 grid((unsigned)((n_vocab + LG_RULES_SLICE - 1) / LG_RULES_SLICE), (unsigned)rows);
+    const unsigned lds = LG_RULES_SLICE * 4 * (r->n_bias ? 2 : r->penalty ? 1 : 0);
+    if (aligned16(d_logits) && aligned16(d_out) && stride % 4 == 0 && out_stride % 4 == 0) hipLaunchKernelGGL(lg_k_rules<true>, grid, dim3(LG_RULES_WG), lds, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL(lg_k_rules<false>, grid, dim3(LG_RULES_WG), lds, (hipStream_t)stream, a);
     LG_TRY(hipGetLastError());
     return 0;
 }

@@ -1,0 +1,226 @@
+// lg_share.h — pages of a cache that sequences share: forks and ends of them, and rows moved and copied in every layer.
+#pragma once
+
+#include "lg_pages.h"
+
+// ---- fork ------------------------------------------------------------------------------------------------------------
+enum { LG_FORK_BAD_LEN = 1, LG_FORK_NO_PAGES = 2, LG_FORK_BAD_SOURCE = 4, LG_FORK_BAD_STACK = 8, LG_FORK_BAD_PAGE = 16, LG_FORK_BAD_SHARES = 32 };   // LG_HIP_FORK_* of lg_hip.h
+
+struct ForkPage { int32_t holders, first, parts, keeper; };      // of a page that the call touches: rows that hold it afterwards, its first release, rows that end in it, the one of them that keeps it
+struct ForkArgs {
+    const int32_t *src, *len_old, *len_new;     // [n_seq]
+    int32_t *table;                             // [n_seq][max_blocks]
+    int32_t *shares, *stack, *n_free;           // [n_pages], [n_pages], height
+    int32_t *from, *to, *rows;                  // [n_seq]
+    int32_t *status;
+    ForkPage *page;                             // [n_pages] working memory: what is used is set first
+    int32_t *stage;                             // [n_seq * max_blocks] the pages that come to a row
+    int n_seq, shift, n_pages, max_blocks;
+};
+
+// Row i afterwards holds the first len_new[i] positions of what row src[i] held.  Only rows that change count: a row that takes another's pages releases all of its own and takes nb(len_new) of
+// that one's, any other releases those behind nb(len_new).  A page's holders afterwards are those before and what comes and goes, in whole numbers, so the order of the additions does not matter; pages with none go on the
+// stack, each at its first release (sequence by sequence, block by block), the first one topmost.  Of the rows that end inside a page one may keep it if no row holds it whole: the first that had it, or
+// else the first; each of the others takes a page off the stack, in order, and is told what to copy.
+// All or nothing: everything is read and counted in working memory, then everything is written.
+// One workgroup: a few words for every page that moves.  Each pass over them is a search in LDS and a round trip or two.
+template <int NT>
+__global__ __launch_bounds__(NT) void lg_k_page_fork(ForkArgs a) {
+    __shared__ int32_t gone[LG_PLAN_SEQS + 1], come[LG_PLAN_SEQS + 1], fresh[LG_PLAN_SEQS];      // releases and arrivals before each row; which of the new pages it takes, -1 none
+    __shared__ lg_u64 part[3 * NT / 64];
+    __shared__ int32_t bad, wrong_page;
+    const int t = threadIdx.x, P = 1 << a.shift, n = a.n_seq;
+    const long long most = (long long)a.max_blocks << a.shift;
+    const int per = (n + NT - 1) / NT, i0 = t * per, i1 = i0 + per < n ? i0 + per : n;
+    const int nf = *a.n_free;
+    if (t == 0) { bad = nf < 0 || nf > a.n_pages ? LG_FORK_BAD_STACK : 0; wrong_page = 0; }
+    auto blocks = [&](int len) { return (int)(((long long)len + P - 1) >> a.shift); };
+    auto place = [&](int i, int block) { return a.table + (size_t)i * a.max_blocks + block; };
+    auto outside = [&](int id) { return id < 0 || id >= a.n_pages; };
+    auto holders = [&](int id) { return __hip_atomic_load(&a.page[id].holders, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    lg_u64 run[3] = { 0, 0, 0 }, all[3];
+    int st = 0;
+    for (int i = i0; i < i1; ++i) {
+        const int s = a.src[i], lo = a.len_old[i], ln = a.len_new[i];
+        const bool named = s >= 0 && s < n;
+        if (s < -1 || s >= n) st |= LG_FORK_BAD_SOURCE;
+        else if (ln > (named ? a.len_old[s] : 0)) st |= LG_FORK_BAD_LEN;
+        if (lo < 0 || lo > most || ln < 0) st |= LG_FORK_BAD_LEN;
+        if (st) break;
+        gone[i] = (int)run[0]; come[i] = (int)run[1];
+        run[0] += s != i ? blocks(lo) : blocks(lo) - blocks(ln);
+        run[1] += s != i ? blocks(ln) : 0;
+    }
+    lg_block_run3<NT>(run, all, part);                        // (run: exclusive now.  A barrier in here also shows `bad`)
+    if (st) atomicOr(&bad, st);
+    __syncthreads();
+    st = bad;
+    const int n_gone = st ? 0 : (int)all[0], n_come = st ? 0 : (int)all[1];
+    if (!st) for (int i = i0; i < i1; ++i) { gone[i] += (int)run[0]; come[i] += (int)run[1]; }
+    if (t == 0) { gone[n] = n_gone; come[n] = n_come; }
+    __syncthreads();
+    auto leaves = [&](int i, int e) { const int b = e - gone[i]; return a.src[i] != i ? b : blocks(a.len_new[i]) + b; };        // the block of release e
+    // every page that the call touches: its holders before
+    auto touch = [&](int id) {
+        if (outside(id)) { atomicOr(&wrong_page, LG_FORK_BAD_PAGE); return; }
+        const int h = a.shares[id];
+        if (h < 0 || h >= LG_PLAN_SEQS) { atomicOr(&wrong_page, LG_FORK_BAD_SHARES); return; }
+        a.page[id] = ForkPage{ h + 1, INT32_MAX, 0, INT32_MAX };
+    };
+    auto ends_in = [&](int i) { const int s = a.src[i], ln = a.len_new[i]; return s >= 0 && (ln & (P - 1)) ? *place(s, ln >> a.shift) : -1; };
+    if (!st) {
+        for (int e = t; e < n_gone; e += NT) { const int i = lg_owner(gone, n, e); touch(*place(i, leaves(i, e))); }
+        for (int e = t; e < n_come; e += NT) { const int i = lg_owner(come, n, e), id = *place(a.src[i], e - come[i]); a.stage[e] = id; touch(id); }
+        for (int i = i0; i < i1; ++i) if (a.src[i] >= 0 && (a.len_new[i] & (P - 1))) touch(ends_in(i));
+        __syncthreads();
+        st = wrong_page;
+    }
+    int F = 0, N = 0, top = nf;
+    if (!st) {
+        for (int e = t; e < n_gone; e += NT) {
+            const int i = lg_owner(gone, n, e), id = *place(i, leaves(i, e));
+            atomicAdd(&a.page[id].holders, -1);
+            atomicMin(&a.page[id].first, e);
+        }
+        for (int e = t; e < n_come; e += NT) atomicAdd(&a.page[a.stage[e]].holders, 1);
+        for (int i = i0; i < i1; ++i) {
+            const int id = ends_in(i);
+            if (id >= 0) { atomicAdd(&a.page[id].parts, 1); atomicMin(&a.page[id].keeper, (a.src[i] != i ? LG_PLAN_SEQS : 0) + i); }
+        }
+        __syncthreads();
+        // releases in a row to a thread, as their places on the stack follow each other
+        const int each = (n_gone + NT - 1) / NT, e0 = t * each < n_gone ? t * each : n_gone, e1 = e0 + each < n_gone ? e0 + each : n_gone;
+        auto releases = [&](auto &&f) {
+            for (int e = e0, i = e0 < e1 ? lg_owner(gone, n, e0) : 0; e < e1; ++e) {
+                while (gone[i + 1] <= e) ++i;
+                const int id = *place(i, leaves(i, e));
+                if (holders(id) < 0) atomicOr(&wrong_page, LG_FORK_BAD_SHARES);
+                if (holders(id) == 0 && __hip_atomic_load(&a.page[id].first, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == e) f(id);
+            }
+        };
+        run[0] = run[1] = run[2] = 0;
+        releases([&](int) { ++run[0]; });
+        for (int i = i0; i < i1; ++i) {
+            const int id = ends_in(i);
+            bool copies = false;
+            if (id >= 0) {
+                const int h = holders(id), p = __hip_atomic_load(&a.page[id].parts, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+                          k = __hip_atomic_load(&a.page[id].keeper, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (p > h) atomicOr(&wrong_page, LG_FORK_BAD_SHARES);
+                copies = p != h || k != (a.src[i] != i ? LG_PLAN_SEQS : 0) + i;
+            }
+            fresh[i] = copies ? (int)run[1] : -1;
+            run[1] += copies;
+        }
+        lg_block_run3<NT>(run, all, part);
+        F = (int)all[0]; N = (int)all[1]; top = nf + F;
+        for (int i = i0; i < i1; ++i) if (fresh[i] >= 0) fresh[i] += (int)run[1];
+        if (t == 0) {
+            if (top > a.n_pages) atomicOr(&wrong_page, LG_FORK_BAD_STACK);
+            else if (N > top) atomicOr(&wrong_page, LG_FORK_NO_PAGES);
+        }
+        if (top <= a.n_pages && N <= top) for (int k = F + t; k < N; k += NT) if (outside(a.stack[top - 1 - k])) atomicOr(&wrong_page, LG_FORK_BAD_PAGE);
+        __syncthreads();
+        st = wrong_page;
+        if (!st) {
+            // counts and the stack first, while the table is as it was
+            auto count = [&](int id) {
+                const int h = holders(id), p = __hip_atomic_load(&a.page[id].parts, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), left = h - (p && p == h ? p - 1 : p);
+                a.shares[id] = left > 0 ? left - 1 : 0;
+            };
+            int at = top - 1 - (int)run[0];
+            releases([&](int id) { a.stack[at--] = id; });
+            for (int e = t; e < n_gone; e += NT) { const int i = lg_owner(gone, n, e); count(*place(i, leaves(i, e))); }
+            for (int e = t; e < n_come; e += NT) count(a.stage[e]);
+            for (int i = i0; i < i1; ++i) {
+                const int id = ends_in(i);
+                if (id >= 0) count(id);
+                a.from[i] = fresh[i] >= 0 ? id : -1;
+                a.rows[i] = fresh[i] >= 0 ? a.len_new[i] & (P - 1) : 0;
+            }
+            __syncthreads();
+            for (int e = t; e < n_gone; e += NT) { const int i = lg_owner(gone, n, e), b = leaves(i, e); if (b >= blocks(a.len_new[i])) *place(i, b) = -1; }
+            for (int e = t; e < n_come; e += NT) {
+                const int i = lg_owner(come, n, e), b = e - come[i];
+                if (!(fresh[i] >= 0 && b == a.len_new[i] >> a.shift)) *place(i, b) = a.stage[e];
+            }
+            for (int i = i0; i < i1; ++i) {
+                const int id = fresh[i] >= 0 ? a.stack[top - 1 - fresh[i]] : -1;
+                a.to[i] = id;
+                if (id >= 0) { *place(i, a.len_new[i] >> a.shift) = id; a.shares[id] = 0; }
+            }
+        }
+    }
+    if (st) for (int i = i0; i < i1; ++i) { a.from[i] = a.to[i] = -1; a.rows[i] = 0; }
+    if (t == 0) { *a.status = st; if (!st) *a.n_free = top - N; }
+}
+
+// ---- rows and pages in every layer -----------------------------------------------------------------------------------
+#define LG_LAYERS 64                // of a launch: they travel as its arguments
+struct PageLayer { uint16_t *k, *v; long long row_stride, page_stride; int units; };          // units: 8 values, 16 bytes
+struct PageLayers { PageLayer l[LG_LAYERS]; };
+
+// The rows of an accepted path to the places behind the committed ones.  Rows only move down and in order (path[k] > path[k - 1]), so a thread that takes 16 bytes of them all, eight
+// at a time, has read every row before it is written over.  Bound by memory: 2 bytes read and 2 written a value.
+#define LG_MOVE_AT_ONCE 8
+__global__ __launch_bounds__(256) void lg_k_page_compact(PageLayers ls, const int32_t *table, const int32_t *len, const int32_t *start, const int32_t *path, const int32_t *count, int max_tree,
+                                                        int max_blocks, int shift, int n_pages) {
+    __shared__ long long s_src[64], s_dst[64];
+    __shared__ int s_n;
+    const int seq = blockIdx.z, lane = threadIdx.x;
+    const PageLayer &L = ls.l[blockIdx.y];
+    if (lane < 64) {
+        const int total = len[seq], kept = count[seq];
+        const long long n = (long long)start[seq + 1] - start[seq];
+        const bool fits = n >= 1 && n <= max_tree && total >= n && total <= (long long)max_blocks << shift;
+        const int mine = lane < max_tree ? path[(long long)seq * max_tree + lane] : -1;
+        const int before = __shfl(mine, lane ? lane - 1 : 0);
+        const bool ok = fits && lane < kept && mine >= 0 && mine < n && (lane == 0 || mine > before);
+        const lg_u64 not_ok = ~__ballot(ok);
+        const int last = not_ok ? (int)__builtin_ctzll(not_ok) : 64;   // rows from here on stay where they are
+        const int P = 1 << shift;
+        bool moves = lane < last && mine != lane;
+        long long src = 0, dst = 0;
+        if (moves) {
+            const int32_t *row = table + (long long)seq * max_blocks;
+            const int base = total - (int)n, sp = base + mine, dp = base + lane, a = row[sp >> shift], b = row[dp >> shift];
+            moves = a >= 0 && a < n_pages && b >= 0 && b < n_pages;
+            src = a * L.page_stride + (sp & (P - 1)) * L.row_stride;
+            dst = b * L.page_stride + (dp & (P - 1)) * L.row_stride;
+        }
+        const lg_u64 all = __ballot(moves);
+        if (moves) { const int k = __popcll(all & ((1ull << lane) - 1)); s_src[k] = src; s_dst[k] = dst; }
+        if (lane == 0) s_n = __popcll(all);
+    }
+    __syncthreads();
+    const int u = (int)(blockIdx.x * 256 + threadIdx.x), n = s_n;
+    if (u >= 2 * L.units) return;
+    uint16_t *const at = (u < L.units ? L.k : L.v) + (u < L.units ? u : u - L.units) * 8;
+    for (int k0 = 0; k0 < n; k0 += LG_MOVE_AT_ONCE) {
+        uint4 x[LG_MOVE_AT_ONCE];
+        #pragma unroll
+        for (int k = 0; k < LG_MOVE_AT_ONCE; ++k) x[k] = *(const uint4 *)(at + s_src[k0 + k < n ? k0 + k : n - 1]);       // (no branch between loads)
+        #pragma unroll
+        for (int k = 0; k < LG_MOVE_AT_ONCE; ++k) if (k0 + k < n) *(uint4 *)(at + s_dst[k0 + k]) = x[k];
+    }
+}
+// The first rows[i] rows of page from[i] to page to[i]: a workgroup takes every `parts`-th 4096 bytes of K or V of one pair in one layer.  Bound by memory, as above.
+__global__ __launch_bounds__(256) void lg_k_page_copy(PageLayers ls, const int32_t *from, const int32_t *to, const int32_t *rows, int shift, int n_pages, int parts) {
+    const int i = blockIdx.z, a = from[i], b = to[i], n = rows[i];
+    if (a < 0 || a >= n_pages || b < 0 || b >= n_pages || a == b || n < 1) return;
+    const PageLayer &L = ls.l[blockIdx.y];
+    const bool second = (int)blockIdx.x >= parts;
+    const int first = second ? blockIdx.x - parts : blockIdx.x, P = 1 << shift, units = (n < P ? n : P) * L.units;
+    const uint16_t *const src = (second ? L.v : L.k) + a * L.page_stride;
+    uint16_t *const dst = (second ? L.v : L.k) + b * L.page_stride;
+    const int step = parts * 256, of = L.units;
+    const bool dense = L.row_stride == of * 8;
+    auto where = [&](int u) { const int r = dense ? 0 : u / of; return r * L.row_stride + (long long)(u - r * of) * 8; };
+    int u = first * 256 + threadIdx.x;
+    for (; u + 3 * step < units; u += 4 * step) {
+        const long long p0 = where(u), p1 = where(u + step), p2 = where(u + 2 * step), p3 = where(u + 3 * step);
+        const uint4 x0 = *(const uint4 *)(src + p0), x1 = *(const uint4 *)(src + p1), x2 = *(const uint4 *)(src + p2), x3 = *(const uint4 *)(src + p3);
+        *(uint4 *)(dst + p0) = x0; *(uint4 *)(dst + p1) = x1; *(uint4 *)(dst + p2) = x2; *(uint4 *)(dst + p3) = x3;
+    }
+    for (; u < units; u += step) *(uint4 *)(dst + where(u)) = *(const uint4 *)(src + where(u));
+}

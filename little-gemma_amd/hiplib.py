@@ -43,6 +43,13 @@ class Sampling(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
 
 
+class LogitRules(C.Structure):
+    """struct lg_hip_logit_rules: what logits are held to ahead of sampling (device pointers)."""
+    _fields_ = [("n_seq", C.c_int32), ("n_bias", C.c_int32), ("n_allow", C.c_int32), ("seq", C.c_void_p), ("penalty", C.c_void_p), ("hist", C.c_void_p), ("hist_len", C.c_void_p),
+                ("hist_stride", C.c_int64), ("tree_mask", C.c_void_p), ("tree_start", C.c_void_p), ("tree_tok", C.c_void_p), ("bias_start", C.c_void_p), ("bias_tok", C.c_void_p),
+                ("bias", C.c_void_p), ("allow", C.c_void_p), ("allow_row", C.c_void_p), ("allow_stride", C.c_int64)]
+
+
 def build():
     """Compile the HIP library for gfx950 and the C backend on top of it."""
     subprocess.run(["make", "-C", CSRC, "-B", "liblg_hip.so"], check=True, stdout=subprocess.DEVNULL,
@@ -105,6 +112,17 @@ def load_hip():
     L.lg_hip_sample_workspace.argtypes = [I, I]
     L.lg_hip_sample_workspace.restype = Z
     L.lg_hip_sample.argtypes = [P, Q, I, I] + [P] * 6 + [Z, P]
+    L.lg_hip_tree_plan.argtypes = [I] * 3 + [P] * 8
+    L.lg_hip_tree_accept.argtypes = [I] * 3 + [P] * 10
+    L.lg_hip_paged_tree_attention_workspace.argtypes = [I] * 7
+    L.lg_hip_paged_tree_attention_workspace.restype = Z
+    L.lg_hip_paged_tree_attention.argtypes = [P, P, Q, I, I, I, I, P, I, P, P, P, P, I, I, C.c_float, P, Q, P, Z, P]
+    L.lg_hip_paged_compact.argtypes = [P, I, I, I, P, I, P, P, P, P, P]
+    L.lg_hip_paged_fork_workspace.argtypes = [I] * 3
+    L.lg_hip_paged_fork_workspace.restype = Z
+    L.lg_hip_paged_fork.argtypes = [I] * 4 + [P] * 12 + [Z, P]
+    L.lg_hip_paged_copy.argtypes = [P, I, I, P, P, P, P]
+    L.lg_hip_adjust_logits.argtypes = [P, P, Q, I, I, P, Q, P]
     L.lg_hip_forward_sample.argtypes = [P, P, i32p, I, I, C.POINTER(Sampling), f32p, i32p, C.POINTER(C.c_int32)]
     _hip = L
     return L
