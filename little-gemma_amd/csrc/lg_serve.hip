@@ -268,20 +268,27 @@ extern "C" int lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int
     return 0;
 }
 
-// 16-pair tiles of a workgroup: as many as a tree has, up to what registers hold of outputs
-static int tree_tiles(int pairs, int hd) { return pairs <= 16 ? 1 : pairs <= 32 || hd == 512 ? 2 : 4; }
-struct TreeCut { AttnCut c; int tiles, groups, slots; };
+// How a workgroup takes pairs: 16 RT by each of WR wavefronts, as many as registers hold of outputs, and no more than a tree has
+struct TreeForm { int rt, wr; };
+static TreeForm tree_form(int pairs, int hd) {
+    if (pairs <= 16) return { 1, 1 };
+    if (hd == 512) return pairs <= 32 ? TreeForm{ 1, 2 } : TreeForm{ 1, 4 };
+    if (pairs <= 32) return { 2, 1 };
+    return hd == 256 ? TreeForm{ 2, 2 } : TreeForm{ 4, 1 };
+}
+struct TreeCut { AttnCut c; TreeForm form; int groups, slots; };
 // As cut_of, for workgroups of several pairs: those of one stretch of keys share the chip's room
 static TreeCut tree_cut_of(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
-    const int pairs = max_tree * (n_head / n_head_kv), rt = tree_tiles(pairs, hd), groups = (pairs + 16 * rt - 1) / (16 * rt);
-    const int slots = std::max(2, 256 * lg_tree_per_simd(hd, rt) / groups);
+    const int pairs = max_tree * (n_head / n_head_kv);
+    const TreeForm form = tree_form(pairs, hd);
+    const int rows = 16 * form.rt * form.wr, groups = (pairs + rows - 1) / rows, slots = std::max(2, 256 * lg_tree_per_simd(hd, form.rt) / groups);
     // (a tree's rows see a window from the first committed position that its row 0 sees to its last row)
     const int64_t reach = window > 0 ? (int64_t)window + max_tree + LG_PA_TILE : max_len, span = std::min<int64_t>(reach, max_len), tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
     const int64_t units = (int64_t)n_seq * n_head_kv;
     const int alone = alone_of(hd, units * groups), min_tiles = tiles <= alone ? alone : 4;
     const int64_t least = (tiles + min_tiles - 1) / min_tiles, rounds = std::max<int64_t>(1, (units + slots / 2 - 1) / (slots / 2));
     const int64_t full = std::max<int64_t>(rounds * slots / n_head_kv, n_seq * tiles / (LG_PA_CHUNK / LG_PA_TILE));
-    return { { std::min<int64_t>(n_seq * std::max<int64_t>(least, 1), full + n_seq), n_seq * tiles, least > 1, min_tiles }, rt, groups, slots };
+    return { { std::min<int64_t>(n_seq * std::max<int64_t>(least, 1), full + n_seq), n_seq * tiles, least > 1, min_tiles }, form, groups, slots };
 }
 extern "C" size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
     if (!attn_shape(n_seq, n_head, n_head_kv, hd, max_len) || max_tree < 1 || max_tree > LG_TREE_ROWS || window < 0) return 0;
@@ -294,9 +301,13 @@ extern "C" size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree,
 template <int HD>
 static void launch_tree(const TreeAttn &a, const TreeCut &t, hipStream_t st) {
     const dim3 grid((unsigned)((a.units + 7) / 8 * 8 * t.groups)), wg(LG_PA_WAVES * 64);
-    if (t.tiles == 1) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1>), grid, wg, 0, st, a);
-    else if (t.tiles == 2) hipLaunchKernelGGL((lg_k_tree_attn<HD, 2>), grid, wg, 0, st, a);
-    else if constexpr (HD <= 256) hipLaunchKernelGGL((lg_k_tree_attn<HD, 4>), grid, wg, 0, st, a);
+    if (t.form.rt * t.form.wr == 1) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 1>), grid, wg, 0, st, a);
+    else if constexpr (HD == 512) {
+        if (t.form.wr == 2) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 2>), grid, wg, 0, st, a);
+        else hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 4>), grid, wg, 0, st, a);
+    } else if (t.form.rt * t.form.wr == 2) hipLaunchKernelGGL((lg_k_tree_attn<HD, 2, 1>), grid, wg, 0, st, a);
+    else if constexpr (HD == 256) hipLaunchKernelGGL((lg_k_tree_attn<HD, 2, 2>), grid, wg, 0, st, a);
+    else hipLaunchKernelGGL((lg_k_tree_attn<HD, 4, 1>), grid, wg, 0, st, a);
     if (!t.c.join) return;
     if (a.n_seq > LG_PA_LANES) hipLaunchKernelGGL((lg_k_page_merge<HD, 1, TreeAttn>), dim3(a.H * a.max_tree, a.n_seq), dim3(64), 0, st, a);
     else hipLaunchKernelGGL((lg_k_page_merge<HD, 8, TreeAttn>), dim3(a.H * a.max_tree, a.n_seq), dim3(512), 0, st, a);

@@ -110,16 +110,19 @@ __device__ __forceinline__ MergeRow lg_merge_row(const TreeAttn &a) {
     return { seq, node < w.n ? (long long)w.row0 + node : -1, (long long)a.max_tree * a.H, blockIdx.x, head };
 }
 
-constexpr int lg_tree_per_simd(int hd, int rt) { return rt == 1 && hd <= 256 ? 2 : rt == 2 && hd <= 128 ? 2 : rt == 4 && hd <= 64 ? 2 : 1; }
-template <int HD, int RT>
+// 1 in each half of a pair of binary16 values that is infinite or NaN (all bits of the exponent: one more carries into the sign's place)
+__device__ __forceinline__ uint32_t lg_not_finite(uint32_t u) { return ((u & 0x7C007C00u) + 0x04000400u) >> 15 & 0x00010001u; }
+// How the four wavefronts of a workgroup share its work: WR of them take 16 RT pairs each, the others different keys
+constexpr int lg_tree_per_simd(int hd, int rt) { return hd * rt <= 128 ? 3 : hd * rt <= 256 ? 2 : 1; }
+template <int HD, int RT, int WR>
 __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg_k_tree_attn(TreeAttn a) {
     constexpr int KS = HD / 32;                     // score steps
     constexpr int DL = HD >= 128 ? 8 : HD / 16;     // dimensions of a value load
     constexpr int CH = HD / (16 * DL);              // value loads of a key row
     constexpr int NT = HD / 16;                     // output tiles
-    constexpr int HALVES = HD > 256 ? 1 : 2, TILE = 16 * HALVES, ROWS = 16 * RT;
-    __shared__ float s_m[LG_PA_WAVES][ROWS], s_l[LG_PA_WAVES][ROWS];
-    __shared__ __align__(16) union { lg_h8 q[RT][KS][2][64]; float o[LG_PA_WAVES][16][HD]; } s;
+    constexpr int HALVES = HD > 256 ? 1 : 2, TILE = 16 * HALVES, ROWS = 16 * RT * WR, WK = LG_PA_WAVES / WR;
+    __shared__ float s_m[WK][ROWS], s_l[WK][ROWS], s_top[LG_PA_WAVES][ROWS];
+    __shared__ __align__(16) union { lg_h8 q[RT * WR][KS][2][64]; float o[LG_PA_WAVES][16][HD]; } s;
     __shared__ int32_t s_ids[LG_PA_CHUNK / 16 + 1], s_pos[LG_TREE_ROWS];
     // The groups of one stretch of keys run on one XCD at a time (workgroups are dealt over 8 of them in turn): what the first asks for is in its L2 for the others
     const int line = blockIdx.x >> 3, unit = line / a.groups * 8 + (blockIdx.x & 7), group = line % a.groups;
@@ -131,7 +134,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
     const TreeSeq w = lg_tree_seq(a, seq);
     const int n_pairs = w.n * G, p0 = group * ROWS;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 15, g = lane >> 4;
+    const int c = lane & 15, g = lane >> 4, wr = wave % WR, wk = wave / WR;
     const int chunk = __builtin_amdgcn_readfirstlane(cut.tiles) * LG_PA_TILE, n_split = __builtin_amdgcn_readfirstlane(cut.n);
     auto tell = [&]() {                             // the joining launch
         if (a.pm && a.n_seq <= LG_PA_LANES && kvh == 0 && cut.index == 0 && group == 0 && threadIdx.x == 0) {
@@ -140,28 +143,33 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
         }
     };
     if (p0 >= n_pairs) { tell(); return; }
-    constexpr int STEP = LG_PA_WAVES * TILE;
+    constexpr int STEP = WK * TILE;
     const int32_t *table = a.table + (long long)seq * a.max_blocks;
     const int first = (w.lo & ~(LG_PA_TILE - 1)) + __builtin_amdgcn_readfirstlane(cut.index) * chunk, end = w.len < first + chunk ? w.len : first + chunk;
 
-    // queries: a wavefront takes every fourth 32 dimensions of each 16 pairs
+    // queries: a wavefront takes every fourth 32 dimensions of all pairs
     constexpr int QS = (KS + LG_PA_WAVES - 1) / LG_PA_WAVES;
     const int qw = KS < LG_PA_WAVES ? wave % KS : wave;
-    float4 qv[RT][QS][2];
-    int lo_row[RT];                                 // of pair c: the first position that it sees, and its set
-    lg_u64 set[RT];
+    float4 qv[RT * WR][QS][2];
     #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int p = p0 + rt * 16 + c, q = p < n_pairs ? p : p0, node = q / G, row = w.row0 + node;
-        const float *src = a.q + row * a.q_stride + (long long)(kvh * G + q % G) * HD + g * 8;
+    for (int rt = 0; rt < RT * WR; ++rt) {
+        const int p = p0 + rt * 16 + c, q = p < n_pairs ? p : p0;
+        const float *src = a.q + (w.row0 + q / G) * a.q_stride + (long long)(kvh * G + q % G) * HD + g * 8;
         #pragma unroll
         for (int i = 0; i < QS; ++i)
             #pragma unroll
             for (int j = 0; j < 2; ++j) qv[rt][i][j] = *(const float4 *)(src + (i * LG_PA_WAVES + qw) * 32 + j * 4);
+    }
+    // of pair c of the wavefront's own: the first position that it sees, and its set
+    int lo_row[RT], whole = w.lo;
+    lg_u64 set[RT];
+    #pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int p = p0 + (wr * RT + rt) * 16 + c, row = w.row0 + (p < n_pairs ? p : p0) / G;
         const int pos = a.pos[row];
-        set[rt] = a.mask[row];
+        set[rt] = pos < w.done ? 0 : a.mask[row] & (w.n < 64 ? (1ull << w.n) - 1 : ~0ull);
         lo_row[rt] = pos < w.done ? INT32_MAX : a.window > 0 ? pos - a.window + 1 : INT32_MIN;
-        if (pos < w.done) set[rt] = 0;
+        if (p < n_pairs && lo_row[rt] > whole) whole = lo_row[rt];
     }
     const int b0 = first >> a.g.shift;
     const bool has_id = (int)threadIdx.x <= ((end - 1) >> a.g.shift) - b0;
@@ -179,9 +187,9 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
     };
     float qs[RT];                                   // factor of the raw scores: base-2 exponents
     {
-        float top[RT];
+        float top[RT * WR];
         #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+        for (int rt = 0; rt < RT * WR; ++rt) {
             top[rt] = 0;
             #pragma unroll
             for (int i = 0; i < QS; ++i)
@@ -190,16 +198,19 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
                     top[rt] = fmaxf(top[rt], fmaxf(fmaxf(fabsf(qv[rt][i][j].x), fabsf(qv[rt][i][j].y)), fmaxf(fabsf(qv[rt][i][j].z), fabsf(qv[rt][i][j].w))));
             top[rt] = fmaxf(top[rt], __shfl_xor(top[rt], 16));
             top[rt] = fmaxf(top[rt], __shfl_xor(top[rt], 32));
-            if (lane < 16) s_m[wave][rt * 16 + lane] = top[rt];
+            if (lane < 16) s_top[wave][rt * 16 + lane] = top[rt];
         }
         lg_barrier_lds();
-        #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+        auto power = [&](int row) {                 // top * 2^-e in [2^14, 2^15)
+            float x = 0;
             #pragma unroll
-            for (int v = 0; v < LG_PA_WAVES; ++v) top[rt] = fmaxf(top[rt], s_m[v][rt * 16 + c]);
-            int e = (int)(__float_as_uint(top[rt]) >> 23) - 127 - 14;       // top * 2^-e in [2^14, 2^15)
-            if (e < -100) e = -100;                                         // (zero and tiny rows; 2^-e stays a float)
-            const float up = __uint_as_float((unsigned)(127 - e) << 23);
+            for (int v = 0; v < LG_PA_WAVES; ++v) x = fmaxf(x, s_top[v][row]);
+            const int e = (int)(__float_as_uint(x) >> 23) - 127 - 14;
+            return e < -100 ? -100 : e;             // (zero and tiny rows; 2^-e stays a float)
+        };
+        #pragma unroll
+        for (int rt = 0; rt < RT * WR; ++rt) {
+            const float up = __uint_as_float((unsigned)(127 - power(rt * 16 + c)) << 23);
             #pragma unroll
             for (int i = 0; i < QS; ++i) {
                 const int step = i * LG_PA_WAVES + wave;
@@ -215,17 +226,22 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
                 s.q[rt][step][0][lane] = hi;
                 s.q[rt][step][1][lane] = lo;
             }
-            qs[rt] = a.scale * 1.44269504088896341f * __uint_as_float((unsigned)(127 + e) << 23);
         }
+        #pragma unroll
+        for (int rt = 0; rt < RT; ++rt) qs[rt] = a.scale * 1.44269504088896341f * __uint_as_float((unsigned)(127 + power((wr * RT + rt) * 16 + c)) << 23);
         lg_barrier_lds();
     }
-    // tiles in [whole, w.done) need no mask
-    int whole = w.lo;
-    #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) if (p0 + rt * 16 + c < n_pairs && lo_row[rt] > whole) whole = lo_row[rt];
+    // tiles in [whole, w.done) need no mask; rows of the tree in front of a window are taken out of the sets
     #pragma unroll
     for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(whole, o); if (x > whole) whole = x; }
     whole = __builtin_amdgcn_readfirstlane(whole);
+    if (whole > w.done)
+        #pragma unroll 1
+        for (int k = 0; k < w.n; ++k) {
+            const int pos = s_pos[k];
+            #pragma unroll
+            for (int rt = 0; rt < RT; ++rt) if (pos < lo_row[rt]) set[rt] &= ~(1ull << k);
+        }
 
     lg_h8 kf[HALVES][KS];
     PageTile now;
@@ -237,7 +253,18 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
             for (int i = 0; i < KS; ++i) kf[h][i] = *(const lg_h8 *)(kp + i * 32);
         }
     };
-    int t0 = first + wave * TILE;
+    typedef uint32_t values[CH][4 * HALVES][DL / 2];
+    auto load_values = [&](const PageTile &p, values &v) {
+        #pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
+            #pragma unroll
+            for (int j = 0; j < 4 * HALVES; ++j) {
+                const uint16_t *vp = a.g.v + p.row[j >> 2] + (4 * g + (j & 3)) * a.g.row_stride + ch * 128 + c * DL;
+                if constexpr (DL == 8) { const uint4 u = *(const uint4 *)vp; v[ch][j][0] = u.x; v[ch][j][1] = u.y; v[ch][j][2] = u.z; v[ch][j][3] = u.w; }
+                else { const uint2 u = *(const uint2 *)vp; v[ch][j][0] = u.x; v[ch][j][1] = u.y; }
+            }
+    };
+    int t0 = p0 + wr * RT * 16 < n_pairs ? first + wk * TILE : end;      // (no pairs: nothing to do)
     if (t0 < end) { now = tile_at(t0); load_keys(now); }
     lg_f4 acc[RT][NT];
     float m[RT], l[RT];                             // of pair c; l of this lane's keys alone
@@ -248,24 +275,45 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
         for (int i = 0; i < NT; ++i) acc[rt][i] = (lg_f4){ 0, 0, 0, 0 };
     }
     typedef _Float16 part __attribute__((ext_vector_type(4 * HALVES)));
-    auto product = [](const part &x, const part &y, const lg_f4 &z) {
+    auto product = [&](const part &x, const part &y, const lg_f4 &z) {
         if constexpr (HALVES == 2) return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, z, 0, 0, 0);
         else return __builtin_amdgcn_mfma_f32_16x16x16f16(x, y, z, 0, 0, 0);
     };
 
-    auto work = [&](auto more) {                    // more: a tile follows (a branch around its loads would have them waited for with this tile's)
-        constexpr bool MORE = decltype(more)::value;
-        const PageTile here = now;
-        if constexpr (MORE) now = tile_at(t0 + STEP);
-        uint32_t v[CH][4 * HALVES][DL / 2];
+    auto turned = [&](const values &v, int ch, int i) {          // dimension ch * 128 + c * DL + i of the lane's keys
+        union { uint32_t u[2 * HALVES]; part h; } b;
         #pragma unroll
-        for (int ch = 0; ch < CH; ++ch)
+        for (int k = 0; k < 2 * HALVES; ++k) b.u[k] = __builtin_amdgcn_perm(v[ch][2 * k + 1][i >> 1], v[ch][2 * k][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
+        return b.h;
+    };
+    auto plain = [&](int t, const PageTile &p) { return t >= whole && t + TILE <= w.done && t + TILE <= end && p.ok[0] && p.ok[HALVES - 1]; };
+    // which of the lane's keys pair c sees: four bits for four keys in a row from the committed positions [lo_row, done) and from the set, none behind the end or in a page that is not there
+    auto seen_in = [&](int t0, const PageTile &p, uint32_t (&sees)[RT]) {
+        auto below = [](int x) { return (1u << (x < 0 ? 0 : x > 4 ? 4 : x)) - 1; };
+        #pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sees[rt] = 0;
+        #pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+            const int t = t0 + 16 * h + 4 * g, k = t - w.done;
+            const uint32_t there = p.ok[h] ? below(end - t) : 0u, old = below(-k);
             #pragma unroll
-            for (int j = 0; j < 4 * HALVES; ++j) {
-                const uint16_t *vp = a.g.v + here.row[j >> 2] + (4 * g + (j & 3)) * a.g.row_stride + ch * 128 + c * DL;
-                if constexpr (DL == 8) { const uint4 u = *(const uint4 *)vp; v[ch][j][0] = u.x; v[ch][j][1] = u.y; v[ch][j][2] = u.z; v[ch][j][3] = u.w; }
-                else { const uint2 u = *(const uint2 *)vp; v[ch][j][0] = u.x; v[ch][j][1] = u.y; }
+            for (int rt = 0; rt < RT; ++rt) {
+                const int ahead = lo_row[rt] < t ? 0 : lo_row[rt] > t + 4 ? 4 : lo_row[rt] - t;
+                const uint32_t tree = k <= -4 || k > 63 ? 0u : k < 0 ? (uint32_t)set[rt] << (-k & 3) : (uint32_t)(set[rt] >> (k & 63));
+                sees[rt] |= (((old & ~below(ahead)) | (tree & ~old)) & there & 15u) << (4 * h);
             }
+        }
+    };
+    // One tile: its values are requested before its scores are made, the next tile's keys before its values are used (behind the last tile its own once more: a branch around the
+    // loads would have them waited for with this tile's)
+    uint32_t odd = 0;
+    const int t_first = t0;
+    for (; t0 < end; t0 += STEP) {
+        const bool masked = !plain(t0, now);
+        const PageTile here = now;
+        now = tile_at(t0 + STEP < end ? t0 + STEP : t0);
+        values v;
+        load_values(here, v);
         __builtin_amdgcn_sched_barrier(0);
         lg_f4 sc[RT][HALVES];
         #pragma unroll
@@ -278,42 +326,32 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
             for (int x = 0; x < 2; ++x)
                 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    const lg_h8 q = s.q[rt][i][x][lane];
+                    const lg_h8 q = s.q[wr * RT + rt][i][x][lane];
                     #pragma unroll
                     for (int h = 0; h < HALVES; ++h) sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][i], q, sc[rt][h], 0, 0, 0);
                 }
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (MORE) load_keys(now);
+        load_keys(now);
         __builtin_amdgcn_sched_barrier(0);
-        const bool plain = t0 >= whole && t0 + TILE <= w.done && t0 + TILE <= end && here.ok[0] && here.ok[HALVES - 1];
-        // which of its 4 HALVES keys pair c sees
         uint32_t sees[RT];
-        #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) sees[rt] = (1u << 4 * HALVES) - 1;
-        if (!plain) {
+        if (masked) seen_in(t0, here, sees);
+        else
             #pragma unroll
-            for (int j = 0; j < 4 * HALVES; ++j) {
-                const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3), k = t - w.done;
-                const bool there = here.ok[j >> 2] && t < end;
-                const int key = k < 0 ? t : s_pos[k < LG_TREE_ROWS ? k : LG_TREE_ROWS - 1];
-                #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const bool ok = there && key >= lo_row[rt] && lo_row[rt] != INT32_MAX && (k < 0 || (set[rt] >> (k & 63) & 1));
-                    if (!ok) sees[rt] &= ~(1u << j);
-                }
-            }
-        }
-        float x[RT][4 * HALVES];
-        bool higher = false;
+            for (int rt = 0; rt < RT; ++rt) sees[rt] = 255;
         float top[RT];
+        bool higher = false;
         #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             top[rt] = -INFINITY;
             #pragma unroll
-            for (int j = 0; j < 4 * HALVES; ++j) {
-                x[rt][j] = sees[rt] >> j & 1 ? sc[rt][j >> 2][j & 3] * qs[rt] : -INFINITY;
-                top[rt] = fmaxf(top[rt], x[rt][j]);
-            }
+            for (int h = 0; h < HALVES; ++h)
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = sc[rt][h][r] * qs[rt];
+                    if (!(sees[rt] >> (4 * h + r) & 1)) x = -INFINITY;
+                    sc[rt][h][r] = x;
+                    top[rt] = fmaxf(top[rt], x);
+                }
             top[rt] = fmaxf(top[rt], __shfl_xor(top[rt], 16));
             top[rt] = fmaxf(top[rt], __shfl_xor(top[rt], 32));
             higher |= top[rt] > m[rt];
@@ -338,89 +376,79 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
         for (int rt = 0; rt < RT; ++rt)
             #pragma unroll
             for (int j = 0; j < 4 * HALVES; ++j) {
-                const float p = x[rt][j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[rt][j] - m[rt] + 14.0f);
+                const float x = sc[rt][j >> 2][j & 3], p = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m[rt] + 14.0f);
                 l[rt] += p;
                 hi[rt][j] = (_Float16)p;
                 lo[rt][j] = (_Float16)(p - (float)hi[rt][j]);
             }
-        auto turned = [&](int ch, int i) {          // dimension ch * 128 + c * DL + i of the lane's keys
-            union { uint32_t u[2 * HALVES]; part h; } b;
-            #pragma unroll
-            for (int k = 0; k < 2 * HALVES; ++k) b.u[k] = __builtin_amdgcn_perm(v[ch][2 * k + 1][i >> 1], v[ch][2 * k][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
-            return b.h;
-        };
-        if (!plain) {
-            // keys that no pair of the group can see may hold anything: zeros in their place.  Of the others, values that are not finite
-            auto inf = [](uint32_t u) { return (u & 0x7C00u) == 0x7C00u || (u & 0x7C000000u) == 0x7C000000u; };
-            bool odd = false;
+        if (masked) {
+            // keys that no pair of the group can see may hold anything: zeros in their place.  So are values that are not finite, until all else is done
             #pragma unroll
             for (int j = 0; j < 4 * HALVES; ++j) {
                 const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                const bool there = here.ok[j >> 2] && t >= w.lo && t < end;
+                const uint32_t there = here.ok[j >> 2] && t >= w.lo && t < end ? ~0u : 0u;
                 #pragma unroll
                 for (int ch = 0; ch < CH; ++ch)
                     #pragma unroll
                     for (int i = 0; i < DL / 2; ++i) {
-                        v[ch][j][i] = there ? v[ch][j][i] : 0;
-                        odd |= inf(v[ch][j][i]);
+                        const uint32_t u = v[ch][j][i] & there, x = lg_not_finite(u);
+                        odd |= x;
+                        v[ch][j][i] = u & ~(x * 0xFFFFu);
                     }
-            }
-            if (__any(odd)) {
-                part seen[RT];
-                #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    #pragma unroll
-                    for (int j = 0; j < 4 * HALVES; ++j) seen[rt][j] = sees[rt] >> j & 1 ? (_Float16)1.0f : (_Float16)0.0f;
-                #pragma unroll
-                for (int ch = 0; ch < CH; ++ch)
-                    #pragma unroll
-                    for (int i = 0; i < DL; ++i) {
-                        union { part h; uint16_t u[4 * HALVES]; } b;
-                        b.h = turned(ch, i);
-                        #pragma unroll
-                        for (int j = 0; j < 4 * HALVES; ++j) b.u[j] = (b.u[j] & 0x7C00u) == 0x7C00u ? 0x3C00u : 0u;        // 1 where it is not finite
-                        #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) {
-                            const lg_f4 mark = product(seen[rt], b.h, (lg_f4){ 0, 0, 0, 0 });
-                            #pragma unroll
-                            for (int r = 0; r < 4; ++r) if (mark[r] != 0.0f) acc[rt][ch * DL + i][r] = NAN;
-                        }
-                    }
-                #pragma unroll
-                for (int ch = 0; ch < CH; ++ch)
-                    #pragma unroll
-                    for (int j = 0; j < 4 * HALVES; ++j)
-                        #pragma unroll
-                        for (int i = 0; i < DL / 2; ++i) {
-                            uint32_t &u = v[ch][j][i];
-                            if ((u & 0x7C00u) == 0x7C00u) u &= 0xFFFF0000u;
-                            if ((u & 0x7C000000u) == 0x7C000000u) u &= 0xFFFFu;
-                        }
             }
         }
         #pragma unroll
         for (int ch = 0; ch < CH; ++ch)
             #pragma unroll
             for (int i = 0; i < DL; ++i) {
-                const part b = turned(ch, i);
+                const part b = turned(v, ch, i);
                 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     acc[rt][ch * DL + i] = product(hi[rt], b, acc[rt][ch * DL + i]);
                     acc[rt][ch * DL + i] = product(lo[rt], b, acc[rt][ch * DL + i]);
                 }
             }
-    };
-    for (; t0 + STEP < end; t0 += STEP) work(std::true_type{});
-    if (t0 < end) work(std::false_type{});
+    }
+    // values that are not finite, of tiles that not all pairs see whole: NaN for the pairs that see them, found by a product of their own
+    if (__any(odd != 0))
+        #pragma unroll 1
+        for (t0 = t_first; t0 < end; t0 += STEP) {
+            const PageTile here = tile_at(t0);
+            if (plain(t0, here)) continue;
+            values v;
+            load_values(here, v);
+            uint32_t sees[RT];
+            seen_in(t0, here, sees);
+            part seen[RT];
+            #pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                #pragma unroll
+                for (int j = 0; j < 4 * HALVES; ++j) seen[rt][j] = sees[rt] >> j & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+            #pragma unroll
+            for (int ch = 0; ch < CH; ++ch)
+                #pragma unroll
+                for (int i = 0; i < DL; ++i) {
+                    union { part h; uint32_t u[2 * HALVES]; } b;
+                    b.h = turned(v, ch, i);
+                    #pragma unroll
+                    for (int k = 0; k < 2 * HALVES; ++k) b.u[k] = lg_not_finite(b.u[k]) * 0x3C00u;       // 1 where it is not
+                    #pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const lg_f4 mark = product(seen[rt], b.h, (lg_f4){ 0, 0, 0, 0 });
+                        #pragma unroll
+                        for (int r = 0; r < 4; ++r) if (mark[r] != 0.0f) acc[rt][ch * DL + i][r] = NAN;
+                    }
+                }
+        }
     #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         l[rt] += __shfl_xor(l[rt], 16);
         l[rt] += __shfl_xor(l[rt], 32);
-        if (lane < 16) { s_m[wave][rt * 16 + lane] = m[rt]; s_l[wave][rt * 16 + lane] = l[rt]; }
+        if (lane < 16) { s_m[wk][(wr * RT + rt) * 16 + lane] = m[rt]; s_l[wk][(wr * RT + rt) * 16 + lane] = l[rt]; }
     }
     // (behind the loads: lengths and page ids come through the scalar cache as long as nothing has been stored)
     tell();
-    // the wavefronts' parts, 16 pairs at a time
+    // the parts of wavefronts with different keys, 16 pairs of every WR at a time
     const bool wide = (((uintptr_t)a.out | (uintptr_t)a.out_stride * 4) & 15) == 0;
     #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -434,16 +462,16 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
                     *(float4 *)&s.o[wave][4 * g + r][ch * 128 + c * DL + i] = make_float4(acc[rt][ch * DL + i][r], acc[rt][ch * DL + i + 1][r], acc[rt][ch * DL + i + 2][r], acc[rt][ch * DL + i + 3][r]);
         __syncthreads();
         #pragma unroll 4
-        for (int id = threadIdx.x; id < 16 * (HD / 4); id += LG_PA_WAVES * 64) {
-            const int row = id / (HD / 4), d = id % (HD / 4) * 4, p = p0 + rt * 16 + row;
+        for (int id = threadIdx.x; id < WR * 16 * (HD / 4); id += LG_PA_WAVES * 64) {
+            const int x = id / (HD / 4), d = id % (HD / 4) * 4, r = x / 16, pair = (r * RT + rt) * 16 + x % 16, p = p0 + pair;
             float M = -INFINITY, L = 0;
             float4 o = make_float4(0, 0, 0, 0);
             #pragma unroll
-            for (int u = 0; u < LG_PA_WAVES; ++u) M = fmaxf(M, s_m[u][rt * 16 + row]);
+            for (int u = 0; u < WK; ++u) M = fmaxf(M, s_m[u][pair]);
             #pragma unroll
-            for (int u = 0; u < LG_PA_WAVES; ++u) {
-                const float lv = s_l[u][rt * 16 + row], f = lv == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_m[u][rt * 16 + row] - M);       // (0: no key; a score of NaN leaves its mark in the sum)
-                const float4 y = *(const float4 *)&s.o[u][row][d];
+            for (int u = 0; u < WK; ++u) {
+                const float lv = s_l[u][pair], f = lv == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_m[u][pair] - M);       // (0: no key; a score of NaN leaves its mark in the sum)
+                const float4 y = *(const float4 *)&s.o[u * WR + r][x % 16][d];
                 L += f * lv;
                 o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
             }
