@@ -110,6 +110,10 @@ __device__ __forceinline__ MergeRow lg_merge_row(const TreeAttn &a) {
     return { seq, node < w.n ? (long long)w.row0 + node : -1, (long long)a.max_tree * a.H, blockIdx.x, head };
 }
 
+// Probabilities are 2^(x - m + SHIFT).  m is the largest score of a while ago, rounded up to a whole number (m - SHIFT and factors between two of them are exact): it is taken anew, and the sums so far scaled,
+// only when a score passes it by SLACK, which few tiles of a long row do.  So they stay below 2^15 in binary16, and what their two parts leave of a small one is at most 2^-32 of the largest
+#define LG_TREE_SLACK 7.0f
+#define LG_TREE_SHIFT 8.0f
 // 1 in each half of a pair of binary16 values that is infinite or NaN (all bits of the exponent: one more carries into the sign's place)
 __device__ __forceinline__ uint32_t lg_not_finite(uint32_t u) { return ((u & 0x7C007C00u) + 0x04000400u) >> 15 & 0x00010001u; }
 // How the four wavefronts of a workgroup share its work: WR of them take 16 RT pairs each, the others different keys
@@ -274,6 +278,8 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
         #pragma unroll
         for (int i = 0; i < NT; ++i) acc[rt][i] = (lg_f4){ 0, 0, 0, 0 };
     }
+    typedef _Float16 lg_h2 __attribute__((ext_vector_type(2)));
+    typedef float lg_f2 __attribute__((ext_vector_type(2)));
     typedef _Float16 part __attribute__((ext_vector_type(4 * HALVES)));
     auto product = [&](const part &x, const part &y, const lg_f4 &z) {
         if constexpr (HALVES == 2) return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, z, 0, 0, 0);
@@ -306,12 +312,41 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
     };
     // One tile: its values are requested before its scores are made, the next tile's keys before its values are used (behind the last tile its own once more: a branch around the
     // loads would have them waited for with this tile's)
+    // Outputs of forms that have a SIMD to themselves stay in the accumulation registers: where a product's sum is also read by an ordinary instruction the compiler keeps it in the others, and moves all of
+    // them there and back for each tile
+    constexpr bool ALONE = lg_tree_per_simd(HD, RT) == 1;
+    auto stay = [&]() {
+        if constexpr (ALONE)
+            #pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                #pragma unroll
+                for (int i = 0; i < NT; ++i) asm volatile("" : "+a"(acc[rt][i]));
+    };
+    auto out_of = [&](float x) {
+        if constexpr (!ALONE) return x;
+        float y;
+        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(y) : "a"(x));
+        return y;
+    };
     uint32_t odd = 0;
     const int t_first = t0;
+    stay();
     for (; t0 < end; t0 += STEP) {
         const bool masked = !plain(t0, now);
         const PageTile here = now;
         now = tile_at(t0 + STEP < end ? t0 + STEP : t0);
+        // queries from LDS a few steps ahead of their products
+        constexpr int AT = RT == 1 && KS > 1 ? 2 : 1, GROUPS = KS / AT;
+        lg_h8 q[2][AT][2][RT];
+        auto ask = [&](int i) {
+            #pragma unroll
+            for (int k = 0; k < AT; ++k)
+                #pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    #pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) q[i & 1][k][x][rt] = s.q[wr * RT + rt][i * AT + k][x][lane];
+        };
+        ask(0);
         values v;
         load_values(here, v);
         __builtin_amdgcn_sched_barrier(0);
@@ -321,15 +356,19 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
             #pragma unroll
             for (int h = 0; h < HALVES; ++h) sc[rt][h] = (lg_f4){ 0, 0, 0, 0 };
         #pragma unroll
-        for (int i = 0; i < KS; ++i)
+        for (int i = 0; i < GROUPS; ++i) {
+            if (i + 1 < GROUPS) ask(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
             #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int k = 0; k < AT; ++k)
                 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const lg_h8 q = s.q[wr * RT + rt][i][x][lane];
+                for (int x = 0; x < 2; ++x)
                     #pragma unroll
-                    for (int h = 0; h < HALVES; ++h) sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][i], q, sc[rt][h], 0, 0, 0);
-                }
+                    for (int rt = 0; rt < RT; ++rt)
+                        #pragma unroll
+                        for (int h = 0; h < HALVES; ++h) sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][i * AT + k], q[i & 1][k][x][rt], sc[rt][h], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         __builtin_amdgcn_sched_barrier(0);
         load_keys(now);
         __builtin_amdgcn_sched_barrier(0);
@@ -354,33 +393,43 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
                 }
             top[rt] = fmaxf(top[rt], __shfl_xor(top[rt], 16));
             top[rt] = fmaxf(top[rt], __shfl_xor(top[rt], 32));
-            higher |= top[rt] > m[rt];
+            higher |= top[rt] > m[rt] + LG_TREE_SLACK;
         }
         if (__any(higher)) {
+            if constexpr (ALONE) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");           // (products write accumulation registers up to 16 cycles after they are issued; out_of reads them where the compiler does not see it)
             #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const float mn = fmaxf(m[rt], top[rt]);
+                const float mn = fmaxf(m[rt], ceilf(top[rt]));
                 const float f = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);       // (both -inf: nothing seen yet)
                 l[rt] *= f; m[rt] = mn;
                 float fr[4];
                 #pragma unroll
                 for (int r = 0; r < 4; ++r) fr[r] = __shfl(f, 4 * g + r);
                 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                for (int i = 0; i < NT; ++i) {
                     #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[rt][i][r] *= fr[r];
+                    for (int r = 0; r < 4; ++r) acc[rt][i][r] = fr[r] * out_of(acc[rt][i][r]);
+                }
             }
+            stay();
         }
         part hi[RT], lo[RT];
         #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+        for (int rt = 0; rt < RT; ++rt) {
+            const float under = (m[rt] == -INFINITY ? 0.0f : m[rt]) - LG_TREE_SHIFT;
             #pragma unroll
-            for (int j = 0; j < 4 * HALVES; ++j) {
-                const float x = sc[rt][j >> 2][j & 3], p = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m[rt] + 14.0f);
-                l[rt] += p;
-                hi[rt][j] = (_Float16)p;
-                lo[rt][j] = (_Float16)(p - (float)hi[rt][j]);
+            for (int j = 0; j < 4 * HALVES; j += 2) {
+                lg_f2 p, left;
+                #pragma unroll
+                for (int k = 0; k < 2; ++k) { p[k] = __builtin_amdgcn_exp2f(sc[rt][j >> 2][j + k & 3] - under); l[rt] += p[k]; }
+                const lg_h2 h = __builtin_convertvector(p, lg_h2);
+                #pragma unroll
+                for (int k = 0; k < 2; ++k) left[k] = __builtin_fmaf((float)h[k], -1.0f, p[k]);
+                const lg_h2 u = __builtin_convertvector(left, lg_h2);
+                #pragma unroll
+                for (int k = 0; k < 2; ++k) { hi[rt][j + k] = h[k]; lo[rt][j + k] = u[k]; }
             }
+        }
         if (masked) {
             // keys that no pair of the group can see may hold anything: zeros in their place.  So are values that are not finite, until all else is done
             #pragma unroll
@@ -408,6 +457,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
                     acc[rt][ch * DL + i] = product(lo[rt], b, acc[rt][ch * DL + i]);
                 }
             }
+        stay();
     }
     // values that are not finite, of tiles that not all pairs see whole: NaN for the pairs that see them, found by a product of their own
     if (__any(odd != 0))
