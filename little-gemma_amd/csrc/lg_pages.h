@@ -247,7 +247,7 @@ __device__ __forceinline__ void lg_pa_range(const PageAttn &a, int seq, int &lo,
     if (len < 0) len = 0;
     lo = a.window > 0 && len > a.window ? len - a.window : 0;
 }
-// What follows serves calls of one row a sequence (PageAttn) and of trees (TreeAttn, lg_tree.h): their lg_pa_range and lg_merge_row differ
+// (calls of one row a sequence, PageAttn, and of trees, TreeAttn of lg_tree.h, whose lg_pa_range and lg_merge_row differ)
 template <class A>
 __device__ __forceinline__ int lg_pa_tiles(const A &a, int seq) {
     int lo, len;
@@ -263,8 +263,8 @@ struct PageCut { int tiles; int seq, index, first, n; };       // tiles of a spl
 // them to splits that are full.  Were every sequence's last split a full one, `some` more than total / size would be needed; ragged ones need half as many, and the size
 // for that is tried first (61 sequences of 4..8192 keys, heads of 256: 74.3 -> 72.1 us).  count(t): the splits of size t
 template <class A, typename Count>
-__device__ __forceinline__ uint32_t lg_pa_split_tiles(const A &a, uint32_t total, uint32_t some, Count count) {
-    const uint32_t units = some * a.nkv, half = (uint32_t)a.slots / 2, rounds = units > half ? (units + half - 1) / half : 1, room = rounds * a.slots / a.nkv;
+__device__ __forceinline__ uint32_t lg_pa_split_tiles(const A &a, uint32_t total, uint32_t some, Count count, uint32_t at_least = 1) {
+    const uint32_t units = some * a.nkv, half = (uint32_t)a.slots / 2, own = units > half ? (units + half - 1) / half : 1, rounds = own > at_least ? own : at_least, room = rounds * a.slots / a.nkv;
     auto size = [&](uint32_t spare) {
         const uint32_t full = room > spare ? room - spare : 1, tiles = (total + full - 1) / full;
         return tiles < (uint32_t)a.least ? a.least : tiles > LG_PA_CHUNK / LG_PA_TILE ? LG_PA_CHUNK / LG_PA_TILE : tiles;
@@ -280,8 +280,7 @@ __device__ __forceinline__ uint32_t lg_pa_split_tiles(const A &a, uint32_t total
     return most;
 }
 __device__ __forceinline__ uint32_t lg_pa_splits(uint32_t of, uint32_t tiles) { const uint32_t x = (of + tiles - 1) / tiles; return x ? x : 1u; }
-template <class A>
-__device__ __forceinline__ PageCut lg_pa_cut(const A &a, int at) {
+__device__ __forceinline__ PageCut lg_pa_cut(const PageAttn &a, int at) {
     if (!a.pm) return { a.least, at, 0, at, 1 };
     if (a.n_seq > LG_PA_LANES) {
         const int seq = a.cut[2 + a.n_seq + at];
@@ -302,8 +301,7 @@ __device__ __forceinline__ PageCut lg_pa_cut(const A &a, int at) {
 // The cut of more sequences than a wavefront has lanes, worked out once: in every workgroup it takes several barriers and passes over the
 // lengths.  400 sequences of all lengths up to 1024, heads of 128: 66.8 -> 48.0 us, with the joining launch's workgroups of one wavefront
 #define LG_PC_WG    1024
-template <class A>
-__global__ __launch_bounds__(LG_PC_WG) void lg_k_page_cut(A a) {
+__global__ __launch_bounds__(LG_PC_WG) void lg_k_page_cut(PageAttn a) {
     __shared__ uint32_t part[LG_PC_WG / 64];
     __shared__ int32_t before[LG_PA_SEQS + 1];
     constexpr int PER = LG_PA_SEQS / LG_PC_WG;

@@ -178,7 +178,7 @@ extern "C" int lg_hip_paged_attention(const struct lg_hip_pages *p, const float 
     const PageAttn a{ g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, (float *)w, need ? (float *)(w + part) : nullptr,
                       need ? (float *)(w + 2 * part) : nullptr, scale, need ? (int32_t *)d_work : nullptr, n_head, p->n_head_kv, n_seq, max_blocks, max_len, window, slots_of(hd), c.least };
     hipStream_t st = (hipStream_t)stream;
-    if (c.join && n_seq > LG_PA_LANES) hipLaunchKernelGGL(lg_k_page_cut<PageAttn>, dim3(1), dim3(LG_PC_WG), 0, st, a);
+    if (c.join && n_seq > LG_PA_LANES) hipLaunchKernelGGL(lg_k_page_cut, dim3(1), dim3(LG_PC_WG), 0, st, a);
     switch (hd) {
         case 64:  launch_attn<64>(a, c, st); break;
         case 128: launch_attn<128>(a, c, st); break;
@@ -268,48 +268,58 @@ extern "C" int lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int
     return 0;
 }
 
-// How a workgroup takes pairs: 16 RT by each of WR wavefronts, as many as registers hold of outputs, and no more than a tree has
-struct TreeForm { int rt, wr; };
+// How a workgroup takes pairs: 16 RT by each of WR wavefronts, no more than a tree has
+struct TreeForm { int rt, wr; bool wide; };
 static TreeForm tree_form(int pairs, int hd) {
-    if (pairs <= 16) return { 1, 1 };
-    if (hd == 512) return pairs <= 32 ? TreeForm{ 1, 2 } : TreeForm{ 1, 4 };
-    if (pairs <= 32) return { 2, 1 };
-    return hd == 256 ? TreeForm{ 2, 2 } : TreeForm{ 4, 1 };
+    if (pairs <= 16) return { 1, 1, false };
+    if (pairs <= 32) return hd == 512 ? TreeForm{ 1, 2, false } : TreeForm{ 2, 1, false };
+    return { 1, LG_PA_WAVES, true };
 }
-struct TreeCut { AttnCut c; TreeForm form; int groups, slots; };
-// As cut_of, for workgroups of several pairs: those of one stretch of keys share the chip's room
+#ifndef LG_WIDE_ALONE0
+#define LG_WIDE_ALONE0 8
+#define LG_WIDE_ALONE1 16
+#define LG_WIDE_ALONE2 32
+#endif
+// Trees of up to so many tiles are left whole, as alone_of says for one row
+static int tree_alone_of(int hd, int64_t units, bool wide) {
+    return wide ? (units < 256 ? LG_WIDE_ALONE0 : units < 512 ? LG_WIDE_ALONE1 : LG_WIDE_ALONE2) : alone_of(hd, units);
+}
+struct TreeCut { AttnCut c; int64_t items; TreeForm form; int rows, groups, slots; };
+// As cut_of, for workgroups of several pairs: a split of a tree takes as many as its pairs need, and those are what the chip's room is counted in.  items: workgroups of a key head, at most
 static TreeCut tree_cut_of(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
     const int pairs = max_tree * (n_head / n_head_kv);
     const TreeForm form = tree_form(pairs, hd);
-    const int rows = 16 * form.rt * form.wr, groups = (pairs + rows - 1) / rows, slots = std::max(2, 256 * lg_tree_per_simd(hd, form.rt) / groups);
+    const int rows = 16 * form.rt * form.wr, groups = (pairs + rows - 1) / rows, slots = 256 * (form.wide ? lg_wide_per_simd(hd, form.rt) : lg_tree_per_simd(hd, form.rt));
     // (a tree's rows see a window from the first committed position that its row 0 sees to its last row)
     const int64_t reach = window > 0 ? (int64_t)window + max_tree + LG_PA_TILE : max_len, span = std::min<int64_t>(reach, max_len), tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
-    const int64_t units = (int64_t)n_seq * n_head_kv;
-    const int alone = alone_of(hd, units * groups), min_tiles = tiles <= alone ? alone : 4;
-    const int64_t least = (tiles + min_tiles - 1) / min_tiles, rounds = std::max<int64_t>(1, (units + slots / 2 - 1) / (slots / 2));
-    const int64_t full = std::max<int64_t>(rounds * slots / n_head_kv, n_seq * tiles / (LG_PA_CHUNK / LG_PA_TILE));
-    return { { std::min<int64_t>(n_seq * std::max<int64_t>(least, 1), full + n_seq), n_seq * tiles, least > 1, min_tiles }, form, groups, slots };
+    const int64_t most = LG_PA_CHUNK / LG_PA_TILE, all = (int64_t)n_seq * groups, units = all * n_head_kv;
+    const int alone = tree_alone_of(hd, units, form.wide), min_tiles = tiles <= alone ? alone : 4;
+    const int64_t least = std::max<int64_t>(1, (tiles + min_tiles - 1) / min_tiles), one = std::max<int64_t>(1, slots / n_head_kv * most);
+    const int64_t rounds = std::max<int64_t>({ 1, (units + slots / 2 - 1) / (slots / 2), (all * tiles + one - 1) / one });
+    const int64_t full = std::max<int64_t>(rounds * slots / n_head_kv, all * tiles / most);
+    return { { std::min<int64_t>(n_seq * least, full + n_seq), all * tiles, least > 1, min_tiles }, std::min<int64_t>(all * least, full + all), form, rows, groups, slots };
 }
+static size_t tree_cut_bytes(int n_seq, const TreeCut &t) { return up256(((size_t)n_seq + 1 + (n_seq > LG_PA_LANES ? n_seq + 2 + t.items : 0)) * 4); }
 extern "C" size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
     if (!attn_shape(n_seq, n_head, n_head_kv, hd, max_len) || max_tree < 1 || max_tree > LG_TREE_ROWS || window < 0) return 0;
-    const AttnCut c = tree_cut_of(n_seq, max_tree, n_head, n_head_kv, hd, max_len, window).c;
-    if (!c.join) return 0;
-    const size_t slots = (size_t)c.splits * max_tree * n_head;
-    return cut_bytes(n_seq, c) + 2 * up256(slots * 4) + slots * hd * 4;
+    const TreeCut t = tree_cut_of(n_seq, max_tree, n_head, n_head_kv, hd, max_len, window);
+    if (!t.c.join) return 0;
+    const size_t slots = (size_t)t.c.splits * max_tree * n_head;
+    return tree_cut_bytes(n_seq, t) + 2 * up256(slots * 4) + slots * hd * 4;
 }
 
+#define LG_TREE_FEW 1024
 template <int HD>
 static void launch_tree(const TreeAttn &a, const TreeCut &t, hipStream_t st) {
-    const dim3 grid((unsigned)((a.units + 7) / 8 * 8 * t.groups)), wg(LG_PA_WAVES * 64);
-    if (t.form.rt * t.form.wr == 1) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 1>), grid, wg, 0, st, a);
-    else if constexpr (HD == 512) {
-        if (t.form.wr == 2) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 2>), grid, wg, 0, st, a);
-        else hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 4>), grid, wg, 0, st, a);
-    } else if (t.form.rt * t.form.wr == 2) hipLaunchKernelGGL((lg_k_tree_attn<HD, 2, 1>), grid, wg, 0, st, a);
-    else if constexpr (HD == 256) hipLaunchKernelGGL((lg_k_tree_attn<HD, 2, 2>), grid, wg, 0, st, a);
-    else hipLaunchKernelGGL((lg_k_tree_attn<HD, 4, 1>), grid, wg, 0, st, a);
+    const dim3 grid((unsigned)(((int64_t)a.items * a.nkv + 63) / 64 * 64)), wg(LG_PA_WAVES * 64);
+    if (t.form.wide) {
+        hipLaunchKernelGGL((lg_k_tree_wide<HD, 1>), grid, wg, 0, st, a);
+    } else if (t.form.rt * t.form.wr == 1) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 1>), grid, wg, 0, st, a);
+    else if constexpr (HD == 512) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 2>), grid, wg, 0, st, a);
+    else hipLaunchKernelGGL((lg_k_tree_attn<HD, 2, 1>), grid, wg, 0, st, a);
     if (!t.c.join) return;
-    if (a.n_seq > LG_PA_LANES) hipLaunchKernelGGL((lg_k_page_merge<HD, 1, TreeAttn>), dim3(a.H * a.max_tree, a.n_seq), dim3(64), 0, st, a);
+    // a wavefront to a row's head, or eight where those are few
+    if ((int64_t)a.H * a.max_tree * a.n_seq > LG_TREE_FEW) hipLaunchKernelGGL((lg_k_page_merge<HD, 1, TreeAttn>), dim3(a.H * a.max_tree, a.n_seq), dim3(64), 0, st, a);
     else hipLaunchKernelGGL((lg_k_page_merge<HD, 8, TreeAttn>), dim3(a.H * a.max_tree, a.n_seq), dim3(512), 0, st, a);
 }
 
@@ -333,18 +343,18 @@ extern "C" int lg_hip_paged_tree_attention(const struct lg_hip_pages *p, const f
     const TreeCut t = tree_cut_of(n_seq, max_tree, n_head, p->n_head_kv, hd, max_len, window);
     const AttnCut &c = t.c;
     // (sums over the sequences are 32 bits on the device, and so are a launch's threads)
-    if (c.tiles > INT32_MAX || c.splits * n_head * max_tree > LG_MOST_GROUPS || (int64_t)n_head * max_tree * n_seq > LG_MOST_GROUPS / 2)
+    if (c.tiles > INT32_MAX || t.items * p->n_head_kv > LG_MOST_GROUPS || (int64_t)n_head * max_tree * n_seq > LG_MOST_GROUPS / 2)
         return lg_fail(-2, "paged_tree_attention: %d sequences of up to %d rows of %d heads in %lld splits in one call", n_seq, max_tree, n_head, (long long)c.splits);
     const size_t need = lg_hip_paged_tree_attention_workspace(n_seq, max_tree, n_head, p->n_head_kv, hd, max_len, window);
     if (need && (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)))
         return lg_fail(-2, "paged_tree_attention: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
     const size_t part = up256((size_t)c.splits * max_tree * n_head * 4);
-    char *const w = need ? (char *)d_work + cut_bytes(n_seq, c) : nullptr;
+    char *const w = need ? (char *)d_work + tree_cut_bytes(n_seq, t) : nullptr;
     const TreeAttn a{ { g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, (float *)w, need ? (float *)(w + part) : nullptr, need ? (float *)(w + 2 * part) : nullptr, scale,
                         need ? (int32_t *)d_work : nullptr, n_head, p->n_head_kv, n_seq, max_blocks, max_len, window, t.slots, c.least },
-                      d_start, d_pos, (const lg_u64 *)d_mask, n_rows, max_tree, t.groups, (int)(c.splits * p->n_head_kv) };
+                      d_start, d_pos, (const lg_u64 *)d_mask, n_rows, max_tree, t.groups, t.rows, (int)t.items };
     hipStream_t st = (hipStream_t)stream;
-    if (c.join && n_seq > LG_PA_LANES) hipLaunchKernelGGL(lg_k_page_cut<TreeAttn>, dim3(1), dim3(LG_PC_WG), 0, st, a);
+    if (c.join && n_seq > LG_PA_LANES) hipLaunchKernelGGL(lg_k_tree_cut, dim3(1), dim3(LG_PC_WG), 0, st, a);
     switch (hd) {
         case 64:  launch_tree<64>(a, t, st); break;
         case 128: launch_tree<128>(a, t, st); break;

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(LG_TREE_WG) void lg_k_tree_accept(const int32_t *st
 struct TreeAttn : PageAttn {        // len: with the tree's rows
     const int32_t *start, *pos;
     const lg_u64 *mask;
-    int n_rows, max_tree, groups, units;        // groups of ROWS pairs; stretches of keys: splits x key heads
+    int n_rows, max_tree, groups, rows, items;  // groups of `rows` pairs, at most; workgroups of a key head, at most
 };
 // The keys that rows of a tree see: [lo, len)
 struct TreeSeq { int row0, n, done, lo, len; };
@@ -104,6 +104,79 @@ __device__ __forceinline__ void lg_pa_range(const TreeAttn &a, int seq, int &lo,
     const TreeSeq s = lg_tree_seq(a, seq);
     lo = s.lo; len = s.len;
 }
+// How a call is cut: as lg_pa_cut does it, with a workgroup for each group of a sequence's pairs in each of its splits.  Workgroups are numbered sequence by sequence, split by split.
+__device__ __forceinline__ uint32_t lg_tree_groups(const TreeAttn &a, int seq) {
+    const int n = lg_tree_rows(a.start, seq, a.n_rows, a.max_tree).n * (a.H / a.nkv);
+    return n > a.rows ? (uint32_t)(n + a.rows - 1) / (uint32_t)a.rows : 1u;
+}
+// `total` tiles, each as often as groups read it, of `some` groups.  (A split has LG_PA_CHUNK keys at most: with fewer rounds than are asked for here all splits would be of that size and the last
+// round of workgroups hardly filled.  One sequence of 100003 keys, 32 pairs: 164 -> 150 us)
+template <typename Count>
+__device__ __forceinline__ uint32_t lg_tree_tiles(const TreeAttn &a, uint32_t total, uint32_t some, Count count) {
+    const uint32_t one = (uint32_t)a.slots / a.nkv * (LG_PA_CHUNK / LG_PA_TILE), most = one ? one : 1;
+    return lg_pa_split_tiles(a, total, some, count, (total + most - 1) / most);
+}
+struct TreePart { int tiles, seq, index, first, n, group; };       // as PageCut; the group of pairs
+__device__ __forceinline__ TreePart lg_tree_part(const TreeAttn &a, int item) {
+    if (!a.pm) { const int seq = item / a.groups; return { a.least, seq < a.n_seq ? seq : -1, 0, seq, 1, item % a.groups }; }
+    if (a.n_seq > LG_PA_LANES) {
+        const int32_t *const items = a.cut + a.n_seq + 2;
+        if (item >= items[a.n_seq]) return { 0, -1, 0, 0, 0, 0 };
+        const int seq = items[a.n_seq + 1 + item], first = a.cut[seq], n = a.cut[seq + 1] - first, k = item - items[seq], groups = (items[seq + 1] - items[seq]) / n;
+        return { a.cut[a.n_seq + 1], seq, k / groups, first, n, k % groups };
+    }
+    // a lane for each, in every wavefront: no barrier
+    const int i = threadIdx.x & 63;
+    const uint32_t mine = i < a.n_seq ? lg_pa_tiles(a, i) : 0, by = i < a.n_seq ? lg_tree_groups(a, i) : 0;
+    const uint32_t tiles = lg_tree_tiles(a, lg_wave_total(mine * by), lg_wave_total(mine ? by : 0), [&](uint32_t t) { return lg_wave_total(by * ((mine + t - 1) / t)); });
+    const uint32_t n = i < a.n_seq ? lg_pa_splits(mine, tiles) : 0, first = lg_wave_run(n) - n, run = lg_wave_run(n * by) - n * by;
+    const lg_u64 it = __ballot((uint32_t)item - run < n * by);
+    if (!it) return { (int)tiles, -1, 0, 0, 0, 0 };
+    const int lane = (int)__builtin_ctzll(it), k = item - (int)lg_lane(run, lane), groups = (int)lg_lane(by, lane);
+    return { (int)tiles, lane, k / groups, (int)lg_lane(first, lane), (int)lg_lane(n, lane), k % groups };
+}
+// The cut of more sequences than a wavefront has lanes, worked out once: splits before each sequence and their tiles, workgroups before each sequence and their sequences
+__global__ __launch_bounds__(LG_PC_WG) void lg_k_tree_cut(TreeAttn a) {
+    __shared__ uint32_t part[LG_PC_WG / 64];
+    __shared__ int32_t before[LG_PA_SEQS + 1];
+    constexpr int PER = LG_PA_SEQS / LG_PC_WG;
+    const int per = (a.n_seq + LG_PC_WG - 1) / LG_PC_WG, i0 = threadIdx.x * per;
+    uint32_t x[PER], by[PER], mine = 0, some = 0, all;
+    #pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const bool is = k < per && i0 + k < a.n_seq;
+        x[k] = is ? lg_pa_tiles(a, i0 + k) : 0;
+        by[k] = is ? lg_tree_groups(a, i0 + k) : 0;
+        mine += x[k] * by[k]; some += x[k] ? by[k] : 0;
+    }
+    const uint32_t total = lg_block_sum<LG_PC_WG>(mine, part);
+    some = lg_block_sum<LG_PC_WG>(some, part);
+    const uint32_t tiles = lg_tree_tiles(a, total, some, [&](uint32_t t) {
+        uint32_t n = 0;
+        #pragma unroll
+        for (int k = 0; k < PER; ++k) n += by[k] * ((x[k] + t - 1) / t);
+        return lg_block_sum<LG_PC_WG>(n, part);
+    });
+    uint32_t n = 0, m = 0;
+    #pragma unroll
+    for (int k = 0; k < PER; ++k) if (by[k]) { const uint32_t s = lg_pa_splits(x[k], tiles); n += s; m += s * by[k]; }
+    uint32_t run = lg_block_run<LG_PC_WG>(n, part, &all) - n;
+    if (threadIdx.x == 0) { a.cut[a.n_seq] = (int32_t)all; a.cut[a.n_seq + 1] = (int32_t)tiles; }
+    uint32_t item = lg_block_run<LG_PC_WG>(m, part, &all) - m;
+    int32_t *const items = a.cut + a.n_seq + 2;
+    #pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (by[k]) {
+            a.cut[i0 + k] = (int32_t)run; items[i0 + k] = before[i0 + k] = (int32_t)item;
+            const uint32_t s = lg_pa_splits(x[k], tiles);
+            run += s; item += s * by[k];
+        }
+    if (threadIdx.x == 0) items[a.n_seq] = before[a.n_seq] = (int32_t)all;
+    __syncthreads();
+    for (int s = threadIdx.x; s < (int)all; s += LG_PC_WG) items[a.n_seq + 1 + s] = lg_owner(before, a.n_seq, s);
+}
+// Workgroups are dealt over 8 XCDs in turn; eight in a row of the numbers above go to one, so that the groups of a split, which read the same keys, find them in its L2
+__device__ __forceinline__ int lg_tree_number(int block) { const int y = block >> 3; return ((y >> 3) * 8 + (block & 7)) * 8 + (y & 7); }
 __device__ __forceinline__ MergeRow lg_merge_row(const TreeAttn &a) {
     const int seq = blockIdx.y, node = blockIdx.x / a.H, head = blockIdx.x % a.H;
     const TreeRows w = lg_tree_rows(a.start, seq, a.n_rows, a.max_tree);
@@ -116,6 +189,63 @@ __device__ __forceinline__ MergeRow lg_merge_row(const TreeAttn &a) {
 #define LG_TREE_SHIFT 8.0f
 // 1 in each half of a pair of binary16 values that is infinite or NaN (all bits of the exponent: one more carries into the sign's place)
 __device__ __forceinline__ uint32_t lg_not_finite(uint32_t u) { return ((u & 0x7C007C00u) + 0x04000400u) >> 15 & 0x00010001u; }
+// The largest `whole` of the wavefront's pairs; rows of the tree in front of a pair's window are taken out of its set (which the usual windows, wider than a tree is deep, do not ask for)
+template <int RT>
+__device__ __forceinline__ void lg_tree_trim(const TreeAttn &a, const TreeSeq &w, const int32_t *s_pos, const int (&lo_row)[RT], lg_u64 (&set)[RT], int &whole) {
+    // (rows of 16 lanes by turning them: 0x128, 0x124, 0x122, 0x121 row_ror 8, 4, 2, 1)
+    auto top = [&](int y) { if (y > whole) whole = y; };
+    top(__builtin_amdgcn_mov_dpp(whole, 0x128, 0xF, 0xF, true)); top(__builtin_amdgcn_mov_dpp(whole, 0x124, 0xF, 0xF, true));
+    top(__builtin_amdgcn_mov_dpp(whole, 0x122, 0xF, 0xF, true)); top(__builtin_amdgcn_mov_dpp(whole, 0x121, 0xF, 0xF, true));
+    whole = __builtin_amdgcn_readfirstlane(whole);
+    if (a.window <= 0) return;
+    const int lane = threadIdx.x & 63;
+    // (lg_wave_max is of numbers from 0 up: positions below 0 count as behind every window)
+    const uint32_t before = lane < w.n ? s_pos[lane] < 0 ? 0x80000000u : 0x7FFFFFFFu - (uint32_t)s_pos[lane] : 0u;
+    const uint32_t most = lg_wave_max(before);
+    if (most < 0x80000000u && (int)(0x7FFFFFFFu - most) >= whole) return;
+    #pragma unroll 1
+    for (int k = 0; k < w.n; ++k) {
+        const int pos = s_pos[k];
+        #pragma unroll
+        for (int rt = 0; rt < RT; ++rt) if (pos < lo_row[rt]) set[rt] &= ~(1ull << k);
+    }
+}
+// Four keys in a row from position t on: which of them are committed, which there are at all, and where they are in the tree
+struct LgQuad { uint32_t old, there; int t, k; };
+__device__ __forceinline__ uint32_t lg_below(int x) { return (1u << (x < 0 ? 0 : x > 4 ? 4 : x)) - 1; }
+__device__ __forceinline__ LgQuad lg_tree_quad(int t, int done, int end) { return { lg_below(done - t), lg_below(end - t), t, t - done }; }
+// Those that a pair sees: of the committed ones the ones from lo on, of the tree's the ones of its set
+__device__ __forceinline__ uint32_t lg_tree_sees(const LgQuad &x, int lo, lg_u64 set) {
+    const int ahead = lo < x.t ? 0 : lo > x.t + 4 ? 4 : lo - x.t;
+    const uint32_t tree = x.k <= -4 || x.k > 63 ? 0u : x.k < 0 ? (uint32_t)set << (-x.k & 3) : (uint32_t)(set >> (x.k & 63));
+    return ((x.old & ~lg_below(ahead)) | (tree & ~x.old)) & x.there & 15u;
+}
+// Scores of eight keys (base-2 exponents) -> their probabilities as two binary16 parts, and their sum
+typedef _Float16 lg_h2 __attribute__((ext_vector_type(2)));
+typedef float lg_f2 __attribute__((ext_vector_type(2)));
+template <int HALVES, class Part>
+__device__ __forceinline__ void lg_tree_parts(const lg_f4 (&x)[HALVES], float m, float &l, Part &hi, Part &lo) {
+    const float under = (m == -INFINITY ? 0.0f : m) - LG_TREE_SHIFT;
+    #pragma unroll
+    for (int j = 0; j < 4 * HALVES; j += 2) {
+        lg_f2 p, left;
+        #pragma unroll
+        for (int k = 0; k < 2; ++k) { p[k] = __builtin_amdgcn_exp2f(x[j >> 2][(j + k) & 3] - under); l += p[k]; }
+        const lg_h2 h = __builtin_convertvector(p, lg_h2);
+        #pragma unroll
+        for (int k = 0; k < 2; ++k) left[k] = __builtin_fmaf((float)h[k], -1.0f, p[k]);
+        const lg_h2 u = __builtin_convertvector(left, lg_h2);
+        #pragma unroll
+        for (int k = 0; k < 2; ++k) { hi[j + k] = h[k]; lo[j + k] = u[k]; }
+    }
+}
+// The largest of the four rows of 16 lanes, lane by lane: rows are exchanged between two registers, without LDS
+__device__ __forceinline__ float lg_max_of_rows(float x) {
+    const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1]));
+    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+}
 // How the four wavefronts of a workgroup share its work: WR of them take 16 RT pairs each, the others different keys
 constexpr int lg_tree_per_simd(int hd, int rt) { return hd * rt <= 128 ? 3 : hd * rt <= 256 ? 2 : 1; }
 template <int HD, int RT, int WR>
@@ -128,15 +258,13 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
     __shared__ float s_m[WK][ROWS], s_l[WK][ROWS], s_top[LG_PA_WAVES][ROWS];
     __shared__ __align__(16) union { lg_h8 q[RT * WR][KS][2][64]; float o[LG_PA_WAVES][16][HD]; } s;
     __shared__ int32_t s_ids[LG_PA_CHUNK / 16 + 1], s_pos[LG_TREE_ROWS];
-    // The groups of one stretch of keys run on one XCD at a time (workgroups are dealt over 8 of them in turn): what the first asks for is in its L2 for the others
-    const int line = blockIdx.x >> 3, unit = line / a.groups * 8 + (blockIdx.x & 7), group = line % a.groups;
-    if (unit >= a.units) return;
-    const int kvh = unit % a.nkv, G = a.H / a.nkv, at = unit / a.nkv;
-    const PageCut cut = lg_pa_cut(a, at);
+    const int number = lg_tree_number(blockIdx.x), kvh = number / a.items, G = a.H / a.nkv;
+    if (kvh >= a.nkv) return;
+    const TreePart cut = lg_tree_part(a, number % a.items);
     const int seq = __builtin_amdgcn_readfirstlane(cut.seq);
     if (seq < 0) return;
     const TreeSeq w = lg_tree_seq(a, seq);
-    const int n_pairs = w.n * G, p0 = group * ROWS;
+    const int group = __builtin_amdgcn_readfirstlane(cut.group), at = __builtin_amdgcn_readfirstlane(cut.first + cut.index), n_pairs = w.n * G, p0 = group * ROWS;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4, wr = wave % WR, wk = wave / WR;
     const int chunk = __builtin_amdgcn_readfirstlane(cut.tiles) * LG_PA_TILE, n_split = __builtin_amdgcn_readfirstlane(cut.n);
@@ -236,16 +364,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
         lg_barrier_lds();
     }
     // tiles in [whole, w.done) need no mask; rows of the tree in front of a window are taken out of the sets
-    #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) { const int x = __shfl_xor(whole, o); if (x > whole) whole = x; }
-    whole = __builtin_amdgcn_readfirstlane(whole);
-    if (whole > w.done)
-        #pragma unroll 1
-        for (int k = 0; k < w.n; ++k) {
-            const int pos = s_pos[k];
-            #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) if (pos < lo_row[rt]) set[rt] &= ~(1ull << k);
-        }
+    lg_tree_trim<RT>(a, w, s_pos, lo_row, set, whole);
 
     lg_h8 kf[HALVES][KS];
     PageTile now;
@@ -278,8 +397,6 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
         #pragma unroll
         for (int i = 0; i < NT; ++i) acc[rt][i] = (lg_f4){ 0, 0, 0, 0 };
     }
-    typedef _Float16 lg_h2 __attribute__((ext_vector_type(2)));
-    typedef float lg_f2 __attribute__((ext_vector_type(2)));
     typedef _Float16 part __attribute__((ext_vector_type(4 * HALVES)));
     auto product = [&](const part &x, const part &y, const lg_f4 &z) {
         if constexpr (HALVES == 2) return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, z, 0, 0, 0);
@@ -295,19 +412,13 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
     auto plain = [&](int t, const PageTile &p) { return t >= whole && t + TILE <= w.done && t + TILE <= end && p.ok[0] && p.ok[HALVES - 1]; };
     // which of the lane's keys pair c sees: four bits for four keys in a row from the committed positions [lo_row, done) and from the set, none behind the end or in a page that is not there
     auto seen_in = [&](int t0, const PageTile &p, uint32_t (&sees)[RT]) {
-        auto below = [](int x) { return (1u << (x < 0 ? 0 : x > 4 ? 4 : x)) - 1; };
         #pragma unroll
         for (int rt = 0; rt < RT; ++rt) sees[rt] = 0;
         #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
-            const int t = t0 + 16 * h + 4 * g, k = t - w.done;
-            const uint32_t there = p.ok[h] ? below(end - t) : 0u, old = below(-k);
+            const LgQuad x = lg_tree_quad(t0 + 16 * h + 4 * g, w.done, p.ok[h] ? end : 0);
             #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const int ahead = lo_row[rt] < t ? 0 : lo_row[rt] > t + 4 ? 4 : lo_row[rt] - t;
-                const uint32_t tree = k <= -4 || k > 63 ? 0u : k < 0 ? (uint32_t)set[rt] << (-k & 3) : (uint32_t)(set[rt] >> (k & 63));
-                sees[rt] |= (((old & ~below(ahead)) | (tree & ~old)) & there & 15u) << (4 * h);
-            }
+            for (int rt = 0; rt < RT; ++rt) sees[rt] |= lg_tree_sees(x, lo_row[rt], set[rt]) << (4 * h);
         }
     };
     // One tile: its values are requested before its scores are made, the next tile's keys before its values are used (behind the last tile its own once more: a branch around the
@@ -415,21 +526,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
         }
         part hi[RT], lo[RT];
         #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const float under = (m[rt] == -INFINITY ? 0.0f : m[rt]) - LG_TREE_SHIFT;
-            #pragma unroll
-            for (int j = 0; j < 4 * HALVES; j += 2) {
-                lg_f2 p, left;
-                #pragma unroll
-                for (int k = 0; k < 2; ++k) { p[k] = __builtin_amdgcn_exp2f(sc[rt][j >> 2][j + k & 3] - under); l[rt] += p[k]; }
-                const lg_h2 h = __builtin_convertvector(p, lg_h2);
-                #pragma unroll
-                for (int k = 0; k < 2; ++k) left[k] = __builtin_fmaf((float)h[k], -1.0f, p[k]);
-                const lg_h2 u = __builtin_convertvector(left, lg_h2);
-                #pragma unroll
-                for (int k = 0; k < 2; ++k) { hi[rt][j + k] = h[k]; lo[rt][j + k] = u[k]; }
-            }
-        }
+        for (int rt = 0; rt < RT; ++rt) lg_tree_parts(sc[rt], m[rt], l[rt], hi[rt], lo[rt]);
         if (masked) {
             // keys that no pair of the group can see may hold anything: zeros in their place.  So are values that are not finite, until all else is done
             #pragma unroll
@@ -538,5 +635,339 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
                 if (d == 0) { a.pm[place] = M; a.pl[place] = L; }
             }
         }
+    }
+}
+
+// The same for more than 32 pairs: their wavefronts share keys and values through LDS.  From memory to registers each of them would ask for the same rows again, and rows of keys as operands are asked for
+// in 16 pieces of 64 bytes, for which the memory pipeline takes four times as long as for whole rows; here a tile of 32 keys and values goes to LDS once, by loads that pass no
+// register, while the tile before is worked on.  Queries stay in registers: a wavefront takes 16 RT pairs, and all keys, so that nothing is joined in the end.
+// A row's 16-byte pieces lie in LDS in an order of the row's own (piece j ^ swap), so that reads of a column of 16 rows touch all banks.
+constexpr int lg_wide_per_simd(int hd, int rt) { return hd * rt <= 256 ? 2 : 1; }
+__device__ __forceinline__ void lg_to_lds(const void *from, uint32_t to) {         // 16 bytes of each lane, one after another from byte `to` on
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to), "v"(from) : "memory");
+}
+template <int HD, int RT>
+__global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg_k_tree_wide(TreeAttn a) {
+    constexpr int KS = HD / 32;                     // score steps
+    constexpr int NT = HD / 16;                     // output tiles
+    constexpr int TILE = LG_PA_TILE, ROWS = 16 * RT * LG_PA_WAVES;
+    constexpr int PIECES = HD / 8, AT_ONCE = 64 / PIECES, LOADS = TILE / AT_ONCE / LG_PA_WAVES;      // 16-byte pieces of a row; rows of a load; loads of a wavefront for a tile's keys, and for its values
+    __shared__ __align__(16) uint16_t s_kv[2][2][TILE * HD];
+    __shared__ int32_t s_pos[LG_TREE_ROWS];
+    const int number = lg_tree_number(blockIdx.x), kvh = number / a.items, G = a.H / a.nkv;
+    if (kvh >= a.nkv) return;
+    const TreePart cut = lg_tree_part(a, number % a.items);
+    const int seq = __builtin_amdgcn_readfirstlane(cut.seq);
+    if (seq < 0) return;
+    const TreeSeq w = lg_tree_seq(a, seq);
+    const int group = __builtin_amdgcn_readfirstlane(cut.group), at = __builtin_amdgcn_readfirstlane(cut.first + cut.index), n_pairs = w.n * G, p0 = group * ROWS;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int chunk = __builtin_amdgcn_readfirstlane(cut.tiles) * LG_PA_TILE, n_split = __builtin_amdgcn_readfirstlane(cut.n);
+    auto tell = [&]() {                             // the joining launch
+        if (a.pm && a.n_seq <= LG_PA_LANES && kvh == 0 && cut.index == 0 && group == 0 && threadIdx.x == 0) {
+            a.cut[seq] = cut.first;
+            if (seq == a.n_seq - 1) a.cut[a.n_seq] = cut.first + cut.n;
+        }
+    };
+    if (p0 >= n_pairs) { tell(); return; }
+    const int32_t *table = a.table + (long long)seq * a.max_blocks;
+    const int first = (w.lo & ~(LG_PA_TILE - 1)) + __builtin_amdgcn_readfirstlane(cut.index) * chunk, end = w.len < first + chunk ? w.len : first + chunk;
+    const int b0 = first >> a.g.shift;
+    // page ids of the stretch, a lane each
+    static_assert(LG_PA_CHUNK / 16 + 1 <= 192, "in three registers");
+    auto id_of = [&](int i) { return i <= ((end - 1) >> a.g.shift) - b0 && b0 + i < a.max_blocks ? table[b0 + i] : -1; };
+    const int ids0 = id_of(lane), ids1 = id_of(64 + lane), ids2 = id_of(128 + lane);
+    auto tile_at = [&](int t) {
+        PageIds p;
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int i = ((t + 16 * h < end ? t + 16 * h : t) >> a.g.shift) - b0;             // (a half behind the end is masked)
+            const int x = __builtin_amdgcn_readlane(ids0, i & 63), y = __builtin_amdgcn_readlane(ids1, i & 63), z = __builtin_amdgcn_readlane(ids2, i & 63);
+            p.id[h] = i < 64 ? x : i < 128 ? y : z;
+        }
+        return lg_pa_tile(a, p, t, kvh * HD);
+    };
+
+    auto swap = [](int row) { return HD == 64 ? row >> 1 & 7 : row & 15; };
+    // of a load: the lane's row and piece; the first row is a multiple of AT_ONCE, so that swap(first ^ row) = swap(first) ^ swap(row)
+    const long long to_row = lane / PIECES * a.g.row_stride * 2;
+    const uint32_t piece = ((lane % PIECES) ^ swap(lane / PIECES)) * 16;
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&s_kv[0][0][0];
+    auto fetch = [&](const PageTile &p, int buffer) {
+        #pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int row0 = (wave * LOADS + i) * AT_ONCE;
+            const long long from = to_row + (piece ^ (uint32_t)(swap(row0) * 16)), at = ((row0 < 16 ? p.row[0] : p.row[1]) + (row0 & 15) * a.g.row_stride) * 2;
+            const uint32_t to = lds + (uint32_t)((buffer * 2 * TILE + row0) * HD * 2);
+            lg_to_lds((const char *)a.g.k + at + from, to);
+            lg_to_lds((const char *)a.g.v + at + from, to + TILE * HD * 2);
+        }
+    };
+    PageTile now;
+    if (first < end) { now = tile_at(first); fetch(now, 0); }
+    if ((int)threadIdx.x < w.n) s_pos[threadIdx.x] = a.pos[w.row0 + threadIdx.x];
+
+    // queries of the wavefront's pairs, as operands
+    lg_h8 q[RT][KS][2];
+    float qs[RT];                                   // factor of the raw scores: base-2 exponents
+    int lo_row[RT], whole = w.lo;                   // of pair c: the first position that it sees, and its set
+    lg_u64 set[RT];
+    #pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int p = p0 + (wave * RT + rt) * 16 + c, x = p < n_pairs ? p : p0, row = w.row0 + x / G;
+        const float *src = a.q + row * a.q_stride + (long long)(kvh * G + x % G) * HD + g * 8;
+        float4 v[KS][2];
+        #pragma unroll
+        for (int i = 0; i < KS; ++i)
+            #pragma unroll
+            for (int j = 0; j < 2; ++j) v[i][j] = *(const float4 *)(src + i * 32 + j * 4);
+        const int pos = a.pos[row];
+        set[rt] = pos < w.done ? 0 : a.mask[row] & (w.n < 64 ? (1ull << w.n) - 1 : ~0ull);
+        lo_row[rt] = pos < w.done ? INT32_MAX : a.window > 0 ? pos - a.window + 1 : INT32_MIN;
+        if (p < n_pairs && lo_row[rt] > whole) whole = lo_row[rt];
+        float top = 0;
+        #pragma unroll
+        for (int i = 0; i < KS; ++i)
+            #pragma unroll
+            for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fmaxf(fabsf(v[i][j].x), fabsf(v[i][j].y)), fmaxf(fabsf(v[i][j].z), fabsf(v[i][j].w))));
+        top = lg_max_of_rows(top);
+        int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;         // top * 2^-e in [2^14, 2^15)
+        if (e < -100) e = -100;                                       // (zero and tiny rows; 2^-e stays a float)
+        const float up = __uint_as_float((unsigned)(127 - e) << 23);
+        #pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            const float y[8] = { v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w, v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w };
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float z = y[j] * up;
+                q[rt][i][0][j] = (_Float16)z;
+                q[rt][i][1][j] = (_Float16)(z - (float)q[rt][i][0][j]);
+            }
+        }
+        qs[rt] = a.scale * 1.44269504088896341f * __uint_as_float((unsigned)(127 + e) << 23);
+    }
+    lg_barrier_lds();                               // (positions)
+    // tiles in [whole, w.done) need no mask; rows of the tree in front of a window are taken out of the sets
+    lg_tree_trim<RT>(a, w, s_pos, lo_row, set, whole);
+
+    const bool busy = p0 + wave * RT * 16 < n_pairs;          // (a wavefront without pairs only fetches)
+    lg_f4 acc[RT][NT];
+    float m[RT], l[RT];                             // of pair c; l of this lane's keys alone
+    auto clear = [&]() {
+        #pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            m[rt] = -INFINITY; l[rt] = 0;
+            #pragma unroll
+            for (int i = 0; i < NT; ++i) acc[rt][i] = (lg_f4){ 0, 0, 0, 0 };
+        }
+    };
+    auto plain = [&](int t, const PageTile &p) { return t >= whole && t + TILE <= w.done && t + TILE <= end && p.ok[0] && p.ok[1]; };
+    auto seen_in = [&](int t0, const PageTile &p, uint32_t (&sees)[RT]) {
+        #pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sees[rt] = 0;
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const LgQuad x = lg_tree_quad(t0 + 16 * h + 4 * g, w.done, p.ok[h] ? end : 0);
+            #pragma unroll
+            for (int rt = 0; rt < RT; ++rt) sees[rt] |= lg_tree_sees(x, lo_row[rt], set[rt]) << (4 * h);
+        }
+    };
+    // where a lane reads, in values: its piece of a key row differs from that of the step before by a piece's place, of those 4 (2) steps before by a whole number of rounds
+    constexpr int KEY_AT = KS < 4 ? KS : 4;
+    int at_key[KEY_AT];
+    #pragma unroll
+    for (int i = 0; i < KEY_AT; ++i) at_key[i] = c * HD + ((4 * i + g) ^ swap(c)) * 8;
+    // Values of 16 dimensions: sixteen lanes give the places of four values each of four keys' rows, and get four keys of one dimension each (ds_read_b64_tr_b16).  A round of places takes VAL_AT tiles
+    constexpr int VAL_AT = HD == 64 ? 4 : 8;
+    int at_val[VAL_AT];
+    #pragma unroll
+    for (int i = 0; i < VAL_AT; ++i) { const int row = 4 * g + (c >> 2); at_val[i] = row * HD + ((2 * i + (c >> 1 & 1)) ^ swap(row)) * 8 + (c & 1) * 4; }
+    typedef short lg_s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) lg_s4 lds_s4;
+    union operand { lg_s4 s[2]; uint32_t u[4]; lg_h8 h; };
+    // A value that is infinite or NaN reaches rows that do not see it as 0 * inf: found in the end, by sums that are not finite, and then all is done again with such values taken out of the products and marked by
+    // products of their own
+    auto run = [&](auto safe) {
+    constexpr bool SAFE = decltype(safe)::value;
+    clear();
+    int buffer = 0;
+    for (int t0 = first; t0 < end; t0 += TILE, buffer ^= 1) {
+        // this tile has arrived, and every wavefront has done with the one before
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const PageTile here = now;
+        if (t0 + TILE < end) { now = tile_at(t0 + TILE); fetch(now, buffer ^ 1); }
+        if (!busy) continue;
+        const uint16_t *const keys = s_kv[buffer][0], *const vals = s_kv[buffer][1];
+        lg_f4 sc[RT][2];
+        #pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = (lg_f4){ 0, 0, 0, 0 };
+        constexpr int DEEP = KS < 3 || RT > 1 ? 2 : 3;      // key operands on their way
+        lg_h8 kf[DEEP][2];
+        auto ask = [&](int i) {
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) kf[i % DEEP][h] = *(const lg_h8 *)(keys + at_key[i % KEY_AT] + (i / KEY_AT) * KEY_AT * 32 + h * 16 * HD);
+        };
+        #pragma unroll
+        for (int i = 0; i < DEEP - 1; ++i) ask(i);
+        #pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            if (i + DEEP - 1 < KS) ask(i + DEEP - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            #pragma unroll
+            for (int x = 0; x < 2; ++x)
+                #pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    #pragma unroll
+                    for (int h = 0; h < 2; ++h) sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i % DEEP][h], q[rt][i][x], sc[rt][h], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        operand b[2][4];
+        auto ask_values = [&](int n) {              // four tiles of 16 dimensions
+            #pragma unroll
+            for (int i = 0; i < 4; ++i)
+                #pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int tile = 4 * n + i;
+                    b[n & 1][i].s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vals + at_val[tile % VAL_AT] + tile / VAL_AT * VAL_AT * 16 + h * 16 * HD));
+                }
+        };
+        ask_values(0);
+        __builtin_amdgcn_sched_barrier(0);
+        const bool masked = !plain(t0, here);
+        #pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) sc[rt][h] *= qs[rt];
+        uint32_t sees[RT];
+        if (masked) {
+            seen_in(t0, here, sees);
+            #pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) if (!(sees[rt] >> j & 1)) sc[rt][j >> 2][j & 3] = -INFINITY;
+        }
+        float top[RT];
+        bool higher = false;
+        #pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            top[rt] = -INFINITY;
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) top[rt] = fmaxf(top[rt], sc[rt][j >> 2][j & 3]);
+            top[rt] = lg_max_of_rows(top[rt]);
+            higher |= top[rt] > m[rt] + LG_TREE_SLACK;
+        }
+        if (__any(higher)) {
+            #pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float mn = fmaxf(m[rt], ceilf(top[rt]));
+                const float f = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);       // (both -inf: nothing seen yet)
+                l[rt] *= f; m[rt] = mn;
+                float fr[4];
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) fr[r] = __shfl(f, 4 * g + r);
+                #pragma unroll
+                for (int i = 0; i < NT; ++i)
+                    #pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[rt][i][r] *= fr[r];
+            }
+        }
+        lg_h8 hi[RT], lo[RT];
+        #pragma unroll
+        for (int rt = 0; rt < RT; ++rt) lg_tree_parts(sc[rt], m[rt], l[rt], hi[rt], lo[rt]);
+        // keys that are not there may hold anything: zeros in their place
+        const bool partly = t0 < w.lo || t0 + TILE > end || !here.ok[0] || !here.ok[1];
+        uint32_t there[4];
+        if (partly)
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {           // keys 4 g + 2 (k % 2) and the next of half k / 2
+                const int t = t0 + 16 * (k >> 1) + 4 * g + 2 * (k & 1);
+                there[k] = !here.ok[k >> 1] ? 0u : (t >= w.lo && t < end ? 0xFFFFu : 0u) | (t + 1 >= w.lo && t + 1 < end ? 0xFFFF0000u : 0u);
+            }
+        #pragma unroll
+        for (int n = 0; n < NT / 4; ++n) {          // (four sums in turn: a product waits for the one before it into the same sum)
+            if (n + 1 < NT / 4) ask_values(n + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            operand (&v)[4] = b[n & 1];
+            if (partly)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) v[i].u[k] &= there[k];
+            if (SAFE && masked)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    operand odd;
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t x = lg_not_finite(v[i].u[k]);
+                        v[i].u[k] &= ~(x * 0xFFFFu);
+                        odd.u[k] = x * 0x3C00u;                   // 1 where it is not finite
+                    }
+                    #pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        lg_h8 seen;
+                        #pragma unroll
+                        for (int j = 0; j < 8; ++j) seen[j] = sees[rt] >> j & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+                        const lg_f4 mark = __builtin_amdgcn_mfma_f32_16x16x32_f16(seen, odd.h, (lg_f4){ 0, 0, 0, 0 }, 0, 0, 0);
+                        #pragma unroll
+                        for (int r = 0; r < 4; ++r) if (mark[r] != 0.0f) acc[rt][4 * n + i][r] = NAN;
+                    }
+                }
+            #pragma unroll
+            for (int x = 0; x < 2; ++x)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    #pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) acc[rt][4 * n + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x ? lo[rt] : hi[rt], v[i].h, acc[rt][4 * n + i], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    };
+    run(std::false_type{});
+    float finite = 0;                               // or NaN
+    #pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+        #pragma unroll
+        for (int n = 0; n < NT; ++n)
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) finite = __builtin_fmaf(acc[rt][n][r], 0.0f, finite);
+    if (__syncthreads_or(finite != 0.0f)) {
+        now = tile_at(first);
+        fetch(now, 0);
+        run(std::true_type{});
+    }
+    tell();
+    __syncthreads();                                // (the last tile's readers)
+    if (!busy) return;
+    float total = l[0];
+    total += __shfl_xor(total, 16);
+    total += __shfl_xor(total, 32);
+    // outputs turned in LDS, each wavefront by itself, for stores of 16 bytes: 16 pairs of 64 dimensions at a time, 4 floats between rows
+    float *const turn = (float *)&s_kv[0][0][0] + wave * 16 * 68;
+    const bool aligned = n_split > 1 || (((uintptr_t)a.out | (uintptr_t)a.out_stride * 4) & 15) == 0;
+    #pragma unroll
+    for (int n = 0; n < NT; n += 4) {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i)
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) turn[(4 * g + r) * 68 + i * 16 + c] = acc[0][n + i][r];
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int pair = 4 * k + g, p = p0 + wave * 16 + pair;
+            float4 y = *(const float4 *)(turn + pair * 68 + c * 4);
+            const float L = __shfl(total, pair), by = n_split > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+            y.x *= by; y.y *= by; y.z *= by; y.w *= by;
+            if (p >= n_pairs) continue;
+            const int node = p / G, head = kvh * G + p % G;
+            float *const to = (n_split == 1 ? a.out + (w.row0 + node) * a.out_stride + (long long)head * HD : a.pacc + (((long long)at * a.max_tree + node) * a.H + head) * HD) + n * 16 + c * 4;
+            if (aligned) *(float4 *)to = y;
+            else { to[0] = y.x; to[1] = y.y; to[2] = y.z; to[3] = y.w; }
+        }
+    }
+    const int p = p0 + wave * 16 + lane;
+    if (n_split > 1 && lane < 16 && p < n_pairs) {
+        const long long place = ((long long)at * a.max_tree + p / G) * a.H + kvh * G + p % G;
+        a.pm[place] = m[0]; a.pl[place] = total;
     }
 }
