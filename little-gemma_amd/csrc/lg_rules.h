@@ -5,7 +5,7 @@
 
 #define LG_RULES_VOCAB 524288
 #define LG_RULES_WG 256
-#define LG_RULES_SLICE 8192         // tokens of a workgroup: their counts lie in LDS
+#define LG_RULES_SLICE 8192         // tokens of a workgroup at most: their counts lie in LDS
 
 struct RulesPenalty { float repetition, presence, frequency; int32_t prompt; };       // struct lg_hip_penalty
 struct RulesArgs {
@@ -20,16 +20,26 @@ struct RulesArgs {
     int rows, n_vocab, n_seq, n_bias, n_allow;
 };
 
-// A workgroup takes LG_RULES_SLICE tokens of one row's vocabulary.  It asks for their logits, goes over the whole text of the row's sequence and counts its own tokens in LDS (whole numbers:
+// A workgroup takes SLICE tokens of one row's vocabulary.  It asks for their logits, goes over the whole text of the row's sequence and counts its own tokens in LDS (whole numbers:
 // the order does not matter), then writes the slice.  Bound by memory where rows are many: 8 bytes a logit; a text is read once for every slice of every row, but from the L2.
 // Logits that a rule changes are computed in 64 bits and rounded once.
-template <bool VEC>
+template <bool VEC, int SLICE>
 __global__ __launch_bounds__(LG_RULES_WG) void lg_k_rules(RulesArgs a) {
     extern __shared__ uint32_t s_word[];            // [SLICE] counts: bit 31 a token of the text, below it how often it was generated; [SLICE] 1 + the bias of a token, where there are any
     constexpr uint32_t SEEN = 1u << 31;
-    constexpr int EACH = LG_RULES_SLICE / (4 * LG_RULES_WG);
-    const int t = threadIdx.x, row = blockIdx.y, base = blockIdx.x * LG_RULES_SLICE;
-    const int size = a.n_vocab - base < LG_RULES_SLICE ? a.n_vocab - base : LG_RULES_SLICE;
+    constexpr int EACH = SLICE / (4 * LG_RULES_WG);
+    const int t = threadIdx.x, row = blockIdx.y, base = blockIdx.x * SLICE;
+    const int size = a.n_vocab - base < SLICE ? a.n_vocab - base : SLICE;
+    // (logits first: what is asked for later arrives later)
+    const float *in = a.logits + row * a.stride + base;
+    float *out = a.out + row * a.out_stride + base;
+    float4 x[EACH];
+    #pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const int i = (k * LG_RULES_WG + t) * 4;
+        if (VEC && i + 4 <= size) x[k] = *(const float4 *)(in + i);
+        else { float *v = (float *)&x[k]; for (int j = 0; j < 4; ++j) v[j] = i + j < size ? in[i + j] : 0.0f; }
+    }
     const int s = a.seq ? a.seq[row] : row;
     const bool named = s >= 0 && s < a.n_seq;
     RulesPenalty p = { 1.0f, 0.0f, 0.0f, 0 };
@@ -47,17 +57,8 @@ __global__ __launch_bounds__(LG_RULES_WG) void lg_k_rules(RulesArgs a) {
     const bool biased = b1 > b0;
     const int grammar = a.n_allow ? a.allow_row ? a.allow_row[row] : row : -1;
     const uint32_t *allow = grammar >= 0 && grammar < a.n_allow ? a.allow + grammar * a.allow_stride : nullptr;
-    const float *in = a.logits + row * a.stride + base;
-    float *out = a.out + row * a.out_stride + base;
     if (in == out && !text && !biased && !allow) return;
-    float4 x[EACH];
-    #pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-        const int i = (k * LG_RULES_WG + t) * 4;
-        if (VEC && i + 4 <= size) x[k] = *(const float4 *)(in + i);
-        else { float *v = (float *)&x[k]; for (int j = 0; j < 4; ++j) v[j] = i + j < size ? in[i + j] : 0.0f; }
-    }
-    uint32_t *const s_bias = s_word + LG_RULES_SLICE;
+    uint32_t *const s_bias = s_word + SLICE;
     if (text || biased) {
         #pragma unroll
         for (int k = 0; k < EACH; ++k) {

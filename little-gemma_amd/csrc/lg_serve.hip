@@ -366,6 +366,7 @@ extern "C" int lg_hip_paged_tree_attention(const struct lg_hip_pages *p, const f
 }
 
 // ---- shared pages -----------------------------------------------------------------------------------------------
+#define LG_FORK_FEW 4096
 static size_t fork_page_bytes(int n_pages) { return up256((size_t)n_pages * sizeof(ForkPage)); }
 static bool fork_shape(int n_seq, int n_pages, int max_blocks) {
     // (entries of the table are counted in 31 bits)
@@ -389,7 +390,8 @@ extern "C" int lg_hip_paged_fork(int n_seq, int page_size, int n_pages, int max_
     if (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)) return lg_fail(-2, "paged_fork: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
     const ForkArgs a{ d_src, d_len_old, d_len_new, d_table, d_shares, d_free, d_n_free, d_from, d_to, d_rows, d_status, (ForkPage *)d_work, (int32_t *)((char *)d_work + fork_page_bytes(n_pages)),
                       n_seq, shift, n_pages, max_blocks };
-    hipLaunchKernelGGL(lg_k_page_fork<1024>, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
+    if (n_seq <= 64 && (int64_t)n_seq * max_blocks <= LG_FORK_FEW) hipLaunchKernelGGL(lg_k_page_fork<256>, dim3(1), dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL(lg_k_page_fork<1024>, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
     LG_TRY(hipGetLastError());
     return 0;
 }
@@ -431,8 +433,8 @@ extern "C" int lg_hip_paged_compact(const struct lg_hip_pages *layers, int n_lay
     if (n_seq == 0) return 0;
     if (!d_table || !d_len || !d_start || !d_path || !d_count) return lg_fail(-1, "paged_compact: null argument");
     each_layers(layers, n_layers, [&](const PageLayers &ls, int n, int most) {
-        hipLaunchKernelGGL(lg_k_page_compact, dim3((unsigned)(2 * most + 255) / 256, (unsigned)n, (unsigned)n_seq), dim3(256), 0, (hipStream_t)stream, ls, d_table, d_len, d_start, d_path, d_count,
-                           max_tree, max_blocks, shift_of(layers->page_size), layers->n_pages);
+        hipLaunchKernelGGL(lg_k_page_compact, dim3((unsigned)(2 * most + LG_MOVE_PLACES - 1) / LG_MOVE_PLACES, (unsigned)n, (unsigned)n_seq), dim3(256), 0, (hipStream_t)stream, ls, d_table, d_len, d_start,
+                           d_path, d_count, max_tree, max_blocks, shift_of(layers->page_size), layers->n_pages);
     });
     LG_TRY(hipGetLastError());
     return 0;
@@ -455,6 +457,18 @@ extern "C" int lg_hip_paged_copy(const struct lg_hip_pages *layers, int n_layers
 }
 
 // ---- rules ------------------------------------------------------------------------------------------------------
+#define LG_RULES_FEW (1 << 21)
+template <bool VEC, int SLICE>
+static void launch_rules_of(const RulesArgs &a, hipStream_t st) {
+    const unsigned lds = SLICE * 4 * (a.bias_start ? 2 : a.penalty ? 1 : 0);
+    hipLaunchKernelGGL((lg_k_rules<VEC, SLICE>), dim3((unsigned)((a.n_vocab + SLICE - 1) / SLICE), (unsigned)a.rows), dim3(LG_RULES_WG), lds, st, a);
+}
+template <bool VEC>
+static void launch_rules(const RulesArgs &a, hipStream_t st) {
+    if ((int64_t)a.rows * a.n_vocab <= LG_RULES_FEW) launch_rules_of<VEC, LG_RULES_SLICE / 4>(a, st);
+    else if (a.bias_start) launch_rules_of<VEC, LG_RULES_SLICE / 2>(a, st);
+    else launch_rules_of<VEC, LG_RULES_SLICE>(a, st);
+}
 extern "C" int lg_hip_adjust_logits(const struct lg_hip_logit_rules *r, const float *d_logits, int64_t stride, int rows, int n_vocab, float *d_out, int64_t out_stride, void *stream) {
     if (!r) return lg_fail(-1, "adjust_logits: null argument");
     if (rows < 0 || rows > 65535) return lg_fail(-2, "adjust_logits: %d rows (0..65535)", rows);
@@ -472,10 +486,8 @@ extern "C" int lg_hip_adjust_logits(const struct lg_hip_logit_rules *r, const fl
     const RulesArgs a{ d_logits, (long long)stride, d_out, (long long)out_stride, r->seq, (const RulesPenalty *)r->penalty, r->hist, r->hist_len, (long long)r->hist_stride,
                        (const lg_u64 *)r->tree_mask, r->tree_start, r->tree_tok, r->n_bias ? r->bias_start : nullptr, r->bias_tok, r->bias, r->allow, r->allow_row, (long long)r->allow_stride,
                        rows, n_vocab, r->n_seq, r->n_bias, r->n_allow };
-    const dim3 grid((unsigned)((n_vocab + LG_RULES_SLICE - 1) / LG_RULES_SLICE), (unsigned)rows);
-    const unsigned lds = LG_RULES_SLICE * 4 * (r->n_bias ? 2 : r->penalty ? 1 : 0);
-    if (aligned16(d_logits) && aligned16(d_out) && stride % 4 == 0 && out_stride % 4 == 0) hipLaunchKernelGGL(lg_k_rules<true>, grid, dim3(LG_RULES_WG), lds, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(lg_k_rules<false>, grid, dim3(LG_RULES_WG), lds, (hipStream_t)stream, a);
+    if (aligned16(d_logits) && aligned16(d_out) && stride % 4 == 0 && out_stride % 4 == 0) launch_rules<true>(a, (hipStream_t)stream);
+    else launch_rules<false>(a, (hipStream_t)stream);
     LG_TRY(hipGetLastError());
     return 0;
 }

@@ -160,9 +160,12 @@ __global__ __launch_bounds__(NT) void lg_k_page_fork(ForkArgs a) {
 struct PageLayer { uint16_t *k, *v; long long row_stride, page_stride; int units; };          // units: 8 values, 16 bytes
 struct PageLayers { PageLayer l[LG_LAYERS]; };
 
-// The rows of an accepted path to the places behind the committed ones.  Rows only move down and in order (path[k] > path[k - 1]), so a thread that takes 16 bytes of them all, eight
-// at a time, has read every row before it is written over.  Bound by memory: 2 bytes read and 2 written a value.
+// The rows of an accepted path to the places behind the committed ones.  Rows only move down and in order (path[k] > path[k - 1]), so a thread that takes 16 bytes of them all, up to eight
+// at a time, has read every row before it is written over.  Bound by memory: 2 bytes read and 2 written a value; where the rows lie is a chain of lengths, path and pages ahead of that, which is why
+// a workgroup takes keys and values of a layer together, two places of 16 bytes a thread.
+typedef uint32_t lg_u4 __attribute__((ext_vector_type(4)));          // (arrays of HIP's own uint4 end up in scratch memory)
 #define LG_MOVE_AT_ONCE 8
+#define LG_MOVE_PLACES  512         // of a workgroup
 __global__ __launch_bounds__(256) void lg_k_page_compact(PageLayers ls, const int32_t *table, const int32_t *len, const int32_t *start, const int32_t *path, const int32_t *count, int max_tree,
                                                         int max_blocks, int shift, int n_pages) {
     __shared__ long long s_src[64], s_dst[64];
@@ -172,8 +175,8 @@ __global__ __launch_bounds__(256) void lg_k_page_compact(PageLayers ls, const in
     if (lane < 64) {
         const int total = len[seq], kept = count[seq];
         const long long n = (long long)start[seq + 1] - start[seq];
-        const bool fits = n >= 1 && n <= max_tree && total >= n && total <= (long long)max_blocks << shift;
         const int mine = lane < max_tree ? path[(long long)seq * max_tree + lane] : -1;
+        const bool fits = n >= 1 && n <= max_tree && total >= n && total <= (long long)max_blocks << shift;
         const int before = __shfl(mine, lane ? lane - 1 : 0);
         const bool ok = fits && lane < kept && mine >= 0 && mine < n && (lane == 0 || mine > before);
         const lg_u64 not_ok = ~__ballot(ok);
@@ -193,15 +196,32 @@ __global__ __launch_bounds__(256) void lg_k_page_compact(PageLayers ls, const in
         if (lane == 0) s_n = __popcll(all);
     }
     __syncthreads();
-    const int u = (int)(blockIdx.x * 256 + threadIdx.x), n = s_n;
-    if (u >= 2 * L.units) return;
-    uint16_t *const at = (u < L.units ? L.k : L.v) + (u < L.units ? u : u - L.units) * 8;
+    const int n = s_n, u0 = (int)(blockIdx.x * LG_MOVE_PLACES + threadIdx.x), u1 = u0 + LG_MOVE_PLACES / 2;
+    if (u0 >= 2 * L.units) return;
+    const bool both = u1 < 2 * L.units;
+    auto place = [&](int u) { return (u < L.units ? L.k : L.v) + (u < L.units ? u : u - L.units) * 8; };
+    uint16_t *const p0 = place(u0), *const p1 = place(both ? u1 : u0);
+    auto move = [&](auto most, int k0) {            // (behind the last one the last again: no branch between loads)
+        constexpr int N = decltype(most)::value;
+        lg_u4 x[N], y[N];
+        #pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const long long at = s_src[k0 + k < n ? k0 + k : n - 1];
+            x[k] = *(const lg_u4 *)(p0 + at);
+            y[k] = *(const lg_u4 *)(p1 + at);
+        }
+        #pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k0 + k < n) {
+                const long long at = s_dst[k0 + k];
+                *(lg_u4 *)(p0 + at) = x[k];
+                if (both) *(lg_u4 *)(p1 + at) = y[k];
+            }
+    };
     for (int k0 = 0; k0 < n; k0 += LG_MOVE_AT_ONCE) {
-        uint4 x[LG_MOVE_AT_ONCE];
-        #pragma unroll
-        for (int k = 0; k < LG_MOVE_AT_ONCE; ++k) x[k] = *(const uint4 *)(at + s_src[k0 + k < n ? k0 + k : n - 1]);       // (no branch between loads)
-        #pragma unroll
-        for (int k = 0; k < LG_MOVE_AT_ONCE; ++k) if (k0 + k < n) *(uint4 *)(at + s_dst[k0 + k]) = x[k];
+        if (n - k0 > 4) move(std::integral_constant<int, LG_MOVE_AT_ONCE>{}, k0);
+        else if (n - k0 > 2) move(std::integral_constant<int, 4>{}, k0);
+        else move(std::integral_constant<int, 2>{}, k0);
     }
 }
 // The first rows[i] rows of page from[i] to page to[i]: a workgroup takes every `parts`-th 4096 bytes of K or V of one pair in one layer.  Bound by memory, as above.
