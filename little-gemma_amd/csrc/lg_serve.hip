@@ -275,14 +275,12 @@ static TreeForm tree_form(int pairs, int hd) {
     if (pairs <= 32) return hd == 512 ? TreeForm{ 1, 2, false } : TreeForm{ 2, 1, false };
     return { 1, LG_PA_WAVES, true };
 }
-#ifndef LG_WIDE_ALONE0
-#define LG_WIDE_ALONE0 8
-#define LG_WIDE_ALONE1 16
-#define LG_WIDE_ALONE2 32
-#endif
-// Trees of up to so many tiles are left whole, as alone_of says for one row
+// Trees of up to so many tiles are left whole, as alone_of says for one row.  A workgroup of 64 pairs spends 10 us beside its tiles, of 1.5 us each, and the joining launch takes 8.  Whole and in splits, us, heads of
+// 256: 2 units (sequences x key heads x groups) of 512 keys 31.6 and 19.3, 16 units 33.9 and 23.2; 128 units of 144 keys 17.6 and 29.4, of 272 24.6 and 30.3, of 528 35.7 and 34.9 (all of
+// these lengths up to it: 36.7 and 33.2); 256 of 272 26.7 and 47.7, of 528 39.6 and 55.6; 512 of 528 65.1 and 114.8
 static int tree_alone_of(int hd, int64_t units, bool wide) {
-    return wide ? (units < 256 ? LG_WIDE_ALONE0 : units < 512 ? LG_WIDE_ALONE1 : LG_WIDE_ALONE2) : alone_of(hd, units);
+    if (!wide) return alone_of(hd, units);
+    return units < 64 ? 8 : units < 256 ? 16 : units < 512 ? 24 : 32;
 }
 struct TreeCut { AttnCut c; int64_t items; TreeForm form; int rows, groups, slots; };
 // As cut_of, for workgroups of several pairs: a split of a tree takes as many as its pairs need, and those are what the chip's room is counted in.  items: workgroups of a key head, at most
@@ -318,7 +316,7 @@ static void launch_tree(const TreeAttn &a, const TreeCut &t, hipStream_t st) {
     else if constexpr (HD == 512) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 2>), grid, wg, 0, st, a);
     else hipLaunchKernelGGL((lg_k_tree_attn<HD, 2, 1>), grid, wg, 0, st, a);
     if (!t.c.join) return;
-    // a wavefront to a row's head, or eight where those are few
+    // a wavefront to a row's head, or eight where those are few (24 sequences with trees of 64: 8.2 and 30 us; one of 100003 keys with 16 rows: 29 and 7.3)
     if ((int64_t)a.H * a.max_tree * a.n_seq > LG_TREE_FEW) hipLaunchKernelGGL((lg_k_page_merge<HD, 1, TreeAttn>), dim3(a.H * a.max_tree, a.n_seq), dim3(64), 0, st, a);
     else hipLaunchKernelGGL((lg_k_page_merge<HD, 8, TreeAttn>), dim3(a.H * a.max_tree, a.n_seq), dim3(512), 0, st, a);
 }
@@ -366,11 +364,12 @@ extern "C" int lg_hip_paged_tree_attention(const struct lg_hip_pages *p, const f
 }
 
 // ---- shared pages -----------------------------------------------------------------------------------------------
-#define LG_FORK_FEW 4096
+// A workgroup of four wavefronts where the table has a few entries: its barriers are shorter.  Eight forks of 16 pages and their end: 23.0 us, with 1024 threads 24.7; 15 of 250 pages 87 and 42
+#define LG_FORK_FEW 16
 static size_t fork_page_bytes(int n_pages) { return up256((size_t)n_pages * sizeof(ForkPage)); }
 static bool fork_shape(int n_seq, int n_pages, int max_blocks) {
     // (entries of the table are counted in 31 bits)
-    return n_seq >= 0 && n_seq <= LG_PLAN_SEQS && n_pages >= 1 && max_blocks >= 1 && (int64_t)n_seq * max_blocks < INT32_MAX;
+    return n_seq >= 0 && n_seq <= LG_PLAN_SEQS && n_pages >= 1 && max_blocks >= 1 && (int64_t)n_seq * max_blocks <= 1 << 30;
 }
 extern "C" size_t lg_hip_paged_fork_workspace(int n_seq, int n_pages, int max_blocks) {
     if (!fork_shape(n_seq, n_pages, max_blocks)) return 0;
@@ -390,8 +389,8 @@ extern "C" int lg_hip_paged_fork(int n_seq, int page_size, int n_pages, int max_
     if (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)) return lg_fail(-2, "paged_fork: %zu bytes of working memory (aligned to 256), given %zu", need, d_work ? work_bytes : 0);
     const ForkArgs a{ d_src, d_len_old, d_len_new, d_table, d_shares, d_free, d_n_free, d_from, d_to, d_rows, d_status, (ForkPage *)d_work, (int32_t *)((char *)d_work + fork_page_bytes(n_pages)),
                       n_seq, shift, n_pages, max_blocks };
-    if (n_seq <= 64 && (int64_t)n_seq * max_blocks <= LG_FORK_FEW) hipLaunchKernelGGL(lg_k_page_fork<256>, dim3(1), dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(lg_k_page_fork<1024>, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
+    if (n_seq <= LG_FORK_FEW && (int64_t)n_seq * max_blocks <= 1024) hipLaunchKernelGGL((lg_k_page_fork<256, LG_FORK_FEW>), dim3(1), dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((lg_k_page_fork<1024, LG_PLAN_SEQS>), dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
     LG_TRY(hipGetLastError());
     return 0;
 }

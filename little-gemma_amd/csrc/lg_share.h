@@ -23,91 +23,107 @@ struct ForkArgs {
 // stack, each at its first release (sequence by sequence, block by block), the first one topmost.  Of the rows that end inside a page one may keep it if no row holds it whole: the first that had it, or
 // else the first; each of the others takes a page off the stack, in order, and is told what to copy.
 // All or nothing: everything is read and counted in working memory, then everything is written.
-// One workgroup: a few words for every page that moves.  Each pass over them is a search in LDS and a round trip or two.
-template <int NT>
+// One workgroup, of NT threads: a few words for every page that moves, its time a chain of round trips to memory (lengths, ids, shares; counts; places; stores).  A thread keeps its first release, arrival and
+// row in registers, so that a call of up to NT of each asks for them once: eight forks of 16 pages 9.7 -> 6.3 us.
+template <int NT, int SEQS>
 __global__ __launch_bounds__(NT) void lg_k_page_fork(ForkArgs a) {
-    __shared__ int32_t gone[LG_PLAN_SEQS + 1], come[LG_PLAN_SEQS + 1], fresh[LG_PLAN_SEQS];      // releases and arrivals before each row; which of the new pages it takes, -1 none
+    __shared__ int32_t gone[SEQS + 1], come[SEQS + 1], fresh[SEQS];      // releases and arrivals before each row; which of the new pages it takes, -1 none
+    __shared__ int32_t s_src[SEQS], s_old[SEQS], s_new[SEQS];
     __shared__ lg_u64 part[3 * NT / 64];
     __shared__ int32_t bad, wrong_page;
     const int t = threadIdx.x, P = 1 << a.shift, n = a.n_seq;
     const long long most = (long long)a.max_blocks << a.shift;
-    const int per = (n + NT - 1) / NT, i0 = t * per, i1 = i0 + per < n ? i0 + per : n;
+    const int per = (n + NT - 1) / NT, i0 = t * per < n ? t * per : n, i1 = i0 + per < n ? i0 + per : n;
     const int nf = *a.n_free;
     if (t == 0) { bad = nf < 0 || nf > a.n_pages ? LG_FORK_BAD_STACK : 0; wrong_page = 0; }
+    for (int i = t; i < n; i += NT) { s_src[i] = a.src[i]; s_old[i] = a.len_old[i]; s_new[i] = a.len_new[i]; }
+    __syncthreads();
     auto blocks = [&](int len) { return (int)(((long long)len + P - 1) >> a.shift); };
     auto place = [&](int i, int block) { return a.table + (size_t)i * a.max_blocks + block; };
     auto outside = [&](int id) { return id < 0 || id >= a.n_pages; };
-    auto holders = [&](int id) { return __hip_atomic_load(&a.page[id].holders, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    auto now = [&](const int32_t &x) { return __hip_atomic_load(&x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     lg_u64 run[3] = { 0, 0, 0 }, all[3];
     int st = 0;
     for (int i = i0; i < i1; ++i) {
-        const int s = a.src[i], lo = a.len_old[i], ln = a.len_new[i];
-        const bool named = s >= 0 && s < n;
+        const int s = s_src[i], lo = s_old[i], ln = s_new[i];
         if (s < -1 || s >= n) st |= LG_FORK_BAD_SOURCE;
-        else if (ln > (named ? a.len_old[s] : 0)) st |= LG_FORK_BAD_LEN;
+        else if (ln > (s >= 0 ? s_old[s] : 0)) st |= LG_FORK_BAD_LEN;
         if (lo < 0 || lo > most || ln < 0) st |= LG_FORK_BAD_LEN;
         if (st) break;
         gone[i] = (int)run[0]; come[i] = (int)run[1];
         run[0] += s != i ? blocks(lo) : blocks(lo) - blocks(ln);
         run[1] += s != i ? blocks(ln) : 0;
     }
-    lg_block_run3<NT>(run, all, part);                        // (run: exclusive now.  A barrier in here also shows `bad`)
     if (st) atomicOr(&bad, st);
-    __syncthreads();
+    lg_block_run3<NT>(run, all, part);                        // (run: exclusive now; its barriers also show `bad`)
     st = bad;
     const int n_gone = st ? 0 : (int)all[0], n_come = st ? 0 : (int)all[1];
     if (!st) for (int i = i0; i < i1; ++i) { gone[i] += (int)run[0]; come[i] += (int)run[1]; }
     if (t == 0) { gone[n] = n_gone; come[n] = n_come; }
     __syncthreads();
-    auto leaves = [&](int i, int e) { const int b = e - gone[i]; return a.src[i] != i ? b : blocks(a.len_new[i]) + b; };        // the block of release e
+    auto leaves = [&](int i, int e) { const int b = e - gone[i]; return s_src[i] != i ? b : blocks(s_new[i]) + b; };            // the block of release e
+    auto ends = [&](int i) { return s_src[i] >= 0 && (s_new[i] & (P - 1)); };
+    auto ends_in = [&](int i) { return place(s_src[i], s_new[i] >> a.shift); };
+    auto key = [&](int i) { return (s_src[i] != i ? LG_PLAN_SEQS : 0) + i; };
+    // the thread's first of each
+    const bool has_g = t < n_gone, has_c = t < n_come, has_r = !st && i0 < i1 && ends(i0);
+    const int gi = has_g ? lg_owner(gone, n, t) : 0, ci = has_c ? lg_owner(come, n, t) : 0;
+    const int g_id = has_g ? *place(gi, leaves(gi, t)) : -1, c_id = has_c ? *place(s_src[ci], t - come[ci]) : -1, r_id = has_r ? *ends_in(i0) : -1;
+    auto gone_of = [&](int e) { return e == t ? gi : lg_owner(gone, n, e); };
+    auto come_of = [&](int e) { return e == t ? ci : lg_owner(come, n, e); };
+    auto gone_id = [&](int e, int i) { return e == t ? g_id : *place(i, leaves(i, e)); };
+    auto come_id = [&](int e) { return e == t ? c_id : a.stage[e]; };
+    auto end_id = [&](int i) { return i == i0 ? r_id : ends(i) ? *ends_in(i) : -1; };
     // every page that the call touches: its holders before
-    auto touch = [&](int id) {
-        if (outside(id)) { atomicOr(&wrong_page, LG_FORK_BAD_PAGE); return; }
-        const int h = a.shares[id];
-        if (h < 0 || h >= LG_PLAN_SEQS) { atomicOr(&wrong_page, LG_FORK_BAD_SHARES); return; }
-        a.page[id] = ForkPage{ h + 1, INT32_MAX, 0, INT32_MAX };
+    auto touch = [&](int id, int shares) {
+        if (outside(id)) atomicOr(&wrong_page, LG_FORK_BAD_PAGE);
+        else if (shares < 0 || shares >= LG_PLAN_SEQS) atomicOr(&wrong_page, LG_FORK_BAD_SHARES);
+        else a.page[id] = ForkPage{ shares + 1, INT32_MAX, 0, INT32_MAX };
     };
-    auto ends_in = [&](int i) { const int s = a.src[i], ln = a.len_new[i]; return s >= 0 && (ln & (P - 1)) ? *place(s, ln >> a.shift) : -1; };
+    auto shares_of = [&](int id) { return outside(id) ? 0 : a.shares[id]; };
     if (!st) {
-        for (int e = t; e < n_gone; e += NT) { const int i = lg_owner(gone, n, e); touch(*place(i, leaves(i, e))); }
-        for (int e = t; e < n_come; e += NT) { const int i = lg_owner(come, n, e), id = *place(a.src[i], e - come[i]); a.stage[e] = id; touch(id); }
-        for (int i = i0; i < i1; ++i) if (a.src[i] >= 0 && (a.len_new[i] & (P - 1))) touch(ends_in(i));
+        const int sg = shares_of(g_id), sc = shares_of(c_id), sr = shares_of(r_id);
+        if (has_g) touch(g_id, sg);
+        if (has_c) touch(c_id, sc);
+        if (has_r) touch(r_id, sr);
+        for (int e = t + NT; e < n_gone; e += NT) { const int i = lg_owner(gone, n, e), id = *place(i, leaves(i, e)); touch(id, shares_of(id)); }
+        for (int e = t + NT; e < n_come; e += NT) { const int i = lg_owner(come, n, e), id = *place(s_src[i], e - come[i]); a.stage[e] = id; touch(id, shares_of(id)); }
+        for (int i = i0 + 1; i < i1; ++i) if (ends(i)) { const int id = *ends_in(i); touch(id, shares_of(id)); }
         __syncthreads();
         st = wrong_page;
     }
     int F = 0, N = 0, top = nf;
     if (!st) {
         for (int e = t; e < n_gone; e += NT) {
-            const int i = lg_owner(gone, n, e), id = *place(i, leaves(i, e));
+            const int id = gone_id(e, gone_of(e));
             atomicAdd(&a.page[id].holders, -1);
             atomicMin(&a.page[id].first, e);
         }
-        for (int e = t; e < n_come; e += NT) atomicAdd(&a.page[a.stage[e]].holders, 1);
+        for (int e = t; e < n_come; e += NT) atomicAdd(&a.page[come_id(e)].holders, 1);
         for (int i = i0; i < i1; ++i) {
-            const int id = ends_in(i);
-            if (id >= 0) { atomicAdd(&a.page[id].parts, 1); atomicMin(&a.page[id].keeper, (a.src[i] != i ? LG_PLAN_SEQS : 0) + i); }
+            const int id = end_id(i);
+            if (id >= 0) { atomicAdd(&a.page[id].parts, 1); atomicMin(&a.page[id].keeper, key(i)); }
         }
         __syncthreads();
         // releases in a row to a thread, as their places on the stack follow each other
         const int each = (n_gone + NT - 1) / NT, e0 = t * each < n_gone ? t * each : n_gone, e1 = e0 + each < n_gone ? e0 + each : n_gone;
         auto releases = [&](auto &&f) {
-            for (int e = e0, i = e0 < e1 ? lg_owner(gone, n, e0) : 0; e < e1; ++e) {
+            for (int e = e0, i = e0 < e1 ? gone_of(e0) : 0; e < e1; ++e) {
                 while (gone[i + 1] <= e) ++i;
-                const int id = *place(i, leaves(i, e));
-                if (holders(id) < 0) atomicOr(&wrong_page, LG_FORK_BAD_SHARES);
-                if (holders(id) == 0 && __hip_atomic_load(&a.page[id].first, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == e) f(id);
+                const int id = gone_id(e, i), h = now(a.page[id].holders), first = now(a.page[id].first);
+                if (h < 0) atomicOr(&wrong_page, LG_FORK_BAD_SHARES);
+                if (h == 0 && first == e) f(id);
             }
         };
         run[0] = run[1] = run[2] = 0;
         releases([&](int) { ++run[0]; });
         for (int i = i0; i < i1; ++i) {
-            const int id = ends_in(i);
+            const int id = end_id(i);
             bool copies = false;
             if (id >= 0) {
-                const int h = holders(id), p = __hip_atomic_load(&a.page[id].parts, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
-                          k = __hip_atomic_load(&a.page[id].keeper, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const int h = now(a.page[id].holders), p = now(a.page[id].parts), k = now(a.page[id].keeper);
                 if (p > h) atomicOr(&wrong_page, LG_FORK_BAD_SHARES);
-                copies = p != h || k != (a.src[i] != i ? LG_PLAN_SEQS : 0) + i;
+                copies = p != h || k != key(i);
             }
             fresh[i] = copies ? (int)run[1] : -1;
             run[1] += copies;
@@ -125,29 +141,29 @@ __global__ __launch_bounds__(NT) void lg_k_page_fork(ForkArgs a) {
         if (!st) {
             // counts and the stack first, while the table is as it was
             auto count = [&](int id) {
-                const int h = holders(id), p = __hip_atomic_load(&a.page[id].parts, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), left = h - (p && p == h ? p - 1 : p);
+                const int h = now(a.page[id].holders), p = now(a.page[id].parts), left = h - (p && p == h ? p - 1 : p);
                 a.shares[id] = left > 0 ? left - 1 : 0;
             };
             int at = top - 1 - (int)run[0];
             releases([&](int id) { a.stack[at--] = id; });
-            for (int e = t; e < n_gone; e += NT) { const int i = lg_owner(gone, n, e); count(*place(i, leaves(i, e))); }
-            for (int e = t; e < n_come; e += NT) count(a.stage[e]);
+            for (int e = t; e < n_gone; e += NT) count(gone_id(e, gone_of(e)));
+            for (int e = t; e < n_come; e += NT) count(come_id(e));
             for (int i = i0; i < i1; ++i) {
-                const int id = ends_in(i);
+                const int id = end_id(i);
                 if (id >= 0) count(id);
                 a.from[i] = fresh[i] >= 0 ? id : -1;
-                a.rows[i] = fresh[i] >= 0 ? a.len_new[i] & (P - 1) : 0;
+                a.rows[i] = fresh[i] >= 0 ? s_new[i] & (P - 1) : 0;
             }
             __syncthreads();
-            for (int e = t; e < n_gone; e += NT) { const int i = lg_owner(gone, n, e), b = leaves(i, e); if (b >= blocks(a.len_new[i])) *place(i, b) = -1; }
+            for (int e = t; e < n_gone; e += NT) { const int i = gone_of(e), b = leaves(i, e); if (b >= blocks(s_new[i])) *place(i, b) = -1; }
             for (int e = t; e < n_come; e += NT) {
-                const int i = lg_owner(come, n, e), b = e - come[i];
-                if (!(fresh[i] >= 0 && b == a.len_new[i] >> a.shift)) *place(i, b) = a.stage[e];
+                const int i = come_of(e), b = e - come[i];
+                if (!(fresh[i] >= 0 && b == s_new[i] >> a.shift)) *place(i, b) = come_id(e);
             }
             for (int i = i0; i < i1; ++i) {
-                const int id = fresh[i] >= 0 ? a.stack[top - 1 - fresh[i]] : -1;
+                const int id = fresh[i] >= 0 ? now(a.stack[top - 1 - fresh[i]]) : -1;
                 a.to[i] = id;
-                if (id >= 0) { *place(i, a.len_new[i] >> a.shift) = id; a.shares[id] = 0; }
+                if (id >= 0) { *place(i, s_new[i] >> a.shift) = id; a.shares[id] = 0; }
             }
         }
     }

@@ -946,24 +946,31 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
     // outputs turned in LDS, each wavefront by itself, for stores of 16 bytes: 16 pairs of 64 dimensions at a time, 4 floats between rows
     float *const turn = (float *)&s_kv[0][0][0] + wave * 16 * 68;
     const bool aligned = n_split > 1 || (((uintptr_t)a.out | (uintptr_t)a.out_stride * 4) & 15) == 0;
+    float *to[4], by[4];                            // of pairs 4 k + g
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int p = p0 + wave * 16 + 4 * k + g, node = p / G, head = kvh * G + p - node * G;
+        const float L = __shfl(total, 4 * k + g);
+        to[k] = p >= n_pairs ? nullptr : (n_split == 1 ? a.out + (w.row0 + node) * a.out_stride + (long long)head * HD : a.pacc + (((long long)at * a.max_tree + node) * a.H + head) * HD) + c * 4;
+        by[k] = n_split > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+    }
     #pragma unroll
     for (int n = 0; n < NT; n += 4) {
         #pragma unroll
         for (int i = 0; i < 4; ++i)
             #pragma unroll
             for (int r = 0; r < 4; ++r) turn[(4 * g + r) * 68 + i * 16 + c] = acc[0][n + i][r];
+        lg_f4 y[4];
         #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int pair = 4 * k + g, p = p0 + wave * 16 + pair;
-            float4 y = *(const float4 *)(turn + pair * 68 + c * 4);
-            const float L = __shfl(total, pair), by = n_split > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
-            y.x *= by; y.y *= by; y.z *= by; y.w *= by;
-            if (p >= n_pairs) continue;
-            const int node = p / G, head = kvh * G + p % G;
-            float *const to = (n_split == 1 ? a.out + (w.row0 + node) * a.out_stride + (long long)head * HD : a.pacc + (((long long)at * a.max_tree + node) * a.H + head) * HD) + n * 16 + c * 4;
-            if (aligned) *(float4 *)to = y;
-            else { to[0] = y.x; to[1] = y.y; to[2] = y.z; to[3] = y.w; }
-        }
+        for (int k = 0; k < 4; ++k) y[k] = *(const lg_f4 *)(turn + (4 * k + g) * 68 + c * 4) * by[k];
+        #pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (to[k]) {
+                if (aligned) *(lg_f4 *)(to[k] + n * 16) = y[k];
+                else
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) to[k][n * 16 + i] = y[k][i];
+            }
     }
     const int p = p0 + wave * 16 + lane;
     if (n_split > 1 && lane < 16 && p < n_pairs) {
