@@ -263,11 +263,11 @@ struct PageCut { int tiles; int seq, index, first, n; };       // tiles of a spl
 // them to splits that are full.  Were every sequence's last split a full one, `some` more than total / size would be needed; ragged ones need half as many, and the size
 // for that is tried first (61 sequences of 4..8192 keys, heads of 256: 74.3 -> 72.1 us).  count(t): the splits of size t
 template <class A, typename Count>
-__device__ __forceinline__ uint32_t lg_pa_split_tiles(const A &a, uint32_t total, uint32_t some, Count count, uint32_t at_least = 1) {
+__device__ __forceinline__ uint32_t lg_pa_split_tiles(const A &a, uint32_t total, uint32_t some, Count count, uint32_t at_least = 1, uint32_t longest = LG_PA_CHUNK / LG_PA_TILE) {
     const uint32_t units = some * a.nkv, half = (uint32_t)a.slots / 2, own = units > half ? (units + half - 1) / half : 1, rounds = own > at_least ? own : at_least, room = rounds * a.slots / a.nkv;
     auto size = [&](uint32_t spare) {
         const uint32_t full = room > spare ? room - spare : 1, tiles = (total + full - 1) / full;
-        return tiles < (uint32_t)a.least ? a.least : tiles > LG_PA_CHUNK / LG_PA_TILE ? LG_PA_CHUNK / LG_PA_TILE : tiles;
+        return tiles < (uint32_t)a.least ? a.least : tiles > longest ? longest : tiles;
     };
     const uint32_t most = size(some);
     if (some < 2 || most == (uint32_t)a.least) return most;

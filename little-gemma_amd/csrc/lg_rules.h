@@ -5,7 +5,8 @@
 
 #define LG_RULES_VOCAB 524288
 #define LG_RULES_WG 256
-#define LG_RULES_SLICE 8192         // tokens of a workgroup at most: their counts lie in LDS
+#define LG_RULES_AHEAD 4
+#define LG_RULES_SLICE 2048         // tokens of a workgroup: their counts lie in LDS
 
 struct RulesPenalty { float repetition, presence, frequency; int32_t prompt; };       // struct lg_hip_penalty
 struct RulesArgs {
@@ -23,11 +24,11 @@ struct RulesArgs {
 // A workgroup takes SLICE tokens of one row's vocabulary.  It asks for their logits, goes over the whole text of the row's sequence and counts its own tokens in LDS (whole numbers:
 // the order does not matter), then writes the slice.  Bound by memory where rows are many: 8 bytes a logit; a text is read once for every slice of every row, but from the L2.
 // Logits that a rule changes are computed in 64 bits and rounded once.
-template <bool VEC, int SLICE>
+template <bool VEC>
 __global__ __launch_bounds__(LG_RULES_WG) void lg_k_rules(RulesArgs a) {
     extern __shared__ uint32_t s_word[];            // [SLICE] counts: bit 31 a token of the text, below it how often it was generated; [SLICE] 1 + the bias of a token, where there are any
     constexpr uint32_t SEEN = 1u << 31;
-    constexpr int EACH = SLICE / (4 * LG_RULES_WG);
+    constexpr int SLICE = LG_RULES_SLICE, EACH = SLICE / (4 * LG_RULES_WG);
     const int t = threadIdx.x, row = blockIdx.y, base = blockIdx.x * SLICE;
     const int size = a.n_vocab - base < SLICE ? a.n_vocab - base : SLICE;
     // (logits first: what is asked for later arrives later)
@@ -77,13 +78,24 @@ __global__ __launch_bounds__(LG_RULES_WG) void lg_k_rules(RulesArgs a) {
             };
             const int head = (int)((16 - ((uintptr_t)h & 15)) & 15) / 4, lead = head < n ? head : n;
             if (t < lead) count(t, h[t]);
-            int i = lead + t * 4;
-            #pragma unroll 2
-            for (; i + 4 <= n; i += 4 * LG_RULES_WG) {
-                const int4 q = *(const int4 *)(h + i);
-                count(i, q.x); count(i + 1, q.y); count(i + 2, q.z); count(i + 3, q.w);
+            // fours of tokens, LG_RULES_AHEAD of them asked for at once
+            const int fours = (n - lead) / 4;
+            typedef int32_t four __attribute__((ext_vector_type(4)));
+            const four *const f = (const four *)(h + lead);
+            for (int k0 = t; k0 < fours; k0 += LG_RULES_AHEAD * LG_RULES_WG) {
+                four q[LG_RULES_AHEAD];
+                #pragma unroll
+                for (int k = 0; k < LG_RULES_AHEAD; ++k) q[k] = f[k0 + k * LG_RULES_WG < fours ? k0 + k * LG_RULES_WG : k0];
+                #pragma unroll
+                for (int k = 0; k < LG_RULES_AHEAD; ++k) {
+                    const int x = k0 + k * LG_RULES_WG;
+                    if (x < fours)
+                        #pragma unroll
+                        for (int j = 0; j < 4; ++j) count(lead + 4 * x + j, q[k][j]);
+                }
             }
-            for (; i < n; ++i) count(i, h[i]);                 // (of the last whole four's successor alone)
+            const int end = lead + 4 * fours;
+            if (end + t < n) count(end + t, h[end + t]);       // (up to three)
         }
         if (text && a.tree_mask && t < 64 && (a.tree_mask[row] >> t & 1)) {
             const long long at = (long long)a.tree_start[s] + t;

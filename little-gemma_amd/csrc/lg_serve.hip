@@ -282,7 +282,7 @@ static int tree_alone_of(int hd, int64_t units, bool wide) {
     if (!wide) return alone_of(hd, units);
     return units < 64 ? 8 : units < 256 ? 16 : units < 512 ? 24 : 32;
 }
-struct TreeCut { AttnCut c; int64_t items; TreeForm form; int rows, groups, slots; };
+struct TreeCut { AttnCut c; int64_t items; TreeForm form; int rows, groups, slots, longest; };
 // As cut_of, for workgroups of several pairs: a split of a tree takes as many as its pairs need, and those are what the chip's room is counted in.  items: workgroups of a key head, at most
 static TreeCut tree_cut_of(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
     const int pairs = max_tree * (n_head / n_head_kv);
@@ -290,12 +290,13 @@ static TreeCut tree_cut_of(int n_seq, int max_tree, int n_head, int n_head_kv, i
     const int rows = 16 * form.rt * form.wr, groups = (pairs + rows - 1) / rows, slots = 256 * (form.wide ? lg_wide_per_simd(hd, form.rt) : lg_tree_per_simd(hd, form.rt));
     // (a tree's rows see a window from the first committed position that its row 0 sees to its last row)
     const int64_t reach = window > 0 ? (int64_t)window + max_tree + LG_PA_TILE : max_len, span = std::min<int64_t>(reach, max_len), tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
-    const int64_t most = LG_PA_CHUNK / LG_PA_TILE, all = (int64_t)n_seq * groups, units = all * n_head_kv;
+    const int longest = form.wide ? LG_PA_CHUNK / LG_PA_TILE : LG_TREE_TILES;
+    const int64_t all = (int64_t)n_seq * groups, units = all * n_head_kv;
     const int alone = tree_alone_of(hd, units, form.wide), min_tiles = tiles <= alone ? alone : 4;
-    const int64_t least = std::max<int64_t>(1, (tiles + min_tiles - 1) / min_tiles), one = std::max<int64_t>(1, slots / n_head_kv * most);
+    const int64_t least = std::max<int64_t>(1, (tiles + min_tiles - 1) / min_tiles), one = std::max<int64_t>(1, slots / n_head_kv * longest);
     const int64_t rounds = std::max<int64_t>({ 1, (units + slots / 2 - 1) / (slots / 2), (all * tiles + one - 1) / one });
-    const int64_t full = std::max<int64_t>(rounds * slots / n_head_kv, all * tiles / most);
-    return { { std::min<int64_t>(n_seq * least, full + n_seq), all * tiles, least > 1, min_tiles }, std::min<int64_t>(all * least, full + all), form, rows, groups, slots };
+    const int64_t full = std::max<int64_t>(rounds * slots / n_head_kv, all * tiles / longest);
+    return { { std::min<int64_t>(n_seq * least, full + n_seq), all * tiles, least > 1, min_tiles }, std::min<int64_t>(all * least, full + all), form, rows, groups, slots, longest };
 }
 static size_t tree_cut_bytes(int n_seq, const TreeCut &t) { return up256(((size_t)n_seq + 1 + (n_seq > LG_PA_LANES ? n_seq + 2 + t.items : 0)) * 4); }
 extern "C" size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
@@ -350,7 +351,7 @@ extern "C" int lg_hip_paged_tree_attention(const struct lg_hip_pages *p, const f
     char *const w = need ? (char *)d_work + tree_cut_bytes(n_seq, t) : nullptr;
     const TreeAttn a{ { g, d_q, (long long)q_stride, d_table, d_len, d_out, (long long)out_stride, (float *)w, need ? (float *)(w + part) : nullptr, need ? (float *)(w + 2 * part) : nullptr, scale,
                         need ? (int32_t *)d_work : nullptr, n_head, p->n_head_kv, n_seq, max_blocks, max_len, window, t.slots, c.least },
-                      d_start, d_pos, (const lg_u64 *)d_mask, n_rows, max_tree, t.groups, t.rows, (int)t.items };
+                      d_start, d_pos, (const lg_u64 *)d_mask, n_rows, max_tree, t.groups, t.rows, (int)t.items, t.longest };
     hipStream_t st = (hipStream_t)stream;
     if (c.join && n_seq > LG_PA_LANES) hipLaunchKernelGGL(lg_k_tree_cut, dim3(1), dim3(LG_PC_WG), 0, st, a);
     switch (hd) {
@@ -456,17 +457,10 @@ extern "C" int lg_hip_paged_copy(const struct lg_hip_pages *layers, int n_layers
 }
 
 // ---- rules ------------------------------------------------------------------------------------------------------
-#define LG_RULES_FEW (1 << 21)
-template <bool VEC, int SLICE>
-static void launch_rules_of(const RulesArgs &a, hipStream_t st) {
-    const unsigned lds = SLICE * 4 * (a.bias_start ? 2 : a.penalty ? 1 : 0);
-    hipLaunchKernelGGL((lg_k_rules<VEC, SLICE>), dim3((unsigned)((a.n_vocab + SLICE - 1) / SLICE), (unsigned)a.rows), dim3(LG_RULES_WG), lds, st, a);
-}
 template <bool VEC>
 static void launch_rules(const RulesArgs &a, hipStream_t st) {
-    if ((int64_t)a.rows * a.n_vocab <= LG_RULES_FEW) launch_rules_of<VEC, LG_RULES_SLICE / 4>(a, st);
-    else if (a.bias_start) launch_rules_of<VEC, LG_RULES_SLICE / 2>(a, st);
-    else launch_rules_of<VEC, LG_RULES_SLICE>(a, st);
+    const unsigned lds = LG_RULES_SLICE * 4 * (a.bias_start ? 2 : a.penalty ? 1 : 0);
+    hipLaunchKernelGGL(lg_k_rules<VEC>, dim3((unsigned)((a.n_vocab + LG_RULES_SLICE - 1) / LG_RULES_SLICE), (unsigned)a.rows), dim3(LG_RULES_WG), lds, st, a);
 }
 extern "C" int lg_hip_adjust_logits(const struct lg_hip_logit_rules *r, const float *d_logits, int64_t stride, int rows, int n_vocab, float *d_out, int64_t out_stride, void *stream) {
     if (!r) return lg_fail(-1, "adjust_logits: null argument");

@@ -6,6 +6,7 @@
 
 #include "lg_pages.h"
 
+#define LG_TREE_TILES 127            // of a split at most, where its page ids lie in LDS: an id for each thread
 #define LG_TREE_ROWS 64             // rows of a tree: a set of them is 64 bits, a lane each
 
 enum { LG_TREE_BAD_ROWS = 1, LG_TREE_BAD_PARENT = 2, LG_TREE_BAD_LEN = 4 };            // LG_HIP_TREE_* of lg_hip.h
@@ -89,6 +90,7 @@ struct TreeAttn : PageAttn {        // len: with the tree's rows
     const int32_t *start, *pos;
     const lg_u64 *mask;
     int n_rows, max_tree, groups, rows, items;  // groups of `rows` pairs, at most; workgroups of a key head, at most
+    int longest;                    // tiles of a split at most
 };
 // The keys that rows of a tree see: [lo, len)
 struct TreeSeq { int row0, n, done, lo, len; };
@@ -109,12 +111,12 @@ __device__ __forceinline__ uint32_t lg_tree_groups(const TreeAttn &a, int seq) {
     const int n = lg_tree_rows(a.start, seq, a.n_rows, a.max_tree).n * (a.H / a.nkv);
     return n > a.rows ? (uint32_t)(n + a.rows - 1) / (uint32_t)a.rows : 1u;
 }
-// `total` tiles, each as often as groups read it, of `some` groups.  (A split has LG_PA_CHUNK keys at most: with fewer rounds than are asked for here all splits would be of that size and the last
-// round of workgroups hardly filled.  One sequence of 100003 keys, 32 pairs: 164 -> 150 us)
+// `total` tiles, each as often as groups read it, of `some` groups.  (A split's page ids have a fixed place, so it has a.longest tiles at most: with fewer rounds than are asked for here all splits would be of
+// that size and the last round of workgroups hardly filled)
 template <typename Count>
 __device__ __forceinline__ uint32_t lg_tree_tiles(const TreeAttn &a, uint32_t total, uint32_t some, Count count) {
-    const uint32_t one = (uint32_t)a.slots / a.nkv * (LG_PA_CHUNK / LG_PA_TILE), most = one ? one : 1;
-    return lg_pa_split_tiles(a, total, some, count, (total + most - 1) / most);
+    const uint32_t one = (uint32_t)a.slots / a.nkv * a.longest, most = one ? one : 1;
+    return lg_pa_split_tiles(a, total, some, count, (total + most - 1) / most, a.longest);
 }
 struct TreePart { int tiles, seq, index, first, n, group; };       // as PageCut; the group of pairs
 __device__ __forceinline__ TreePart lg_tree_part(const TreeAttn &a, int item) {
@@ -257,7 +259,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
     constexpr int HALVES = HD > 256 ? 1 : 2, TILE = 16 * HALVES, ROWS = 16 * RT * WR, WK = LG_PA_WAVES / WR;
     __shared__ float s_m[WK][ROWS], s_l[WK][ROWS], s_top[LG_PA_WAVES][ROWS];
     __shared__ __align__(16) union { lg_h8 q[RT * WR][KS][2][64]; float o[LG_PA_WAVES][16][HD]; } s;
-    __shared__ int32_t s_ids[LG_PA_CHUNK / 16 + 1], s_pos[LG_TREE_ROWS];
+    __shared__ int32_t s_ids[LG_TREE_TILES * 2 + 1], s_pos[LG_TREE_ROWS];
     const int number = lg_tree_number(blockIdx.x), kvh = number / a.items, G = a.H / a.nkv;
     if (kvh >= a.nkv) return;
     const TreePart cut = lg_tree_part(a, number % a.items);
