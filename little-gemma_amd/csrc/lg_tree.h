@@ -258,6 +258,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
     constexpr int NT = HD / 16;                     // output tiles
     constexpr int HALVES = HD > 256 ? 1 : 2, TILE = 16 * HALVES, ROWS = 16 * RT * WR, WK = LG_PA_WAVES / WR;
     __shared__ float s_m[WK][ROWS], s_l[WK][ROWS], s_top[LG_PA_WAVES][ROWS];
+    __shared__ long long s_to[ROWS];
     __shared__ __align__(16) union { lg_h8 q[RT * WR][KS][2][64]; float o[LG_PA_WAVES][16][HD]; } s;
     __shared__ int32_t s_ids[LG_TREE_TILES * 2 + 1], s_pos[LG_TREE_ROWS];
     const int number = lg_tree_number(blockIdx.x), kvh = number / a.items, G = a.H / a.nkv;
@@ -308,8 +309,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
     const int b0 = first >> a.g.shift;
     const bool has_id = (int)threadIdx.x <= ((end - 1) >> a.g.shift) - b0;
     const int my_id = has_id && b0 + (int)threadIdx.x < a.max_blocks ? table[b0 + threadIdx.x] : -1;
-    if ((int)threadIdx.x < w.n) s_pos[threadIdx.x] = a.pos[w.row0 + threadIdx.x];
-    if (has_id) s_ids[threadIdx.x] = my_id;
+    const int my_pos = (int)threadIdx.x < w.n ? a.pos[w.row0 + threadIdx.x] : 0;
     auto tile_at = [&](int t) {
         PageIds p;
         #pragma unroll
@@ -319,8 +319,21 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
         }
         return lg_pa_tile(a, p, t, kvh * HD);
     };
+    lg_h8 kf[HALVES][KS];
+    int t0 = p0 + wr * RT * 16 < n_pairs ? first + wk * TILE : end;      // (no pairs: nothing to do)
+    PageTile now = lg_pa_tile(a, lg_pa_ids(a, table, t0 < end ? t0 : first), t0 < end ? t0 : first, kvh * HD);
+    auto load_keys = [&](const PageTile &p) {
+        #pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+            const uint16_t *kp = a.g.k + p.row[h] + c * a.g.row_stride + g * 8;
+            #pragma unroll
+            for (int i = 0; i < KS; ++i) kf[h][i] = *(const lg_h8 *)(kp + i * 32);
+        }
+    };
     float qs[RT];                                   // factor of the raw scores: base-2 exponents
-    {
+    auto queries = [&]() {
+        if ((int)threadIdx.x < w.n) s_pos[threadIdx.x] = my_pos;
+        if (has_id) s_ids[threadIdx.x] = my_id;
         float top[RT * WR];
         #pragma unroll
         for (int rt = 0; rt < RT * WR; ++rt) {
@@ -364,20 +377,20 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
         #pragma unroll
         for (int rt = 0; rt < RT; ++rt) qs[rt] = a.scale * 1.44269504088896341f * __uint_as_float((unsigned)(127 + power((wr * RT + rt) * 16 + c)) << 23);
         lg_barrier_lds();
+    };
+    // (on either side of the branch: behind it they would have to wait for everything in flight)
+    if (t0 < end) {
+        __builtin_amdgcn_sched_barrier(0);
+        load_keys(now);
+        __builtin_amdgcn_sched_barrier(0);
+        queries();
+    } else {
+        queries();
+        asm volatile("");                           // (so that the two sides stay apart)
     }
     // tiles in [whole, w.done) need no mask; rows of the tree in front of a window are taken out of the sets
     lg_tree_trim<RT>(a, w, s_pos, lo_row, set, whole);
 
-    lg_h8 kf[HALVES][KS];
-    PageTile now;
-    auto load_keys = [&](const PageTile &p) {
-        #pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
-            const uint16_t *kp = a.g.k + p.row[h] + c * a.g.row_stride + g * 8;
-            #pragma unroll
-            for (int i = 0; i < KS; ++i) kf[h][i] = *(const lg_h8 *)(kp + i * 32);
-        }
-    };
     typedef uint32_t values[CH][4 * HALVES][DL / 2];
     auto load_values = [&](const PageTile &p, values &v) {
         #pragma unroll
@@ -389,8 +402,6 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
                 else { const uint2 u = *(const uint2 *)vp; v[ch][j][0] = u.x; v[ch][j][1] = u.y; }
             }
     };
-    int t0 = p0 + wr * RT * 16 < n_pairs ? first + wk * TILE : end;      // (no pairs: nothing to do)
-    if (t0 < end) { now = tile_at(t0); load_keys(now); }
     lg_f4 acc[RT][NT];
     float m[RT], l[RT];                             // of pair c; l of this lane's keys alone
     #pragma unroll
@@ -597,11 +608,29 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
     }
     // (behind the loads: lengths and page ids come through the scalar cache as long as nothing has been stored)
     tell();
-    // the parts of wavefronts with different keys, 16 pairs of every WR at a time
-    const bool wide = (((uintptr_t)a.out | (uintptr_t)a.out_stride * 4) & 15) == 0;
+    // the parts of wavefronts with different keys: their factors and where a pair's output goes, once for each pair; then 16 pairs of every WR at a time
+    __syncthreads();
+    if ((int)threadIdx.x < ROWS) {
+        const int pair = threadIdx.x, p = p0 + pair, node = p / G, head = kvh * G + p - node * G;
+        float M = -INFINITY, L = 0;
+        #pragma unroll
+        for (int u = 0; u < WK; ++u) M = fmaxf(M, s_m[u][pair]);
+        #pragma unroll
+        for (int u = 0; u < WK; ++u) {
+            const float lv = s_l[u][pair], f = lv == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_m[u][pair] - M);       // (0: no key; a score of NaN leaves its mark in the sum)
+            L += f * lv;
+            s_m[u][pair] = f;
+        }
+        const long long place = ((long long)at * a.max_tree + node) * a.H + head;
+        s_l[0][pair] = n_split > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+        s_to[pair] = p >= n_pairs ? -1 : n_split == 1 ? (w.row0 + node) * a.out_stride + (long long)head * HD : place * HD;
+        if (n_split > 1 && p < n_pairs) { a.pm[place] = M; a.pl[place] = L; }
+    }
+    float *const to = n_split == 1 ? a.out : a.pacc;
+    const bool wide = n_split > 1 || (((uintptr_t)a.out | (uintptr_t)a.out_stride * 4) & 15) == 0;
     #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        __syncthreads();                            // (the queries' last reader; the sums' of the 16 before)
+        if (rt) __syncthreads();                    // (the sums' readers of the 16 before)
         #pragma unroll
         for (int ch = 0; ch < CH; ++ch)
             #pragma unroll
@@ -610,32 +639,22 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
                 for (int i = 0; i < DL; i += 4)
                     *(float4 *)&s.o[wave][4 * g + r][ch * 128 + c * DL + i] = make_float4(acc[rt][ch * DL + i][r], acc[rt][ch * DL + i + 1][r], acc[rt][ch * DL + i + 2][r], acc[rt][ch * DL + i + 3][r]);
         __syncthreads();
-        #pragma unroll 4
-        for (int id = threadIdx.x; id < WR * 16 * (HD / 4); id += LG_PA_WAVES * 64) {
-            const int x = id / (HD / 4), d = id % (HD / 4) * 4, r = x / 16, pair = (r * RT + rt) * 16 + x % 16, p = p0 + pair;
-            float M = -INFINITY, L = 0;
-            float4 o = make_float4(0, 0, 0, 0);
+        constexpr int SUMS = WR * 16 * (HD / 4), EACH = (SUMS + LG_PA_WAVES * 64 - 1) / (LG_PA_WAVES * 64);
+        #pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            const int id = threadIdx.x + k * LG_PA_WAVES * 64, x = id / (HD / 4), d = id % (HD / 4) * 4, r = x / 16, pair = (r * RT + rt) * 16 + x % 16;
+            static_assert(SUMS % (LG_PA_WAVES * 64) == 0, "one for each thread in every round");
+            lg_f4 o = { 0, 0, 0, 0 };
             #pragma unroll
-            for (int u = 0; u < WK; ++u) M = fmaxf(M, s_m[u][pair]);
-            #pragma unroll
-            for (int u = 0; u < WK; ++u) {
-                const float lv = s_l[u][pair], f = lv == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_m[u][pair] - M);       // (0: no key; a score of NaN leaves its mark in the sum)
-                const float4 y = *(const float4 *)&s.o[u * WR + r][x % 16][d];
-                L += f * lv;
-                o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
-            }
-            if (p >= n_pairs) continue;
-            const int node = p / G, head = kvh * G + p % G;
-            if (n_split == 1) {
-                float *const to = a.out + (w.row0 + node) * a.out_stride + (long long)head * HD + d;
-                const float4 y = L == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(o.x / L, o.y / L, o.z / L, o.w / L);
-                if (wide) *(float4 *)to = y;
-                else { to[0] = y.x; to[1] = y.y; to[2] = y.z; to[3] = y.w; }
-            } else {
-                const long long place = ((long long)at * a.max_tree + node) * a.H + head;
-                *(float4 *)(a.pacc + place * HD + d) = o;
-                if (d == 0) { a.pm[place] = M; a.pl[place] = L; }
-            }
+            for (int u = 0; u < WK; ++u) o += s_m[u][pair] * *(const lg_f4 *)&s.o[u * WR + r][x % 16][d];
+            o *= s_l[0][pair];
+            const long long base = s_to[pair];
+            if (base < 0) continue;
+            float *const z = to + base + d;
+            if (wide) *(lg_f4 *)z = o;
+            else
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) z[i] = o[i];
         }
     }
 }
