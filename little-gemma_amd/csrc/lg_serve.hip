@@ -331,6 +331,7 @@ extern "C" int lg_hip_paged_tree_attention(const struct lg_hip_pages *p, const f
     const int hd = p->head_dim;
     if (!attn_shape(n_seq, n_head, p->n_head_kv, hd, max_len))
         return lg_fail(-2, "paged_tree_attention: %d query heads on %d key heads (at most 8 each), lengths up to %d", n_head, p->n_head_kv, max_len);
+    if (p->row_stride > 1 << 27) return lg_fail(-2, "paged_tree_attention: rows %lld values apart (at most 2^27)", (long long)p->row_stride);
     if (max_blocks < 1 || (int64_t)max_blocks * p->page_size > INT32_MAX) return lg_fail(-2, "paged_tree_attention: %d blocks of %d positions", max_blocks, p->page_size);
     if (window < 0) return lg_fail(-2, "paged_tree_attention: a window of %d", window);
     if (n_seq == 0 || n_rows == 0) return 0;

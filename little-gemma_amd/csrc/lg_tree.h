@@ -664,8 +664,9 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
 // register, while the tile before is worked on.  Queries stay in registers: a wavefront takes 16 RT pairs, and all keys, so that nothing is joined in the end.
 // A row's 16-byte pieces lie in LDS in an order of the row's own (piece j ^ swap), so that reads of a column of 16 rows touch all banks.
 constexpr int lg_wide_per_simd(int hd, int rt) { return hd * rt <= 256 ? 2 : 1; }
-__device__ __forceinline__ void lg_to_lds(const void *from, uint32_t to) {         // 16 bytes of each lane, one after another from byte `to` on
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to), "v"(from) : "memory");
+// 16 bytes of each lane, from a common place and its own distance behind it, to LDS, one after another from byte `to` on
+__device__ __forceinline__ void lg_to_lds(const void *from, uint32_t behind, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(to), "v"(behind), "s"(from) : "memory");
 }
 template <int HD, int RT>
 __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg_k_tree_wide(TreeAttn a) {
@@ -699,33 +700,47 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
     static_assert(LG_PA_CHUNK / 16 + 1 <= 192, "in three registers");
     auto id_of = [&](int i) { return i <= ((end - 1) >> a.g.shift) - b0 && b0 + i < a.max_blocks ? table[b0 + i] : -1; };
     const int ids0 = id_of(lane), ids1 = id_of(64 + lane), ids2 = id_of(128 + lane);
+    const int n_ids = ((end - 1) >> a.g.shift) - b0 + 1;
+    auto is_page = [&](int id) { return id >= 0 && id < a.g.n_pages; };
+    const bool all_there = __ballot((lane < n_ids && !is_page(ids0)) || (64 + lane < n_ids && !is_page(ids1)) || (128 + lane < n_ids && !is_page(ids2))) == 0;
+    auto id_at = [&](int t) {
+        const int i = (t >> a.g.shift) - b0;
+        int x = __builtin_amdgcn_readlane(ids0, i & 63);
+        if (n_ids > 64) { const int y = __builtin_amdgcn_readlane(ids1, i & 63), z = __builtin_amdgcn_readlane(ids2, i & 63); x = i < 64 ? x : i < 128 ? y : z; }
+        return x;
+    };
+    // a tile, for this wavefront: which half tiles are there, and where the half that it fetches from begins
+    constexpr int OWN = TILE / LG_PA_WAVES;         // its rows
+    const int half = wave * OWN / 16;
+    struct Tile { long long row; bool ok[2]; };
     auto tile_at = [&](int t) {
-        PageIds p;
-        #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int i = ((t + 16 * h < end ? t + 16 * h : t) >> a.g.shift) - b0;             // (a half behind the end is masked)
-            const int x = __builtin_amdgcn_readlane(ids0, i & 63), y = __builtin_amdgcn_readlane(ids1, i & 63), z = __builtin_amdgcn_readlane(ids2, i & 63);
-            p.id[h] = i < 64 ? x : i < 128 ? y : z;
-        }
-        return lg_pa_tile(a, p, t, kvh * HD);
+        Tile p;
+        const int mine = t + 16 * half, id = id_at(mine < end ? mine : t);      // (a half behind the end is masked)
+        p.row = (is_page(id) ? id : 0) * a.g.page_stride + (mine & ((1 << a.g.shift) - 1)) * a.g.row_stride;
+        p.ok[0] = p.ok[1] = true;
+        if (!all_there) { p.ok[0] = is_page(id_at(t)); p.ok[1] = is_page(id_at(t + 16 < end ? t + 16 : t)); }
+        return p;
     };
 
     auto swap = [](int row) { return HD == 64 ? row >> 1 & 7 : row & 15; };
-    // of a load: the lane's row and piece; the first row is a multiple of AT_ONCE, so that swap(first ^ row) = swap(first) ^ swap(row)
-    const long long to_row = lane / PIECES * a.g.row_stride * 2;
-    const uint32_t piece = ((lane % PIECES) ^ swap(lane / PIECES)) * 16;
-    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&s_kv[0][0][0];
-    auto fetch = [&](const PageTile &p, int buffer) {
+    // of its loads: the lane's row and piece, in bytes behind the half tile's first row (rows are at most 2^27 values apart: 32 bits)
+    uint32_t behind[LOADS];
+    #pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int row = (wave * OWN + i * AT_ONCE + lane / PIECES) & 15;
+        behind[i] = (uint32_t)row * (uint32_t)(a.g.row_stride * 2) + (uint32_t)((lane % PIECES) ^ swap(row)) * 16;
+    }
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&s_kv[0][0][0] + (uint32_t)(wave * OWN * HD * 2);
+    const uint16_t *const keys_of = a.g.k + kvh * HD, *const values_of = a.g.v + kvh * HD;
+    auto fetch = [&](const Tile &p, int buffer) {
+        const uint32_t to = lds + (uint32_t)(buffer * 2 * TILE * HD * 2);
         #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int row0 = (wave * LOADS + i) * AT_ONCE;
-            const long long from = to_row + (piece ^ (uint32_t)(swap(row0) * 16)), at = ((row0 < 16 ? p.row[0] : p.row[1]) + (row0 & 15) * a.g.row_stride) * 2;
-            const uint32_t to = lds + (uint32_t)((buffer * 2 * TILE + row0) * HD * 2);
-            lg_to_lds((const char *)a.g.k + at + from, to);
-            lg_to_lds((const char *)a.g.v + at + from, to + TILE * HD * 2);
+            lg_to_lds(keys_of + p.row, behind[i], to + i * AT_ONCE * HD * 2);
+            lg_to_lds(values_of + p.row, behind[i], to + i * AT_ONCE * HD * 2 + TILE * HD * 2);
         }
     };
-    PageTile now;
+    Tile now;
     if (first < end) { now = tile_at(first); fetch(now, 0); }
     if ((int)threadIdx.x < w.n) s_pos[threadIdx.x] = a.pos[w.row0 + threadIdx.x];
 
@@ -783,8 +798,8 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
             for (int i = 0; i < NT; ++i) acc[rt][i] = (lg_f4){ 0, 0, 0, 0 };
         }
     };
-    auto plain = [&](int t, const PageTile &p) { return t >= whole && t + TILE <= w.done && t + TILE <= end && p.ok[0] && p.ok[1]; };
-    auto seen_in = [&](int t0, const PageTile &p, uint32_t (&sees)[RT]) {
+    auto plain = [&](int t, const Tile &p) { return t >= whole && t + TILE <= w.done && t + TILE <= end && p.ok[0] && p.ok[1]; };
+    auto seen_in = [&](int t0, const Tile &p, uint32_t (&sees)[RT]) {
         #pragma unroll
         for (int rt = 0; rt < RT; ++rt) sees[rt] = 0;
         #pragma unroll
@@ -816,7 +831,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
     for (int t0 = first; t0 < end; t0 += TILE, buffer ^= 1) {
         // this tile has arrived, and every wavefront has done with the one before
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const PageTile here = now;
+        const Tile here = now;
         if (t0 + TILE < end) { now = tile_at(t0 + TILE); fetch(now, buffer ^ 1); }
         if (!busy) continue;
         const uint16_t *const keys = s_kv[buffer][0], *const vals = s_kv[buffer][1];
@@ -843,17 +858,19 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
                     for (int h = 0; h < 2; ++h) sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i % DEEP][h], q[rt][i][x], sc[rt][h], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
-        operand b[2][4];
+        constexpr int FAR = NT / 4 < 3 ? NT / 4 : 3;          // groups of values on their way
+        operand b[FAR][4];
         auto ask_values = [&](int n) {              // four tiles of 16 dimensions
             #pragma unroll
             for (int i = 0; i < 4; ++i)
                 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int tile = 4 * n + i;
-                    b[n & 1][i].s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vals + at_val[tile % VAL_AT] + tile / VAL_AT * VAL_AT * 16 + h * 16 * HD));
+                    b[n % FAR][i].s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vals + at_val[tile % VAL_AT] + tile / VAL_AT * VAL_AT * 16 + h * 16 * HD));
                 }
         };
-        ask_values(0);
+        #pragma unroll
+        for (int n = 0; n < FAR - 1 || n < 1; ++n) ask_values(n);
         __builtin_amdgcn_sched_barrier(0);
         const bool masked = !plain(t0, here);
         #pragma unroll
@@ -907,9 +924,9 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
             }
         #pragma unroll
         for (int n = 0; n < NT / 4; ++n) {          // (four sums in turn: a product waits for the one before it into the same sum)
-            if (n + 1 < NT / 4) ask_values(n + 1);
+            if (FAR > 1 && n + FAR - 1 < NT / 4) ask_values(n + FAR - 1);
             __builtin_amdgcn_sched_barrier(0);
-            operand (&v)[4] = b[n & 1];
+            operand (&v)[4] = b[n % FAR];
             if (partly)
                 #pragma unroll
                 for (int i = 0; i < 4; ++i)
