@@ -287,7 +287,7 @@ struct TreeCut { AttnCut c; int64_t items; TreeForm form; int rows, groups, slot
 static TreeCut tree_cut_of(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
     const int pairs = max_tree * (n_head / n_head_kv);
     const TreeForm form = tree_form(pairs, hd);
-    const int rows = 16 * form.rt * form.wr, groups = (pairs + rows - 1) / rows, slots = 256 * (form.wide ? lg_wide_per_simd(hd, form.rt) : lg_tree_per_simd(hd, form.rt));
+    const int rows = 16 * form.rt * form.wr, groups = (pairs + rows - 1) / rows, slots = 256 * (form.wide ? lg_wide_per_simd(hd) : lg_tree_per_simd(hd, form.rt));
     // (a tree's rows see a window from the first committed position that its row 0 sees to its last row)
     const int64_t reach = window > 0 ? (int64_t)window + max_tree + LG_PA_TILE : max_len, span = std::min<int64_t>(reach, max_len), tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
     const int longest = form.wide ? LG_PA_CHUNK / LG_PA_TILE : LG_TREE_TILES;
@@ -312,7 +312,7 @@ template <int HD>
 static void launch_tree(const TreeAttn &a, const TreeCut &t, hipStream_t st) {
     const dim3 grid((unsigned)(((int64_t)a.items * a.nkv + 63) / 64 * 64)), wg(LG_PA_WAVES * 64);
     if (t.form.wide) {
-        hipLaunchKernelGGL((lg_k_tree_wide<HD, 1>), grid, wg, 0, st, a);
+        hipLaunchKernelGGL(lg_k_tree_wide<HD>, grid, wg, 0, st, a);
     } else if (t.form.rt * t.form.wr == 1) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 1>), grid, wg, 0, st, a);
     else if constexpr (HD == 512) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 2>), grid, wg, 0, st, a);
     else hipLaunchKernelGGL((lg_k_tree_attn<HD, 2, 1>), grid, wg, 0, st, a);

@@ -192,8 +192,8 @@ __device__ __forceinline__ MergeRow lg_merge_row(const TreeAttn &a) {
 // 1 in each half of a pair of binary16 values that is infinite or NaN (all bits of the exponent: one more carries into the sign's place)
 __device__ __forceinline__ uint32_t lg_not_finite(uint32_t u) { return ((u & 0x7C007C00u) + 0x04000400u) >> 15 & 0x00010001u; }
 // The largest `whole` of the wavefront's pairs; rows of the tree in front of a pair's window are taken out of its set (which the usual windows, wider than a tree is deep, do not ask for)
-template <int RT>
-__device__ __forceinline__ void lg_tree_trim(const TreeAttn &a, const TreeSeq &w, const int32_t *s_pos, const int (&lo_row)[RT], lg_u64 (&set)[RT], int &whole) {
+template <class Trim>
+__device__ __forceinline__ void lg_tree_trim(const TreeAttn &a, const TreeSeq &w, const int32_t *s_pos, int &whole, Trim trim) {
     // (rows of 16 lanes by turning them: 0x128, 0x124, 0x122, 0x121 row_ror 8, 4, 2, 1)
     auto top = [&](int y) { if (y > whole) whole = y; };
     top(__builtin_amdgcn_mov_dpp(whole, 0x128, 0xF, 0xF, true)); top(__builtin_amdgcn_mov_dpp(whole, 0x124, 0xF, 0xF, true));
@@ -206,11 +206,7 @@ __device__ __forceinline__ void lg_tree_trim(const TreeAttn &a, const TreeSeq &w
     const uint32_t most = lg_wave_max(before);
     if (most < 0x80000000u && (int)(0x7FFFFFFFu - most) >= whole) return;
     #pragma unroll 1
-    for (int k = 0; k < w.n; ++k) {
-        const int pos = s_pos[k];
-        #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) if (pos < lo_row[rt]) set[rt] &= ~(1ull << k);
-    }
+    for (int k = 0; k < w.n; ++k) trim(s_pos[k], 1ull << k);
 }
 // Four keys in a row from position t on: which of them are committed, which there are at all, and where they are in the tree
 struct LgQuad { uint32_t old, there; int t, k; };
@@ -389,7 +385,10 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
         asm volatile("");                           // (so that the two sides stay apart)
     }
     // tiles in [whole, w.done) need no mask; rows of the tree in front of a window are taken out of the sets
-    lg_tree_trim<RT>(a, w, s_pos, lo_row, set, whole);
+    lg_tree_trim(a, w, s_pos, whole, [&](int pos, lg_u64 row) {
+        #pragma unroll
+        for (int rt = 0; rt < RT; ++rt) if (pos < lo_row[rt]) set[rt] &= ~row;
+    });
 
     typedef uint32_t values[CH][4 * HALVES][DL / 2];
     auto load_values = [&](const PageTile &p, values &v) {
@@ -661,20 +660,21 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
 
 // The same for more than 32 pairs: their wavefronts share keys and values through LDS.  From memory to registers each of them would ask for the same rows again, and rows of keys as operands are asked for
 // in 16 pieces of 64 bytes, for which the memory pipeline takes four times as long as for whole rows; here a tile of 32 keys and values goes to LDS once, by loads that pass no
-// register, while the tile before is worked on.  Queries stay in registers: a wavefront takes 16 RT pairs, and all keys, so that nothing is joined in the end.
+// register, while the tile before is worked on.  Queries stay in registers: a wavefront takes 16 pairs, and all keys, so that nothing is joined in the end.
 // A row's 16-byte pieces lie in LDS in an order of the row's own (piece j ^ swap), so that reads of a column of 16 rows touch all banks.
-constexpr int lg_wide_per_simd(int hd, int rt) { return hd * rt <= 256 ? 2 : 1; }
+constexpr int lg_wide_per_simd(int hd) { return hd <= 256 ? 2 : 1; }
 // 16 bytes of each lane, from a common place and its own distance behind it, to LDS, one after another from byte `to` on
 __device__ __forceinline__ void lg_to_lds(const void *from, uint32_t behind, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(to), "v"(behind), "s"(from) : "memory");
 }
-template <int HD, int RT>
-__global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg_k_tree_wide(TreeAttn a) {
+template <int HD>
+__global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD)) void lg_k_tree_wide(TreeAttn a) {
     constexpr int KS = HD / 32;                     // score steps
     constexpr int NT = HD / 16;                     // output tiles
-    constexpr int TILE = LG_PA_TILE, ROWS = 16 * RT * LG_PA_WAVES;
+    constexpr int TILE = LG_PA_TILE, ROWS = 16 * LG_PA_WAVES;
     constexpr int PIECES = HD / 8, AT_ONCE = 64 / PIECES, LOADS = TILE / AT_ONCE / LG_PA_WAVES;      // 16-byte pieces of a row; rows of a load; loads of a wavefront for a tile's keys, and for its values
-    __shared__ __align__(16) uint16_t s_kv[2][2][TILE * HD];
+    constexpr int TURN = 64 + 4;                    // floats between rows of the outputs' turn: no two of a column in a bank
+    __shared__ __align__(16) union { uint16_t kv[2][2][TILE * HD]; float turn[LG_PA_WAVES][16][TURN]; } s;
     __shared__ int32_t s_pos[LG_TREE_ROWS];
     const int number = lg_tree_number(blockIdx.x), kvh = number / a.items, G = a.H / a.nkv;
     if (kvh >= a.nkv) return;
@@ -730,7 +730,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
         const int row = (wave * OWN + i * AT_ONCE + lane / PIECES) & 15;
         behind[i] = (uint32_t)row * (uint32_t)(a.g.row_stride * 2) + (uint32_t)((lane % PIECES) ^ swap(row)) * 16;
     }
-    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&s_kv[0][0][0] + (uint32_t)(wave * OWN * HD * 2);
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&s.kv[0][0][0] + (uint32_t)(wave * OWN * HD * 2);
     const uint16_t *const keys_of = a.g.k + kvh * HD, *const values_of = a.g.v + kvh * HD;
     auto fetch = [&](const Tile &p, int buffer) {
         const uint32_t to = lds + (uint32_t)(buffer * 2 * TILE * HD * 2);
@@ -745,69 +745,62 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
     if ((int)threadIdx.x < w.n) s_pos[threadIdx.x] = a.pos[w.row0 + threadIdx.x];
 
     // queries of the wavefront's pairs, as operands
-    lg_h8 q[RT][KS][2];
-    float qs[RT];                                   // factor of the raw scores: base-2 exponents
-    int lo_row[RT], whole = w.lo;                   // of pair c: the first position that it sees, and its set
-    lg_u64 set[RT];
+    lg_h8 q[KS][2];
+    float qs;                                       // factor of the raw scores: base-2 exponents
+    int lo_row, whole = w.lo;                       // of pair c: the first position that it sees, and its set
+    lg_u64 set;
+    const int pair = p0 + wave * 16 + c, x = pair < n_pairs ? pair : p0, row = w.row0 + x / G;
+    const float *src = a.q + row * a.q_stride + (long long)(kvh * G + x % G) * HD + g * 8;
+    float4 v[KS][2];
     #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int p = p0 + (wave * RT + rt) * 16 + c, x = p < n_pairs ? p : p0, row = w.row0 + x / G;
-        const float *src = a.q + row * a.q_stride + (long long)(kvh * G + x % G) * HD + g * 8;
-        float4 v[KS][2];
+    for (int i = 0; i < KS; ++i)
         #pragma unroll
-        for (int i = 0; i < KS; ++i)
-            #pragma unroll
-            for (int j = 0; j < 2; ++j) v[i][j] = *(const float4 *)(src + i * 32 + j * 4);
-        const int pos = a.pos[row];
-        set[rt] = pos < w.done ? 0 : a.mask[row] & (w.n < 64 ? (1ull << w.n) - 1 : ~0ull);
-        lo_row[rt] = pos < w.done ? INT32_MAX : a.window > 0 ? pos - a.window + 1 : INT32_MIN;
-        if (p < n_pairs && lo_row[rt] > whole) whole = lo_row[rt];
-        float top = 0;
+        for (int j = 0; j < 2; ++j) v[i][j] = *(const float4 *)(src + i * 32 + j * 4);
+    const int pos = a.pos[row];
+    set = pos < w.done ? 0 : a.mask[row] & (w.n < 64 ? (1ull << w.n) - 1 : ~0ull);
+    lo_row = pos < w.done ? INT32_MAX : a.window > 0 ? pos - a.window + 1 : INT32_MIN;
+    if (pair < n_pairs && lo_row > whole) whole = lo_row;
+    float top = 0;
+    #pragma unroll
+    for (int i = 0; i < KS; ++i)
         #pragma unroll
-        for (int i = 0; i < KS; ++i)
-            #pragma unroll
-            for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fmaxf(fabsf(v[i][j].x), fabsf(v[i][j].y)), fmaxf(fabsf(v[i][j].z), fabsf(v[i][j].w))));
-        top = lg_max_of_rows(top);
-        int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;         // top * 2^-e in [2^14, 2^15)
-        if (e < -100) e = -100;                                       // (zero and tiny rows; 2^-e stays a float)
-        const float up = __uint_as_float((unsigned)(127 - e) << 23);
+        for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fmaxf(fabsf(v[i][j].x), fabsf(v[i][j].y)), fmaxf(fabsf(v[i][j].z), fabsf(v[i][j].w))));
+    top = lg_max_of_rows(top);
+    int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;         // top * 2^-e in [2^14, 2^15)
+    if (e < -100) e = -100;                                       // (zero and tiny rows; 2^-e stays a float)
+    const float up = __uint_as_float((unsigned)(127 - e) << 23);
+    #pragma unroll
+    for (int i = 0; i < KS; ++i) {
+        const float y[8] = { v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w, v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w };
         #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            const float y[8] = { v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w, v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w };
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float z = y[j] * up;
-                q[rt][i][0][j] = (_Float16)z;
-                q[rt][i][1][j] = (_Float16)(z - (float)q[rt][i][0][j]);
-            }
+        for (int j = 0; j < 8; ++j) {
+            const float z = y[j] * up;
+            q[i][0][j] = (_Float16)z;
+            q[i][1][j] = (_Float16)(z - (float)q[i][0][j]);
         }
-        qs[rt] = a.scale * 1.44269504088896341f * __uint_as_float((unsigned)(127 + e) << 23);
     }
+    qs = a.scale * 1.44269504088896341f * __uint_as_float((unsigned)(127 + e) << 23);
     lg_barrier_lds();                               // (positions)
     // tiles in [whole, w.done) need no mask; rows of the tree in front of a window are taken out of the sets
-    lg_tree_trim<RT>(a, w, s_pos, lo_row, set, whole);
+    lg_tree_trim(a, w, s_pos, whole, [&](int pos, lg_u64 row) { if (pos < lo_row) set &= ~row; });
 
-    const bool busy = p0 + wave * RT * 16 < n_pairs;          // (a wavefront without pairs only fetches)
-    lg_f4 acc[RT][NT];
-    float m[RT], l[RT];                             // of pair c; l of this lane's keys alone
+    const bool busy = p0 + wave * 16 < n_pairs;     // (a wavefront without pairs only fetches)
+    lg_f4 acc[NT];
+    float m, l;                                     // of pair c; l of this lane's keys alone
     auto clear = [&]() {
+        m = -INFINITY; l = 0;
         #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            m[rt] = -INFINITY; l[rt] = 0;
-            #pragma unroll
-            for (int i = 0; i < NT; ++i) acc[rt][i] = (lg_f4){ 0, 0, 0, 0 };
-        }
+        for (int i = 0; i < NT; ++i) acc[i] = (lg_f4){ 0, 0, 0, 0 };
     };
     auto plain = [&](int t, const Tile &p) { return t >= whole && t + TILE <= w.done && t + TILE <= end && p.ok[0] && p.ok[1]; };
-    auto seen_in = [&](int t0, const Tile &p, uint32_t (&sees)[RT]) {
-        #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) sees[rt] = 0;
+    auto seen_in = [&](int t0, const Tile &p) {
+        uint32_t sees = 0;
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const LgQuad x = lg_tree_quad(t0 + 16 * h + 4 * g, w.done, p.ok[h] ? end : 0);
-            #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) sees[rt] |= lg_tree_sees(x, lo_row[rt], set[rt]) << (4 * h);
+            sees |= lg_tree_sees(x, lo_row, set) << (4 * h);
         }
+        return sees;
     };
     // where a lane reads, in values: its piece of a key row differs from that of the step before by a piece's place, of those 4 (2) steps before by a whole number of rounds
     constexpr int KEY_AT = KS < 4 ? KS : 4;
@@ -834,11 +827,9 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
         const Tile here = now;
         if (t0 + TILE < end) { now = tile_at(t0 + TILE); fetch(now, buffer ^ 1); }
         if (!busy) continue;
-        const uint16_t *const keys = s_kv[buffer][0], *const vals = s_kv[buffer][1];
-        lg_f4 sc[RT][2];
-        #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = (lg_f4){ 0, 0, 0, 0 };
-        constexpr int DEEP = KS < 3 || RT > 1 ? 2 : 3;      // key operands on their way
+        const uint16_t *const keys = s.kv[buffer][0], *const vals = s.kv[buffer][1];
+        lg_f4 sc[2] = {};
+        constexpr int DEEP = KS < 3 ? 2 : 3;     // key operands on their way
         lg_h8 kf[DEEP][2];
         auto ask = [&](int i) {
             #pragma unroll
@@ -853,9 +844,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
             #pragma unroll
             for (int x = 0; x < 2; ++x)
                 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    #pragma unroll
-                    for (int h = 0; h < 2; ++h) sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i % DEEP][h], q[rt][i][x], sc[rt][h], 0, 0, 0);
+                for (int h = 0; h < 2; ++h) sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i % DEEP][h], q[i][x], sc[h], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
         constexpr int FAR = NT / 4 < 3 ? NT / 4 : 3;          // groups of values on their way
@@ -874,45 +863,31 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
         __builtin_amdgcn_sched_barrier(0);
         const bool masked = !plain(t0, here);
         #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-            #pragma unroll
-            for (int h = 0; h < 2; ++h) sc[rt][h] *= qs[rt];
-        uint32_t sees[RT];
+        for (int h = 0; h < 2; ++h) sc[h] *= qs;
+        uint32_t sees;
         if (masked) {
-            seen_in(t0, here, sees);
+            sees = seen_in(t0, here);
             #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) if (!(sees[rt] >> j & 1)) sc[rt][j >> 2][j & 3] = -INFINITY;
+            for (int j = 0; j < 8; ++j) if (!(sees >> j & 1)) sc[j >> 2][j & 3] = -INFINITY;
         }
-        float top[RT];
-        bool higher = false;
+        float top = -INFINITY;
         #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            top[rt] = -INFINITY;
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[j >> 2][j & 3]);
+        top = lg_max_of_rows(top);
+        if (__any(top > m + LG_TREE_SLACK)) {
+            const float mn = fmaxf(m, ceilf(top));
+            const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);       // (both -inf: nothing seen yet)
+            l *= f; m = mn;
+            float fr[4];
             #pragma unroll
-            for (int j = 0; j < 8; ++j) top[rt] = fmaxf(top[rt], sc[rt][j >> 2][j & 3]);
-            top[rt] = lg_max_of_rows(top[rt]);
-            higher |= top[rt] > m[rt] + LG_TREE_SLACK;
-        }
-        if (__any(higher)) {
+            for (int r = 0; r < 4; ++r) fr[r] = __shfl(f, 4 * g + r);
             #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const float mn = fmaxf(m[rt], ceilf(top[rt]));
-                const float f = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);       // (both -inf: nothing seen yet)
-                l[rt] *= f; m[rt] = mn;
-                float fr[4];
+            for (int i = 0; i < NT; ++i)
                 #pragma unroll
-                for (int r = 0; r < 4; ++r) fr[r] = __shfl(f, 4 * g + r);
-                #pragma unroll
-                for (int i = 0; i < NT; ++i)
-                    #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[rt][i][r] *= fr[r];
-            }
+                for (int r = 0; r < 4; ++r) acc[i][r] *= fr[r];
         }
-        lg_h8 hi[RT], lo[RT];
-        #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) lg_tree_parts(sc[rt], m[rt], l[rt], hi[rt], lo[rt]);
+        lg_h8 hi, lo;
+        lg_tree_parts(sc, m, l, hi, lo);
         // keys that are not there may hold anything: zeros in their place
         const bool partly = t0 < w.lo || t0 + TILE > end || !here.ok[0] || !here.ok[1];
         uint32_t there[4];
@@ -942,22 +917,18 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
                         v[i].u[k] &= ~(x * 0xFFFFu);
                         odd.u[k] = x * 0x3C00u;                   // 1 where it is not finite
                     }
+                    lg_h8 seen;
                     #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        lg_h8 seen;
-                        #pragma unroll
-                        for (int j = 0; j < 8; ++j) seen[j] = sees[rt] >> j & 1 ? (_Float16)1.0f : (_Float16)0.0f;
-                        const lg_f4 mark = __builtin_amdgcn_mfma_f32_16x16x32_f16(seen, odd.h, (lg_f4){ 0, 0, 0, 0 }, 0, 0, 0);
-                        #pragma unroll
-                        for (int r = 0; r < 4; ++r) if (mark[r] != 0.0f) acc[rt][4 * n + i][r] = NAN;
-                    }
+                    for (int j = 0; j < 8; ++j) seen[j] = sees >> j & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+                    const lg_f4 mark = __builtin_amdgcn_mfma_f32_16x16x32_f16(seen, odd.h, (lg_f4){ 0, 0, 0, 0 }, 0, 0, 0);
+                    #pragma unroll
+                    for (int r = 0; r < 4; ++r) if (mark[r] != 0.0f) acc[4 * n + i][r] = NAN;
                 }
             #pragma unroll
             for (int x = 0; x < 2; ++x)
                 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) acc[rt][4 * n + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x ? lo[rt] : hi[rt], v[i].h, acc[rt][4 * n + i], 0, 0, 0);
+                    acc[4 * n + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x ? lo : hi, v[i].h, acc[4 * n + i], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -965,11 +936,9 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
     run(std::false_type{});
     float finite = 0;                               // or NaN
     #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int n = 0; n < NT; ++n)
         #pragma unroll
-        for (int n = 0; n < NT; ++n)
-            #pragma unroll
-            for (int r = 0; r < 4; ++r) finite = __builtin_fmaf(acc[rt][n][r], 0.0f, finite);
+        for (int r = 0; r < 4; ++r) finite = __builtin_fmaf(acc[n][r], 0.0f, finite);
     if (__syncthreads_or(finite != 0.0f)) {
         now = tile_at(first);
         fetch(now, 0);
@@ -978,11 +947,11 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
     tell();
     __syncthreads();                                // (the last tile's readers)
     if (!busy) return;
-    float total = l[0];
+    float total = l;
     total += __shfl_xor(total, 16);
     total += __shfl_xor(total, 32);
-    // outputs turned in LDS, each wavefront by itself, for stores of 16 bytes: 16 pairs of 64 dimensions at a time, 4 floats between rows
-    float *const turn = (float *)&s_kv[0][0][0] + wave * 16 * 68;
+    // outputs turned in LDS, each wavefront by itself, for stores of 16 bytes: 16 pairs of 64 dimensions at a time
+    float (&turn)[16][TURN] = s.turn[wave];
     const bool aligned = n_split > 1 || (((uintptr_t)a.out | (uintptr_t)a.out_stride * 4) & 15) == 0;
     float *to[4], by[4];                            // of pairs 4 k + g
     #pragma unroll
@@ -997,10 +966,10 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
         #pragma unroll
         for (int i = 0; i < 4; ++i)
             #pragma unroll
-            for (int r = 0; r < 4; ++r) turn[(4 * g + r) * 68 + i * 16 + c] = acc[0][n + i][r];
+            for (int r = 0; r < 4; ++r) turn[4 * g + r][i * 16 + c] = acc[n + i][r];
         lg_f4 y[4];
         #pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = *(const lg_f4 *)(turn + (4 * k + g) * 68 + c * 4) * by[k];
+        for (int k = 0; k < 4; ++k) y[k] = *(const lg_f4 *)&turn[4 * k + g][c * 4] * by[k];
         #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (to[k]) {
@@ -1013,6 +982,6 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD, RT)) void lg
     const int p = p0 + wave * 16 + lane;
     if (n_split > 1 && lane < 16 && p < n_pairs) {
         const long long place = ((long long)at * a.max_tree + p / G) * a.H + kvh * G + p % G;
-        a.pm[place] = m[0]; a.pl[place] = total;
+        a.pm[place] = m; a.pl[place] = total;
     }
 }
