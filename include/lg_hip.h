@@ -341,7 +341,7 @@ int    lg_hip_sample(const float *d_logits, int64_t stride, int rows, int n_voca
 
 /* Before the step, from d_parent [n_rows] (a tree's rows count from 0; row 0's parent is not read): d_mask (aligned to 8 bytes), the row and the rows above it up to row 0 as a set of 64 bits; d_pos,
  * the position that the row stands for, committed positions + rows above it (rotations and windows go by it); d_seq, its sequence.  *d_status [n_seq]: 0, or the
- * LG_HIP_TREE_ bits of what is wrong with a tree: its rows then get an empty set and position -1 (nothing is written for LG_HIP_TREE_BAD_ROWS). */
+ * LG_HIP_TREE_ bits of what is wrong with a tree: its rows then get an empty set and position -1 (nothing is written for LG_HIP_TREE_BAD_ROWS).  Rows of no tree are left as they are. */
 enum { LG_HIP_TREE_BAD_ROWS = 1,       /* d_start falls, a tree has more than max_tree rows, or a row is outside 0..n_rows-1 */
        LG_HIP_TREE_BAD_PARENT = 2,     /* a parent that is not an earlier row */
        LG_HIP_TREE_BAD_LENGTH = 4 };   /* a length below the tree's rows */
@@ -356,7 +356,8 @@ int    lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int32_t *d_
  * that its set d_mask names, of which only those with t > d_pos[row] - window and d_pos[row k] > d_pos[row] - window where window is not 0.  d_len [n_seq] counts the trees' rows.  Sets need not come from lg_hip_tree_plan: any rows of the
  * same tree may be named, later ones too; positions are at least the committed length, a row with another one sees nothing.  A row that sees nothing gets
  * zeros, so do the rows of a sequence whose length is below its rows or above max_len or max_blocks * page_size; rows of a tree with LG_HIP_TREE_BAD_ROWS and rows of no tree are left as they are.
- * Positions whose page is outside 0..n_pages-1 are left out.  What is not seen by a row does not reach it, whatever it holds, also where other rows of the tree see it; infinities and NaN that are seen
+ * Positions whose page is outside 0..n_pages-1 are left out.  Arguments as lg_hip_paged_attention's (n_head / n_head_kv <= 8, q_stride a multiple of 4, d_q aligned to 16 bytes; max_len bounds the lengths
+ * of a captured call, and the working memory), d_mask aligned to 8 bytes, the pages' row_stride at most 2^27.  What is not seen by a row does not reach it, whatever it holds, also where other rows of the tree see it; infinities and NaN that are seen
  * spoil the heads that read them (NaN as a rule) and no others. */
 size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree, int n_head, int n_head_kv, int head_dim, int max_len, int window);
 int    lg_hip_paged_tree_attention(const struct lg_hip_pages *pages, const float *d_q, int64_t q_stride, int n_rows, int n_seq, int max_tree, int n_head,
@@ -373,7 +374,7 @@ int    lg_hip_paged_compact(const struct lg_hip_pages *layers, int n_layers, int
  * name one source, rows may change places).  Whole pages are shared: d_shares [n_pages] counts for each page the rows that hold it beyond the first, 0 at the start and for free pages.  A last page that is not
  * full belongs to its row alone, so that the row may grow into it: where others hold it too, the row gets a page off the stack, and d_from, d_to, d_rows [n_seq] say what lg_hip_paged_copy has to copy (-1, -1, 0 for the other rows).
  * Pages that no row holds any longer go on the stack first, row by row, the first one topmost.  *d_status: 0, or the LG_HIP_FORK_ bits of what was wrong; then nothing but d_from, d_to and d_rows (nothing to copy) is written.
- * lg_hip_paged_plan goes on working on such a table for growth, and for taking back pages that were grown since; pages with shares are given back here. A row holds a page once; that is not looked for. */
+ * n_seq * max_blocks is at most 2^30.  lg_hip_paged_plan goes on working on such a table for growth, and for taking back pages that were grown since; pages with shares are given back here. A row holds a page once; that is not looked for. */
 enum { LG_HIP_FORK_BAD_LENGTH = 1,     /* a length below 0 or above max_blocks * page_size, or a new one above the source's old one */
        LG_HIP_FORK_NO_PAGES = 2,       /* not enough free pages for the copies */
        LG_HIP_FORK_BAD_SOURCE = 4,     /* a source outside -1..n_seq-1 */

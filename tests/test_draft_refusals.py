@@ -62,6 +62,12 @@ def test_bad_pages_are_refused(lg, change, code, words):
     refused(lg, H.lg_hip_paged_copy(two, 2, 3, P16, P16, P16, None), code, words)
 
 
+def test_rows_too_far_apart_for_tree_attention_are_refused(lg):
+    H, far = lg.hiplib.load_hip(), (1 << 27) + 8
+    refused(lg, attend(H, pages(lg, dict(row_stride=far, page_stride=far * 16))), -2, "at most 2^27")
+    assert attend(H, pages(lg, dict(row_stride=1 << 27, page_stride=1 << 31)), rows=0) == 0
+
+
 def test_calls_beyond_what_a_launch_holds_are_refused(lg):
     H = lg.hiplib.load_hip()
     for seqs, heads, kv, most in ((4096, 2, 1, 1), (128, 2, 1, 64), (4096, 1024, 128, 64)):
