@@ -268,11 +268,16 @@ extern "C" int lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int
     return 0;
 }
 
-// How a workgroup takes pairs: 16 RT by each of WR wavefronts, no more than a tree has
+// How a workgroup takes pairs: 16 RT by each of WR wavefronts.  `work`: tiles of all sequences and key heads, as often as groups of 64 pairs read them.
+// 16 pairs to one where a tree has no more (trees of 32 and of 16 pairs in workgroups of 32, us: 64 sequences in windows of 512 tokens, heads of 256, 25.5 and 24.3, in those of 16 the latter 20.4; 4096 tokens
+// 114 both).  32 (lg_k_tree_attn) and 64 (lg_k_tree_wide) of 64 pairs and more: the wide one reads keys once for all four wavefronts but spends 10 us beside its tiles, the other less, and twice as many of
+// its workgroups are at work.  Us, 32 and 64 to a workgroup, heads of 256: windows of 512 of 64 sequences (2304 tiles) 27.0 and 33.3, of 96 (3456) 46.5 and 36, of 128 (4608) 48.4 and 36.2; 4096 tokens of 8
+// sequences (2048) 33.0 and 33.7, 20 (5120) 47.3 and 45.7, 32 (8192) 75.9 and 63.5.  Heads of 128: 4608 tiles 31.8 and 24.8.  Heads of 512: 576 tiles 33.0 and 37.7, 1152 48.7 and 46.0, 2304 62.6 and 55.9.
+// Trees of up to 32 pairs in wide workgroups: 100003 tokens 166 for 147, 64 sequences in windows of 512 31.1 for 25.5
 struct TreeForm { int rt, wr; bool wide; };
-static TreeForm tree_form(int pairs, int hd) {
+static TreeForm tree_form(int pairs, int hd, int64_t work) {
     if (pairs <= 16) return { 1, 1, false };
-    if (pairs <= 32) return hd == 512 ? TreeForm{ 1, 2, false } : TreeForm{ 2, 1, false };
+    if (pairs <= 32 || work <= (hd == 512 ? 1024 : 2560)) return hd == 512 ? TreeForm{ 1, 2, false } : TreeForm{ 2, 1, false };
     return { 1, LG_PA_WAVES, true };
 }
 // Trees of up to so many tiles are left whole, as alone_of says for one row.  A workgroup of 64 pairs spends 10 us beside its tiles, of 1.5 us each, and the joining launch takes 8.  Whole and in splits, us, heads of
@@ -280,16 +285,16 @@ static TreeForm tree_form(int pairs, int hd) {
 // these lengths up to it: 36.7 and 33.2); 256 of 272 26.7 and 47.7, of 528 39.6 and 55.6; 512 of 528 65.1 and 114.8
 static int tree_alone_of(int hd, int64_t units, bool wide) {
     if (!wide) return alone_of(hd, units);
-    return units < 64 ? 8 : units < 256 ? 16 : units < 512 ? 24 : 32;
+    return units < 64 ? 8 : units < 160 ? 16 : units < 512 ? 24 : 32;
 }
 struct TreeCut { AttnCut c; int64_t items; TreeForm form; int rows, groups, slots, longest; };
 // As cut_of, for workgroups of several pairs: a split of a tree takes as many as its pairs need, and those are what the chip's room is counted in.  items: workgroups of a key head, at most
 static TreeCut tree_cut_of(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
     const int pairs = max_tree * (n_head / n_head_kv);
-    const TreeForm form = tree_form(pairs, hd);
-    const int rows = 16 * form.rt * form.wr, groups = (pairs + rows - 1) / rows, slots = 256 * (form.wide ? lg_wide_per_simd(hd) : lg_tree_per_simd(hd, form.rt));
     // (a tree's rows see a window from the first committed position that its row 0 sees to its last row)
     const int64_t reach = window > 0 ? (int64_t)window + max_tree + LG_PA_TILE : max_len, span = std::min<int64_t>(reach, max_len), tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
+    const TreeForm form = tree_form(pairs, hd, tiles * n_seq * n_head_kv * ((pairs + 63) / 64));
+    const int rows = 16 * form.rt * form.wr, groups = (pairs + rows - 1) / rows, slots = 256 * (form.wide ? lg_wide_per_simd(hd) : lg_tree_per_simd(hd, form.rt));
     const int longest = form.wide ? LG_PA_CHUNK / LG_PA_TILE : LG_TREE_TILES;
     const int64_t all = (int64_t)n_seq * groups, units = all * n_head_kv;
     const int alone = tree_alone_of(hd, units, form.wide), min_tiles = tiles <= alone ? alone : 4;

@@ -245,7 +245,7 @@ __device__ __forceinline__ float lg_max_of_rows(float x) {
     return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
 }
 // How the four wavefronts of a workgroup share its work: WR of them take 16 RT pairs each, the others different keys
-constexpr int lg_tree_per_simd(int hd, int rt) { return hd * rt <= 128 ? 3 : hd * rt <= 256 ? 2 : 1; }
+constexpr int lg_tree_per_simd(int hd, int rt) { return hd * rt <= 128 ? 3 : hd * rt < 256 ? 2 : 1; }
 template <int HD, int RT, int WR>
 __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg_k_tree_attn(TreeAttn a) {
     constexpr int KS = HD / 32;                     // score steps
