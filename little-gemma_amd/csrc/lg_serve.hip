@@ -268,16 +268,18 @@ extern "C" int lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int
     return 0;
 }
 
-// How a workgroup takes pairs: 16 RT by each of WR wavefronts.  `work`: tiles of all sequences and key heads, as often as groups of 64 pairs read them.
-// 16 pairs to one where a tree has no more (trees of 32 and of 16 pairs in workgroups of 32, us: 64 sequences in windows of 512 tokens, heads of 256, 25.5 and 24.3, in those of 16 the latter 20.4; 4096 tokens
-// 114 both).  32 (lg_k_tree_attn) and 64 (lg_k_tree_wide) of 64 pairs and more: the wide one reads keys once for all four wavefronts but spends 10 us beside its tiles, the other less, and twice as many of
-// its workgroups are at work.  Us, 32 and 64 to a workgroup, heads of 256: windows of 512 of 64 sequences (2304 tiles) 27.0 and 33.3, of 96 (3456) 46.5 and 36, of 128 (4608) 48.4 and 36.2; 4096 tokens of 8
-// sequences (2048) 33.0 and 33.7, 20 (5120) 47.3 and 45.7, 32 (8192) 75.9 and 63.5.  Heads of 128: 4608 tiles 31.8 and 24.8.  Heads of 512: 576 tiles 33.0 and 37.7, 1152 48.7 and 46.0, 2304 62.6 and 55.9.
-// Trees of up to 32 pairs in wide workgroups: 100003 tokens 166 for 147, 64 sequences in windows of 512 31.1 for 25.5
+// How many pairs a workgroup takes, 16 RT by each of WR wavefronts, goes by how much there is to read: tiles of all sequences and key heads, as often as groups of so many pairs read them.
+// Few pairs make short workgroups, and many of them; where the chip is full their reads of the same keys again cost more.  Us of trees of 8 and 16 rows, heads of 256, 4 query heads to a key head:
+//   16 to a workgroup and 32: windows of 512 of 32 sequences (4608 tiles, read by sixteens) 20.3 and 25.2, of 40 (5760) 36.9 and 25.4; 4096 tokens of 4 (4096) 23.3 and 24.7, of 8 (8192) 36.0 and 32.0; 100
+//     tokens of one, trees of 5, 9.7 and 12.9; heads of 128: 2048 14.8 and 15.8, 4096 20.3 and 18.3, in windows 4608 12.5 and 15.9, 9216 18.5 and 17.3; heads of 64: 8192 19.3 and 20.5, 16384 28.1 and 21.5;
+//     heads of 512: 4096 38.4 and 42.8, in windows 4352 32.9 and 54.8
+//   32 (lg_k_tree_attn) and 64 (lg_k_tree_wide, which reads keys once for all four wavefronts but spends 10 us beside its tiles): windows of 64 sequences (2304 tiles, read by sixty-fours) 27.0 and 33.3, of 96
+//     (3456) 46.5 and 36, of 128 (4608) 48.4 and 36.2; 4096 tokens of 8 (2048) 33.0 and 33.7, of 20 (5120) 47.3 and 45.7, of 32 (8192) 75.9 and 63.5; heads of 128: 4608 31.8 and 24.8; heads of 512: 2304 62.6 and
+//     55.9.  Trees of up to 32 pairs in wide workgroups: 100003 tokens 166 for 147, 64 sequences in windows of 512 31.1 for 25.5
 struct TreeForm { int rt, wr; bool wide; };
-static TreeForm tree_form(int pairs, int hd, int64_t work) {
-    if (pairs <= 16) return { 1, 1, false };
-    if (pairs <= 32 || work <= (hd == 512 ? 1024 : 2560)) return hd == 512 ? TreeForm{ 1, 2, false } : TreeForm{ 2, 1, false };
+static TreeForm tree_form(int pairs, int hd, int64_t tiles) {
+    if (pairs <= 16 || tiles * ((pairs + 15) / 16) <= (hd == 64 ? 9216 : 4608)) return { 1, 1, false };
+    if (pairs <= 32 || (hd < 512 && tiles * ((pairs + 63) / 64) <= 2560)) return hd == 512 ? TreeForm{ 1, 2, false } : TreeForm{ 2, 1, false };
     return { 1, LG_PA_WAVES, true };
 }
 // Trees of up to so many tiles are left whole, as alone_of says for one row.  A workgroup of 64 pairs spends 10 us beside its tiles, of 1.5 us each, and the joining launch takes 8.  Whole and in splits, us, heads of
@@ -293,7 +295,7 @@ static TreeCut tree_cut_of(int n_seq, int max_tree, int n_head, int n_head_kv, i
     const int pairs = max_tree * (n_head / n_head_kv);
     // (a tree's rows see a window from the first committed position that its row 0 sees to its last row)
     const int64_t reach = window > 0 ? (int64_t)window + max_tree + LG_PA_TILE : max_len, span = std::min<int64_t>(reach, max_len), tiles = (span + LG_PA_TILE - 1) / LG_PA_TILE;
-    const TreeForm form = tree_form(pairs, hd, tiles * n_seq * n_head_kv * ((pairs + 63) / 64));
+    const TreeForm form = tree_form(pairs, hd, tiles * n_seq * n_head_kv);
     const int rows = 16 * form.rt * form.wr, groups = (pairs + rows - 1) / rows, slots = 256 * (form.wide ? lg_wide_per_simd(hd) : lg_tree_per_simd(hd, form.rt));
     const int longest = form.wide ? LG_PA_CHUNK / LG_PA_TILE : LG_TREE_TILES;
     const int64_t all = (int64_t)n_seq * groups, units = all * n_head_kv;
