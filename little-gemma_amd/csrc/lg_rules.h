@@ -23,6 +23,8 @@ struct RulesArgs {
 
 // A workgroup takes SLICE tokens of one row's vocabulary.  It asks for their logits, goes over the whole text of the row's sequence and counts its own tokens in LDS (whole numbers:
 // the order does not matter), then writes the slice.  Bound by memory where rows are many: 8 bytes a logit; a text is read once for every slice of every row, but from the L2.
+// 64 rows of 262144 with penalties, biases and sets, 135 MB: 28 us, 4.8 TB/s; one row with a text of 3001 tokens 4.8 us, the launch and the chain of parameters, text and logits.  Slices of 2048 at all sizes: of 4096 64
+// rows took 34.6, one row 5.1.  Rows that are not aligned to 16 bytes (VEC false): 39.6 and 5.2.
 // Logits that a rule changes are computed in 64 bits and rounded once.
 template <bool VEC>
 __global__ __launch_bounds__(LG_RULES_WG) void lg_k_rules(RulesArgs a) {

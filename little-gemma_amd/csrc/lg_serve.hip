@@ -454,7 +454,8 @@ extern "C" int lg_hip_paged_copy(const struct lg_hip_pages *layers, int n_layers
     if (n == 0 || n_layers == 0) return 0;
     if (!d_from || !d_to || !d_rows) return lg_fail(-1, "paged_copy: null argument");
     each_layers(layers, n_layers, [&](const PageLayers &ls, int k, int most) {
-        // several workgroups to a page where there are few pages
+        // several workgroups to a page where there are few pages, up to 4096 in all.  Forks and copy, one workgroup to a page, this, and one to every 4 loads of a thread: two pages of 256
+        // positions of one layer 33.7, 16.3 and 16.3 us, of 48 layers 47.6, 42.7 and 47.6, nine of 48 261, 240 and 235, 244 pages of 32 positions of 48 layers 394, 394 and 408
         const int64_t pages = (int64_t)n * k * 2, whole = ((int64_t)layers->page_size * most + 1023) / 1024;
         const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(whole, 4096 / pages));
         hipLaunchKernelGGL(lg_k_page_copy, dim3((unsigned)(2 * parts), (unsigned)k, (unsigned)n), dim3(256), 0, (hipStream_t)stream, ls, d_from, d_to, d_rows, shift_of(layers->page_size),

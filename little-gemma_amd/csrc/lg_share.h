@@ -24,7 +24,8 @@ struct ForkArgs {
 // else the first; each of the others takes a page off the stack, in order, and is told what to copy.
 // All or nothing: everything is read and counted in working memory, then everything is written.
 // One workgroup, of NT threads: a few words for every page that moves, its time a chain of round trips to memory (lengths, ids, shares; counts; places; stores).  A thread keeps its first release, arrival and
-// row in registers, so that a call of up to NT of each asks for them once: eight forks of 16 pages 9.7 -> 6.3 us.
+// row in registers, so that a call of up to NT of each asks for them once: eight forks of 16 pages 9.7 -> 7.1 us.  61 conversations with three forks each 11.8 us; 63 forks of
+// 250 pages of one page list 70 (atomics on the same pages, one after another).
 template <int NT, int SEQS>
 __global__ __launch_bounds__(NT) void lg_k_page_fork(ForkArgs a) {
     __shared__ int32_t gone[SEQS + 1], come[SEQS + 1], fresh[SEQS];      // releases and arrivals before each row; which of the new pages it takes, -1 none
@@ -178,7 +179,8 @@ struct PageLayers { PageLayer l[LG_LAYERS]; };
 
 // The rows of an accepted path to the places behind the committed ones.  Rows only move down and in order (path[k] > path[k - 1]), so a thread that takes 16 bytes of them all, up to eight
 // at a time, has read every row before it is written over.  Bound by memory: 2 bytes read and 2 written a value; where the rows lie is a chain of lengths, path and pages ahead of that, which is why
-// a workgroup takes keys and values of a layer together, two places of 16 bytes a thread.
+// a workgroup takes keys and values of a layer together, two places of 16 bytes a thread.  64 sequences of 48 layers of 8 heads of 256, 176 MB read and written: 28 to 30 us where caches hold a part of it (5.8 TB/s),
+// 44 where they do not (4.0); one sequence of 42 layers 3.6.
 typedef uint32_t lg_u4 __attribute__((ext_vector_type(4)));          // (arrays of HIP's own uint4 end up in scratch memory)
 #define LG_MOVE_AT_ONCE 8
 #define LG_MOVE_PLACES  512         // of a workgroup
@@ -240,7 +242,7 @@ __global__ __launch_bounds__(256) void lg_k_page_compact(PageLayers ls, const in
         else move(std::integral_constant<int, 2>{}, k0);
     }
 }
-// The first rows[i] rows of page from[i] to page to[i]: a workgroup takes every `parts`-th 4096 bytes of K or V of one pair in one layer.  Bound by memory, as above.
+// The first rows[i] rows of page from[i] to page to[i]: a workgroup takes every `parts`-th 4096 bytes of K or V of one pair in one layer.  Bound by memory: 1.81 GB read and written 372 us, 4.9 TB/s, as much as any copy; nine pages of 42 layers, 55 MB, 8 to 9 us.
 __global__ __launch_bounds__(256) void lg_k_page_copy(PageLayers ls, const int32_t *from, const int32_t *to, const int32_t *rows, int shift, int n_pages, int parts) {
     const int i = blockIdx.z, a = from[i], b = to[i], n = rows[i];
     if (a < 0 || a >= n_pages || b < 0 || b >= n_pages || a == b || n < 1) return;

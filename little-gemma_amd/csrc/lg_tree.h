@@ -20,7 +20,7 @@ __device__ __forceinline__ TreeRows lg_tree_rows(const int32_t *start, int seq, 
 }
 
 // ---- plan and accept -------------------------------------------------------------------------------------------------
-// A wavefront to a tree, a lane to a row.  Both are chains of a few hundred clocks behind two round trips to memory.
+// A wavefront to a tree, a lane to a row.  Both are chains of a few hundred clocks behind two round trips to memory: one tree of 8 rows 1.4 us each, 256 of 64 rows (a few hundred KB) 2.6.
 #define LG_TREE_WG 256
 // anc(j) = anc(parent j) + {j}: every lane takes over what the row it points at has reached, then points where that one points; the reach doubles, so six steps do for 64 rows.
 __global__ __launch_bounds__(LG_TREE_WG) void lg_k_tree_plan(const int32_t *start, const int32_t *parent, const int32_t *len, lg_u64 *mask, int32_t *pos, int32_t *seq_of,
@@ -79,13 +79,15 @@ __global__ __launch_bounds__(LG_TREE_WG) void lg_k_tree_accept(const int32_t *st
 // ---- attend ----------------------------------------------------------------------------------------------------------
 // o[j, h] = sum_t softmax_t(scale q[j, h].k[t]) v[t] over the committed positions t of a row's window and the rows of its tree that its set names.
 //
-// A workgroup takes a stretch of keys of one key head and up to ROWS = 16 RT of the n G (row, query head) pairs that share them; its four wavefronts take tiles of 32 keys in
+// A workgroup takes a stretch of keys of one key head and up to ROWS = 16 RT WR of the n G (row, query head) pairs that share them; its four wavefronts take tiles of 32 keys in
 // turn, as lg_k_page_attn does, and for the same reason no key or value passes through LDS: a lane's 16 bytes of a key row are the operand of the scores as they lie in memory, and the 8 x 8 values
 // that a lane loads are turned in registers, here once for all pairs.
 // Queries and probabilities are f32 and keep their precision as two binary16 parts (22 bits together) whose products go into one sum: two instructions for each 16 pairs, where the one-row
 // kernel puts the second part into rows that it has anyway.  Queries lie in LDS as operands; maxima, sums and outputs are in f32.
 // A tile that all pairs see whole (every tile but those at a window's border and of the tree) has no mask.  In the others a value that is infinite or NaN must not reach rows that
 // do not see it through 0 * inf: it is taken out of the product and marked by a product of its own.
+// Bound by memory where there is much to read (one tree of 16 rows over 100003 tokens, 8 key heads of 256: 820 MB in 139 to 145 us, 5.7 TB/s), by the chain lengths -> ids, queries -> keys -> products ->
+// joining in LDS where there is little (a chain of 5 over 100 tokens 6 us, heads of 256 9.7): 64 trees of 16 in windows of 512, 65 MB, take 27 us, a workgroup to each compute unit.
 struct TreeAttn : PageAttn {        // len: with the tree's rows
     const int32_t *start, *pos;
     const lg_u64 *mask;
@@ -661,6 +663,10 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
 // The same for more than 32 pairs: their wavefronts share keys and values through LDS.  From memory to registers each of them would ask for the same rows again, and rows of keys as operands are asked for
 // in 16 pieces of 64 bytes, for which the memory pipeline takes four times as long as for whole rows; here a tile of 32 keys and values goes to LDS once, by loads that pass no
 // register, while the tile before is worked on.  Queries stay in registers: a wavefront takes 16 pairs, and all keys, so that nothing is joined in the end.
+// Measured: 24 trees of up to 64 rows over up to 8192 tokens, heads of 256 (159 MB of keys and values, 57 GFLOP issued) 93 us (121 in lg_k_tree_attn's groups of 32 pairs); without the loads of later tiles it would take 79, and
+// those alone 41; its matrix units are busy a quarter of the time, its compute units three quarters, since splits are of 31 tiles where 26 would be even.  64 trees of 16 over 4096 tokens 123 to 131 us, 537 MB, of
+// which loads alone take 117.  Tried: values read once a workgroup, by wavefronts that take a quarter of the dimensions for all pairs and get the probabilities through LDS (heads of 256 131 -> 123 us and 99 -> 97, but
+// heads of 64 28 -> 32, 128 38 -> 41, 512 137 -> 236); 32 pairs to a wavefront (spills); loads of the next tile between score steps, four chains of scores, priorities around products (nothing).
 // A row's 16-byte pieces lie in LDS in an order of the row's own (piece j ^ swap), so that reads of a column of 16 rows touch all banks.
 constexpr int lg_wide_per_simd(int hd) { return hd <= 256 ? 2 : 1; }
 // 16 bytes of each lane, from a common place and its own distance behind it, to LDS, one after another from byte `to` on
