@@ -660,12 +660,12 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
     }
 }
 
-// The same for more than 32 pairs: their wavefronts share keys and values through LDS.  From memory to registers each of them would ask for the same rows again, and rows of keys as operands are asked for
+// The same for more than 32 pairs, where there is much to read: their wavefronts share keys and values through LDS.  From memory to registers each of them would ask for the same rows again, and rows of keys as operands are asked for
 // in 16 pieces of 64 bytes, for which the memory pipeline takes four times as long as for whole rows; here a tile of 32 keys and values goes to LDS once, by loads that pass no
 // register, while the tile before is worked on.  Queries stay in registers: a wavefront takes 16 pairs, and all keys, so that nothing is joined in the end.
 // Measured: 24 trees of up to 64 rows over up to 8192 tokens, heads of 256 (159 MB of keys and values, 57 GFLOP issued) 93 us (121 in lg_k_tree_attn's groups of 32 pairs); without the loads of later tiles it would take 79, and
-// those alone 41; its matrix units are busy a quarter of the time, its compute units three quarters, since splits are of 31 tiles where 26 would be even.  64 trees of 16 over 4096 tokens 123 to 131 us, 537 MB, of
-// which loads alone take 117.  Tried: values read once a workgroup, by wavefronts that take a quarter of the dimensions for all pairs and get the probabilities through LDS (heads of 256 131 -> 123 us and 99 -> 97, but
+// those alone 41; its matrix units are busy a quarter of the time, its compute units three quarters, since splits are of 31 tiles where 26 would be even.  64 trees of 16 over 4096 tokens 129 us, 537 MB, of
+// which loads alone take 116.  Tried: values read once a workgroup, by wavefronts that take a quarter of the dimensions for all pairs and get the probabilities through LDS (heads of 256 131 -> 123 us and 99 -> 97, but
 // heads of 64 28 -> 32, 128 38 -> 41, 512 137 -> 236); 32 pairs to a wavefront (spills); loads of the next tile between score steps, four chains of scores, priorities around products (nothing).
 // A row's 16-byte pieces lie in LDS in an order of the row's own (piece j ^ swap), so that reads of a column of 16 rows touch all banks.
 constexpr int lg_wide_per_simd(int hd) { return hd <= 256 ? 2 : 1; }
