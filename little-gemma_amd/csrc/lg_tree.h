@@ -48,7 +48,8 @@ __global__ __launch_bounds__(LG_TREE_WG) void lg_k_tree_plan(const int32_t *star
     }
     if (j == 0) status[seq] = st;
 }
-// From row 0 on to the first row behind the current one that hangs on it and carries the token picked after it, as long as there is one
+// From row 0 on to the first row behind the current one that hangs on it and carries the token picked after it, as long as there is one.  Trees that lg_k_tree_plan refuses have been given no sets: what was
+// picked behind their rows comes of no attention, so none of it is accepted, and the sequence stays at its committed length (at the length it has, where that is below the rows)
 __global__ __launch_bounds__(LG_TREE_WG) void lg_k_tree_accept(const int32_t *start, const int32_t *parent, const int32_t *token, const int32_t *next, const int32_t *len,
                                                               int32_t *path, int32_t *count, int32_t *len_out, int32_t *last, int n_seq, int n_rows, int max_tree) {
     const int seq = (int)(blockIdx.x * (LG_TREE_WG / 64) + (threadIdx.x >> 6)), j = threadIdx.x & 63;
@@ -57,21 +58,23 @@ __global__ __launch_bounds__(LG_TREE_WG) void lg_k_tree_accept(const int32_t *st
     const int total = len[seq];
     const bool live = j < w.n;
     const int up = live ? parent[w.row0 + j] : -1, tok = live ? token[w.row0 + j] : -1, picked = live ? next[w.row0 + j] : -1;
+    const bool orphan = __any(live && j && (up < 0 || up >= j)), fits = w.n > 0 && total >= w.n;
     int cur = 0, n = 0, mine = -1, want = -1;
-    if (w.n > 0) {
+    if (fits) {
         for (;;) {                                            // (rows only rise: at most 64 rounds)
             if (j == n) mine = cur;
             ++n;
+            if (orphan) break;
             want = __builtin_amdgcn_readlane(picked, cur);
-            const lg_u64 fits = __ballot(live && j > cur && up == cur && tok == want && want >= 0);
-            if (!fits) break;
-            cur = (int)__builtin_ctzll(fits);
+            const lg_u64 goes_on = __ballot(live && j > cur && up == cur && tok == want && want >= 0);
+            if (!goes_on) break;
+            cur = (int)__builtin_ctzll(goes_on);
         }
     }
     if (j < max_tree) path[(long long)seq * max_tree + j] = mine;
     if (j == 0) {
         count[seq] = n;
-        len_out[seq] = w.n > 0 ? total - w.n + n : total;
+        len_out[seq] = fits ? total - w.n + (orphan ? 0 : n) : total;
         last[seq] = want;
     }
 }
