@@ -244,16 +244,28 @@ static int check_trees(const char *who, int n_seq, int max_tree, int n_rows) {
 }
 static dim3 waves_for(int n_seq) { return dim3((unsigned)((n_seq + LG_TREE_WG / 64 - 1) / (LG_TREE_WG / 64))); }
 
+static int launch_tree_plan(const char *who, int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_len, int32_t *d_grown, uint64_t *d_mask,
+                            int32_t *d_pos, int32_t *d_seq, int32_t *d_status, void *stream) {
+    if (!d_start || !d_len || !d_status || (n_rows && (!d_parent || !d_mask || !d_pos || !d_seq))) return lg_fail(-1, "%s: null argument", who);
+    if ((uintptr_t)d_mask & 7) return lg_fail(-2, "%s: sets that are not aligned to 8 bytes", who);
+    hipLaunchKernelGGL(lg_k_tree_plan, waves_for(n_seq), dim3(LG_TREE_WG), 0, (hipStream_t)stream, d_start, d_parent, d_len, d_grown, (lg_u64 *)d_mask, d_pos, d_seq, d_status, n_seq, n_rows,
+                       max_tree);
+    LG_TRY(hipGetLastError());
+    return 0;
+}
 extern "C" int lg_hip_tree_plan(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_len, uint64_t *d_mask, int32_t *d_pos,
                                 int32_t *d_seq, int32_t *d_status, void *stream) {
     const int rc = check_trees("tree_plan", n_seq, max_tree, n_rows);
-    if (rc) return rc;
-    if (n_seq == 0) return 0;
-    if (!d_start || !d_len || !d_status || (n_rows && (!d_parent || !d_mask || !d_pos || !d_seq))) return lg_fail(-1, "tree_plan: null argument");
-    if ((uintptr_t)d_mask & 7) return lg_fail(-2, "tree_plan: sets that are not aligned to 8 bytes");
-    hipLaunchKernelGGL(lg_k_tree_plan, waves_for(n_seq), dim3(LG_TREE_WG), 0, (hipStream_t)stream, d_start, d_parent, d_len, (lg_u64 *)d_mask, d_pos, d_seq, d_status, n_seq, n_rows, max_tree);
-    LG_TRY(hipGetLastError());
-    return 0;
+    if (rc || n_seq == 0) return rc;
+    return launch_tree_plan("tree_plan", n_seq, max_tree, n_rows, d_start, d_parent, d_len, nullptr, d_mask, d_pos, d_seq, d_status, stream);
+}
+extern "C" int lg_hip_tree_plan_from(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_len, int32_t *d_len_grown, uint64_t *d_mask,
+                                     int32_t *d_pos, int32_t *d_seq, int32_t *d_status, void *stream) {
+    const int rc = check_trees("tree_plan_from", n_seq, max_tree, n_rows);
+    if (rc || n_seq == 0) return rc;
+    if (!d_len_grown) return lg_fail(-1, "tree_plan_from: null argument");
+    if (d_len_grown == d_len) return lg_fail(-2, "tree_plan_from: lengths before and behind the plan in one place");
+    return launch_tree_plan("tree_plan_from", n_seq, max_tree, n_rows, d_start, d_parent, d_len, d_len_grown, d_mask, d_pos, d_seq, d_status, stream);
 }
 
 extern "C" int lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_token, const int32_t *d_next, const int32_t *d_len,

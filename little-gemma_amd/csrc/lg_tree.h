@@ -23,12 +23,18 @@ __device__ __forceinline__ TreeRows lg_tree_rows(const int32_t *start, int seq, 
 // A wavefront to a tree, a lane to a row.  Both are chains of a few hundred clocks behind two round trips to memory: one tree of 8 rows 1.4 us each, 256 of 64 rows (a few hundred KB) 2.6.
 #define LG_TREE_WG 256
 // anc(j) = anc(parent j) + {j}: every lane takes over what the row it points at has reached, then points where that one points; the reach doubles, so six steps do for 64 rows.
-__global__ __launch_bounds__(LG_TREE_WG) void lg_k_tree_plan(const int32_t *start, const int32_t *parent, const int32_t *len, lg_u64 *mask, int32_t *pos, int32_t *seq_of,
+// With `grown`, len holds the lengths ahead of the plan that made `start`, and grown gets those behind it: by the rows that the plan has given, which are none where it was refused
+__global__ __launch_bounds__(LG_TREE_WG) void lg_k_tree_plan(const int32_t *start, const int32_t *parent, const int32_t *len, int32_t *grown, lg_u64 *mask, int32_t *pos, int32_t *seq_of,
                                                             int32_t *status, int n_seq, int n_rows, int max_tree) {
     const int seq = (int)(blockIdx.x * (LG_TREE_WG / 64) + (threadIdx.x >> 6)), j = threadIdx.x & 63;
     if (seq >= n_seq) return;
     const TreeRows w = lg_tree_rows(start, seq, n_rows, max_tree);
-    const int total = len[seq];
+    int total = len[seq];
+    if (grown) {
+        const long long rows = (long long)start[seq + 1] - start[seq], sum = total + rows;
+        if (rows > 0 && sum <= INT32_MAX) total = (int)sum;
+        if (j == 0) grown[seq] = total;
+    }
     if (w.n < 0) { if (j == 0) status[seq] = LG_TREE_BAD_ROWS; return; }
     const bool live = j < w.n;
     int up = live ? parent[w.row0 + j] : 0;

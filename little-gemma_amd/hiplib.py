@@ -113,6 +113,7 @@ def load_hip():
     L.lg_hip_sample_workspace.restype = Z
     L.lg_hip_sample.argtypes = [P, Q, I, I] + [P] * 6 + [Z, P]
     L.lg_hip_tree_plan.argtypes = [I] * 3 + [P] * 8
+    L.lg_hip_tree_plan_from.argtypes = [I] * 3 + [P] * 9
     L.lg_hip_tree_accept.argtypes = [I] * 3 + [P] * 10
     L.lg_hip_paged_tree_attention_workspace.argtypes = [I] * 7
     L.lg_hip_paged_tree_attention_workspace.restype = Z
