@@ -326,10 +326,13 @@ extern "C" size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree,
     return tree_cut_bytes(n_seq, t) + 2 * up256(slots * 4) + slots * hd * 4;
 }
 
+// (lg_tree_number turns 64 workgroups in a row: launches are of whole sixty-fours)
+static int64_t tree_groups(const TreeCut &t, int n_head_kv) { return (t.items * n_head_kv + 63) / 64 * 64; }
+
 #define LG_TREE_FEW 1024
 template <int HD>
 static void launch_tree(const TreeAttn &a, const TreeCut &t, hipStream_t st) {
-    const dim3 grid((unsigned)(((int64_t)a.items * a.nkv + 63) / 64 * 64)), wg(LG_PA_WAVES * 64);
+    const dim3 grid((unsigned)tree_groups(t, a.nkv)), wg(LG_PA_WAVES * 64);
     if (t.form.wide) {
         hipLaunchKernelGGL(lg_k_tree_wide<HD>, grid, wg, 0, st, a);
     } else if (t.form.rt * t.form.wr == 1) hipLaunchKernelGGL((lg_k_tree_attn<HD, 1, 1>), grid, wg, 0, st, a);
@@ -361,8 +364,8 @@ extern "C" int lg_hip_paged_tree_attention(const struct lg_hip_pages *p, const f
     if ((uintptr_t)d_mask & 7) return lg_fail(-2, "paged_tree_attention: sets that are not aligned to 8 bytes");
     const TreeCut t = tree_cut_of(n_seq, max_tree, n_head, p->n_head_kv, hd, max_len, window);
     const AttnCut &c = t.c;
-    // (sums over the sequences are 32 bits on the device, and so are a launch's threads)
-    if (c.tiles > INT32_MAX || t.items * p->n_head_kv > LG_MOST_GROUPS || (int64_t)n_head * max_tree * n_seq > LG_MOST_GROUPS / 2)
+    // (sums over the sequences are 32 bits on the device, and so are a launch's threads; the joining launch has 512 to a row's head)
+    if (c.tiles > INT32_MAX || tree_groups(t, p->n_head_kv) > LG_MOST_GROUPS || (c.join && (int64_t)n_head * max_tree * n_seq > LG_MOST_GROUPS / 2))
         return lg_fail(-2, "paged_tree_attention: %d sequences of up to %d rows of %d heads in %lld splits in one call", n_seq, max_tree, n_head, (long long)c.splits);
     const size_t need = lg_hip_paged_tree_attention_workspace(n_seq, max_tree, n_head, p->n_head_kv, hd, max_len, window);
     if (need && (!d_work || work_bytes < need || ((uintptr_t)d_work & 255)))

@@ -3,7 +3,7 @@ import ctypes as C
 
 import pytest
 
-from test_serving_refusals import P16, refused
+from test_serving_refusals import P16, pages, refused
 
 P32 = C.c_void_p(1 << 22)
 
@@ -18,3 +18,23 @@ def test_tree_plans_from_earlier_lengths_refuse(lg, change, code, words):
     H = lg.hiplib.load_hip()
     refused(lg, H.lg_hip_tree_plan_from(a["n_seq"], a["most"], a["rows"], *(None if a["null"] == k else x for k, x in enumerate(p)), None), code, words)
     assert H.lg_hip_tree_plan_from(0, 4, 9, *[None] * 8, None) == 0
+
+
+def attend(H, lg, seqs, heads, kv, most, max_len, hd=64):
+    p = pages(lg, dict(n_head_kv=kv, head_dim=hd, row_stride=kv * hd, page_stride=kv * hd * 16))
+    return H.lg_hip_paged_tree_attention(C.byref(p), P16, hd * heads, 9, seqs, most, heads, P16, 1 << 26, P16, P16, P16, P16, max_len, 0, 1.0, P16, hd * heads, P16, 1 << 62, None)
+
+
+@pytest.mark.parametrize("below", [1, 20, 63])
+def test_launches_are_counted_as_they_are_made(lg, below):
+    """A call of 2^24 - below workgroups is launched in whole sixty-fours: 2^24, whose threads pass 32 bits.  Splits of 127 tiles in rounds of 768 workgroups, 2^24 - 256 of them, and one more for each sequence."""
+    seqs = 256 - below
+    tiles = (2 ** 24 - 256) * 127 // seqs
+    assert tiles * seqs < 1 << 31
+    refused(lg, attend(lg.hiplib.load_hip(), lg, seqs, 1, 1, 1, tiles * 32), -2, "in one call")
+
+
+@pytest.mark.parametrize("seqs, heads, kv, most", [(3813, 4400, 550, 64), (2713, 6184, 773, 64)])
+def test_launches_of_whole_trees_are_counted_as_they_are_made(lg, seqs, heads, kv, most):
+    """2^24 - 16 and 2^24 - 24 workgroups of 64 pairs, and no joining launch."""
+    refused(lg, attend(lg.hiplib.load_hip(), lg, seqs, heads, kv, most, 32), -2, "in one call")
