@@ -196,10 +196,16 @@ __device__ __forceinline__ MergeRow lg_merge_row(const TreeAttn &a) {
     return { seq, node < w.n ? (long long)w.row0 + node : -1, (long long)a.max_tree * a.H, blockIdx.x, head };
 }
 
-// Probabilities are 2^(x - m + SHIFT).  m is the largest score of a while ago, rounded up to a whole number (m - SHIFT and factors between two of them are exact): it is taken anew, and the sums so far scaled,
-// only when a score passes it by SLACK, which few tiles of a long row do.  So they stay below 2^15 in binary16, and what their two parts leave of a small one is at most 2^-32 of the largest
+// Probabilities are 2^(x - m), m the largest score of a while ago, rounded up to a whole number, less SHIFT (both and factors between two of them are exact): it is taken anew, and the sums so far scaled,
+// only when a score passes it by SLACK more, which few tiles of a long row do.  So they stay below 2^15 in binary16, and what their two parts leave of a small one is at most 2^-32 of the largest.
+// Where f32 does not hold the difference, from 2^27 on, where scores lie 16 and more apart, nothing is taken off (rounded, it was 16 for half of them, and the largest probability 2^16)
 #define LG_TREE_SLACK 7.0f
 #define LG_TREE_SHIFT 8.0f
+__device__ __forceinline__ float lg_tree_base(float top) {
+    const float c = ceilf(top), m = c - LG_TREE_SHIFT;
+    return c - m > LG_TREE_SHIFT ? c : m;           // (infinities stay: their difference is NaN)
+}
+__device__ __forceinline__ bool lg_tree_passes(float top, float m) { return top - m > LG_TREE_SHIFT + LG_TREE_SLACK; }         // (both -inf: no)
 // 1 in each half of a pair of binary16 values that is infinite or NaN (all bits of the exponent: one more carries into the sign's place)
 __device__ __forceinline__ uint32_t lg_not_finite(uint32_t u) { return ((u & 0x7C007C00u) + 0x04000400u) >> 15 & 0x00010001u; }
 // The largest `whole` of the wavefront's pairs; rows of the tree in front of a pair's window are taken out of its set (which the usual windows, wider than a tree is deep, do not ask for)
@@ -234,7 +240,7 @@ typedef _Float16 lg_h2 __attribute__((ext_vector_type(2)));
 typedef float lg_f2 __attribute__((ext_vector_type(2)));
 template <int HALVES, class Part>
 __device__ __forceinline__ void lg_tree_parts(const lg_f4 (&x)[HALVES], float m, float &l, Part &hi, Part &lo) {
-    const float under = (m == -INFINITY ? 0.0f : m) - LG_TREE_SHIFT;
+    const float under = m == -INFINITY ? 0.0f : m;
     #pragma unroll
     for (int j = 0; j < 4 * HALVES; j += 2) {
         lg_f2 p, left;
@@ -527,13 +533,13 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
                 }
             top[rt] = fmaxf(top[rt], __shfl_xor(top[rt], 16));
             top[rt] = fmaxf(top[rt], __shfl_xor(top[rt], 32));
-            higher |= top[rt] > m[rt] + LG_TREE_SLACK;
+            higher |= lg_tree_passes(top[rt], m[rt]);
         }
         if (__any(higher)) {
             if constexpr (ALONE) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");           // (products write accumulation registers up to 16 cycles after they are issued; out_of reads them where the compiler does not see it)
             #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const float mn = fmaxf(m[rt], ceilf(top[rt]));
+                const float mn = fmaxf(m[rt], lg_tree_base(top[rt]));
                 const float f = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);       // (both -inf: nothing seen yet)
                 l[rt] *= f; m[rt] = mn;
                 float fr[4];
@@ -889,8 +895,8 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD)) void lg_k_t
         #pragma unroll
         for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[j >> 2][j & 3]);
         top = lg_max_of_rows(top);
-        if (__any(top > m + LG_TREE_SLACK)) {
-            const float mn = fmaxf(m, ceilf(top));
+        if (__any(lg_tree_passes(top, m))) {
+            const float mn = fmaxf(m, lg_tree_base(top));
             const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);       // (both -inf: nothing seen yet)
             l *= f; m = mn;
             float fr[4];
