@@ -686,7 +686,7 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
 constexpr int lg_wide_per_simd(int hd) { return hd <= 256 ? 2 : 1; }
 // 16 bytes of each lane, from a common place and its own distance behind it, to LDS, one after another from byte `to` on
 __device__ __forceinline__ void lg_to_lds(const void *from, uint32_t behind, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(to), "v"(behind), "s"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(to), "v"(behind), "s"(from) : "m0", "memory");
 }
 template <int HD>
 __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_wide_per_simd(HD)) void lg_k_tree_wide(TreeAttn a) {
