@@ -367,6 +367,8 @@ int    lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int32_t *d_
  * of a captured call, and the working memory), d_mask aligned to 8 bytes, the pages' row_stride at most 2^27.  What is not seen by a row does not reach it, whatever it holds, also where other rows of the tree see it; infinities and NaN that are seen
  * spoil the heads that read them (NaN as a rule) and no others. */
 size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree, int n_head, int n_head_kv, int head_dim, int max_len, int window);
+/* How many of a tree's pairs of a row and a query head a workgroup takes in a call of these sizes: 16, 32 or 64, a kernel each (for profiles and tests; 0: not served). */
+int    lg_hip_paged_tree_attention_pairs(int n_seq, int max_tree, int n_head, int n_head_kv, int head_dim, int max_len, int window);
 int    lg_hip_paged_tree_attention(const struct lg_hip_pages *pages, const float *d_q, int64_t q_stride, int n_rows, int n_seq, int max_tree, int n_head,
                                    const int32_t *d_table, int max_blocks, const int32_t *d_len, const int32_t *d_start, const uint64_t *d_mask, const int32_t *d_pos,
                                    int max_len, int window, float scale, float *d_out, int64_t out_stride, void *d_work, size_t work_bytes, void *stream);

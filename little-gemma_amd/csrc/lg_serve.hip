@@ -326,6 +326,10 @@ extern "C" size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree,
     return tree_cut_bytes(n_seq, t) + 2 * up256(slots * 4) + slots * hd * 4;
 }
 
+extern "C" int lg_hip_paged_tree_attention_pairs(int n_seq, int max_tree, int n_head, int n_head_kv, int hd, int max_len, int window) {
+    if (!attn_shape(n_seq, n_head, n_head_kv, hd, max_len) || max_tree < 1 || max_tree > LG_TREE_ROWS || window < 0) return 0;
+    return tree_cut_of(n_seq, max_tree, n_head, n_head_kv, hd, max_len, window).rows;
+}
 // (lg_tree_number turns 64 workgroups in a row: launches are of whole sixty-fours)
 static int64_t tree_groups(const TreeCut &t, int n_head_kv) { return (t.items * n_head_kv + 63) / 64 * 64; }
 

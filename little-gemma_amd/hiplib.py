@@ -117,6 +117,7 @@ def load_hip():
     L.lg_hip_tree_accept.argtypes = [I] * 3 + [P] * 10
     L.lg_hip_paged_tree_attention_workspace.argtypes = [I] * 7
     L.lg_hip_paged_tree_attention_workspace.restype = Z
+    L.lg_hip_paged_tree_attention_pairs.argtypes = [I] * 7
     L.lg_hip_paged_tree_attention.argtypes = [P, P, Q, I, I, I, I, P, I, P, P, P, P, I, I, C.c_float, P, Q, P, Z, P]
     L.lg_hip_paged_compact.argtypes = [P, I, I, I, P, I, P, P, P, P, P]
     L.lg_hip_paged_fork_workspace.argtypes = [I] * 3

@@ -21,8 +21,10 @@ def small(lg, dev, s, kv, most, max_len, window=0):
 @pytest.mark.parametrize("form, heads, kv, hd, most", FORMS + [(16, 8, 2, 128, 7)])
 def test_in_splits(lg, dev, form, heads, kv, hd, most):
     rng = np.random.default_rng(form + hd + most)
-    s = scene(rng, [100, 0, 1200, 33, 500], [most, max(1, most - 1), most, 1, most], heads, kv, hd, 16)
-    small(lg, dev, s, kv, most, max(int(s["lens"].max()), room_of(form, 5, heads, kv, hd, most)))
+    s = scene(rng, [100, 0, 600 if form == 16 else 1200, 33, 500], [most, max(1, most - 1), most, 1, most], heads, kv, hd, 16)
+    room = max(int(s["lens"].max()), room_of(form, 5, heads, kv, hd, most))
+    assert dev.H.lg_hip_paged_tree_attention_pairs(5, most, heads, kv, hd, room, 0) == form
+    small(lg, dev, s, kv, most, room)
 
 
 @pytest.mark.parametrize("form, heads, kv, hd, most", [x for x in FORMS if x[0] > 16])
@@ -31,4 +33,6 @@ def test_whole(lg, dev, form, heads, kv, hd, most, window):
     rng = np.random.default_rng(form + hd + most)
     n = min(4096, -(-tiles_for(form, most * (heads // kv), hd) // ((window + most + 63) // 32 * kv if window else 8 * kv)))
     s = scene(rng, with_empty([0, 40, 120, 190 if not window else 1500], n), with_empty([most, most, 1, most], n), heads, kv, hd, 16)
-    small(lg, dev, s, kv, most, int(s["lens"].max()) if window else 256, window)
+    room = int(s["lens"].max()) if window else 256
+    assert dev.H.lg_hip_paged_tree_attention_pairs(n, most, heads, kv, hd, room, window) == form
+    small(lg, dev, s, kv, most, room, window)
