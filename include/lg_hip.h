@@ -347,7 +347,7 @@ enum { LG_HIP_TREE_BAD_ROWS = 1,       /* d_start falls, a tree has more than ma
        LG_HIP_TREE_BAD_LENGTH = 4 };   /* a length below the tree's rows */
 int    lg_hip_tree_plan(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_len, uint64_t *d_mask, int32_t *d_pos,
                         int32_t *d_seq, int32_t *d_status, void *stream);
-/* The same from the lengths ahead of lg_hip_paged_plan: d_len_grown [n_seq] (not d_len itself) gets d_len and the rows that the plan has given a sequence, which are none where it was refused.  What comes behind takes its
+/* The same from the lengths ahead of lg_hip_paged_plan: d_len_grown [n_seq] (not d_len itself; the array of the lengths that the plan was asked for will do) gets d_len and the rows that the plan has given a sequence, which are none where it was refused.  What comes behind takes its
  * lengths from there: after a refused plan every tree is empty, nothing is accepted, and d_len_out of lg_hip_tree_accept is d_len again, with no word from the host.  (A program that hands on lengths of its own after a
  * refused plan says that sequences hold pages which they do not.) */
 int    lg_hip_tree_plan_from(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_len, int32_t *d_len_grown, uint64_t *d_mask, int32_t *d_pos,
@@ -365,7 +365,8 @@ int    lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int32_t *d_
  * zeros, so do the rows of a sequence whose length is below its rows or above max_len or max_blocks * page_size; rows of a tree with LG_HIP_TREE_BAD_ROWS and rows of no tree are left as they are.
  * Positions whose page is outside 0..n_pages-1 are left out.  Arguments as lg_hip_paged_attention's (n_head / n_head_kv <= 8, q_stride a multiple of 4, d_q aligned to 16 bytes; max_len bounds the lengths
  * of a captured call, and the working memory), d_mask aligned to 8 bytes, the pages' row_stride at most 2^27.  What is not seen by a row does not reach it, whatever it holds, also where other rows of the tree see it; infinities and NaN that are seen
- * spoil the heads that read them (NaN as a rule) and no others. */
+ * spoil the heads that read them (NaN as a rule) and no others.  Queries and probabilities enter the products as two binary16 parts each, 22 bits (lg_hip_paged_attention's do as well), all sums are of f32: outputs are
+ * off by 3e-7 to 1.1e-6 of their size, by 6e-8 where a row sees one key, by 1.4e-7 to 2.8e-7 (heads of 64 to 512) where it sees four. */
 size_t lg_hip_paged_tree_attention_workspace(int n_seq, int max_tree, int n_head, int n_head_kv, int head_dim, int max_len, int window);
 /* How many of a tree's pairs of a row and a query head a workgroup takes in a call of these sizes: 16, 32 or 64, a kernel each (for profiles and tests; 0: not served). */
 int    lg_hip_paged_tree_attention_pairs(int n_seq, int max_tree, int n_head, int n_head_kv, int head_dim, int max_len, int window);
@@ -409,7 +410,8 @@ struct lg_hip_logit_rules {
     const struct lg_hip_penalty *penalty;/* [n_seq] */
     const int32_t *hist, *hist_len;      /* [n_seq][hist_stride] the texts, [n_seq] how much of them counts (at most hist_stride, at most 2^30); needs penalty */
     int64_t hist_stride;
-    const uint64_t *tree_mask;           /* [rows] sets of rows of a tree, as lg_hip_tree_plan's: their tokens count as generated too; needs penalty, tree_start, tree_tok */
+    const uint64_t *tree_mask;           /* [rows] sets of rows of a tree, as lg_hip_tree_plan's: their tokens count as generated too; needs penalty, tree_start, tree_tok.  Bit k of a row of sequence i is row
+                                          * tree_start[i] + k of the call, none outside it: unlike attention this does not ask whether the tree has that row, so sets of the caller's own name no more than their tree's */
     const int32_t *tree_start, *tree_tok;/* [n_seq + 1] the first row of each sequence's tree, [rows] tokens */
     const int32_t *bias_start, *bias_tok;/* [n_seq + 1], [n_bias]: sequence i adds bias[j] to the logit of bias_tok[j], bias_start[i] <= j < bias_start[i + 1]; of a token named more than once the last counts */
     const float *bias;                   /* [n_bias] */

@@ -25,6 +25,8 @@ struct RulesArgs {
 // the order does not matter), then writes the slice.  Bound by memory where rows are many: 8 bytes a logit; a text is read once for every slice of every row, but from the L2.
 // 64 rows of 262144 with penalties, biases and sets, 135 MB: 28 us, 4.8 TB/s; one row with a text of 3001 tokens 4.8 us, the launch and the chain of parameters, text and logits.  Slices of 2048 at all sizes: of 4096 64
 // rows took 34.6, one row 5.1.  Rows that are not aligned to 16 bytes (VEC false): 39.6 and 5.2.
+// Long texts take longer, for each slice goes over all of its row's text: one row with 32768 and 100000 tokens 10.9 and 25.4 us; 64 rows with texts of their own, penalties alone, 3001, 32768 and 100000 tokens 23.0, 36.6
+// and 62.4.
 // Logits that a rule changes are computed in 64 bits and rounded once.
 template <bool VEC>
 __global__ __launch_bounds__(LG_RULES_WG) void lg_k_rules(RulesArgs a) {

@@ -281,22 +281,32 @@ extern "C" int lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int
 }
 
 // How many pairs a workgroup takes, 16 RT by each of WR wavefronts, goes by how much there is to read: tiles of all sequences and key heads, as often as groups of so many pairs read them.
-// Few pairs make short workgroups, and many of them; where the chip is full their reads of the same keys again cost more.  Us of trees of 8 and 16 rows, heads of 256, 4 query heads to a key head:
-//   16 to a workgroup and 32: windows of 512 of 32 sequences (4608 tiles, read by sixteens) 20.3 and 25.2, of 40 (5760) 36.9 and 25.4; 4096 tokens of 4 (4096) 23.3 and 24.7, of 8 (8192) 36.0 and 32.0; 100
-//     tokens of one, trees of 5, 9.7 and 12.9; heads of 128: 2048 14.8 and 15.8, 4096 20.3 and 18.3, in windows 4608 12.5 and 15.9, 9216 18.5 and 17.3; heads of 64: 8192 19.3 and 20.5, 16384 28.1 and 21.5;
-//     heads of 512: 4096 38.4 and 42.8, in windows 4352 32.9 and 54.8
-//   32 (lg_k_tree_attn) and 64 (lg_k_tree_wide, which reads keys once for all four wavefronts but spends 10 us beside its tiles): windows of 64 sequences (2304 tiles, read by sixty-fours) 27.0 and 33.3, of 96
-//     (3456) 46.5 and 36, of 128 (4608) 48.4 and 36.2; 4096 tokens of 8 (2048) 33.0 and 33.7, of 20 (5120) 47.3 and 45.7, of 32 (8192) 75.9 and 63.5; heads of 128: 4608 31.8 and 24.8; heads of 512: 2304 62.6 and
-//     55.9.  Trees of up to 32 pairs in wide workgroups: 100003 tokens 166 for 147, 64 sequences in windows of 512 31.1 for 25.5
+// Few pairs make short workgroups, and many of them; where the chip is full their reads of the same keys again cost more.  Us, trees of 8 and 16 rows, 4 query heads to a key head:
+//
+//   heads  keys of sequences     tiles, read by 16   16 pairs  32       heads  keys of sequences     tiles, read by 64   32 pairs  64
+//   256    windows of 512, 32    4608                20.3      25.2     256    windows of 512, 64    2304                27.0      33.3
+//          windows of 512, 40    5760                36.9      25.4            windows of 512, 96    3456                46.5      36
+//          4096, 4               4096                23.3      24.7            windows of 512, 128   4608                48.4      36.2
+//          4096, 8               8192                36.0      32.0            4096, 8               2048                33.0      33.7
+//          100, 1 (trees of 5)   8                   9.7       12.9            4096, 20              5120                47.3      45.7
+//   128    all                   2048                14.8      15.8            4096, 32              8192                75.9      63.5
+//          all                   4096                20.3      18.3     128    windows               4608                31.8      24.8
+//          windows               4608                12.5      15.9     512    windows               2304                62.6      55.9
+//          windows               9216                18.5      17.3
+//   64     all                   8192                19.3      20.5     (64 pairs: lg_k_tree_wide, which reads keys once for all four wavefronts but
+//          all                   16384               28.1      21.5     spends 10 us beside its tiles.  Trees of up to 32 pairs in its workgroups:
+//   512    all                   4096                38.4      42.8     100003 tokens 166 for 147, 64 sequences in windows of 512 31.1 for 25.5)
+//          windows               4352                32.9      54.8
 struct TreeForm { int rt, wr; bool wide; };
 static TreeForm tree_form(int pairs, int hd, int64_t tiles) {
     if (pairs <= 16 || tiles * ((pairs + 15) / 16) <= (hd == 64 ? 9216 : 4608)) return { 1, 1, false };
     if (pairs <= 32 || (hd < 512 && tiles * ((pairs + 63) / 64) <= 2560)) return hd == 512 ? TreeForm{ 1, 2, false } : TreeForm{ 2, 1, false };
     return { 1, LG_PA_WAVES, true };
 }
-// Trees of up to so many tiles are left whole, as alone_of says for one row.  A workgroup of 64 pairs spends 10 us beside its tiles, of 1.5 us each, and the joining launch takes 8.  Whole and in splits, us, heads of
-// 256: 2 units (sequences x key heads x groups) of 512 keys 31.6 and 19.3, 16 units 33.9 and 23.2; 128 units of 144 keys 17.6 and 29.4, of 272 24.6 and 30.3, of 528 35.7 and 34.9 (all of
-// these lengths up to it: 36.7 and 33.2); 256 of 272 26.7 and 47.7, of 528 39.6 and 55.6; 512 of 528 65.1 and 114.8
+// Trees of up to so many tiles are left whole, as alone_of says for one row.  A workgroup of 64 pairs spends 10 us beside its tiles, of 1.5 us each, and the joining launch takes 8.
+// Whole and in splits, us, heads of 256, by units (sequences x key heads x groups) and keys:
+//   2 units    512 31.6 and 19.3                      128 units  144 17.6 and 29.4, 272 24.6 and 30.3, 528 35.7 and 34.9 (all lengths up to it: 36.7 and 33.2)
+//   16 units   512 33.9 and 23.2                      256 units  272 26.7 and 47.7, 528 39.6 and 55.6                512 units  528 65.1 and 114.8
 static int tree_alone_of(int hd, int64_t units, bool wide) {
     if (!wide) return alone_of(hd, units);
     return units < 64 ? 8 : units < 160 ? 16 : units < 512 ? 24 : 32;

@@ -25,7 +25,7 @@ struct ForkArgs {
 // All or nothing: everything is read and counted in working memory, then everything is written.
 // One workgroup, of NT threads: a few words for every page that moves, its time a chain of round trips to memory (lengths, ids, shares; counts; places; stores).  A thread keeps its first release, arrival and
 // row in registers, so that a call of up to NT of each asks for them once: eight forks of 16 pages 9.7 -> 7.1 us.  61 conversations with three forks each 11.8 us; 63 forks of
-// 250 pages of one page list 70 (atomics on the same pages, one after another).
+// 250 pages of one page list 70, eight of 1563 pages 80: atomics for each page of each fork, on the same pages one after another, from one workgroup.
 template <int NT, int SEQS>
 __global__ __launch_bounds__(NT) void lg_k_page_fork(ForkArgs a) {
     __shared__ int32_t gone[SEQS + 1], come[SEQS + 1], fresh[SEQS];      // releases and arrivals before each row; which of the new pages it takes, -1 none

@@ -96,7 +96,9 @@ __global__ __launch_bounds__(LG_TREE_WG) void lg_k_tree_accept(const int32_t *st
 // A tile that all pairs see whole (every tile but those at a window's border and of the tree) has no mask.  In the others a value that is infinite or NaN must not reach rows that
 // do not see it through 0 * inf: it is taken out of the product and marked by a product of its own.
 // Bound by memory where there is much to read (one tree of 16 rows over 100003 tokens, 8 key heads of 256: 820 MB in 139 to 145 us, 5.7 TB/s), by the chain lengths -> ids, queries -> keys -> products ->
-// joining in LDS where there is little (a chain of 5 over 100 tokens 6 us, heads of 256 9.7): 64 trees of 16 in windows of 512, 65 MB, take 27 us, a workgroup to each compute unit.
+// joining in LDS where there is little (a chain of 5 over 100 tokens 6 us, heads of 256 9.7): 64 trees of 16 in windows of 512, 65 MB, take 26 us, a workgroup to each compute unit.  Of a workgroup's 23 us, by clock stamps,
+// 1.6 go by until starts and lengths are there, 3.8 until pages, sets and queries are and the first keys are on their way, 5.6 until the first tile is done (its keys, then its values, arrive), 9.3 with the three or four other tiles
+// of a wavefront, 2.9 with the joining of the four and the stores.
 struct TreeAttn : PageAttn {        // len: with the tree's rows
     const int32_t *start, *pos;
     const lg_u64 *mask;
@@ -678,10 +680,11 @@ __global__ __launch_bounds__(LG_PA_WAVES * 64, lg_tree_per_simd(HD, RT)) void lg
 // The same for more than 32 pairs, where there is much to read: their wavefronts share keys and values through LDS.  From memory to registers each of them would ask for the same rows again, and rows of keys as operands are asked for
 // in 16 pieces of 64 bytes, for which the memory pipeline takes four times as long as for whole rows; here a tile of 32 keys and values goes to LDS once, by loads that pass no
 // register, while the tile before is worked on.  Queries stay in registers: a wavefront takes 16 pairs, and all keys, so that nothing is joined in the end.
-// Measured: 24 trees of up to 64 rows over up to 8192 tokens, heads of 256 (159 MB of keys and values, 57 GFLOP issued) 93 us (121 in lg_k_tree_attn's groups of 32 pairs); without the loads of later tiles it would take 79, and
-// those alone 41; its matrix units are busy a quarter of the time, its compute units three quarters, since splits are of 31 tiles where 26 would be even.  64 trees of 16 over 4096 tokens 129 us, 537 MB, of
-// which loads alone take 116.  Tried: values read once a workgroup, by wavefronts that take a quarter of the dimensions for all pairs and get the probabilities through LDS (heads of 256 131 -> 123 us and 99 -> 97, but
-// heads of 64 28 -> 32, 128 38 -> 41, 512 137 -> 236); 32 pairs to a wavefront (spills); loads of the next tile between score steps, four chains of scores, priorities around products (nothing).
+// Measured: 24 trees of up to 64 rows over up to 8192 tokens, heads of 256 (159 MB of keys and values, 57 GFLOP issued) 87.5 us in a row of calls, and 7.6 the joining launch behind it (121 in lg_k_tree_attn's groups of 32 pairs;
+// 95 and more by itself under a profiler).  Without the loads of later tiles it would take 79, and those alone 41; its matrix units are busy a quarter of the time, its compute units three quarters, since splits are of 31 tiles where 26
+// would be even.  64 trees of 16 over 4096 tokens 129 us, 537 MB, of which loads alone take 116: a workgroup's loads drain at each tile's barrier.
+// Tried: values read once a workgroup, by wavefronts that take a quarter of the dimensions for all pairs and get the probabilities through LDS (heads of 256 131 -> 123 us and 99 -> 97, but heads of 64 28 -> 32, 128 38 -> 41,
+// 512 137 -> 236); 32 pairs to a wavefront (spills); loads of the next tile between score steps, four chains of scores, priorities around products (nothing).
 // A row's 16-byte pieces lie in LDS in an order of the row's own (piece j ^ swap), so that reads of a column of 16 rows touch all banks.
 constexpr int lg_wide_per_simd(int hd) { return hd <= 256 ? 2 : 1; }
 // 16 bytes of each lane, from a common place and its own distance behind it, to LDS, one after another from byte `to` on

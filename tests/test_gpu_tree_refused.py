@@ -202,6 +202,13 @@ def test_lengths_behind_a_plan(dev):
     assert pos[[0, 1, 2, 9, 10, 12]].tolist() == [7, 8, 9, 0, -1, -1] and seq[[0, 9, 12]].tolist() == [0, 2, 5]
 
 
+def test_a_step_without_rows_has_the_lengths_ahead_of_it(dev):
+    p = [dev.up(x, np.int32) for x in ([0, 0, 0, 0], [5, 0, 70], [77] * 3, [77] * 3)]
+    dev.check(dev.H.lg_hip_tree_plan_from(3, 4, 0, p[0], None, p[1], p[2], None, None, None, p[3], None), "tree_plan_from")
+    assert dev.back(p[2], 3, np.int32).tolist() == [5, 0, 70] and dev.back(p[3], 3, np.int32).tolist() == [0, 0, 0]
+    dev.free()
+
+
 @pytest.mark.parametrize("n, most", [(1, 64), (257, 9)])
 def test_both_forms_of_the_tree_plan_agree(dev, n, most):
     rng = np.random.default_rng(n)
