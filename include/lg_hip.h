@@ -347,16 +347,16 @@ enum { LG_HIP_TREE_BAD_ROWS = 1,       /* d_start falls, a tree has more than ma
        LG_HIP_TREE_BAD_LENGTH = 4 };   /* a length below the tree's rows */
 int    lg_hip_tree_plan(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_len, uint64_t *d_mask, int32_t *d_pos,
                         int32_t *d_seq, int32_t *d_status, void *stream);
-/* The same from the lengths ahead of lg_hip_paged_plan: d_len_grown [n_seq] (not d_len itself; the array of the lengths that the plan was asked for will do) gets d_len and the rows that the plan has given a sequence, which are none where it was refused.  What comes behind takes its
- * lengths from there: after a refused plan every tree is empty, nothing is accepted, and d_len_out of lg_hip_tree_accept is d_len again, with no word from the host.  (A program that hands on lengths of its own after a
- * refused plan says that sequences hold pages which they do not.) */
+/* The same from the lengths ahead of lg_hip_paged_plan: d_len_grown [n_seq] (not d_len itself; the array of the lengths that the plan was asked for will do) gets d_len and the rows that the plan has
+ * given a sequence, which are none where it was refused.  What comes behind takes its lengths from there: after a refused plan every tree is empty, nothing is accepted, and d_len_out of
+ * lg_hip_tree_accept is d_len again, with no word from the host.  (A program that hands on lengths of its own after a refused plan says that sequences hold pages which they do not.) */
 int    lg_hip_tree_plan_from(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_len, int32_t *d_len_grown, uint64_t *d_mask, int32_t *d_pos,
                              int32_t *d_seq, int32_t *d_status, void *stream);
 /* After it, from d_token [n_rows], the rows' tokens, and d_next [n_rows], the token picked behind each row (lg_hip_sample, or the likeliest): from row 0 on to the first row that hangs on
  * the current one and holds the token picked behind it, as long as there is one.  d_path [n_seq][max_tree]: the rows passed, the rest -1; d_count: how many (0 for a tree without rows,
  * or with LG_HIP_TREE_BAD_ROWS); d_len_out: the sequence's length with them alone; d_last: the token picked behind the last one (-1 where there is no row). A picked token below 0 fits no row.
  * Nothing that was picked in a tree that lg_hip_tree_plan refuses is accepted: d_last is -1; with LG_HIP_TREE_BAD_PARENT the path ends at row 0 and d_len_out is the committed length, without that row (its attention
- * was refused as well, the step can be run again); with LG_HIP_TREE_BAD_LENGTH there is no path and d_len_out is the length as given. */
+ * was refused as well, the step can be run again); with LG_HIP_TREE_BAD_LENGTH, and with LG_HIP_TREE_BAD_ROWS, whose rows nothing has computed, there is no path and d_len_out is the length as given. */
 int    lg_hip_tree_accept(int n_seq, int max_tree, int n_rows, const int32_t *d_start, const int32_t *d_parent, const int32_t *d_token, const int32_t *d_next,
                           const int32_t *d_len, int32_t *d_path, int32_t *d_count, int32_t *d_len_out, int32_t *d_last, void *stream);
 /* Attention of every row of the trees, as lg_hip_paged_attention: out = softmax(scale * q.k) v over the committed positions t of the row's sequence and the tree's positions committed + k for the rows k
