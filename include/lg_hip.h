@@ -413,7 +413,7 @@ struct lg_hip_logit_rules {
     const uint64_t *tree_mask;           /* [rows] sets of rows of a tree, as lg_hip_tree_plan's: their tokens count as generated too; needs penalty, tree_start, tree_tok.  Bit k of a row of sequence i is row
                                           * tree_start[i] + k of the call, none outside it: unlike attention this does not ask whether the tree has that row, so sets of the caller's own name no more than their tree's */
     const int32_t *tree_start, *tree_tok;/* [n_seq + 1] the first row of each sequence's tree, [rows] tokens */
-    const int32_t *bias_start, *bias_tok;/* [n_seq + 1], [n_bias]: sequence i adds bias[j] to the logit of bias_tok[j], bias_start[i] <= j < bias_start[i + 1]; of a token named more than once the last counts */
+    const int32_t *bias_start, *bias_tok;/* [n_seq + 1], [n_bias] (at most 2^30): sequence i adds bias[j] to the logit of bias_tok[j], bias_start[i] <= j < bias_start[i + 1]; of a token named more than once the last counts */
     const float *bias;                   /* [n_bias] */
     const uint32_t *allow;               /* [n_allow][allow_stride] sets of tokens, token t bit t % 32 of word t / 32: logits of the others become -inf */
     const int32_t *allow_row;            /* [rows] the set of each row, outside 0..n_allow-1: none (NULL: row i has set i) */

@@ -506,6 +506,7 @@ extern "C" int lg_hip_adjust_logits(const struct lg_hip_logit_rules *r, const fl
     if (n_vocab < 1 || n_vocab > LG_RULES_VOCAB) return lg_fail(-2, "adjust_logits: a vocabulary of %d (1..%d)", n_vocab, LG_RULES_VOCAB);
     if (stride < n_vocab || out_stride < n_vocab) return lg_fail(-2, "adjust_logits: rows of %d logits, %lld and %lld apart", n_vocab, (long long)stride, (long long)out_stride);
     if (r->n_seq < 0 || r->n_bias < 0 || r->n_allow < 0) return lg_fail(-2, "adjust_logits: %d sequences, %d biases, %d grammars", r->n_seq, r->n_bias, r->n_allow);
+    if (r->n_bias > 1 << 30) return lg_fail(-2, "adjust_logits: %d biases (at most 2^30: a workgroup counts past the last one by its threads)", r->n_bias);
     if (r->hist && (r->hist_stride < 1 || r->hist_stride > 1 << 30)) return lg_fail(-2, "adjust_logits: texts %lld tokens apart", (long long)r->hist_stride);
     if (r->n_allow && r->allow_stride < (n_vocab + 31) / 32) return lg_fail(-2, "adjust_logits: sets of %d tokens, %lld words apart", n_vocab, (long long)r->allow_stride);
     if (rows == 0) return 0;

@@ -3,6 +3,7 @@ import ctypes as C
 
 import pytest
 
+from test_draft_refusals import RULES
 from test_serving_refusals import P16, pages, refused
 
 P32 = C.c_void_p(1 << 22)
@@ -38,3 +39,10 @@ def test_launches_are_counted_as_they_are_made(lg, below):
 def test_launches_of_whole_trees_are_counted_as_they_are_made(lg, seqs, heads, kv, most):
     """2^24 - 16 and 2^24 - 24 workgroups of 64 pairs, and no joining launch."""
     refused(lg, attend(lg.hiplib.load_hip(), lg, seqs, heads, kv, most, 32), -2, "in one call")
+
+
+@pytest.mark.parametrize("n", [(1 << 30) + 1, (1 << 31) - 1])
+def test_more_biases_than_a_workgroup_counts_are_refused(lg, n):
+    """Its threads count on behind the last one: near 2^31 past what 32 bits hold."""
+    r = lg.hiplib.LogitRules(**{**RULES, "n_bias": n})
+    refused(lg, lg.hiplib.load_hip().lg_hip_adjust_logits(C.byref(r), P16, 100, 3, 100, P32, 100, None), -2, "biases")
